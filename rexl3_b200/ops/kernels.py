@@ -392,6 +392,135 @@ def topk(logits: torch.Tensor, count: int, scratch, ids: torch.Tensor, vals: tor
     _lib.count(2)
 
 
+def _operand(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, like: "torch.Tensor | None" = None) -> int:
+    """The device pointer of a contiguous operand of the current device; a None in `shape` stands for any extent."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{name}: a CUDA tensor is needed")
+    if t.device.index != (torch.cuda.current_device() if like is None else like.device.index):
+        raise ValueError(f"{name} is on {t.device}" + (f", not on the current device cuda:{torch.cuda.current_device()}" if like is None else f", not on {like.device}"))
+    if t.dtype != dtype or t.ndim != len(shape) or any(want is not None and want != got for want, got in zip(shape, t.shape)):
+        raise ValueError(f"{name}: {dtype} {tuple('any' if x is None else x for x in shape)} is needed, not {t.dtype} {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: must be contiguous")
+    return t.data_ptr()
+
+
+def topk_adjusted(logits: torch.Tensor, count: int, scratch: torch.Tensor, ids: torch.Tensor, vals: torch.Tensor, row_slot: "torch.Tensor | None" = None, *,
+                  counts=None, penalties=None, bias=None, mask=None, window=None) -> None:
+    """`topk` of the logits under sampling rules, in one pass over them: ids int32 / vals f32 [rows, count], value descending, then id ascending.
+    logits: f32 [rows, vocab], rows may be further apart than vocab.  row_slot (int32 [rows]): the slot whose rules row r is under; a value outside the slots
+    (-1): no penalties, no biases.  Each step rounds to f32:
+    counts (int16 [slots, vocab], see `token_counts`) with penalties (f32 [slots, 3]: repetition > 0, frequency, presence): an id that the prompt holds or
+    that was generated is divided by repetition (multiplied where it is <= 0); then frequency * (times generated) and, where that is not 0, presence go off.
+    window = (first, fed), int32 [rows] each: rows first[r] .. r feed the tokens fed of a verify window; those after first[r] count as generated for row r.
+    bias = (ids int32 [slots, n], values f32 [slots, n]), n up to 1024: added; an id outside the vocabulary (-1) is an unused place, equal ids add up in order.
+    mask = (bits int32 [n, ceil(vocab / 32)], row int32 [rows]): row r may take the ids whose bit of bits[row[r]] is set (id i: bit i % 32 of word i // 32), every
+    id where row[r] is outside 0 .. n - 1.  What is masked stands at -inf, whatever its logit.  Where a row has fewer than count ids above -inf, the rest are
+    its lowest other ids at -inf.  A NaN that is not masked is above everything.  scratch: `topk_scratch`; calls that may overlap need one each."""
+    if not isinstance(logits, torch.Tensor) or logits.ndim != 2 or logits.dtype != torch.float32 or not logits.is_cuda:
+        raise ValueError("logits: a CUDA float32 [rows, vocab] tensor is needed")
+    rows, vocab = logits.shape
+    if logits.device.index != torch.cuda.current_device():
+        raise ValueError(f"logits is on {logits.device}, not on the current device cuda:{torch.cuda.current_device()}")
+    if rows > 1 and (logits.stride(0) < vocab) or vocab > 1 and logits.stride(1) != 1:
+        raise ValueError("logits: a row's values must stand side by side, and rows must not overlap")
+    if not 1 <= count <= min(64, vocab) or (vocab + 4095) // 4096 * count > 4096:
+        raise ValueError(f"count {count}: 1 .. 64, no more than the vocabulary of {vocab}, and ceil(vocab / 4096) * count <= 4096")
+    if rows > 65535:
+        raise ValueError(f"{rows} rows: at most 65535")
+    p_ids, p_vals = _operand(ids, "ids", torch.int32, (rows, count), logits), _operand(vals, "vals", torch.float32, (rows, count), logits)
+    if rows == 0:
+        return
+    if not scratch.is_cuda or scratch.device != logits.device or not scratch.is_contiguous() or \
+            scratch.numel() * scratch.element_size() < _lib.load().rx_topk_scratch_bytes(rows, vocab, count):
+        raise ValueError("scratch: too small (see topk_scratch), not contiguous or on another device")
+    if (counts is None) != (penalties is None):
+        raise ValueError("counts and penalties go together")
+    if row_slot is None and (counts is not None or bias is not None):
+        raise ValueError("penalties and biases need row_slot")
+    p_slot = None if row_slot is None else _operand(row_slot, "row_slot", torch.int32, (rows,), logits)
+    slots, p_counts, p_pen, p_bid, p_bval, nb, p_mask, p_mrow, nm, p_first, p_fed = 0, None, None, None, None, 0, None, None, 0, None, None
+    if counts is not None:
+        p_counts = _operand(counts, "counts", torch.int16, (None, vocab), logits)
+        slots = counts.shape[0]
+        p_pen = _operand(penalties, "penalties", torch.float32, (slots, 3), logits)
+    if bias is not None:
+        n_slots = slots if counts is not None else None
+        p_bid = _operand(bias[0], "bias ids", torch.int32, (n_slots, None), logits)
+        slots, nb = bias[0].shape
+        p_bval = _operand(bias[1], "bias values", torch.float32, (slots, nb), logits)
+        if nb > 1024:
+            raise ValueError(f"{nb} biases a slot: at most 1024")
+    if mask is not None:
+        p_mask, p_mrow = _operand(mask[0], "mask bits", torch.int32, (None, (vocab + 31) // 32), logits), _operand(mask[1], "mask row", torch.int32, (rows,), logits)
+        nm = mask[0].shape[0]
+    if window is not None:
+        p_first, p_fed = (_operand(t, n, torch.int32, (rows,), logits) for t, n in zip(window, ("window first", "window fed")))
+    _lib.check(_lib.load().rx_topk_adjusted(logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab, count, scratch.data_ptr(),
+                                            p_ids, p_vals, p_slot, p_counts, p_pen, slots, p_bid, p_bval, nb, p_mask, p_mrow, nm, p_first, p_fed, _lib.stream_ptr()),
+               "rx_topk_adjusted")
+    _lib.count(2)
+
+
+def token_counts(counts: torch.Tensor, slots: torch.Tensor, starts: torch.Tensor, prompt_len: torch.Tensor, tokens: torch.Tensor, status: torch.Tensor) -> None:
+    """Rebuilds the token counts of some slots from their histories (a request is admitted or resumed).  counts: int16 [n_slots, vocab], bit 15 = the prompt holds
+    the id, bits 0 .. 14 = times generated, up to 32767.  Request i's history is tokens[starts[i]:starts[i + 1]], its first prompt_len[i] tokens the prompt; row
+    slots[i] of counts is written whole, the others stay.  int32 tensors; starts has one more entry than slots.  A token outside the vocabulary is left out, a slot
+    outside the table, a slot's second request and a range outside `tokens` are passed over; each sets the status."""
+    p_counts = _operand(counts, "counts", torch.int16, (None, None))
+    n = slots.numel()
+    p = [_operand(t, name, torch.int32, shape, counts) for t, name, shape in ((slots, "slots", (n,)), (starts, "starts", (n + 1,)), (prompt_len, "prompt_len", (n,)),
+                                                                             (tokens, "tokens", (None,)), (status, "status", (STATUS_WORDS,)))]
+    if n > 65535:
+        raise ValueError(f"{n} requests: at most 65535")
+    if n == 0 or counts.numel() == 0:
+        return
+    _lib.check(_lib.load().rx_token_counts(p_counts, counts.shape[0], counts.shape[1], p[0], p[1], p[2], p[3], tokens.numel(), n, p[4], _lib.stream_ptr()), "rx_token_counts")
+    _lib.count()
+
+
+def token_counts_add(counts: torch.Tensor, slots: torch.Tensor, tokens: torch.Tensor, status: torch.Tensor, prompt: bool = False) -> None:
+    """counts[slots[i], tokens[i]] takes one more generated token (`prompt`: the prompt bit), for the tokens that a step committed; a pair may stand more than
+    once.  int32 [n] each.  A slot or token outside the table is left out and sets the status."""
+    p_counts = _operand(counts, "counts", torch.int16, (None, None))
+    n = slots.numel()
+    p = [_operand(t, name, torch.int32, shape, counts) for t, name, shape in ((slots, "slots", (n,)), (tokens, "tokens", (n,)), (status, "status", (STATUS_WORDS,)))]
+    if n == 0 or counts.numel() == 0:
+        return
+    _lib.check(_lib.load().rx_token_counts_add(p_counts, counts.shape[0], counts.shape[1], p[0], p[1], n, 1 if prompt else 0, p[2], _lib.stream_ptr()),
+               "rx_token_counts_add")
+    _lib.count()
+
+
+def window_rows(seq: torch.Tensor, have: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor, rows: torch.Tensor, starts: torch.Tensor, status: torch.Tensor, *,
+                free=None, free_at=None, free_next=None) -> None:
+    """Row maps of a window or a prompt slice, and the pages that it begins, from the requests' lengths, on the device.  Request i (up to 1024) holds have[i] cached
+    tokens in table row seq[i] and feeds new[i] >= 0 more; its rows begin at starts[i] (int32 [n + 1], the last entry is the total).  rows: int32 [5, cap],
+    written up to the total, the rest stays: position | KV slot | table row | keys seen (position + 1) | leading pages that the request's table has in
+    common with the request before it that has rows (among pages with cached tokens of both; see `attn_shared`).
+    free (int32 [m]) with free_at, free_next (int32 [1] each): page ids free[free_at:], in request order, become the table entries of the pages that
+    the new tokens begin, and free_next = free_at + their number (it may be the same tensor as free_at).  Without them the table holds those pages already.
+    All or nothing: a length below 0, tokens beyond the table, more rows than cap, more pages than there are, a table row outside the table or
+    given twice sets the status and changes nothing else.  A table entry below 0 where a row is to be written gives slot -1 (the row is not cached) and sets the status."""
+    n, cap = seq.numel(), rows.shape[-1] if isinstance(rows, torch.Tensor) and rows.ndim else 0
+    p_table = _operand(block_table, "block_table", torch.int32, (None, None))
+    tables, width = block_table.shape
+    p = [_operand(t, name, torch.int32, shape, block_table) for t, name, shape in (
+        (seq, "seq", (n,)), (have, "have", (n,)), (new, "new", (n,)), (rows, "rows", (5, None)), (starts, "starts", (n + 1,)), (status, "status", (STATUS_WORDS,)))]
+    if not 1 <= n <= _lib.load().rx_window_rows_max():
+        raise ValueError(f"{n} requests: 1 .. {_lib.load().rx_window_rows_max()}")
+    if not 1 <= tables <= 32768 or not 1 <= width <= 1 << 24 or cap > 1 << 20:
+        raise ValueError("block_table: 1 .. 32768 rows of 1 .. 2^24 pages; rows: at most 2^20")
+    if (free is None) != (free_at is None) or (free is None) != (free_next is None):
+        raise ValueError("free, free_at and free_next go together")
+    f = [None, None, None]
+    if free is not None:
+        f = [_operand(t, name, torch.int32, shape, block_table) for t, name, shape in ((free, "free", (None,)), (free_at, "free_at", (1,)), (free_next, "free_next", (1,)))]
+    _lib.check(_lib.load().rx_window_rows(p[0], p[1], p[2], n, p_table, tables, width, f[0], 0 if free is None else free.numel(), f[1], f[2], p[3], cap, p[4], p[5],
+                                          _lib.stream_ptr()), "rx_window_rows")
+    _lib.count()
+
+
 class KvTensorMap:
     """Host-side TMA descriptors of one layer's K or V cache (bf16 or bytes [pages, n_kv, 64, hd]): `ptr` for decode attention, `rows_ptr` for prefill
     (they differ for E4M3 bytes, whose decode kernel takes its pages swizzled)."""

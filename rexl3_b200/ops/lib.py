@@ -132,6 +132,12 @@ def _declare(lib):
         "rx_hc_apply": (c_int, [c_void, c_void, c_void, c_int, c_int, c_void]),
         "rx_topk_scratch_bytes": (c_ll, [c_int, c_int, c_int]),
         "rx_topk": (c_int, [c_void, c_int, c_int, c_int, c_void, c_void, c_void, c_void]),
+        "rx_topk_adjusted": (c_int, [c_void, c_ll, c_int, c_int, c_int, c_void, c_void, c_void, c_void, c_void, c_void, c_int, c_void, c_void, c_int, c_void,
+                                     c_void, c_int, c_void, c_void, c_void]),
+        "rx_token_counts": (c_int, [c_void, c_int, c_int, c_void, c_void, c_void, c_void, c_int, c_int, c_void, c_void]),
+        "rx_token_counts_add": (c_int, [c_void, c_int, c_int, c_void, c_void, c_int, c_int, c_void, c_void]),
+        "rx_window_rows_max": (c_int, []),
+        "rx_window_rows": (c_int, [c_void, c_void, c_void, c_int, c_void, c_int, c_int, c_void, c_int, c_void, c_void, c_void, c_int, c_void, c_void, c_void]),
         "rx_make_kv_tmap": (c_int, [c_void, c_void, c_ll, c_int]),
         "rx_make_kv_tmap8": (c_int, [c_void, c_void, c_ll, c_int]),
         "rx_make_kv_tmap_f8": (c_int, [c_void, c_void, c_ll, c_int]),
