@@ -581,6 +581,73 @@ def attn_decode(tk: KvTensorMap, tv: KvTensorMap, q, block_table, row_seq, ctx_l
     _lib.count(2 if plan is not None else 3)
 
 
+def attn_shared_scratch(rows: int, n_q: int, n_kv: int, hd: int, device="cuda") -> torch.Tensor:
+    """Workspace of `attn_shared` for windows of up to `rows` rows; calls that may overlap need one each."""
+    n = _lib.load().rx_attn_shared_scratch_floats(rows, n_q, n_kv, hd)
+    if n <= 0:
+        raise ValueError(f"{rows} rows of {n_q} query and {n_kv} KV heads: n_kv must divide n_q, and at most 128 query heads share a KV head")
+    return torch.empty(n, dtype=torch.float32, device=device)
+
+
+def attn_shared_plan_buffer(device="cuda") -> torch.Tensor:
+    return torch.zeros(_lib.load().rx_attn_shared_plan_ints(), dtype=torch.int32, device=device)
+
+
+def _shared_window(block_table, row_seq, ctx_len, common, status, n_q: int, n_kv: int):
+    p_table = _operand(block_table, "block_table", torch.int32, (None, None))
+    rows = row_seq.numel()
+    p = [p_table] + [_operand(t, name, torch.int32, shape, block_table) for t, name, shape in (
+        (row_seq, "row_seq", (rows,)), (ctx_len, "ctx_len", (rows,)), (common, "common", (rows,)), (status, "status", (STATUS_WORDS,)))]
+    if not 1 <= rows <= 1024 or n_kv < 1 or n_q % n_kv or not 1 <= n_q // n_kv <= 128:
+        raise ValueError(f"{rows} rows of {n_q} query and {n_kv} KV heads: 1 .. 1024 rows, n_kv divides n_q, at most 128 query heads share a KV head")
+    if block_table.numel() == 0 or rows * block_table.shape[1] * n_kv >= 1 << 29:
+        raise ValueError("block_table: empty, or rows * pages a sequence * n_kv reaches 2^29")
+    return rows, p
+
+
+def attn_shared_plan(block_table, row_seq, ctx_len, common, n_q: int, n_kv: int, plan: torch.Tensor, status: torch.Tensor) -> None:
+    """The work plan of `attn_shared` for one window: a function of these tensors' values (of block_table only its extents), so one plan serves every layer."""
+    rows, p = _shared_window(block_table, row_seq, ctx_len, common, status, n_q, n_kv)
+    L = _lib.load()
+    p_plan = _operand(plan, "plan", torch.int32, (L.rx_attn_shared_plan_ints(),), block_table)
+    _lib.check(L.rx_attn_shared_plan(p[1], p[2], p[3], rows, block_table.shape[0], block_table.shape[1], n_q, n_kv, p_plan, p[4], _lib.stream_ptr()), "rx_attn_shared_plan")
+    _lib.count()
+
+
+def attn_shared(tk: KvTensorMap, tv: KvTensorMap, q, block_table, row_seq, ctx_len, common, scratch, n_q: int, n_kv: int, hd: int, scale: float, out, status, *,
+                suh=None, xr=None, kv_scale=None, plan=None) -> None:
+    """Decode / verify-window attention that reads the pages neighbouring sequences have in common once for all of them (`attn_decode` reads them once per
+    sequence).  q bf16 [rows, n_q * hd]; row r sees the first ctx_len[r] keys of table row row_seq[r] (0: its output is 0); the rows of a sequence are
+    adjacent.  common (int32 [rows], read at the first row of each sequence): how many leading page ids of its table row are also those of the sequence before
+    it; sequences whose pages agree should stand side by side, and 0 is always right.  `window_rows` writes all three.
+    out bf16 [rows, n_q * hd] or None; with suh also xr fp16, `attn_decode`'s rotated output.  bf16 caches, or E4M3 ones with kv_scale (f32 [2, n_kv]); heads of
+    64 or 128; n_q * hd a multiple of 128.  A row's last bits depend on the rows beside it: the cut of the work follows the whole window.
+    A table row or a context outside the table sets the status and stands for a context of 0.
+    `plan`: from `attn_shared_plan` for this window (one serves every layer); None: the call plans for itself."""
+    rows, p = _shared_window(block_table, row_seq, ctx_len, common, status, n_q, n_kv)
+    if hd not in (64, 128) or n_q * hd % 128:
+        raise ValueError(f"heads of {hd}: 64 or 128, and n_q * hd a multiple of 128")
+    for t, name in ((tk, "K"), (tv, "V")):
+        if t.i8 or t.fp8 != (kv_scale is not None) or tuple(t._keep.shape[1:]) != (n_kv, 64, hd) or t._keep.device != block_table.device:
+            raise ValueError(f"{name} cache: bf16, or E4M3 bytes with kv_scale, [pages, {n_kv}, 64, {hd}] on {block_table.device} is needed")
+    if out is None and xr is None or (suh is None) != (xr is None):
+        raise ValueError("out, or suh with xr, or both are needed")
+    L, width = _lib.load(), n_q * hd
+    p_q = _operand(q, "q", torch.bfloat16, (rows, width), block_table)
+    p_out = None if out is None else _operand(out, "out", torch.bfloat16, (rows, width), block_table)
+    p_suh, p_xr = (None, None) if xr is None else (_operand(suh, "suh", torch.float16, (width,), block_table), _operand(xr, "xr", torch.float16, (rows, width), block_table))
+    p_scale = None if kv_scale is None else _operand(kv_scale, "kv_scale", torch.float32, (2, n_kv), block_table)
+    p_plan = None if plan is None else _operand(plan, "plan", torch.int32, (L.rx_attn_shared_plan_ints(),), block_table)
+    p_scratch = _operand(scratch, "scratch", torch.float32, (None,), block_table)
+    if scratch.numel() < L.rx_attn_shared_scratch_floats(rows, n_q, n_kv, hd):
+        raise ValueError("scratch: too small (see attn_shared_scratch)")
+    if (p_q | p_scratch | (p_plan or 0)) & 15 or ((p_out or 0) | (p_xr or 0)) & 7:
+        raise ValueError("q, scratch and plan begin on 16-byte boundaries, out and xr on 8-byte ones")
+    _lib.check(L.rx_attn_shared(tk.rows_ptr, tv.rows_ptr, p_q, p[0], block_table.shape[0], block_table.shape[1], p[1], p[2], p[3], p_scratch, rows, n_q, n_kv, hd, scale,
+                                p_scale, p_suh, p_xr, p_out, p_plan, p[4], _lib.stream_ptr()), "rx_attn_shared")
+    _lib.count(2 if plan is not None else 3)
+
+
 def kv_move_rows(tensor_ptrs, row_bytes: int, n_kv: int, moves, n_moves: int) -> None:
     """Copies runs of cache rows, moves[i] = (source slot, destination slot, rows), in every cache whose base address is in `tensor_ptrs`
     (int64 device tensor); caches are [pages, n_kv, 64, row_bytes]; a run stays inside one page; no destination row is a source or a

@@ -138,6 +138,11 @@ def _declare(lib):
         "rx_token_counts_add": (c_int, [c_void, c_int, c_int, c_void, c_void, c_int, c_int, c_void, c_void]),
         "rx_window_rows_max": (c_int, []),
         "rx_window_rows": (c_int, [c_void, c_void, c_void, c_int, c_void, c_int, c_int, c_void, c_int, c_void, c_void, c_void, c_int, c_void, c_void, c_void]),
+        "rx_attn_shared_plan_ints": (c_int, []),
+        "rx_attn_shared_scratch_floats": (c_ll, [c_int, c_int, c_int, c_int]),
+        "rx_attn_shared_plan": (c_int, [c_void, c_void, c_void, c_int, c_int, c_int, c_int, c_int, c_void, c_void, c_void]),
+        "rx_attn_shared": (c_int, [c_void, c_void, c_void, c_void, c_int, c_int, c_void, c_void, c_void, c_void, c_int, c_int, c_int, c_int, c_f, c_void, c_void,
+                                   c_void, c_void, c_void, c_void, c_void]),
         "rx_make_kv_tmap": (c_int, [c_void, c_void, c_ll, c_int]),
         "rx_make_kv_tmap8": (c_int, [c_void, c_void, c_ll, c_int]),
         "rx_make_kv_tmap_f8": (c_int, [c_void, c_void, c_ll, c_int]),
