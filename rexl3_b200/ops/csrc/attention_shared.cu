@@ -9,10 +9,17 @@
 // read its 33.5 MB per layer once instead of 64 times.
 //
 // All pages of all (block, KV head) units stand in one line, cut into equal pieces, one for each of 296 CTAs (two per SM): a CTA's piece may end in
-// one unit and begin in another.  Each (unit, CTA) leaves partial outputs in fp32 with their maxima and sums, and a merge kernel joins a row's in a fixed order.
-// Where the pieces end depends on the whole window, and with it the order of a row's sum: unlike attn_decode's, a row's last bits depend on its window mates.
+// one unit and begin in another.  Each (unit, CTA) segment leaves partial outputs in fp32 with their maxima and sums, and a merge kernel joins a row's in a
+// fixed order.  Where the pieces end depends on the whole window, and with it the order of a row's sum: unlike attn_decode's, a row's last bits depend on
+// its window mates.
 //
-// Warps: 0 = TMA producer, 1 = MMA issuer (owns the tensor memory), 2..5 = softmax, for E4M3 caches 6..7 = expansion of byte pages to fp16 operand tiles.
+// A page's 64 scores a pair go to tensor memory, come back as exponentials in 16 bits over the same columns, and are the A operand of the product with V.
+// The QKs run two pages ahead of the PVs, also into the next segment.
+//
+// Warps: 0..3 = softmax, 4 = feeder (queries and descriptions of the segments; TMA), 5 = MMA issuer (owns the tensor memory), for E4M3 caches 6, 7 = expansion
+// of byte pages of K and of V to fp16 operand tiles, in place of TMA.
+// A block of up to 64 or 32 pairs would leave two or three quarters idle and the others bound by one warp's exponentials: its queries
+// stand in the tensor memory two or four times, each copy takes its part of a page's keys - the rest of its P is zero - and leaves its own partial output.
 // All waits are bounded (status words), no cluster multicast.
 #include <cuda.h>
 #include <cuda_fp8.h>
@@ -23,15 +30,16 @@ namespace rx {
 
 constexpr int SH_PAGE = 64, SH_PAIRS = 128, SH_CTAS = 296, SH_MAX_ROWS = 1024;
 constexpr int SH_MIN_SHARED = 1;                        // pages that a group must have in common
+constexpr int SH_SEGMENT = 2;                           // what a unit costs beside its pages, in pages: its place in the line is that much longer
 
 // ------------------------------------------------------------------------------------------------ plan
-// Layout (int32): [0] pages of all units  [1] pages per CTA  [2] blocks  [3] n_kv, then the block at which each CTA begins, the blocks, and per row its
+// Layout (int32): [0] length of the line  [1] a CTA's piece  [2] blocks  [3] n_kv, then the block at which each CTA begins, the blocks, and per row its
 // block over common pages, its block over own pages (-1: none), the keys it sees and nothing.
 struct ShBlock {
   int row, rows;          // first row, rows
   int seq;                // table row
   int page, pages;        // first page, pages
-  int before;             // pages of the blocks before (times n_kv: where the block's units begin in the line)
+  int before;             // length of the blocks before (times n_kv: where the block's units begin in the line)
   int part;               // partial vectors (times n_q) of the blocks before
   int most;               // keys that some row of the block's group sees: what stands behind them is never multiplied
 };
@@ -41,6 +49,9 @@ constexpr int SH_AT_ROWS = SH_AT_BLOCKS + 2 * SH_MAX_ROWS * 8;
 constexpr int SH_PLAN_INTS = SH_AT_ROWS + 4 * SH_MAX_ROWS + 4;      // (with room to align it)
 
 __device__ __forceinline__ int sh_slots(int pages, int L) { return (pages + L - 1) / L + 1; }      // CTAs that a unit of `pages` pages can meet
+__device__ __forceinline__ int sh_copies(int pairs) { return pairs <= 32 ? 4 : pairs <= 64 ? 2 : 1; }
+// where the pages of a unit begin in the line
+__device__ __forceinline__ int sh_unit(const ShBlock& b, int kvh, int n_kv) { return b.before * n_kv + kvh * (b.pages + SH_SEGMENT) + SH_SEGMENT; }
 
 // inclusive sum over the block's threads; `all` gets the total
 __device__ __forceinline__ int block_scan(int v, int* s_warp, int& all) {
@@ -69,12 +80,12 @@ __device__ __forceinline__ int block_scan(int v, int* s_warp, int& all) {
 // before it) is at least SH_MIN_SHARED pages and at least half of each neighbouring link: a group shares its smallest link, and one pair of
 // strangers with nothing but a first page in common must not take a long prompt away from the pairs on both sides.
 __global__ void __launch_bounds__(SH_MAX_ROWS) shared_plan_kernel(const int* __restrict__ row_seq, const int* __restrict__ ctx_len, const int* __restrict__ common,
-                                                                  int rows, int n_tables, int width, int rt, int n_kv, int* __restrict__ plan, int* status) {
+                                                                  int rows, int n_tables, int width, int G, int n_kv, int* __restrict__ plan, int* status) {
   pdl_launch();
   __shared__ int s_seq[SH_MAX_ROWS], s_first[SH_MAX_ROWS + 1], s_link[SH_MAX_ROWS + 1], s_group[SH_MAX_ROWS], s_shared[SH_MAX_ROWS], s_gfirst[SH_MAX_ROWS + 1],
       s_gmost[SH_MAX_ROWS], s_most[SH_MAX_ROWS], s_before[2 * SH_MAX_ROWS], s_warp[32];
   pdl_wait();
-  const int r = threadIdx.x;
+  const int r = threadIdx.x, rt = SH_PAIRS / G;
   const bool live = r < rows;
   int seq = live ? row_seq[r] : -1, ctx = live ? ctx_len[r] : 0;
   const int link = live ? min(max(common[r], 0), width) : 0;
@@ -114,26 +125,28 @@ __global__ void __launch_bounds__(SH_MAX_ROWS) shared_plan_kernel(const int* __r
   const bool lead_s = live && shared > 0 && r == tile, lead_o = live && own > 0 && r == chunk;
   int pages_s, pages_o, blocks;
   const int b_in = block_scan((lead_s ? 1 : 0) | (lead_o ? 1 << 16 : 0), s_warp, blocks);
-  const int p_s = block_scan(lead_s ? shared : 0, s_warp, pages_s), p_o = block_scan(lead_o ? own : 0, s_warp, pages_o);
+  const int len_s = shared + SH_SEGMENT, len_o = own + SH_SEGMENT;
+  const int p_s = block_scan(lead_s ? len_s : 0, s_warp, pages_s), p_o = block_scan(lead_o ? len_o : 0, s_warp, pages_o);
   const int nb_s = blocks & 0xFFFF, nb = nb_s + (blocks >> 16);
   const int total = (pages_s + pages_o) * n_kv, L = max((total + SH_CTAS - 1) / SH_CTAS, 1);
   const int n_s = live ? min(rt, s_gfirst[group + 1] - tile) : 0, n_o = live ? min(rt, s_first[run + 1] - chunk) : 0;
-  const int v_s = block_scan(lead_s ? n_s * sh_slots(shared, L) : 0, s_warp, all);
+  const int k_s = n_s * sh_slots(shared, L) * sh_copies(n_s * G), k_o = n_o * sh_slots(own, L) * sh_copies(n_o * G);
+  const int v_s = block_scan(lead_s ? k_s : 0, s_warp, all);
   const int all_s = all;
-  const int v_o = block_scan(lead_o ? n_o * sh_slots(own, L) : 0, s_warp, all);
+  const int v_o = block_scan(lead_o ? k_o : 0, s_warp, all);
   ShBlock* blk = reinterpret_cast<ShBlock*>(plan + SH_AT_BLOCKS);
   // (s_seq and s_link are free: the ids of the blocks that begin at a row)
   __syncthreads();
   if (lead_s) {
     const int id = (b_in & 0xFFFF) - 1;
-    s_link[r] = id, s_before[id] = p_s - shared;
-    blk[id] = ShBlock{r, n_s, s_seq[gfirst], 0, shared, p_s - shared, v_s - n_s * sh_slots(shared, L), s_gmost[group]};
+    s_link[r] = id, s_before[id] = p_s - len_s;
+    blk[id] = ShBlock{r, n_s, s_seq[gfirst], 0, shared, p_s - len_s, v_s - k_s, s_gmost[group]};
   }
   __syncthreads();
   if (lead_o) {
     const int id = nb_s + (b_in >> 16) - 1;
-    s_seq[r] = id, s_before[id] = pages_s + p_o - own;
-    blk[id] = ShBlock{r, n_o, seq, shared, own, pages_s + p_o - own, all_s + v_o - n_o * sh_slots(own, L), s_most[chunk]};
+    s_seq[r] = id, s_before[id] = pages_s + p_o - len_o;
+    blk[id] = ShBlock{r, n_o, seq, shared, own, pages_s + p_o - len_o, all_s + v_o - k_o, s_most[chunk]};
   }
   __syncthreads();
   if (live) {
@@ -151,17 +164,6 @@ __global__ void __launch_bounds__(SH_MAX_ROWS) shared_plan_kernel(const int* __r
 }
 
 // ------------------------------------------------------------------------------------------------ attention
-__device__ __forceinline__ void sh_ld_x32(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
-      "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
-        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
-        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
-        "=r"(r[31])
-      : "r"(taddr)
-      : "memory");
-}
 __device__ __forceinline__ float sh_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -178,39 +180,67 @@ __device__ __forceinline__ uint32_t sh_pack(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&v);
   }
 }
-// V page as the B operand: keys x head_dim with the head dimension contiguous (MN-major, 128-byte swizzle; see attention_tc.cu)
-__device__ __forceinline__ uint64_t sh_desc_v(uint32_t smem_addr) {
-  return (uint64_t)((smem_addr & 0x3FFFF) >> 4) | (uint64_t)(8192 >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+// V as the B operand: keys x head_dim with the head dimension contiguous (MN-major, 128-byte swizzle; see attention_tc.cu)
+__device__ __forceinline__ uint64_t sh_desc_v(uint32_t smem_addr, uint32_t box) {
+  return (uint64_t)((smem_addr & 0x3FFFF) >> 4) | (uint64_t)(box >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+// mbar_wait reads the clock and the host's limit before it polls again: some 1000 cycles, of 2100 that a page took where every wait of its chain
+// (scores, softmax, products) was met a little early.  Here that begins after polls that a page's work never outlasts.
+__device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool sh_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int site) {
+#pragma unroll 1
+  for (int i = 0; i < 64; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(4000)          // asleep for up to 4 us
+        : "memory");
+    if (ok) return true;
+  }
+  return mbar_wait(bar, parity, abort_flag, status, site);
 }
 
 struct ShArgs {
-  const uint16_t* q;
   const int* block_table;
   const int* plan;
   const float* kv_scale;
+  const uint8_t *k8, *v8;              // E4M3 caches, and their pages
   float* part_o;
   float* part_ml;
   int* status;
-  int max_blocks, n_q, n_kv;
+  int max_blocks, n_q, n_kv, n_pages;
   float scale_log2;
 };
 
 template <int HD, bool F8>
 struct Sh {
-  static constexpr int TILE = SH_PAGE * HD * 2, RAW = SH_PAGE * HD, QBOX = SH_PAIRS * 128;
-  static constexpr int KS = F8 ? 1 : 2, VS = F8 ? 1 : 2, RS = 2;            // stages of K, of V, of byte pages
-  static constexpr int OPERANDS = (KS + VS) * TILE, RAWS = F8 ? 2 * RS * RAW : 0, Q = HD / 64 * QBOX;
-  static constexpr int SMEM = OPERANDS + RAWS + Q + 256 + 1024;
-  static constexpr int THREADS = F8 ? 256 : 192;
-  static constexpr int S_COLS = 64, O = 128;                                // tensor memory: two S buffers of 64 columns | O
-  static constexpr int COLS = 256;
+  static constexpr int TILE = SH_PAGE * HD * 2, QBOX = SH_PAIRS * 128;      // a page of K or V as an operand; 64 values of all pairs
+  static constexpr int KS = 3, VS = 2;                                      // stages of K, of V
+  static constexpr int SMEM = (KS + VS) * TILE + HD / 64 * QBOX + 512;      // two CTAs an SM: 115,712 bytes at most
+  static_assert(SMEM <= 115712, "two CTAs an SM");
+  static constexpr int THREADS = 32 * (F8 ? 8 : 6);
+  static constexpr int S_COLS = 64, O = 128, COLS = 256;                    // tensor memory: two buffers of S (P over the first 32 columns of one) | O
 };
 
 // a wait's outcome for the whole warp: what follows it is done by all lanes or by none
 __device__ __forceinline__ bool all_ok(bool ok) { return __all_sync(0xffffffffu, ok); }
 
 struct ShSegment { ShBlock b; int kvh, page, pages, slot, slots; };          // a CTA's pages of one unit
-// The CTA's piece of the line as segments; every role walks it by itself.
+// The CTA's piece of the line as segments.
 struct ShWalk {
   const ShBlock* blk;
   int b, pos, end, L, n_kv;
@@ -222,65 +252,136 @@ struct ShWalk {
     b = plan[SH_HEAD + blockIdx.x];
   }
   __device__ __forceinline__ bool next(ShSegment& s) {
-    if (pos >= end) return false;
-    const int4* p = reinterpret_cast<const int4*>(blk + b);
-    int4 x = p[0], y = p[1];
-    int rel = pos - y.y * n_kv;
-    if (rel >= y.x * n_kv) {                                                // the block is done
-      p = reinterpret_cast<const int4*>(blk + ++b);
-      x = p[0], y = p[1];
-      rel = pos - y.y * n_kv;
+    while (pos < end) {
+      const int4* p = reinterpret_cast<const int4*>(blk + b);
+      int4 x = p[0], y = p[1];
+      int rel = pos - y.y * n_kv;
+      if (rel >= (y.x + SH_SEGMENT) * n_kv) {                               // the block is done
+        p = reinterpret_cast<const int4*>(blk + ++b);
+        x = p[0], y = p[1];
+        rel = pos - y.y * n_kv;
+      }
+      s.b = ShBlock{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+      s.kvh = rel / (s.b.pages + SH_SEGMENT);
+      const int unit = sh_unit(s.b, s.kvh, n_kv), stop = min(end, unit + s.b.pages);
+      pos = max(pos, unit);
+      s.page = pos - unit, s.pages = stop - pos;
+      s.slot = (int)blockIdx.x - unit / L, s.slots = sh_slots(s.b.pages, L);
+      pos = max(pos, stop);
+      if (s.pages > 0) return true;                                         // (else the piece ended before the unit's first page)
     }
-    s.b = ShBlock{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-    s.kvh = rel / s.b.pages, s.page = rel - s.kvh * s.b.pages;
-    s.pages = min(end - pos, s.b.pages - s.page);
-    const int unit = s.b.before * n_kv + s.kvh * s.b.pages;
-    s.slot = (int)blockIdx.x - unit / L, s.slots = sh_slots(s.b.pages, L);
-    pos += s.pages;
-    return true;
+    return false;
   }
 };
 
+// What the warps know of a segment; the four last are in shared memory.  pages == 0: there are no more.
+struct ShDesc {
+  int row, rows, kvh, key0, pages, part, stride, most;
+  const int* table;       // its page ids
+  long long pad;
+};
+
+// N columns of the thread's lane, once they are there (load and wait in one statement: no copy of a register comes between them)
+template <int N>
+__device__ __forceinline__ void sh_ld(uint32_t taddr, uint32_t (&r)[N]) {
+  static_assert(N == 64 || N == 32 || N == 16, "16, 32 or 64 columns");
+  if constexpr (N == 64)
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
+                 "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, "
+                 "%46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+                   "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
+                   "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]),
+                   "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]),
+                   "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+                   "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+                 : "r"(taddr)
+                 : "memory");
+  else if constexpr (N == 32)
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
+                 "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+                   "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
+                   "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr)
+                 : "memory");
+  else if constexpr (N == 16)
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+                 "[%16];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+                   "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr)
+                 : "memory");
+}
+template <int N>
+__device__ __forceinline__ void sh_st(uint32_t taddr, const uint32_t (&r)[N]) {
+  static_assert(N == 32 || N == 16 || N == 8, "8, 16 or 32 columns");
+  if constexpr (N == 32) tc_st_32x32b_x32(taddr, r);
+  else if constexpr (N == 16) tc_st_32x32b_x16(taddr, r);
+  else if constexpr (N == 8)
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
+                 "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+template <int N>
+__device__ __forceinline__ void sh_st_zero(uint32_t taddr) {
+  const uint32_t z[N] = {};
+  sh_st(taddr, z);
+}
+
+// One row's query heads of a KV head: 64 of their values each, from [rows][n_q][hd]
+__device__ __forceinline__ void sh_load_q(void* dst, const void* tmap, int x, int head, int row, uint64_t* bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)), "l"(tmap),
+               "r"(smem_u32(bar)), "r"(x), "r"(head), "r"(row)
+               : "memory");
+}
+
 template <int HD, bool F8>
 __global__ void __launch_bounds__((Sh<HD, F8>::THREADS), 2)
-attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const __grid_constant__ ShArgs a) {
+attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tq, const __grid_constant__ ShArgs a) {
   using C = Sh<HD, F8>;
-  constexpr int TILE = C::TILE, BOXES = HD / 64;
+  constexpr int BOXES = HD / 64, TILE = C::TILE, KS = C::KS, VS = C::VS;
   pdl_launch();
-  extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if ((smem_u32(smem) & 1023) != 0) {                     // (a kernel without static shared memory begins on a 1024-byte boundary)
+    if (threadIdx.x == 0) set_status(a.status, ST_BAD_ARG, 109);
+    return;
+  }
   uint8_t* k_sm = smem;                                   // [stage][box (64 d)][64 keys][128 B]
-  uint8_t* v_sm = smem + C::KS * TILE;
-  uint8_t* q_sm = smem + C::OPERANDS;                     // [box][128 pairs][128 B]
-  uint8_t* raw = q_sm + C::Q;                             // [stage][K, V][64 keys][HD]
-  uint64_t* bars = (uint64_t*)(raw + C::RAWS);
-  uint64_t* k_full = bars;                                // [KS] the copy, or both expanding warps
-  uint64_t* v_full = k_full + 2;
-  uint64_t* k_empty = v_full + 2;                         // commit after QK
-  uint64_t* v_empty = k_empty + 2;                        // commit after PV
-  uint64_t* s_full = v_empty + 2;                         // [2] commit after QK
-  uint64_t* p_ready = s_full + 2;                         // [2] the 4 softmax warps
-  uint64_t* pv_done = p_ready + 2;                        // [1] commit after PV
-  uint64_t* q_ready = pv_done + 1;                        // [1] the 4 softmax warps, once per segment
-  uint64_t* drained = q_ready + 1;
-  uint64_t* raw_full = drained + 1;                       // [RS]
-  uint64_t* raw_empty = raw_full + 2;                     // [RS] both expanding warps
-  uint32_t* tmem_slot = (uint32_t*)(raw_empty + 2);
+  uint8_t* v_sm = smem + KS * TILE;
+  uint8_t* q_sm = smem + (KS + VS) * TILE;                // [box][128 pairs][128 B]
+  uint64_t* bars = (uint64_t*)(q_sm + BOXES * C::QBOX);   // all of one arrival but p_ready
+  uint64_t* k_full = bars;                                // [KS] the copies, or the expanding warp
+  uint64_t* v_full = k_full + KS;                         // [VS]
+  uint64_t* k_empty = v_full + VS;                        // [KS] commit after QK
+  uint64_t* v_empty = k_empty + KS;                       // [VS] commit after PV
+  uint64_t* s_full = v_empty + VS;                        // [2] commit after QK
+  uint64_t* pv_done = s_full + 2;                         // [2] commit after PV
+  uint64_t* q_ready = pv_done + 2;                        // [4] a segment's queries and description are there
+  uint64_t* q_free = q_ready + 4;                         // commit after a segment's last QK
+  uint64_t* drained = q_free + 1;
+  uint64_t* q_there = drained + 1;                        // (E4M3 caches) the queries as they are
+  uint64_t* spare = q_there + 1;
+  uint64_t* p_ready = spare + 1;                          // [2] the 4 softmax warps
+  ShDesc* desc = (ShDesc*)(p_ready + 2);                  // [4] (behind an even number of words: on a 16-byte boundary)
+  static_assert((2 * (KS + VS)) % 2 == 0, "see desc");
+  uint32_t* tmem_slot = (uint32_t*)(desc + 4);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&k_full[i], F8 ? 2 : 1); mbar_init(&v_full[i], F8 ? 2 : 1); mbar_init(&k_empty[i], 1); mbar_init(&v_empty[i], 1);
-      mbar_init(&s_full[i], 1); mbar_init(&p_ready[i], 4); mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 2);
-    }
-    mbar_init(pv_done, 1); mbar_init(q_ready, 4); mbar_init(drained, 1);
+    for (uint64_t* bar = bars; bar < p_ready; ++bar) mbar_init(bar, 1);
+    mbar_init(&p_ready[0], 4);
+    mbar_init(&p_ready[1], 4);
     *abort_flag = 0;
     fence_barrier_init();
-    prefetch_tmap(&tk);
-    prefetch_tmap(&tv);
+    prefetch_tmap(&tq);
+    if constexpr (!F8) {
+      prefetch_tmap(&tk);
+      prefetch_tmap(&tv);
+    }
   }
-  if (warp == 1) {
+  if (warp == 5) {
     tmem_alloc(tmem_slot, C::COLS);
     tmem_relinquish();
   }
@@ -290,216 +391,142 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
   pdl_wait();                                             // the plan, q and the caches were written by the previous kernels
   const uint32_t tmem_base = *tmem_slot;
   const int G = a.n_q / a.n_kv;
-  ShWalk walk(a.plan, a.n_kv);
-  ShSegment sg;
 
-  if (warp == 0) {
-    // ---------------------------------------------------------------- TMA producer
-    if (elect_one()) {
-      int n = 0, n_v = 0;                                 // pages (bf16: of K, of V) issued
-      bool ok = true;
-      while (ok && walk.next(sg)) {
-        const int* bt = a.block_table + (size_t)sg.b.seq * a.max_blocks + sg.b.page + sg.page;
-        for (int j = 0; j < sg.pages && ok; ++j) {
-          const int y = (bt[j] * a.n_kv + sg.kvh) * SH_PAGE;
-          if constexpr (F8) {
-            const int st = n % C::RS;
-            if (n >= C::RS) ok = mbar_wait(&raw_empty[st], ((n / C::RS) - 1) & 1, abort_flag, a.status, 96, 100);
-            if (!ok) break;
-            mbar_arrive_expect_tx(&raw_full[st], 2 * C::RAW);
-            tma_load_2d(raw + st * 2 * C::RAW, &tk, 0, y, &raw_full[st]);
-            tma_load_2d(raw + st * 2 * C::RAW + C::RAW, &tv, 0, y, &raw_full[st]);
-            ++n;
-          } else {
-            const int st = n % C::KS;
-            if (n >= C::KS) ok = mbar_wait(&k_empty[st], ((n / C::KS) - 1) & 1, abort_flag, a.status, 96, 100);
-            if (!ok) break;
-            mbar_arrive_expect_tx(&k_full[st], TILE);
-            for (int x = 0; x < BOXES; ++x) tma_load_2d(k_sm + st * TILE + x * 8192, &tk, x * 64, y, &k_full[st]);
-            ++n;
-            if (n_v >= C::VS) ok = mbar_wait(&v_empty[st], ((n_v / C::VS) - 1) & 1, abort_flag, a.status, 97, 100);
-            if (!ok) break;
-            mbar_arrive_expect_tx(&v_full[st], TILE);
-            for (int x = 0; x < BOXES; ++x) tma_load_2d(v_sm + st * TILE + x * 8192, &tv, x * 64, y, &v_full[st]);
-            ++n_v;
-          }
-        }
-      }
-      if constexpr (F8) ring_landed(raw_full, C::RS, n);
-      else {
-        ring_landed(k_full, C::KS, n);
-        ring_landed(v_full, C::VS, n_v);
-      }
-    }
-  } else if (warp == 1) {
-    // ---------------------------------------------------------------- MMA issuer
-    if (elect_one()) {
-      constexpr uint32_t fmt = F8 ? 0 : 1;
-      constexpr uint32_t idesc_qk = umma_idesc_f16(SH_PAIRS, SH_PAGE, fmt, fmt);              // both K-major
-      constexpr uint32_t idesc_pv = umma_idesc_f16(SH_PAIRS, HD, fmt, fmt) | (1u << 16);      // B (V) is MN-major
-      const uint64_t qd = umma_desc_k_sw128(smem_u32(q_sm));
-      int done = 0, segs = 0;                             // pages and segments before this one
-      bool ok = true;
-      // S = Q K(j)^T of the CTA's page `n` into buffer n & 1
-      auto qk = [&](int n) {
-        const int st = n % C::KS;
-        if (!mbar_wait(&k_full[st], (n / C::KS) & 1, abort_flag, a.status, 98)) return false;
-        tc_fence_after();
-        const uint64_t kd = umma_desc_k_sw128(smem_u32(k_sm + st * TILE));
+  if (warp < 4) {
+    // ---------------------------------------------------------------- softmax warps: thread = (row, head) pair or a copy of it = TMEM lane
+    const uint32_t lane_addr = tmem_base + ((uint32_t)(warp * 32) << 16);
+    int n = 0;                                            // pages so far
+    bool ok = true;
+    for (int seg = 0; ok; ++seg) {
+      ok = all_ok(sh_wait(&q_ready[seg & 3], (seg >> 2) & 1, abort_flag, a.status, 110));
+      if (!ok) break;
+      const ShDesc d = desc[seg & 3];
+      if (d.pages == 0) break;
+      const int pairs = d.rows * G, copies = sh_copies(pairs);
+      const int copy = copies == 4 ? warp : copies == 2 ? warp >> 1 : 0, pair = copies == 4 ? lane : copies == 2 ? (warp & 1) * 32 + lane : warp * 32 + lane;
+      const int rb = pair / G, hq = d.kvh * G + pair % G;
+      const bool live = rb < d.rows, some = copies > 1 || warp * 32 < pairs;         // (uniform) the warp holds a pair
+      // keys from the segment's first on that the pair sees (a lane without a pair: nothing to mask, nothing comes of it)
+      const int keys = live ? a.plan[SH_AT_ROWS + 4 * (d.row + rb) + 2] - d.key0 : 0x7FFFFFFF;
+      const float scale_log2 = F8 ? a.scale_log2 * a.kv_scale[d.kvh] : a.scale_log2;
+      float m = -INFINITY, l = 0.f;                       // running maximum (log2 units), sum
+      // Keys that no row sees yet: their V may hold anything, and 0 * NaN would reach every pair.  (The barrier of V's stage cannot stand a page's use behind: that
+      // PV was over before the scores of this page were.)
+      auto tail = [&](int j) {
+        const int first = max(d.most - d.key0 - j * SH_PAGE, 0);
+        if (first >= SH_PAGE) return true;
+        if (!all_ok(sh_wait(&v_full[n % VS], (n / VS) & 1, abort_flag, a.status, 104))) return false;
+        for (int i = first * 8 + (int)threadIdx.x; i < SH_PAGE * 8; i += 128)
 #pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk)
-          tc_mma_f16(tmem_base + (n & 1) * C::S_COLS, qd + (uint64_t)((kk >> 2) * (C::QBOX >> 4) + (kk & 3) * 2), kd + (uint64_t)((kk >> 2) * (8192 >> 4) + (kk & 3) * 2),
-                     idesc_qk, kk != 0);
-        tc_commit(&s_full[n & 1]);
-        tc_commit(&k_empty[st]);
+          for (int x = 0; x < BOXES; ++x) *reinterpret_cast<uint4*>(v_sm + (n % VS) * TILE + x * 8192 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+        fence_proxy_async();
         return true;
       };
-      while (ok && walk.next(sg)) {
-        ok = mbar_wait(q_ready, segs & 1, abort_flag, a.status, 99);
-        for (int j = 0; j < 2 && j < sg.pages && ok; ++j) ok = qk(done + j);
-        for (int j = 0; j < sg.pages && ok; ++j) {
-          const int n = done + j, st = n % C::VS;
-          ok = mbar_wait(&v_full[st], (n / C::VS) & 1, abort_flag, a.status, 100) && mbar_wait(&p_ready[n & 1], (n >> 1) & 1, abort_flag, a.status, 101);
-          if (!ok) break;
+      // the segment's pages, NC columns a thread: all of a page's scores, or a copy's part of them
+      auto pages = [&](auto nc) {
+        constexpr int NC = decltype(nc)::value;
+        const int col = NC * copy;
+        uint32_t s[NC];
+        auto scores = [&](int at) {                       // the scores of the CTA's page `at`
           tc_fence_after();
-          const uint32_t vbase = smem_u32(v_sm + st * TILE);
+          sh_ld(lane_addr + (at & 1) * C::S_COLS + col, s);
+        };
+        if (!all_ok(sh_wait(&s_full[n & 1], (n >> 1) & 1, abort_flag, a.status, 102))) return false;
+        scores(n);
+        for (int j = 0;; ++j, ++n) {
+          const uint32_t s_addr = lane_addr + (n & 1) * C::S_COLS;
+          int seen = keys == 0x7FFFFFFF ? NC : keys - j * SH_PAGE - col;
+          asm volatile("" : "+r"(seen));                  // (else the bounds of all columns are held in registers over the whole segment)
+          if (seen < NC) {
 #pragma unroll
-          for (int kk = 0; kk < SH_PAGE / 16; ++kk)
-            tc_mma_f16_ts(tmem_base + C::O, tmem_base + (n & 1) * C::S_COLS + kk * 8, sh_desc_v(vbase + kk * 2048), idesc_pv, (j | kk) != 0);
-          tc_commit(pv_done);
-          tc_commit(&v_empty[st]);
-          if (j + 2 < sg.pages) ok = qk(n + 2);           // overwrites P(n) after PV(n) has read it (a thread's MMAs run in issue order)
-        }
-        done += sg.pages;
-        ++segs;
-      }
-      // every MMA issued so far has completed when this commit arrives: the columns may then be returned
-      tc_commit(drained);
-      for (int i = 0; i < (1 << 22) && !mbar_try_wait(drained, 0); ++i) {}   // bounded, and not cut short by the abort word
-    }
-  } else if (warp < 6) {
-    // ---------------------------------------------------------------- softmax warps: thread = (row, head) pair = TMEM lane
-    const int quarter = warp & 3, pair = quarter * 32 + lane;
-    const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
-    int done = 0;
-    bool ok = true;
-    while (ok && walk.next(sg)) {
-      const int rb = pair / G, hq = sg.kvh * G + pair % G;
-      const bool live = rb < sg.b.rows, some = quarter * 32 < sg.b.rows * G;   // (uniform) the warp holds a pair
-      const int row = sg.b.row + (live ? rb : 0);
-      const int keys = live ? a.plan[SH_AT_ROWS + 4 * row + 2] : 0;     // keys the pair sees
-      if (some) {
-        // q -> shared memory: 128-byte rows, 16-byte chunk c of a box at c ^ (row & 7).  The MMAs that read the segment before's have completed: this
-        // warp has seen the scores of its last page.
-        const uint4* src = reinterpret_cast<const uint4*>(a.q + ((size_t)row * a.n_q + (live ? hq : 0)) * HD);
-        uint8_t* dst = q_sm + pair * 128;
-#pragma unroll
-        for (int i = 0; i < HD / 8; ++i) {
-          uint4 v = live ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
-          if constexpr (F8) {
-            uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-            for (int u = 0; u < 4; ++u) w[u] = sh_pack<true>(__uint_as_float(w[u] << 16), __uint_as_float(w[u] & 0xFFFF0000u));
+            for (int i = 0; i < NC; ++i)
+              if (i >= seen) s[i] = 0xFF800000u;
           }
-          *reinterpret_cast<uint4*>(dst + (i >> 3) * C::QBOX + (((i & 7) ^ (pair & 7)) << 4)) = v;
-        }
-        fence_proxy_async();
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_ready);
-      const float scale_log2 = F8 ? a.scale_log2 * a.kv_scale[sg.kvh] : a.scale_log2;
-      float m = -INFINITY, l = 0.f;
-      for (int j = 0; j < sg.pages && ok; ++j) {
-        const int n = done + j;
-        const uint32_t s_addr = lane_addr + (n & 1) * C::S_COLS;
-        ok = all_ok(mbar_wait(&s_full[n & 1], (n >> 1) & 1, abort_flag, a.status, 102));
-        if (!ok) break;
-        const int key0 = (sg.b.page + sg.page + j) * SH_PAGE;
-        if (some) {
-          tc_fence_after();
-          uint32_t s0[32], s1[32];
-          sh_ld_x32(s_addr, s0);
-          sh_ld_x32(s_addr + 32, s1);
-          tc_wait_ld();
-          if (key0 + SH_PAGE > keys) {
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              if (key0 + i >= keys) s0[i] = 0xFF800000u;
-              if (key0 + 32 + i >= keys) s1[i] = 0xFF800000u;
-            }
-          }
-          float mx = -INFINITY;
-#pragma unroll
-          for (int i = 0; i < 32; ++i) mx = fmaxf(mx, fmaxf(__uint_as_float(s0[i]), __uint_as_float(s1[i])));
-          const float ms = mx * scale_log2;
-          float alpha = 1.f;
+          for (int i = 0; i < NC; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[i]));
+          const float ms = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2;
           // the running maximum moves only by more than 2^8: the probabilities stay below 2^8, harmless in 16-bit operands and fp32 sums
-          if (ms > m + 8.f || m == -INFINITY) {
-            const float m_new = fmaxf(m, ms);
-            alpha = (m == -INFINITY) ? 1.f : sh_ex2(m - m_new);
-            m = m_new;
-          }
-          const float m_use = (m == -INFINITY) ? 0.f : m;
-          float lsum = 0.f;
-          uint32_t pk[32];
+          const bool moves = ms > m + 8.f;
+          if (__any_sync(0xffffffffu, moves)) {           // all pages but a segment's first few: no
+            float alpha = 1.f;
+            if (moves) {
+              if (m != -INFINITY) alpha = sh_ex2(m - ms);
+              m = ms;
+            }
+            l *= alpha;
+            if (__any_sync(0xffffffffu, alpha != 1.f)) {  // O, as the PV before leaves it
+              if (!all_ok(sh_wait(&pv_done[(n - 1) & 1], ((n - 1) >> 1) & 1, abort_flag, a.status, 103))) return false;
+              tc_fence_after();
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float pa = sh_ex2(fmaf(__uint_as_float(s0[2 * i]), scale_log2, -m_use));
-            const float pb = sh_ex2(fmaf(__uint_as_float(s0[2 * i + 1]), scale_log2, -m_use));
-            const float pc = sh_ex2(fmaf(__uint_as_float(s1[2 * i]), scale_log2, -m_use));
-            const float pd = sh_ex2(fmaf(__uint_as_float(s1[2 * i + 1]), scale_log2, -m_use));
-            lsum += (pa + pb) + (pc + pd);
-            pk[i] = sh_pack<F8>(pa, pb);
-            pk[16 + i] = sh_pack<F8>(pc, pd);
-          }
-          tc_st_32x32b_x32(s_addr, pk);
-          l = l * alpha + lsum;
-          if (j > 0) {                                    // O was last written by the PV before: rescale it where a pair's maximum moved
-            ok = all_ok(mbar_wait(pv_done, (n - 1) & 1, abort_flag, a.status, 103));
-            if (!ok) break;
-            tc_fence_after();
-            if (__any_sync(0xffffffffu, alpha != 1.f)) {
+              for (int ch = 0; ch < HD / 16; ++ch) {
+                uint32_t r[16];
+                sh_ld(lane_addr + C::O + ch * 16, r);
 #pragma unroll
-              for (int ch = 0; ch < HD / 32; ++ch) {
-                uint32_t r[32];
-                sh_ld_x32(lane_addr + C::O + ch * 32, r);
-                tc_wait_ld();
-#pragma unroll
-                for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
-                tc_st_32x32b_x32(lane_addr + C::O + ch * 32, r);
+                for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
+                sh_st(lane_addr + C::O + ch * 16, r);
               }
             }
           }
-          tc_wait_st();
-          tc_fence_before();
-        }
-        // Keys that no row sees yet: their V may hold anything, and 0 * NaN would reach every pair
-        if (key0 + SH_PAGE > sg.b.most) {
-          ok = all_ok(mbar_wait(&v_full[n % C::VS], (n / C::VS) & 1, abort_flag, a.status, 104));
-          if (!ok) break;
-          uint8_t* v = v_sm + (n % C::VS) * TILE;
-          for (int i = max(sg.b.most - key0, 0) * 8 + (warp - 2) * 32 + lane; i < SH_PAGE * 8; i += 128)
+          const float m_use = (m == -INFINITY) ? 0.f : m;
+          float lsum[4] = {0.f, 0.f, 0.f, 0.f};
+          uint32_t pk[NC / 2];
 #pragma unroll
-            for (int x = 0; x < BOXES; ++x) *reinterpret_cast<uint4*>(v + x * 8192 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
-          fence_proxy_async();
+          for (int i = 0; i < NC / 2; ++i) {
+            const float pa = sh_ex2(fmaf(__uint_as_float(s[2 * i]), scale_log2, -m_use)), pb = sh_ex2(fmaf(__uint_as_float(s[2 * i + 1]), scale_log2, -m_use));
+            lsum[i & 3] += pa + pb;
+            pk[i] = sh_pack<F8>(pa, pb);
+          }
+          l += (lsum[0] + lsum[1]) + (lsum[2] + lsum[3]);
+          sh_st(s_addr + col / 2, pk);
+          // the other copies' columns of P
+          if constexpr (NC == 32) sh_st_zero<16>(s_addr + 16 * (1 - copy));
+          if constexpr (NC == 16) {
+#pragma unroll
+            for (int o = 1; o < 4; ++o) sh_st_zero<8>(s_addr + 8 * ((copy + o) & 3));
+          }
+          auto done = [&]() {                             // P is there
+            tc_wait_st();
+            tc_fence_before();
+            if (!tail(j)) return false;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_ready[n & 1]);
+            return true;
+          };
+          if (j + 1 == d.pages) {
+            if (!done()) return false;
+            ++n;
+            return true;
+          }
+          // the next page's scores: while the probabilities are on their way, if they are there
+          if (all_ok(mbar_test_wait(&s_full[(n + 1) & 1], ((n + 1) >> 1) & 1))) {
+            scores(n + 1);
+            if (!done()) return false;
+          } else {
+            if (!done() || !all_ok(sh_wait(&s_full[(n + 1) & 1], ((n + 1) >> 1) & 1, abort_flag, a.status, 102))) return false;
+            scores(n + 1);
+          }
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_ready[n & 1]);
+      };
+      if (!some) {
+        for (int j = 0; j < d.pages && ok; ++j, ++n) {
+          ok = all_ok(sh_wait(&s_full[n & 1], (n >> 1) & 1, abort_flag, a.status, 102)) && tail(j);
+          if (ok && lane == 0) mbar_arrive(&p_ready[n & 1]);
+          __syncwarp();
+        }
+      } else {
+        ok = copies == 1 ? pages(std::integral_constant<int, 64>()) : copies == 2 ? pages(std::integral_constant<int, 32>()) : pages(std::integral_constant<int, 16>());
       }
-      done += sg.pages;
-      if (!ok) break;
-      ok = all_ok(mbar_wait(pv_done, (done - 1) & 1, abort_flag, a.status, 105));
-      if (!ok) break;
-      if (some) {
+      if (ok) ok = all_ok(sh_wait(&pv_done[(n - 1) & 1], ((n - 1) >> 1) & 1, abort_flag, a.status, 105));
+      if (ok && some) {
         tc_fence_after();
-        const float v_scale = F8 ? a.kv_scale[a.n_kv + sg.kvh] : 1.f;
-        const size_t at = (size_t)(sg.b.part + rb * sg.slots + sg.slot) * a.n_q + hq;
+        const float v_scale = F8 ? a.kv_scale[a.n_kv + d.kvh] : 1.f;
+        const size_t at = (size_t)(d.part + rb * d.stride + copy) * a.n_q + hq;
         float4* dst = reinterpret_cast<float4*>(a.part_o + at * HD);
 #pragma unroll
         for (int ch = 0; ch < HD / 32; ++ch) {
           uint32_t r[32];
-          sh_ld_x32(lane_addr + C::O + ch * 32, r);
-          tc_wait_ld();
+          sh_ld(lane_addr + C::O + ch * 32, r);
           if (live) {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
@@ -508,55 +535,238 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
           }
         }
         if (live) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m, l);
-        tc_fence_before();                                // the reads of O are ordered before the next segment's first PV by q_ready / p_ready
+        tc_fence_before();                                // the reads of O are ordered before the next segment's first PV by p_ready
       }
+    }
+  } else if (warp == 4) {
+    // ---------------------------------------------------------------- feeder: descriptions and queries of the segments; K and V each at their own pace
+    // One warp's ordinary code is slow (some five cycles an instruction), so it does little of it: a segment is looked up once for everybody, and its
+    // queries come by TMA, a row's heads of one KV head per copy (by plain copies, 125 pairs took 25,000 cycles).
+    // (With K and V in turn, K page n + 2 waited for V page n + 1 and so for PV(n - 1), and a page took as long as a K page's way from memory.)
+    // Of four descriptions the one that is overwritten, segment w - 4's, is out of use.  bf16: V has begun segment w - 1; that copy waited for the PV of a page two
+    // earlier, in segment w - 3 or later, and that PV for all softmax warps to leave the segment before.  E4M3: the last QK of segment w - 1 is over, which was
+    // issued after the PV of a page two earlier.
+    ShWalk walk(a.plan, a.n_kv);
+    struct Ring { int seg, j, n; };                       // segment, its next page, pages issued
+    Ring ring[2] = {{0, 0, 0}, {0, 0, 0}};
+    int known = 0, asked = 0, queries = 0, idle = 0;      // segments with a description, with queries; the last one whose queries were fetched, + 1
+    bool more = true;
+    uint64_t since = 0;
+    while (more || asked < known || (!F8 && (ring[0].seg < known - 1 || ring[1].seg < known - 1))) {
+      bool moved = false;
+      if constexpr (!F8) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          constexpr int S[2] = {KS, VS};
+          Ring& r = ring[u];
+          const int st = r.n % S[u];
+          uint64_t *full = (u ? v_full : k_full) + st, *empty = (u ? v_empty : k_empty) + st;
+          if (r.seg >= known) continue;
+          const ShDesc& d = desc[r.seg & 3];
+          const int left = d.pages - r.j;
+          if (left == 0 || (r.n >= S[u] && !all_ok(mbar_test_wait(empty, ((r.n / S[u]) - 1) & 1)))) continue;
+          if (elect_one()) {
+            const int y = (d.table[r.j] * a.n_kv + d.kvh) * SH_PAGE;
+            mbar_arrive_expect_tx(full, TILE);
+#pragma unroll
+            for (int x = 0; x < BOXES; ++x) tma_load_2d((u ? v_sm : k_sm) + st * TILE + x * 8192, u ? &tv : &tk, x * 64, y, full);
+          }
+          __syncwarp();
+          ++r.n, ++r.j;
+          if (left == 1) ++r.seg, r.j = 0;
+          moved = true;
+        }
+      }
+      if (more && (known < 4 || (F8 ? asked == known && all_ok(mbar_test_wait(q_free, (known - 1) & 1)) : ring[1].seg >= known || (ring[1].seg == known - 1 && ring[1].j > 0)))) {
+        ShSegment sg;
+        more = walk.next(sg);
+        const int copies = sh_copies(sg.b.rows * G);
+        if (lane == 0)
+          desc[known & 3] = ShDesc{sg.b.row, sg.b.rows, sg.kvh, (sg.b.page + sg.page) * SH_PAGE, more ? sg.pages : 0, sg.b.part + sg.slot * copies, sg.slots * copies, sg.b.most,
+                                   a.block_table + (size_t)sg.b.seq * a.max_blocks + sg.b.page + sg.page, 0};
+        __syncwarp();
+        ++known;
+        moved = true;
+      }
+      if (asked < known && (asked == 0 || all_ok(mbar_test_wait(q_free, (asked - 1) & 1)))) {
+        const ShDesc& d = desc[asked & 3];
+        const int rows = d.pages != 0 ? d.rows : 0, copies = sh_copies(rows * G), bytes = rows * copies * G * HD * 2;
+        uint64_t* bar = F8 ? q_there : &q_ready[asked & 3];
+        if (lane == 0) {
+          if (bytes != 0) mbar_arrive_expect_tx(bar, bytes);
+          else mbar_arrive(&q_ready[asked & 3]);
+        }
+        __syncwarp();
+        // 128-byte rows at any multiple of 128 bytes: the swizzle goes by the address, so chunk c of pair p stands at c ^ (p & 7)
+        for (int i = lane; i < rows * copies * BOXES; i += 32) {
+          const int x = i % BOXES, t = i / BOXES % copies, r = i / BOXES / copies;
+          sh_load_q(q_sm + x * C::QBOX + (t * (SH_PAIRS / copies) + r * G) * 128, &tq, x * 64, d.kvh * G, d.row + r, bar);
+        }
+        __syncwarp();
+        if (rows != 0) queries = asked + 1;
+        if (F8 && rows != 0) {                            // bf16 -> fp16 in place, beside the fp16 values of an E4M3 cache
+          if (!all_ok(sh_wait(q_there, asked & 1, abort_flag, a.status, 112))) break;
+          for (int t = 0; t < copies; ++t)
+#pragma unroll
+            for (int x = 0; x < BOXES; ++x) {
+              const uint32_t at = smem_u32(q_sm + x * C::QBOX + t * (SH_PAIRS / copies) * 128);
+#pragma unroll 4
+              for (int i = lane; i < rows * G * 8; i += 32) {
+                uint4 v = lds128(at + i * 16);
+                uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) w[u] = sh_pack<true>(__uint_as_float(w[u] << 16), __uint_as_float(w[u] & 0xFFFF0000u));
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + i * 16), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+              }
+            }
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&q_ready[asked & 3]);
+        }
+        ++asked;
+        moved = true;
+      }
+      if (moved) {
+        idle = 0;
+      } else if (++idle > 16) {
+        __nanosleep(40);
+        if ((idle & 255) == 0) {                          // (a bounded wait, as mbar_wait's, for whatever can go on first)
+          if (idle == 256) since = globaltimer_ns();
+          const bool stop = host_abort(a.status), late = globaltimer_ns() - since > wait_limit_ns(a.status);
+          if (lane == 0 && (stop || late)) set_status(a.status, stop ? ST_ABORTED : ST_TIMEOUT, 96), *abort_flag = 1;
+          __syncwarp();
+          if (__any_sync(0xffffffffu, *abort_flag != 0)) break;
+        }
+      }
+    }
+    if (lane == 0) {
+      if constexpr (!F8) {
+        ring_landed(k_full, KS, ring[0].n);
+        ring_landed(v_full, VS, ring[1].n);
+      }
+      // (where the others gave up, nobody has waited for the last queries)
+      uint64_t* last = F8 ? q_there : &q_ready[(queries - 1) & 3];
+      const int parity = (F8 ? queries - 1 : (queries - 1) >> 2) & 1;
+      if (*abort_flag != 0 && queries > 0)
+        for (int i = 0; i < (1 << 20) && !mbar_try_wait(last, parity); ++i) __nanosleep(100);
+    }
+  } else if (warp == 5) {
+    // ---------------------------------------------------------------- MMA issuer
+    if (elect_one()) {
+      constexpr uint32_t fmt = F8 ? 0 : 1;
+      constexpr uint32_t idesc_qk = umma_idesc_f16(SH_PAIRS, SH_PAGE, fmt, fmt);              // both K-major
+      constexpr uint32_t idesc_pv = umma_idesc_f16(SH_PAIRS, HD, fmt, fmt) | (1u << 16);      // B (V) is MN-major
+      const uint64_t qd = umma_desc_k_sw128(smem_u32(q_sm));
+      int n_qk = 0, seg_qk = 0, left_qk = 0, seg = 0, left = 0;      // pages with a QK, segments begun, pages left of the segment; the PVs' segments and pages
+      bool more = true;
+      // S = Q K^T of the next page, of this segment or the next one
+      auto qk = [&]() {
+        if (left_qk == 0) {
+          if (!sh_wait(&q_ready[seg_qk & 3], (seg_qk >> 2) & 1, abort_flag, a.status, 99)) return false;
+          left_qk = desc[seg_qk & 3].pages;
+          more = left_qk != 0;
+          if (!more) return true;
+          ++seg_qk;
+        }
+        const int n = n_qk++, st = n % KS;
+        if (!sh_wait(&k_full[st], (n / KS) & 1, abort_flag, a.status, 98)) return false;
+        tc_fence_after();
+        const uint64_t kd = umma_desc_k_sw128(smem_u32(k_sm + st * TILE));
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk)
+          tc_mma_f16(tmem_base + (n & 1) * C::S_COLS, qd + (uint64_t)((kk >> 2) * (C::QBOX >> 4) + (kk & 3) * 2), kd + (uint64_t)((kk >> 2) * (8192 >> 4) + (kk & 3) * 2),
+                     idesc_qk, kk != 0);
+        tc_commit(&s_full[n & 1]);
+        tc_commit(&k_empty[st]);
+        if (--left_qk == 0) tc_commit(q_free);
+        return true;
+      };
+      bool ok = qk();
+      if (ok && more) ok = qk();
+      for (int n = 0; ok && n < n_qk; ++n) {
+        const int st = n % VS;
+        const bool fresh = left == 0;
+        if (fresh) left = desc[seg++ & 3].pages;
+        --left;
+        ok = sh_wait(&v_full[st], (n / VS) & 1, abort_flag, a.status, 100) && sh_wait(&p_ready[n & 1], (n >> 1) & 1, abort_flag, a.status, 101);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t vd = sh_desc_v(smem_u32(v_sm + st * TILE), 8192);
+#pragma unroll
+        for (int kk = 0; kk < SH_PAGE / 16; ++kk)
+          tc_mma_f16_ts(tmem_base + C::O, tmem_base + (n & 1) * C::S_COLS + kk * 8, vd + (uint64_t)(kk * (2048 >> 4)), idesc_pv, !fresh || kk != 0);
+        tc_commit(&pv_done[n & 1]);
+        tc_commit(&v_empty[st]);
+        if (more) ok = qk();                              // into P(n)'s buffer, after PV(n) has read it (a thread's MMAs run in issue order)
+      }
+      // every MMA issued so far has completed when this commit arrives: the columns may then be returned
+      tc_commit(drained);
+      for (int i = 0; i < (1 << 22) && !mbar_try_wait(drained, 0); ++i) {}   // bounded, and not cut short by the abort word
     }
   } else if constexpr (F8) {
     // ---------------------------------------------------------------- expansion of byte pages: E4M3 -> fp16 (exact) in the operand layout
-    const int tid = threadIdx.x - 192;
-    constexpr int CHUNKS = C::RAW / 16;
-    auto expand = [&](const uint8_t* src, uint8_t* dst) {
-#pragma unroll 4
-      for (int c = tid; c < CHUNKS; c += 64) {
-        const int key = c / (HD / 16), x = c % (HD / 16);
-        const uint4 b = lds128(smem_u32(src) + c * 16);
-        const uint32_t w[4] = {b.x, b.y, b.z, b.w};
-        uint32_t h[8];
+    // Straight from global memory: three quarters of a page are on their way in registers while one is expanded.
+    const int v = warp - 6, S = v ? VS : KS;
+    constexpr int QC = SH_PAGE * HD / 16 / 128;           // 16-byte chunks of a quarter page per lane
+    uint64_t *full = v ? v_full : k_full, *empty = v ? v_empty : k_empty;
+    const uint8_t* cache = v ? a.v8 : a.k8;
+    ShWalk walk(a.plan, a.n_kv);
+    ShSegment sg;
+    bool more = walk.next(sg);
+    int j = 0;
+    // the next page's address (a page outside the cache: zeros)
+    auto page = [&]() -> const uint4* {
+      if (!more) return nullptr;
+      const int id = a.block_table[(size_t)sg.b.seq * a.max_blocks + sg.b.page + sg.page + j];
+      const uint4* p = id >= 0 && id < a.n_pages ? reinterpret_cast<const uint4*>(cache + ((size_t)id * a.n_kv + sg.kvh) * SH_PAGE * HD) : nullptr;
+      if (++j == sg.pages) j = 0, more = walk.next(sg);
+      return p;
+    };
+    uint4 b[4][QC];
+    auto load = [&](uint4 (&to)[QC], const uint4* p, int quarter) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(h[2 * i]), "=r"(h[2 * i + 1]) : "r"(w[i]));
+      for (int i = 0; i < QC; ++i) to[i] = p != nullptr ? __ldg(p + (quarter * QC + i) * 32 + lane) : make_uint4(0u, 0u, 0u, 0u);
+    };
+    bool here = more;
+    const uint4* src = page();
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int ch = 2 * x + u;                       // 16-byte chunk of the fp16 row
-          *reinterpret_cast<uint4*>(dst + (ch >> 3) * 8192 + key * 128 + (((ch & 7) ^ (key & 7)) << 4)) = make_uint4(h[4 * u], h[4 * u + 1], h[4 * u + 2], h[4 * u + 3]);
+    for (int q = 0; q < 3; ++q) load(b[q], src, q);
+    int st = 0, round = 0;
+    while (here) {
+      const bool then = more;
+      const uint4* next = page();
+      if (round > 0 && !all_ok(sh_wait(&empty[st], (round - 1) & 1, abort_flag, a.status, 107))) break;
+      uint8_t* dst = (v ? v_sm : k_sm) + st * TILE;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (q == 0) load(b[3], src, 3);
+        else load(b[q - 1], next, q - 1);
+#pragma unroll
+        for (int i = 0; i < QC; ++i) {
+          const int c = (q * QC + i) * 32 + lane, key = c / (HD / 16), x = c % (HD / 16);
+          const uint32_t w[4] = {b[q][i].x, b[q][i].y, b[q][i].z, b[q][i].w};
+          uint32_t e[8];
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(e[2 * u]), "=r"(e[2 * u + 1]) : "r"(w[u]));
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int ch = 2 * x + u;                     // 16-byte chunk of the fp16 row
+            *reinterpret_cast<uint4*>(dst + (ch >> 3) * 8192 + key * 128 + (((ch & 7) ^ (key & 7)) << 4)) = make_uint4(e[4 * u], e[4 * u + 1], e[4 * u + 2], e[4 * u + 3]);
+          }
         }
       }
       fence_proxy_async();
       __syncwarp();
-    };
-    int n = 0;
-    bool ok = true;
-    while (ok && walk.next(sg)) {
-      for (int j = 0; j < sg.pages && ok; ++j, ++n) {
-        const int st = n % C::RS;
-        ok = all_ok(mbar_wait(&raw_full[st], (n / C::RS) & 1, abort_flag, a.status, 106));
-        if (ok && n >= C::KS) ok = all_ok(mbar_wait(&k_empty[n % C::KS], ((n / C::KS) - 1) & 1, abort_flag, a.status, 107));
-        if (!ok) break;
-        expand(raw + st * 2 * C::RAW, k_sm + (n % C::KS) * TILE);
-        if (lane == 0) mbar_arrive(&k_full[n % C::KS]);
-        if (n >= C::VS) ok = all_ok(mbar_wait(&v_empty[n % C::VS], ((n / C::VS) - 1) & 1, abort_flag, a.status, 108));
-        if (!ok) break;
-        expand(raw + st * 2 * C::RAW + C::RAW, v_sm + (n % C::VS) * TILE);
-        if (lane == 0) {
-          mbar_arrive(&v_full[n % C::VS]);
-          mbar_arrive(&raw_empty[st]);
-        }
-      }
+      if (lane == 0) mbar_arrive(&full[st]);
+      src = next;
+      here = then;
+      if (++st == S) st = 0, ++round;
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem_base, C::COLS);
+  if (warp == 5) tmem_dealloc(tmem_base, C::COLS);
 }
 
 // ------------------------------------------------------------------------------------------------ merge
@@ -579,9 +789,9 @@ __global__ void __launch_bounds__(128) attn_shared_merge_kernel(const int* plan,
     const int id = plan[SH_AT_ROWS + 4 * row + u];
     if (id < 0) continue;
     const ShBlock s = blk[id];
-    const int unit = s.before * n_kv + kvh * s.pages;
-    n[u] = (unit + s.pages - 1) / L - unit / L + 1;
-    at[u] = (size_t)(s.part + (row - s.row) * sh_slots(s.pages, L)) * n_q + hq;
+    const int unit = sh_unit(s, kvh, n_kv), copies = sh_copies(s.rows * (n_q / n_kv));
+    n[u] = ((unit + s.pages - 1) / L - unit / L + 1) * copies;
+    at[u] = (size_t)(s.part + (row - s.row) * sh_slots(s.pages, L) * copies) * n_q + hq;
   }
   auto slot = [&](int s) { return s < n[0] ? at[0] + (size_t)s * n_q : at[1] + (size_t)(s - n[0]) * n_q; };
   const int all = n[0] + n[1];
@@ -610,14 +820,31 @@ __global__ void __launch_bounds__(128) attn_shared_merge_kernel(const int* plan,
 }
 
 template <int HD, bool F8>
-static cudaError_t launch_shared(int dev, const CUtensorMap& tk, const CUtensorMap& tv, const ShArgs& a, cudaStream_t st) {
+static cudaError_t launch_shared(int dev, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tq, const ShArgs& a, cudaStream_t st) {
   static bool configured[64];
   if (dev >= 64 || !configured[dev]) {
     const cudaError_t e = cudaFuncSetAttribute(attn_shared_kernel<HD, F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh<HD, F8>::SMEM);
     if (e != cudaSuccess) return e;
     if (dev < 64) configured[dev] = true;
   }
-  return rx::launch(attn_shared_kernel<HD, F8>, dim3(SH_CTAS), dim3(Sh<HD, F8>::THREADS), Sh<HD, F8>::SMEM, st, tk, tv, a);
+  return rx::launch(attn_shared_kernel<HD, F8>, dim3(SH_CTAS), dim3(Sh<HD, F8>::THREADS), Sh<HD, F8>::SMEM, st, tk, tv, tq, a);
+}
+
+// The queries [rows][n_q][hd] by boxes of one row's G heads, 64 values of each.
+static bool sh_query_map(CUtensorMap* map, const void* q, int rows, int n_q, int G, int hd) {
+  typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                             CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static Encode encode = nullptr;
+  if (encode == nullptr) {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) return false;
+    encode = (Encode)p;
+  }
+  const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)n_q, (cuuint64_t)rows}, strides[2] = {(cuuint64_t)hd * 2, (cuuint64_t)n_q * hd * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)G, 1}, steps[3] = {1, 1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 }  // namespace rx
@@ -626,16 +853,17 @@ using namespace rx;
 
 RX_API int rx_attn_shared_plan_ints() { return SH_PLAN_INTS; }
 
-// Partial vectors: a block of n rows meets at most pages / L + 2 CTAs per KV head, and all blocks' pages / L together at most SH_CTAS / n_kv; a row is in two blocks.
+// Partial vectors: a unit meets at most pages / L + 2 CTAs, a block of n rows leaves n * copies from each, at most SH_PAIRS / G; all blocks' pages / L together
+// are at most SH_CTAS / n_kv; a row is in two blocks, with up to four copies of it in each.
 RX_API long long rx_attn_shared_scratch_floats(int rows, int n_q, int n_kv, int hd) {
   if (rows < 1 || n_q < 1 || n_kv < 1 || n_q % n_kv != 0 || n_q / n_kv > SH_PAIRS) return 0;
-  const long long rt = SH_PAIRS / (n_q / n_kv), vectors = (rt * SH_CTAS / n_kv + 1 + 4ll * rows) * n_q;
+  const long long rt = SH_PAIRS / (n_q / n_kv), vectors = (rt * SH_CTAS / n_kv + 1 + 16ll * rows) * n_q;
   return vectors * (hd + 2) + SH_PLAN_INTS;
 }
 
 static bool sh_takes(int rows, int n_q, int n_kv, int n_tables, int max_blocks) {
   return rows >= 1 && rows <= SH_MAX_ROWS && n_kv >= 1 && n_q >= n_kv && n_q % n_kv == 0 && n_q / n_kv <= SH_PAIRS && n_tables >= 1 && max_blocks >= 1 &&
-         (long long)rows * max_blocks * n_kv < (1ll << 29) && max_blocks < (1 << 24);
+         (long long)rows * (max_blocks + SH_SEGMENT) * n_kv < (1ll << 29) && max_blocks < (1 << 24);
 }
 
 RX_API int rx_attn_shared_plan(const void* row_seq, const void* ctx_len, const void* common, int rows, int n_tables, int max_blocks, int n_q, int n_kv, void* plan,
@@ -643,15 +871,16 @@ RX_API int rx_attn_shared_plan(const void* row_seq, const void* ctx_len, const v
   if (!sh_takes(rows, n_q, n_kv, n_tables, max_blocks)) return (int)cudaErrorInvalidValue;
   const int threads = rows <= 128 ? 128 : (rows + 31) / 32 * 32;
   return (int)rx::launch(shared_plan_kernel, dim3(1), dim3(threads), 0, (cudaStream_t)stream, (const int*)row_seq, (const int*)ctx_len, (const int*)common, rows,
-                         n_tables, max_blocks, SH_PAIRS / (n_q / n_kv), n_kv, (int*)plan, status);
+                         n_tables, max_blocks, n_q / n_kv, n_kv, (int*)plan, status);
 }
 
-// scratch: rx_attn_shared_scratch_floats floats, 16-byte aligned.  plan == nullptr: the call plans into the scratch.  kv_scale == nullptr: bf16 caches.
+// scratch: rx_attn_shared_scratch_floats floats, 16-byte aligned.  plan == nullptr: the call plans into the scratch.  kv_scale == nullptr: bf16 caches by their tensor
+// maps; else E4M3 caches of n_pages pages at k8, v8.
 RX_API int rx_attn_shared(const void* tmap_k, const void* tmap_v, const void* q, const void* block_table, int n_tables, int max_blocks, const void* row_seq,
                           const void* ctx_len, const void* common, void* scratch, int rows, int n_q, int n_kv, int hd, float scale, const void* kv_scale,
-                          const void* suh, void* xr, void* out, const void* plan, int* status, void* stream) {
+                          const void* suh, void* xr, void* out, const void* plan, const void* k8, const void* v8, int n_pages, int* status, void* stream) {
   if (!sh_takes(rows, n_q, n_kv, n_tables, max_blocks) || (hd != 64 && hd != 128) || n_q * hd % 128 != 0 || (out == nullptr && xr == nullptr) ||
-      (suh == nullptr) != (xr == nullptr))
+      (suh == nullptr) != (xr == nullptr) || (kv_scale != nullptr && (k8 == nullptr || v8 == nullptr || n_pages < 0)))
     return (int)cudaErrorInvalidValue;
   cudaStream_t st = (cudaStream_t)stream;
   int dev = 0;
@@ -662,15 +891,18 @@ RX_API int rx_attn_shared(const void* tmap_k, const void* tmap_v, const void* q,
   a.part_o = (float*)scratch; a.part_ml = a.part_o + vectors * hd;
   int* own_plan = (int*)(a.part_ml + vectors * 2);
   own_plan = (int*)(((uintptr_t)own_plan + 15) & ~(uintptr_t)15);
-  a.q = (const uint16_t*)q; a.block_table = (const int*)block_table; a.plan = plan != nullptr ? (const int*)plan : own_plan;
+  a.block_table = (const int*)block_table; a.plan = plan != nullptr ? (const int*)plan : own_plan;
+  a.k8 = (const uint8_t*)k8; a.v8 = (const uint8_t*)v8; a.n_pages = n_pages;
   a.kv_scale = (const float*)kv_scale; a.status = status; a.max_blocks = max_blocks; a.n_q = n_q; a.n_kv = n_kv; a.scale_log2 = scale * 1.4426950408889634f;
   if (plan == nullptr) {
     const int r = rx_attn_shared_plan(row_seq, ctx_len, common, rows, n_tables, max_blocks, n_q, n_kv, own_plan, status, stream);
     if (r != 0) return r;
   }
+  CUtensorMap tq;
+  if (!sh_query_map(&tq, q, rows, n_q, n_q / n_kv, hd)) return (int)cudaErrorInvalidValue;
   const CUtensorMap &tk = *(const CUtensorMap*)tmap_k, &tv = *(const CUtensorMap*)tmap_v;
-  if (hd == 128) e = kv_scale != nullptr ? launch_shared<128, true>(dev, tk, tv, a, st) : launch_shared<128, false>(dev, tk, tv, a, st);
-  else e = kv_scale != nullptr ? launch_shared<64, true>(dev, tk, tv, a, st) : launch_shared<64, false>(dev, tk, tv, a, st);
+  if (hd == 128) e = kv_scale != nullptr ? launch_shared<128, true>(dev, tk, tv, tq, a, st) : launch_shared<128, false>(dev, tk, tv, tq, a, st);
+  else e = kv_scale != nullptr ? launch_shared<64, true>(dev, tk, tv, tq, a, st) : launch_shared<64, false>(dev, tk, tv, tq, a, st);
   if (e != cudaSuccess) return (int)e;
   return (int)rx::launch(hd == 128 ? attn_shared_merge_kernel<128> : attn_shared_merge_kernel<64>, dim3(rows, (n_q * hd / 128 + 3) / 4), dim3(128), 0, st, a.plan, a.part_o,
                          a.part_ml, n_q, n_kv, (const __half*)suh, (__half*)xr, (uint16_t*)out);

@@ -142,7 +142,7 @@ def _declare(lib):
         "rx_attn_shared_scratch_floats": (c_ll, [c_int, c_int, c_int, c_int]),
         "rx_attn_shared_plan": (c_int, [c_void, c_void, c_void, c_int, c_int, c_int, c_int, c_int, c_void, c_void, c_void]),
         "rx_attn_shared": (c_int, [c_void, c_void, c_void, c_void, c_int, c_int, c_void, c_void, c_void, c_void, c_int, c_int, c_int, c_int, c_f, c_void, c_void,
-                                   c_void, c_void, c_void, c_void, c_void]),
+                                   c_void, c_void, c_void, c_void, c_void, c_int, c_void, c_void]),
         "rx_make_kv_tmap": (c_int, [c_void, c_void, c_ll, c_int]),
         "rx_make_kv_tmap8": (c_int, [c_void, c_void, c_ll, c_int]),
         "rx_make_kv_tmap_f8": (c_int, [c_void, c_void, c_ll, c_int]),
