@@ -16,8 +16,8 @@
 // A page's 64 scores a pair go to tensor memory, come back as exponentials in 16 bits over the same columns, and are the A operand of the product with V.
 // The QKs run two pages ahead of the PVs, also into the next segment.
 //
-// Warps: 0..3 = softmax, 4 = feeder (queries and descriptions of the segments; TMA), 5 = MMA issuer (owns the tensor memory), for E4M3 caches 6, 7 = expansion
-// of byte pages of K and of V to fp16 operand tiles, in place of TMA.
+// Warps: 0..3 = softmax, 4 = feeder (queries and descriptions of the segments; TMA), 5 = MMA issuer (owns the tensor memory), for E4M3 caches 6, 7 and 8, 9 =
+// expansion of byte pages of K and of V to fp16 operand tiles, in place of TMA.
 // A block of up to 64 or 32 pairs would leave two or three quarters idle and the others bound by one warp's exponentials: its queries
 // stand in the tensor memory two or four times, each copy takes its part of a page's keys - the rest of its P is zero - and leaves its own partial output.
 // All waits are bounded (status words), no cluster multicast.
@@ -180,6 +180,16 @@ __device__ __forceinline__ uint32_t sh_pack(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&v);
   }
 }
+// two probabilities of a word, times a factor
+template <bool F16>
+__device__ __forceinline__ uint32_t sh_scale(uint32_t w, float f) {
+  if constexpr (F16) {
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    return sh_pack<true>(v.x * f, v.y * f);
+  } else {
+    return sh_pack<false>(__uint_as_float(w << 16) * f, __uint_as_float(w & 0xFFFF0000u) * f);
+  }
+}
 // V as the B operand: keys x head_dim with the head dimension contiguous (MN-major, 128-byte swizzle; see attention_tc.cu)
 __device__ __forceinline__ uint64_t sh_desc_v(uint32_t smem_addr, uint32_t box) {
   return (uint64_t)((smem_addr & 0x3FFFF) >> 4) | (uint64_t)(box >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
@@ -198,20 +208,14 @@ __device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-__device__ __forceinline__ bool sh_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int site) {
+__device__ __noinline__ bool sh_wait_long(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int site) {
 #pragma unroll 1
-  for (int i = 0; i < 64; ++i) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity), "r"(4000)          // asleep for up to 4 us
-        : "memory");
-    if (ok) return true;
-  }
+  for (int i = 0; i < 64; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
   return mbar_wait(bar, parity, abort_flag, status, site);
+}
+__device__ __forceinline__ bool sh_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int site) {
+  return mbar_try_wait(bar, parity) || sh_wait_long(bar, parity, abort_flag, status, site);      // (a call: in line, the waits were half of the kernel's code)
 }
 
 struct ShArgs {
@@ -232,7 +236,7 @@ struct Sh {
   static constexpr int KS = 3, VS = 2;                                      // stages of K, of V
   static constexpr int SMEM = (KS + VS) * TILE + HD / 64 * QBOX + 512;      // two CTAs an SM: 115,712 bytes at most
   static_assert(SMEM <= 115712, "two CTAs an SM");
-  static constexpr int THREADS = 32 * (F8 ? 8 : 6);
+  static constexpr int THREADS = 32 * (F8 ? 10 : 6);
   static constexpr int S_COLS = 64, O = 128, COLS = 256;                    // tensor memory: two buffers of S (P over the first 32 columns of one) | O
 };
 
@@ -284,7 +288,7 @@ struct ShDesc {
 // N columns of the thread's lane, once they are there (load and wait in one statement: no copy of a register comes between them)
 template <int N>
 __device__ __forceinline__ void sh_ld(uint32_t taddr, uint32_t (&r)[N]) {
-  static_assert(N == 64 || N == 32 || N == 16, "16, 32 or 64 columns");
+  static_assert(N == 64 || N == 32 || N == 16 || N == 8, "8, 16, 32 or 64 columns");
   if constexpr (N == 64)
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
                  "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, "
@@ -303,6 +307,11 @@ __device__ __forceinline__ void sh_ld(uint32_t taddr, uint32_t (&r)[N]) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
                    "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
                    "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr)
+                 : "memory");
+  else if constexpr (N == 8)
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                  : "r"(taddr)
                  : "memory");
   else if constexpr (N == 16)
@@ -336,6 +345,14 @@ __device__ __forceinline__ void sh_load_q(void* dst, const void* tmap, int x, in
                : "memory");
 }
 
+// the rows of a V page from `first` on, by the four softmax warps
+__device__ __noinline__ bool sh_zero_rows(uint8_t* page, int boxes, int first) {
+  for (int x = 0; x < boxes; ++x)
+    for (int i = first * 8 + (int)threadIdx.x; i < SH_PAGE * 8; i += 128) *reinterpret_cast<uint4*>(page + x * 8192 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+  fence_proxy_async();
+  return true;
+}
+
 template <int HD, bool F8>
 __global__ void __launch_bounds__((Sh<HD, F8>::THREADS), 2)
 attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tq, const __grid_constant__ ShArgs a) {
@@ -350,8 +367,8 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
   uint8_t* k_sm = smem;                                   // [stage][box (64 d)][64 keys][128 B]
   uint8_t* v_sm = smem + KS * TILE;
   uint8_t* q_sm = smem + (KS + VS) * TILE;                // [box][128 pairs][128 B]
-  uint64_t* bars = (uint64_t*)(q_sm + BOXES * C::QBOX);   // all of one arrival but p_ready
-  uint64_t* k_full = bars;                                // [KS] the copies, or the expanding warp
+  uint64_t* bars = (uint64_t*)(q_sm + BOXES * C::QBOX);   // of one arrival each but p_ready
+  uint64_t* k_full = bars;                                // [KS] the copies, or the expanding warps
   uint64_t* v_full = k_full + KS;                         // [VS]
   uint64_t* k_empty = v_full + VS;                        // [KS] commit after QK
   uint64_t* v_empty = k_empty + KS;                       // [VS] commit after PV
@@ -370,7 +387,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (uint64_t* bar = bars; bar < p_ready; ++bar) mbar_init(bar, 1);
+    for (uint64_t* bar = bars; bar < p_ready; ++bar) mbar_init(bar, F8 && bar < k_empty ? 2 : 1);      // (of E4M3 caches: two expanding warps)
     mbar_init(&p_ready[0], 4);
     mbar_init(&p_ready[1], 4);
     *abort_flag = 0;
@@ -414,28 +431,21 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
       // PV was over before the scores of this page were.)
       auto tail = [&](int j) {
         const int first = max(d.most - d.key0 - j * SH_PAGE, 0);
-        if (first >= SH_PAGE) return true;
-        if (!all_ok(sh_wait(&v_full[n % VS], (n / VS) & 1, abort_flag, a.status, 104))) return false;
-        for (int i = first * 8 + (int)threadIdx.x; i < SH_PAGE * 8; i += 128)
-#pragma unroll
-          for (int x = 0; x < BOXES; ++x) *reinterpret_cast<uint4*>(v_sm + (n % VS) * TILE + x * 8192 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
-        fence_proxy_async();
-        return true;
+        return first >= SH_PAGE || (all_ok(sh_wait(&v_full[n % VS], (n / VS) & 1, abort_flag, a.status, 104)) && sh_zero_rows(v_sm + (n % VS) * TILE, BOXES, first));
       };
-      // the segment's pages, NC columns a thread: all of a page's scores, or a copy's part of them
-      auto pages = [&](auto nc) {
+      // The segment's pages, NC columns a thread at a time: `parts` times for the 64 / copies scores of a page that are the thread's.  (The code is kept small: the
+      // warps of two CTAs run five programs at once, and where those outgrew the instruction cache, warps waited for it five cycles an instruction.)
+      auto pages = [&](auto nc, int parts) {
         constexpr int NC = decltype(nc)::value;
-        const int col = NC * copy;
+        const int col = NC * parts * copy;
         uint32_t s[NC];
-        auto scores = [&](int at) {                       // the scores of the CTA's page `at`
+        auto scores = [&](int at, int part) {             // of the CTA's page `at`
           tc_fence_after();
-          sh_ld(lane_addr + (at & 1) * C::S_COLS + col, s);
+          sh_ld(lane_addr + (at & 1) * C::S_COLS + col + part * NC, s);
         };
-        if (!all_ok(sh_wait(&s_full[n & 1], (n >> 1) & 1, abort_flag, a.status, 102))) return false;
-        scores(n);
-        for (int j = 0;; ++j, ++n) {
-          const uint32_t s_addr = lane_addr + (n & 1) * C::S_COLS;
-          int seen = keys == 0x7FFFFFFF ? NC : keys - j * SH_PAGE - col;
+        // scores -> probabilities, over the first half of the columns: those have been read
+        auto exponentials = [&](int j, int part) {
+          int seen = keys == 0x7FFFFFFF ? NC : keys - j * SH_PAGE - col - part * NC;
           asm volatile("" : "+r"(seen));                  // (else the bounds of all columns are held in registers over the whole segment)
           if (seen < NC) {
 #pragma unroll
@@ -446,7 +456,8 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
 #pragma unroll
           for (int i = 0; i < NC; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[i]));
           const float ms = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2;
-          // the running maximum moves only by more than 2^8: the probabilities stay below 2^8, harmless in 16-bit operands and fp32 sums
+          // The running maximum moves only by more than 2^8: the probabilities stay below 2^8, harmless in 16-bit operands and fp32 sums.  (A move in a page's second
+          // part comes before the first part's product: those probabilities would be of the old maximum.  So they move with O.)
           const bool moves = ms > m + 8.f;
           if (__any_sync(0xffffffffu, moves)) {           // all pages but a segment's first few: no
             float alpha = 1.f;
@@ -455,16 +466,30 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
               m = ms;
             }
             l *= alpha;
-            if (__any_sync(0xffffffffu, alpha != 1.f)) {  // O, as the PV before leaves it
-              if (!all_ok(sh_wait(&pv_done[(n - 1) & 1], ((n - 1) >> 1) & 1, abort_flag, a.status, 103))) return false;
-              tc_fence_after();
+            if (__any_sync(0xffffffffu, alpha != 1.f)) {
+              if (part > 0) {                             // this page's first probabilities
+                tc_wait_st();
+#pragma unroll 1
+                for (int p = 0; p < part; ++p) {
+                  uint32_t r[NC / 2];
+                  const uint32_t at = lane_addr + (n & 1) * C::S_COLS + (col + p * NC) / 2;
+                  sh_ld(at, r);
 #pragma unroll
-              for (int ch = 0; ch < HD / 16; ++ch) {
-                uint32_t r[16];
-                sh_ld(lane_addr + C::O + ch * 16, r);
+                  for (int i = 0; i < NC / 2; ++i) r[i] = sh_scale<F8>(r[i], alpha);
+                  sh_st(at, r);
+                }
+              }
+              if (j > 0) {                                // O, as the PV before leaves it
+                if (!all_ok(sh_wait(&pv_done[(n - 1) & 1], ((n - 1) >> 1) & 1, abort_flag, a.status, 103))) return false;
+                tc_fence_after();
+#pragma unroll 1
+                for (int ch = 0; ch < HD / 16; ++ch) {
+                  uint32_t r[16];
+                  sh_ld(lane_addr + C::O + ch * 16, r);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
-                sh_st(lane_addr + C::O + ch * 16, r);
+                  for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
+                  sh_st(lane_addr + C::O + ch * 16, r);
+                }
               }
             }
           }
@@ -478,33 +503,39 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             pk[i] = sh_pack<F8>(pa, pb);
           }
           l += (lsum[0] + lsum[1]) + (lsum[2] + lsum[3]);
-          sh_st(s_addr + col / 2, pk);
+          sh_st(lane_addr + (n & 1) * C::S_COLS + (col + part * NC) / 2, pk);
+          return true;
+        };
+        if (!all_ok(sh_wait(&s_full[n & 1], (n >> 1) & 1, abort_flag, a.status, 102))) return false;
+        scores(n, 0);
+        for (int j = 0;; ++j, ++n) {
+#pragma unroll 1
+          for (int part = 0;;) {
+            if (!exponentials(j, part)) return false;
+            if (++part == parts) break;
+            scores(n, part);
+          }
           // the other copies' columns of P
-          if constexpr (NC == 32) sh_st_zero<16>(s_addr + 16 * (1 - copy));
-          if constexpr (NC == 16) {
+          const uint32_t s_addr = lane_addr + (n & 1) * C::S_COLS;
+          if (copies == 2) sh_st_zero<16>(s_addr + 16 * (1 - copy));
+          if (copies == 4) {
 #pragma unroll
             for (int o = 1; o < 4; ++o) sh_st_zero<8>(s_addr + 8 * ((copy + o) & 3));
           }
-          auto done = [&]() {                             // P is there
-            tc_wait_st();
-            tc_fence_before();
-            if (!tail(j)) return false;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_ready[n & 1]);
-            return true;
-          };
-          if (j + 1 == d.pages) {
-            if (!done()) return false;
+          // The next page's scores are fetched while the probabilities are on their way.  (They do not wait for these: the QKs are two pages ahead.)
+          const bool last = j + 1 == d.pages;
+          if (!last) {
+            if (!all_ok(sh_wait(&s_full[(n + 1) & 1], ((n + 1) >> 1) & 1, abort_flag, a.status, 102))) return false;
+            scores(n + 1, 0);
+          }
+          tc_wait_st();
+          tc_fence_before();
+          if (!tail(j)) return false;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_ready[n & 1]);
+          if (last) {
             ++n;
             return true;
-          }
-          // the next page's scores: while the probabilities are on their way, if they are there
-          if (all_ok(mbar_test_wait(&s_full[(n + 1) & 1], ((n + 1) >> 1) & 1))) {
-            scores(n + 1);
-            if (!done()) return false;
-          } else {
-            if (!done() || !all_ok(sh_wait(&s_full[(n + 1) & 1], ((n + 1) >> 1) & 1, abort_flag, a.status, 102))) return false;
-            scores(n + 1);
           }
         }
       };
@@ -515,7 +546,9 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
           __syncwarp();
         }
       } else {
-        ok = copies == 1 ? pages(std::integral_constant<int, 64>()) : copies == 2 ? pages(std::integral_constant<int, 32>()) : pages(std::integral_constant<int, 16>());
+        // 64 / copies = NC * parts
+        if constexpr (F8) ok = copies == 4 ? pages(std::integral_constant<int, 16>(), 1) : pages(std::integral_constant<int, 32>(), 2 / copies);
+        else ok = copies == 1 ? pages(std::integral_constant<int, 64>(), 1) : pages(std::integral_constant<int, 16>(), 4 / copies);
       }
       if (ok) ok = all_ok(sh_wait(&pv_done[(n - 1) & 1], ((n - 1) >> 1) & 1, abort_flag, a.status, 105));
       if (ok && some) {
@@ -523,7 +556,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         const float v_scale = F8 ? a.kv_scale[a.n_kv + d.kvh] : 1.f;
         const size_t at = (size_t)(d.part + rb * d.stride + copy) * a.n_q + hq;
         float4* dst = reinterpret_cast<float4*>(a.part_o + at * HD);
-#pragma unroll
+#pragma unroll 1
         for (int ch = 0; ch < HD / 32; ++ch) {
           uint32_t r[32];
           sh_ld(lane_addr + C::O + ch * 32, r);
@@ -657,19 +690,40 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
       constexpr uint32_t idesc_qk = umma_idesc_f16(SH_PAIRS, SH_PAGE, fmt, fmt);              // both K-major
       constexpr uint32_t idesc_pv = umma_idesc_f16(SH_PAIRS, HD, fmt, fmt) | (1u << 16);      // B (V) is MN-major
       const uint64_t qd = umma_desc_k_sw128(smem_u32(q_sm));
-      int n_qk = 0, seg_qk = 0, left_qk = 0, seg = 0, left = 0;      // pages with a QK, segments begun, pages left of the segment; the PVs' segments and pages
-      bool more = true;
-      // S = Q K^T of the next page, of this segment or the next one
-      auto qk = [&]() {
+      int seg_qk = 0, left_qk = 0, seg = 0, left = 0, pages = 1 << 30;      // segments begun, pages left of the segment, of the QKs and of the PVs; all pages, once known
+      bool ok = true;
+      // round n: PV of page n - 2, then QK of page n into the same buffer (a thread's MMAs run in issue order)
+#pragma unroll 1
+      for (int n = 0; n < pages + 2; ++n) {
+        if (n >= 2) {
+          const int p = n - 2, st = p % VS;
+          const bool fresh = left == 0;
+          if (fresh) left = desc[seg++ & 3].pages;
+          --left;
+          ok = sh_wait(&v_full[st], (p / VS) & 1, abort_flag, a.status, 100) && sh_wait(&p_ready[p & 1], (p >> 1) & 1, abort_flag, a.status, 101);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t vd = sh_desc_v(smem_u32(v_sm + st * TILE), 8192);
+#pragma unroll
+          for (int kk = 0; kk < SH_PAGE / 16; ++kk)
+            tc_mma_f16_ts(tmem_base + C::O, tmem_base + (p & 1) * C::S_COLS + kk * 8, vd + (uint64_t)(kk * (2048 >> 4)), idesc_pv, !fresh || kk != 0);
+          tc_commit(&pv_done[p & 1]);
+          tc_commit(&v_empty[st]);
+        }
+        if (n >= pages) continue;
         if (left_qk == 0) {
-          if (!sh_wait(&q_ready[seg_qk & 3], (seg_qk >> 2) & 1, abort_flag, a.status, 99)) return false;
+          ok = sh_wait(&q_ready[seg_qk & 3], (seg_qk >> 2) & 1, abort_flag, a.status, 99);
+          if (!ok) break;
           left_qk = desc[seg_qk & 3].pages;
-          more = left_qk != 0;
-          if (!more) return true;
+          if (left_qk == 0) {
+            pages = n;                                    // (the PVs of the last two are left)
+            continue;
+          }
           ++seg_qk;
         }
-        const int n = n_qk++, st = n % KS;
-        if (!sh_wait(&k_full[st], (n / KS) & 1, abort_flag, a.status, 98)) return false;
+        const int st = n % KS;
+        ok = sh_wait(&k_full[st], (n / KS) & 1, abort_flag, a.status, 98);
+        if (!ok) break;
         tc_fence_after();
         const uint64_t kd = umma_desc_k_sw128(smem_u32(k_sm + st * TILE));
 #pragma unroll
@@ -679,25 +733,6 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         tc_commit(&s_full[n & 1]);
         tc_commit(&k_empty[st]);
         if (--left_qk == 0) tc_commit(q_free);
-        return true;
-      };
-      bool ok = qk();
-      if (ok && more) ok = qk();
-      for (int n = 0; ok && n < n_qk; ++n) {
-        const int st = n % VS;
-        const bool fresh = left == 0;
-        if (fresh) left = desc[seg++ & 3].pages;
-        --left;
-        ok = sh_wait(&v_full[st], (n / VS) & 1, abort_flag, a.status, 100) && sh_wait(&p_ready[n & 1], (n >> 1) & 1, abort_flag, a.status, 101);
-        if (!ok) break;
-        tc_fence_after();
-        const uint64_t vd = sh_desc_v(smem_u32(v_sm + st * TILE), 8192);
-#pragma unroll
-        for (int kk = 0; kk < SH_PAGE / 16; ++kk)
-          tc_mma_f16_ts(tmem_base + C::O, tmem_base + (n & 1) * C::S_COLS + kk * 8, vd + (uint64_t)(kk * (2048 >> 4)), idesc_pv, !fresh || kk != 0);
-        tc_commit(&pv_done[n & 1]);
-        tc_commit(&v_empty[st]);
-        if (more) ok = qk();                              // into P(n)'s buffer, after PV(n) has read it (a thread's MMAs run in issue order)
       }
       // every MMA issued so far has completed when this commit arrives: the columns may then be returned
       tc_commit(drained);
@@ -705,63 +740,67 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
     }
   } else if constexpr (F8) {
     // ---------------------------------------------------------------- expansion of byte pages: E4M3 -> fp16 (exact) in the operand layout
-    // Straight from global memory: three quarters of a page are on their way in registers while one is expanded.
-    const int v = warp - 6, S = v ? VS : KS;
-    constexpr int QC = SH_PAGE * HD / 16 / 128;           // 16-byte chunks of a quarter page per lane
+    // A warp takes half of every page of K or of V, straight from global memory: the next page's half is on its way in registers while one is expanded, and the id
+    // of the page behind that.
+    const int v = (warp - 6) >> 1, half = warp & 1, S = v ? VS : KS;
+    constexpr int N = SH_PAGE * HD / 16 / 64;             // 16-byte chunks of half a page per lane
     uint64_t *full = v ? v_full : k_full, *empty = v ? v_empty : k_empty;
-    const uint8_t* cache = v ? a.v8 : a.k8;
+    const uint8_t* cache = (v ? a.v8 : a.k8) + half * (SH_PAGE * HD / 2) + lane * 16;
     ShWalk walk(a.plan, a.n_kv);
-    ShSegment sg;
-    bool more = walk.next(sg);
-    int j = 0;
-    // the next page's address (a page outside the cache: zeros)
-    auto page = [&]() -> const uint4* {
-      if (!more) return nullptr;
-      const int id = a.block_table[(size_t)sg.b.seq * a.max_blocks + sg.b.page + sg.page + j];
-      const uint4* p = id >= 0 && id < a.n_pages ? reinterpret_cast<const uint4*>(cache + ((size_t)id * a.n_kv + sg.kvh) * SH_PAGE * HD) : nullptr;
-      if (++j == sg.pages) j = 0, more = walk.next(sg);
-      return p;
+    ShSegment sg = {};
+    const int* table = nullptr;
+    int j = 0, kvh = 0, id = 0;
+    bool any = false;                                     // there is a page behind the one on its way; id, kvh: which
+    auto look = [&]() {
+      if (table == nullptr || ++j == sg.pages) {
+        any = walk.next(sg);
+        j = 0, kvh = sg.kvh;
+        table = a.block_table + (size_t)sg.b.seq * a.max_blocks + sg.b.page + sg.page;
+      }
+      if (any) id = table[j];
     };
-    uint4 b[4][QC];
-    auto load = [&](uint4 (&to)[QC], const uint4* p, int quarter) {
+    auto fetch = [&](uint4 (&to)[N]) {                    // the page that was looked up (one outside the cache: zeros), then looks up the next
+      const uint8_t* p = cache + ((size_t)id * a.n_kv + kvh) * (SH_PAGE * HD);
+      const bool there = any && id >= 0 && id < a.n_pages;
 #pragma unroll
-      for (int i = 0; i < QC; ++i) to[i] = p != nullptr ? __ldg(p + (quarter * QC + i) * 32 + lane) : make_uint4(0u, 0u, 0u, 0u);
+      for (int i = 0; i < N; ++i) to[i] = there ? __ldg(reinterpret_cast<const uint4*>(p + i * 512)) : make_uint4(0u, 0u, 0u, 0u);
+      if (any) look();
     };
-    bool here = more;
-    const uint4* src = page();
-#pragma unroll
-    for (int q = 0; q < 3; ++q) load(b[q], src, q);
     int st = 0, round = 0;
-    while (here) {
-      const bool then = more;
-      const uint4* next = page();
-      if (round > 0 && !all_ok(sh_wait(&empty[st], (round - 1) & 1, abort_flag, a.status, 107))) break;
-      uint8_t* dst = (v ? v_sm : k_sm) + st * TILE;
+    auto expand = [&](const uint4 (&from)[N]) {
+      if (round > 0 && !all_ok(sh_wait(&empty[st], (round - 1) & 1, abort_flag, a.status, 107))) return false;
+      uint8_t* dst = (v ? v_sm : k_sm) + st * TILE + half * 4096;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        if (q == 0) load(b[3], src, 3);
-        else load(b[q - 1], next, q - 1);
+      for (int i = 0; i < N; ++i) {
+        const int c = i * 32 + lane, key = c / (HD / 16), x = c % (HD / 16);
+        const uint32_t w[4] = {from[i].x, from[i].y, from[i].z, from[i].w};
+        uint32_t e[8];
 #pragma unroll
-        for (int i = 0; i < QC; ++i) {
-          const int c = (q * QC + i) * 32 + lane, key = c / (HD / 16), x = c % (HD / 16);
-          const uint32_t w[4] = {b[q][i].x, b[q][i].y, b[q][i].z, b[q][i].w};
-          uint32_t e[8];
+        for (int u = 0; u < 4; ++u)
+          asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(e[2 * u]), "=r"(e[2 * u + 1]) : "r"(w[u]));
 #pragma unroll
-          for (int u = 0; u < 4; ++u)
-            asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(e[2 * u]), "=r"(e[2 * u + 1]) : "r"(w[u]));
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int ch = 2 * x + u;                     // 16-byte chunk of the fp16 row
-            *reinterpret_cast<uint4*>(dst + (ch >> 3) * 8192 + key * 128 + (((ch & 7) ^ (key & 7)) << 4)) = make_uint4(e[4 * u], e[4 * u + 1], e[4 * u + 2], e[4 * u + 3]);
-          }
+        for (int u = 0; u < 2; ++u) {
+          const int ch = 2 * x + u;                       // 16-byte chunk of the fp16 row
+          *reinterpret_cast<uint4*>(dst + (ch >> 3) * 8192 + key * 128 + (((ch & 7) ^ (key & 7)) << 4)) = make_uint4(e[4 * u], e[4 * u + 1], e[4 * u + 2], e[4 * u + 3]);
         }
       }
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(&full[st]);
-      src = next;
-      here = then;
       if (++st == S) st = 0, ++round;
+      return true;
+    };
+    uint4 b[N], next[N];
+    look();
+    bool now = any;
+    fetch(b);
+#pragma unroll 1
+    while (now) {
+      now = any;
+      fetch(next);
+      if (!expand(b)) break;
+#pragma unroll
+      for (int i = 0; i < N; ++i) b[i] = next[i];
     }
   }
   tc_fence_before();
