@@ -16,8 +16,8 @@
 // A page's 64 scores a pair go to tensor memory, come back as exponentials in 16 bits over the same columns, and are the A operand of the product with V.
 // The QKs run two pages ahead of the PVs, also into the next segment.
 //
-// Warps: 0..3 = softmax, 4 = feeder (queries and descriptions of the segments; TMA), 5 = MMA issuer (owns the tensor memory), for E4M3 caches 6, 7 and 8, 9 =
-// expansion of byte pages of K and of V to fp16 operand tiles, in place of TMA.
+// Warps: 0..3 = softmax, 4 = feeder (descriptions of the segments; TMA), 5 = MMA issuer (owns the tensor memory), for E4M3 caches 6, 7 and 8, 9 = expansion of
+// byte pages of K and of V to fp16 operand tiles.
 // A block of up to 64 or 32 pairs would leave two or three quarters idle and the others bound by one warp's exponentials: its queries
 // stand in the tensor memory two or four times, each copy takes its part of a page's keys - the rest of its P is zero - and leaves its own partial output.
 // All waits are bounded (status words), no cluster multicast.
@@ -222,19 +222,20 @@ struct ShArgs {
   const int* block_table;
   const int* plan;
   const float* kv_scale;
-  const uint8_t *k8, *v8;              // E4M3 caches, and their pages
   float* part_o;
   float* part_ml;
   int* status;
-  int max_blocks, n_q, n_kv, n_pages;
+  int max_blocks, n_q, n_kv;
   float scale_log2;
 };
 
 template <int HD, bool F8>
 struct Sh {
   static constexpr int TILE = SH_PAGE * HD * 2, QBOX = SH_PAIRS * 128;      // a page of K or V as an operand; 64 values of all pairs
-  static constexpr int KS = 3, VS = 2;                                      // stages of K, of V
-  static constexpr int SMEM = (KS + VS) * TILE + HD / 64 * QBOX + 512;      // two CTAs an SM: 115,712 bytes at most
+  static constexpr int RAW = SH_PAGE * HD, RS = F8 ? 2 : 0;                 // a byte page; stages of those, of K and of V each
+  static constexpr int KS = F8 ? 1 : 3, VS = 2;                             // stages of operand pages of K, of V
+  static constexpr int KC = F8 ? RS : KS, VC = F8 ? RS : VS, COPY = F8 ? RAW : TILE;      // what the copies fill
+  static constexpr int SMEM = (KS + VS) * TILE + 2 * RS * RAW + HD / 64 * QBOX + 1024;    // two CTAs an SM: 115,712 bytes at most
   static_assert(SMEM <= 115712, "two CTAs an SM");
   static constexpr int THREADS = 32 * (F8 ? 10 : 6);
   static constexpr int S_COLS = 64, O = 128, COLS = 256;                    // tensor memory: two buffers of S (P over the first 32 columns of one) | O
@@ -278,7 +279,7 @@ struct ShWalk {
   }
 };
 
-// What the warps know of a segment; the four last are in shared memory.  pages == 0: there are no more.
+// What the warps know of a segment; the eight last are in shared memory.  pages == 0: there are no more.
 struct ShDesc {
   int row, rows, kvh, key0, pages, part, stride, most;
   const int* table;       // its page ids
@@ -367,10 +368,13 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
   uint8_t* k_sm = smem;                                   // [stage][box (64 d)][64 keys][128 B]
   uint8_t* v_sm = smem + KS * TILE;
   uint8_t* q_sm = smem + (KS + VS) * TILE;                // [box][128 pairs][128 B]
-  uint64_t* bars = (uint64_t*)(q_sm + BOXES * C::QBOX);   // of one arrival each but p_ready
-  uint64_t* k_full = bars;                                // [KS] the copies, or the expanding warps
+  uint8_t* raw = q_sm + BOXES * C::QBOX;                  // [K, V][stage][64 keys][HD]
+  uint64_t* bars = (uint64_t*)(raw + 2 * C::RS * C::RAW);
+  uint64_t* k_full = bars;                                // [KS] the copies, or the two expanding warps
   uint64_t* v_full = k_full + KS;                         // [VS]
-  uint64_t* k_empty = v_full + VS;                        // [KS] commit after QK
+  uint64_t* raw_empty = v_full + VS;                      // [K, V][RS] the two expanding warps
+  uint64_t* raw_full = raw_empty + 2 * C::RS;             // [K, V][RS] the copy
+  uint64_t* k_empty = raw_full + 2 * C::RS;               // [KS] commit after QK
   uint64_t* v_empty = k_empty + KS;                       // [VS] commit after PV
   uint64_t* s_full = v_empty + VS;                        // [2] commit after QK
   uint64_t* pv_done = s_full + 2;                         // [2] commit after PV
@@ -380,23 +384,22 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
   uint64_t* q_there = drained + 1;                        // (E4M3 caches) the queries as they are
   uint64_t* spare = q_there + 1;
   uint64_t* p_ready = spare + 1;                          // [2] the 4 softmax warps
-  ShDesc* desc = (ShDesc*)(p_ready + 2);                  // [4] (behind an even number of words: on a 16-byte boundary)
-  static_assert((2 * (KS + VS)) % 2 == 0, "see desc");
-  uint32_t* tmem_slot = (uint32_t*)(desc + 4);
+  ShDesc* desc = (ShDesc*)(p_ready + 2);                  // [8] (behind an even number of words: on a 16-byte boundary)
+  uint32_t* tmem_slot = (uint32_t*)(desc + 8);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+  volatile int* pages_all = abort_flag + 1;               // (E4M3 caches) pages of the CTA's piece, once the last has been asked for
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (uint64_t* bar = bars; bar < p_ready; ++bar) mbar_init(bar, F8 && bar < k_empty ? 2 : 1);      // (of E4M3 caches: two expanding warps)
+    for (uint64_t* bar = bars; bar < p_ready; ++bar) mbar_init(bar, F8 && bar < raw_full ? 2 : 1);      // (two expanding warps)
     mbar_init(&p_ready[0], 4);
     mbar_init(&p_ready[1], 4);
     *abort_flag = 0;
+    *pages_all = 0x7FFFFFFF;
     fence_barrier_init();
     prefetch_tmap(&tq);
-    if constexpr (!F8) {
-      prefetch_tmap(&tk);
-      prefetch_tmap(&tv);
-    }
+    prefetch_tmap(&tk);
+    prefetch_tmap(&tv);
   }
   if (warp == 5) {
     tmem_alloc(tmem_slot, C::COLS);
@@ -417,7 +420,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
     for (int seg = 0; ok; ++seg) {
       ok = all_ok(sh_wait(&q_ready[seg & 3], (seg >> 2) & 1, abort_flag, a.status, 110));
       if (!ok) break;
-      const ShDesc d = desc[seg & 3];
+      const ShDesc d = desc[seg & 7];
       if (d.pages == 0) break;
       const int pairs = d.rows * G, copies = sh_copies(pairs);
       const int copy = copies == 4 ? warp : copies == 2 ? warp >> 1 : 0, pair = copies == 4 ? lane : copies == 2 ? (warp & 1) * 32 + lane : warp * 32 + lane;
@@ -576,53 +579,51 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
     // One warp's ordinary code is slow (some five cycles an instruction), so it does little of it: a segment is looked up once for everybody, and its
     // queries come by TMA, a row's heads of one KV head per copy (by plain copies, 125 pairs took 25,000 cycles).
     // (With K and V in turn, K page n + 2 waited for V page n + 1 and so for PV(n - 1), and a page took as long as a K page's way from memory.)
-    // Of four descriptions the one that is overwritten, segment w - 4's, is out of use.  bf16: V has begun segment w - 1; that copy waited for the PV of a page two
-    // earlier, in segment w - 3 or later, and that PV for all softmax warps to leave the segment before.  E4M3: the last QK of segment w - 1 is over, which was
-    // issued after the PV of a page two earlier.
+    // Of eight descriptions the one that is overwritten, segment w - 8's, is out of use: V has begun segment w - 1, with a page whose copy waited for the PV of a page
+    // two (E4M3: four) earlier, in segment w - 5 or later, and that PV for all softmax warps to leave the segments before.
     ShWalk walk(a.plan, a.n_kv);
     struct Ring { int seg, j, n; };                       // segment, its next page, pages issued
     Ring ring[2] = {{0, 0, 0}, {0, 0, 0}};
     int known = 0, asked = 0, queries = 0, idle = 0;      // segments with a description, with queries; the last one whose queries were fetched, + 1
     bool more = true;
     uint64_t since = 0;
-    while (more || asked < known || (!F8 && (ring[0].seg < known - 1 || ring[1].seg < known - 1))) {
+    while (more || asked < known || ring[0].seg < known - 1 || ring[1].seg < known - 1) {
       bool moved = false;
-      if constexpr (!F8) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          constexpr int S[2] = {KS, VS};
-          Ring& r = ring[u];
-          const int st = r.n % S[u];
-          uint64_t *full = (u ? v_full : k_full) + st, *empty = (u ? v_empty : k_empty) + st;
-          if (r.seg >= known) continue;
-          const ShDesc& d = desc[r.seg & 3];
-          const int left = d.pages - r.j;
-          if (left == 0 || (r.n >= S[u] && !all_ok(mbar_test_wait(empty, ((r.n / S[u]) - 1) & 1)))) continue;
-          if (elect_one()) {
-            const int y = (d.table[r.j] * a.n_kv + d.kvh) * SH_PAGE;
-            mbar_arrive_expect_tx(full, TILE);
+      for (int u = 0; u < 2; ++u) {
+        constexpr int S[2] = {C::KC, C::VC};
+        Ring& r = ring[u];
+        const int st = r.n % S[u];
+        uint64_t *full = (F8 ? raw_full + u * C::RS : u ? v_full : k_full) + st, *empty = (F8 ? raw_empty + u * C::RS : u ? v_empty : k_empty) + st;
+        if (r.seg >= known) continue;
+        const ShDesc& d = desc[r.seg & 7];
+        const int left = d.pages - r.j;
+        if (left == 0 || (r.n >= S[u] && !all_ok(mbar_test_wait(empty, ((r.n / S[u]) - 1) & 1)))) continue;
+        if (elect_one()) {
+          const int y = (d.table[r.j] * a.n_kv + d.kvh) * SH_PAGE;
+          uint8_t* dst = (F8 ? raw + u * C::RS * C::RAW : u ? v_sm : k_sm) + st * C::COPY;
+          mbar_arrive_expect_tx(full, C::COPY);
 #pragma unroll
-            for (int x = 0; x < BOXES; ++x) tma_load_2d((u ? v_sm : k_sm) + st * TILE + x * 8192, u ? &tv : &tk, x * 64, y, full);
-          }
-          __syncwarp();
-          ++r.n, ++r.j;
-          if (left == 1) ++r.seg, r.j = 0;
-          moved = true;
+          for (int x = 0; x < (F8 ? 1 : BOXES); ++x) tma_load_2d(dst + x * 8192, u ? &tv : &tk, x * 64, y, full);
         }
+        __syncwarp();
+        ++r.n, ++r.j;
+        if (left == 1) ++r.seg, r.j = 0;
+        moved = true;
       }
-      if (more && (known < 4 || (F8 ? asked == known && all_ok(mbar_test_wait(q_free, (known - 1) & 1)) : ring[1].seg >= known || (ring[1].seg == known - 1 && ring[1].j > 0)))) {
+      if (more && (known < 8 || ring[1].seg >= known || (ring[1].seg == known - 1 && ring[1].j > 0))) {
         ShSegment sg;
         more = walk.next(sg);
         const int copies = sh_copies(sg.b.rows * G);
         if (lane == 0)
-          desc[known & 3] = ShDesc{sg.b.row, sg.b.rows, sg.kvh, (sg.b.page + sg.page) * SH_PAGE, more ? sg.pages : 0, sg.b.part + sg.slot * copies, sg.slots * copies, sg.b.most,
+          desc[known & 7] = ShDesc{sg.b.row, sg.b.rows, sg.kvh, (sg.b.page + sg.page) * SH_PAGE, more ? sg.pages : 0, sg.b.part + sg.slot * copies, sg.slots * copies, sg.b.most,
                                    a.block_table + (size_t)sg.b.seq * a.max_blocks + sg.b.page + sg.page, 0};
         __syncwarp();
         ++known;
         moved = true;
       }
       if (asked < known && (asked == 0 || all_ok(mbar_test_wait(q_free, (asked - 1) & 1)))) {
-        const ShDesc& d = desc[asked & 3];
+        const ShDesc& d = desc[asked & 7];
         const int rows = d.pages != 0 ? d.rows : 0, copies = sh_copies(rows * G), bytes = rows * copies * G * HD * 2;
         uint64_t* bar = F8 ? q_there : &q_ready[asked & 3];
         if (lane == 0) {
@@ -673,9 +674,12 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
       }
     }
     if (lane == 0) {
-      if constexpr (!F8) {
-        ring_landed(k_full, KS, ring[0].n);
-        ring_landed(v_full, VS, ring[1].n);
+      ring_landed(F8 ? raw_full : k_full, C::KC, ring[0].n);
+      ring_landed(F8 ? raw_full + C::RS : v_full, C::VC, ring[1].n);
+      if constexpr (F8) {                                 // the expanding warps learn that there are no more
+        *pages_all = ring[0].n;
+        mbar_arrive(&raw_full[ring[0].n % C::RS]);
+        mbar_arrive(&raw_full[C::RS + ring[1].n % C::RS]);
       }
       // (where the others gave up, nobody has waited for the last queries)
       uint64_t* last = F8 ? q_there : &q_ready[(queries - 1) & 3];
@@ -698,7 +702,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         if (n >= 2) {
           const int p = n - 2, st = p % VS;
           const bool fresh = left == 0;
-          if (fresh) left = desc[seg++ & 3].pages;
+          if (fresh) left = desc[seg++ & 7].pages;
           --left;
           ok = sh_wait(&v_full[st], (p / VS) & 1, abort_flag, a.status, 100) && sh_wait(&p_ready[p & 1], (p >> 1) & 1, abort_flag, a.status, 101);
           if (!ok) break;
@@ -714,7 +718,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         if (left_qk == 0) {
           ok = sh_wait(&q_ready[seg_qk & 3], (seg_qk >> 2) & 1, abort_flag, a.status, 99);
           if (!ok) break;
-          left_qk = desc[seg_qk & 3].pages;
+          left_qk = desc[seg_qk & 7].pages;
           if (left_qk == 0) {
             pages = n;                                    // (the PVs of the last two are left)
             continue;
@@ -740,40 +744,22 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
     }
   } else if constexpr (F8) {
     // ---------------------------------------------------------------- expansion of byte pages: E4M3 -> fp16 (exact) in the operand layout
-    // A warp takes half of every page of K or of V, straight from global memory: the next page's half is on its way in registers while one is expanded, and the id
-    // of the page behind that.
+    // A warp takes half of every page of K or of V.  (Straight from global memory, a page ahead in registers, a page took 3300 cycles: the way of plain loads.)
     const int v = (warp - 6) >> 1, half = warp & 1, S = v ? VS : KS;
-    constexpr int N = SH_PAGE * HD / 16 / 64;             // 16-byte chunks of half a page per lane
-    uint64_t *full = v ? v_full : k_full, *empty = v ? v_empty : k_empty;
-    const uint8_t* cache = (v ? a.v8 : a.k8) + half * (SH_PAGE * HD / 2) + lane * 16;
-    ShWalk walk(a.plan, a.n_kv);
-    ShSegment sg = {};
-    const int* table = nullptr;
-    int j = 0, kvh = 0, id = 0;
-    bool any = false;                                     // there is a page behind the one on its way; id, kvh: which
-    auto look = [&]() {
-      if (table == nullptr || ++j == sg.pages) {
-        any = walk.next(sg);
-        j = 0, kvh = sg.kvh;
-        table = a.block_table + (size_t)sg.b.seq * a.max_blocks + sg.b.page + sg.page;
-      }
-      if (any) id = table[j];
-    };
-    auto fetch = [&](uint4 (&to)[N]) {                    // the page that was looked up (one outside the cache: zeros), then looks up the next
-      const uint8_t* p = cache + ((size_t)id * a.n_kv + kvh) * (SH_PAGE * HD);
-      const bool there = any && id >= 0 && id < a.n_pages;
-#pragma unroll
-      for (int i = 0; i < N; ++i) to[i] = there ? __ldg(reinterpret_cast<const uint4*>(p + i * 512)) : make_uint4(0u, 0u, 0u, 0u);
-      if (any) look();
-    };
-    int st = 0, round = 0;
-    auto expand = [&](const uint4 (&from)[N]) {
-      if (round > 0 && !all_ok(sh_wait(&empty[st], (round - 1) & 1, abort_flag, a.status, 107))) return false;
-      uint8_t* dst = (v ? v_sm : k_sm) + st * TILE + half * 4096;
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int c = i * 32 + lane, key = c / (HD / 16), x = c % (HD / 16);
-        const uint32_t w[4] = {from[i].x, from[i].y, from[i].z, from[i].w};
+    uint64_t *full = v ? v_full : k_full, *empty = v ? v_empty : k_empty, *rfull = raw_full + v * C::RS, *rempty = raw_empty + v * C::RS;
+    for (int n = 0;; ++n) {
+      const int rs = n % C::RS, st = n % S;
+      if (!all_ok(sh_wait(&rfull[rs], (n / C::RS) & 1, abort_flag, a.status, 106)) || n >= *pages_all) break;
+      if (n >= S && !all_ok(sh_wait(&empty[st], ((n / S) - 1) & 1, abort_flag, a.status, 107))) break;
+      const uint32_t src = smem_u32(raw + (v * C::RS + rs) * C::RAW);
+      uint8_t* dst = (v ? v_sm : k_sm) + st * TILE;
+#pragma unroll 4
+      for (int i = 0; i < HD / 16; ++i) {
+        // eight lanes take two keys, of 128-byte rows a half each: neither loads nor stores then meet in a bank
+        const int key = half * 32 + (HD == 128 ? (i >> 1) * 8 + (lane >> 3) * 2 + (lane >> 2 & 1) : i * 8 + (lane >> 2));
+        const int x = (lane & 3) + (HD == 128 ? 4 * ((lane >> 2 & 1) ^ (i & 1)) : 0);
+        const uint4 b = lds128(src + key * HD + x * 16);
+        const uint32_t w[4] = {b.x, b.y, b.z, b.w};
         uint32_t e[8];
 #pragma unroll
         for (int u = 0; u < 4; ++u)
@@ -786,21 +772,10 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
       }
       fence_proxy_async();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&full[st]);
-      if (++st == S) st = 0, ++round;
-      return true;
-    };
-    uint4 b[N], next[N];
-    look();
-    bool now = any;
-    fetch(b);
-#pragma unroll 1
-    while (now) {
-      now = any;
-      fetch(next);
-      if (!expand(b)) break;
-#pragma unroll
-      for (int i = 0; i < N; ++i) b[i] = next[i];
+      if (lane == 0) {
+        mbar_arrive(&full[st]);
+        mbar_arrive(&rempty[rs]);
+      }
     }
   }
   tc_fence_before();
@@ -913,13 +888,12 @@ RX_API int rx_attn_shared_plan(const void* row_seq, const void* ctx_len, const v
                          n_tables, max_blocks, n_q / n_kv, n_kv, (int*)plan, status);
 }
 
-// scratch: rx_attn_shared_scratch_floats floats, 16-byte aligned.  plan == nullptr: the call plans into the scratch.  kv_scale == nullptr: bf16 caches by their tensor
-// maps; else E4M3 caches of n_pages pages at k8, v8.
+// scratch: rx_attn_shared_scratch_floats floats, 16-byte aligned.  plan == nullptr: the call plans into the scratch.  kv_scale == nullptr: bf16 caches.
 RX_API int rx_attn_shared(const void* tmap_k, const void* tmap_v, const void* q, const void* block_table, int n_tables, int max_blocks, const void* row_seq,
                           const void* ctx_len, const void* common, void* scratch, int rows, int n_q, int n_kv, int hd, float scale, const void* kv_scale,
-                          const void* suh, void* xr, void* out, const void* plan, const void* k8, const void* v8, int n_pages, int* status, void* stream) {
+                          const void* suh, void* xr, void* out, const void* plan, int* status, void* stream) {
   if (!sh_takes(rows, n_q, n_kv, n_tables, max_blocks) || (hd != 64 && hd != 128) || n_q * hd % 128 != 0 || (out == nullptr && xr == nullptr) ||
-      (suh == nullptr) != (xr == nullptr) || (kv_scale != nullptr && (k8 == nullptr || v8 == nullptr || n_pages < 0)))
+      (suh == nullptr) != (xr == nullptr))
     return (int)cudaErrorInvalidValue;
   cudaStream_t st = (cudaStream_t)stream;
   int dev = 0;
@@ -931,7 +905,6 @@ RX_API int rx_attn_shared(const void* tmap_k, const void* tmap_v, const void* q,
   int* own_plan = (int*)(a.part_ml + vectors * 2);
   own_plan = (int*)(((uintptr_t)own_plan + 15) & ~(uintptr_t)15);
   a.block_table = (const int*)block_table; a.plan = plan != nullptr ? (const int*)plan : own_plan;
-  a.k8 = (const uint8_t*)k8; a.v8 = (const uint8_t*)v8; a.n_pages = n_pages;
   a.kv_scale = (const float*)kv_scale; a.status = status; a.max_blocks = max_blocks; a.n_q = n_q; a.n_kv = n_kv; a.scale_log2 = scale * 1.4426950408889634f;
   if (plan == nullptr) {
     const int r = rx_attn_shared_plan(row_seq, ctx_len, common, rows, n_tables, max_blocks, n_q, n_kv, own_plan, status, stream);

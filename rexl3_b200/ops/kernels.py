@@ -644,8 +644,7 @@ def attn_shared(tk: KvTensorMap, tv: KvTensorMap, q, block_table, row_seq, ctx_l
     if (p_q | p_scratch | (p_plan or 0)) & 15 or ((p_out or 0) | (p_xr or 0)) & 7:
         raise ValueError("q, scratch and plan begin on 16-byte boundaries, out and xr on 8-byte ones")
     _lib.check(L.rx_attn_shared(tk.rows_ptr, tv.rows_ptr, p_q, p[0], block_table.shape[0], block_table.shape[1], p[1], p[2], p[3], p_scratch, rows, n_q, n_kv, hd, scale,
-                                p_scale, p_suh, p_xr, p_out, p_plan, tk._keep.data_ptr(), tv._keep.data_ptr(), min(tk._keep.shape[0], tv._keep.shape[0]), p[4],
-                                _lib.stream_ptr()), "rx_attn_shared")
+                                p_scale, p_suh, p_xr, p_out, p_plan, p[4], _lib.stream_ptr()), "rx_attn_shared")
     _lib.count(2 if plan is not None else 3)
 
 

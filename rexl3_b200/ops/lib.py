@@ -110,7 +110,7 @@ def _declare(lib):
         "rx_tp_cand_push": (c_int, [c_void, c_void, c_int, c_int, c_void, c_void]),
         "rx_tp_cand_merge": (c_int, [c_void, c_void, c_void, c_int, c_int, c_int, c_int, c_void, ctypes.c_uint, c_void, c_void, c_void, c_void]),
         "rx_ssm_mixer": (c_int, [c_void, c_int, c_int, c_int, c_int, c_int, c_int, c_void, c_void, c_void, c_void, c_int, c_void, c_void, c_void, c_void,
-                                 c_void, c_void, c_f, c_void, c_void, c_void, c_void, c_void, c_void, c_int, c_void, c_void]),
+                                 c_void, c_void, c_f, c_void, c_void, c_void, c_void, c_void, c_void]),
         "rx_gdn_mixer": (c_int, [c_void, c_int, c_int, c_int, c_int, c_int, c_void, c_void, c_void, c_void, c_int, c_void, c_void, c_void, c_void, c_void,
                                  c_f, c_void, c_void, c_void, c_void, c_void, c_int, c_int, c_void, c_void, c_void]),
         "rx_dev_alloc": (c_int, [c_ll, ctypes.POINTER(ctypes.c_void_p)]),
@@ -142,7 +142,7 @@ def _declare(lib):
         "rx_attn_shared_scratch_floats": (c_ll, [c_int, c_int, c_int, c_int]),
         "rx_attn_shared_plan": (c_int, [c_void, c_void, c_void, c_int, c_int, c_int, c_int, c_int, c_void, c_void, c_void]),
         "rx_attn_shared": (c_int, [c_void, c_void, c_void, c_void, c_int, c_int, c_void, c_void, c_void, c_void, c_int, c_int, c_int, c_int, c_f, c_void, c_void,
-                                   c_void, c_void, c_void, c_void, c_void, c_int, c_void, c_void]),
+                                   c_void, c_void, c_void, c_void, c_void]),
         "rx_make_kv_tmap": (c_int, [c_void, c_void, c_ll, c_int]),
         "rx_make_kv_tmap8": (c_int, [c_void, c_void, c_ll, c_int]),
         "rx_make_kv_tmap_f8": (c_int, [c_void, c_void, c_ll, c_int]),
