@@ -36,7 +36,7 @@ constexpr int SH_SEGMENT = 2;                           // what a unit costs bes
 // Layout (int32): [0] length of the line  [1] a CTA's piece  [2] blocks  [3] n_kv, then the block at which each CTA begins, the blocks, and per row its
 // block over common pages, its block over own pages (-1: none), the keys it sees and nothing.
 struct ShBlock {
-  int row, rows;          // first row, rows
+  int row, rows;          // first row; rows, and << 8 how many CTAs a unit can meet
   int seq;                // table row
   int page, pages;        // first page, pages
   int before;             // length of the blocks before (times n_kv: where the block's units begin in the line)
@@ -140,13 +140,13 @@ __global__ void __launch_bounds__(SH_MAX_ROWS) shared_plan_kernel(const int* __r
   if (lead_s) {
     const int id = (b_in & 0xFFFF) - 1;
     s_link[r] = id, s_before[id] = p_s - len_s;
-    blk[id] = ShBlock{r, n_s, s_seq[gfirst], 0, shared, p_s - len_s, v_s - k_s, s_gmost[group]};
+    blk[id] = ShBlock{r, n_s | sh_slots(shared, L) << 8, s_seq[gfirst], 0, shared, p_s - len_s, v_s - k_s, s_gmost[group]};
   }
   __syncthreads();
   if (lead_o) {
     const int id = nb_s + (b_in >> 16) - 1;
     s_seq[r] = id, s_before[id] = pages_s + p_o - len_o;
-    blk[id] = ShBlock{r, n_o, seq, shared, own, pages_s + p_o - len_o, all_s + v_o - k_o, s_most[chunk]};
+    blk[id] = ShBlock{r, n_o | sh_slots(own, L) << 8, seq, shared, own, pages_s + p_o - len_o, all_s + v_o - k_o, s_most[chunk]};
   }
   __syncthreads();
   if (live) {
@@ -244,35 +244,40 @@ struct Sh {
 // a wait's outcome for the whole warp: what follows it is done by all lanes or by none
 __device__ __forceinline__ bool all_ok(bool ok) { return __all_sync(0xffffffffu, ok); }
 
-struct ShSegment { ShBlock b; int kvh, page, pages, slot, slots; };          // a CTA's pages of one unit
-// The CTA's piece of the line as segments.
+// The CTA's piece of the line as segments: its pages of one unit each.
+struct ShSegment { int row, rows, slots, seq, kvh, page, pages, slot, part, most; };
 struct ShWalk {
-  const ShBlock* blk;
-  int b, pos, end, L, n_kv;
+  const int4* blk;
+  int4 x, y, nx, ny;                                                        // the block and the one behind it, on its way
+  int b, last, kvh, pos, end, n_kv, L;
+  __device__ __forceinline__ void fetch() {
+    const int at = min(b + 1, last) * 2;
+    nx = blk[at], ny = blk[at + 1];
+  }
   __device__ __forceinline__ ShWalk(const int* plan, int n_kv_) : n_kv(n_kv_) {
     const int total = plan[0];
-    L = plan[1];
-    blk = reinterpret_cast<const ShBlock*>(plan + SH_AT_BLOCKS);
+    L = plan[1], last = plan[2] - 1;
+    blk = reinterpret_cast<const int4*>(plan + SH_AT_BLOCKS);
     pos = (int)min((long long)total, (long long)blockIdx.x * L), end = (int)min((long long)total, (long long)pos + L);
     b = plan[SH_HEAD + blockIdx.x];
+    if (pos >= end) return;
+    x = blk[2 * b], y = blk[2 * b + 1];
+    fetch();
+    kvh = (pos - y.y * n_kv) / (y.x + SH_SEGMENT);                          // (the plan gives the block that holds the piece's begin)
   }
   __device__ __forceinline__ bool next(ShSegment& s) {
     while (pos < end) {
-      const int4* p = reinterpret_cast<const int4*>(blk + b);
-      int4 x = p[0], y = p[1];
-      int rel = pos - y.y * n_kv;
-      if (rel >= (y.x + SH_SEGMENT) * n_kv) {                               // the block is done
-        p = reinterpret_cast<const int4*>(blk + ++b);
-        x = p[0], y = p[1];
-        rel = pos - y.y * n_kv;
+      const int len = y.x + SH_SEGMENT, unit = y.y * n_kv + kvh * len + SH_SEGMENT, stop = min(end, unit + y.x);
+      s.page = max(pos - unit, 0), s.pages = stop - max(pos, unit);
+      // a unit that begins in this piece meets this CTA first
+      s.slot = s.page > 0 ? (int)blockIdx.x - unit / L : 0;
+      s.row = x.x, s.rows = x.y & 255, s.slots = x.y >> 8, s.seq = x.z, s.page += x.w, s.kvh = kvh, s.part = y.z, s.most = y.w;
+      pos = unit + y.x;
+      if (++kvh == n_kv) {
+        kvh = 0, ++b;
+        x = nx, y = ny;
+        fetch();
       }
-      s.b = ShBlock{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-      s.kvh = rel / (s.b.pages + SH_SEGMENT);
-      const int unit = sh_unit(s.b, s.kvh, n_kv), stop = min(end, unit + s.b.pages);
-      pos = max(pos, unit);
-      s.page = pos - unit, s.pages = stop - pos;
-      s.slot = (int)blockIdx.x - unit / L, s.slots = sh_slots(s.b.pages, L);
-      pos = max(pos, stop);
       if (s.pages > 0) return true;                                         // (else the piece ended before the unit's first page)
     }
     return false;
@@ -322,6 +327,14 @@ __device__ __forceinline__ void sh_ld(uint32_t taddr, uint32_t (&r)[N]) {
                    "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                  : "r"(taddr)
                  : "memory");
+}
+// 32 columns of 16 lanes: thread t has columns 8 k + 2 (t % 4) and the next of lane t / 4 in r[4 k], r[4 k + 1] and of lane t / 4 + 8 in r[4 k + 2], r[4 k + 3]
+__device__ __forceinline__ void sh_ld_16x256b_x4(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+                 "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(taddr)
+               : "memory");
 }
 template <int N>
 __device__ __forceinline__ void sh_st(uint32_t taddr, const uint32_t (&r)[N]) {
@@ -557,20 +570,30 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
       if (ok && some) {
         tc_fence_after();
         const float v_scale = F8 ? a.kv_scale[a.n_kv + d.kvh] : 1.f;
-        const size_t at = (size_t)(d.part + rb * d.stride + copy) * a.n_q + hq;
-        float4* dst = reinterpret_cast<float4*>(a.part_o + at * HD);
+        const int at = live ? (d.part + rb * d.stride + copy) * a.n_q + hq : -1;
+        if (live) *reinterpret_cast<float2*>(a.part_ml + (size_t)at * 2) = make_float2(m, l);
+        // Eight lanes' rows by four lanes each: two neighbouring lanes swap pairs, so that a store writes 64 bytes of each of eight rows.  (A row by its own thread, 32
+        // rows a store, took 6300 cycles a segment.)
 #pragma unroll 1
-        for (int ch = 0; ch < HD / 32; ++ch) {
-          uint32_t r[32];
-          sh_ld(lane_addr + C::O + ch * 32, r);
-          if (live) {
+        for (int ch = 0; ch < HD / 16; ++ch) {
+          const int cols = ch >> 1, h = ch & 1;           // 32 columns of the upper or lower 16 rows
+          uint32_t r[16];
+          sh_ld_16x256b_x4(lane_addr + ((uint32_t)(h * 16) << 16) + C::O + cols * 32, r);
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              dst[ch * 8 + i] = make_float4(__uint_as_float(r[4 * i]) * v_scale, __uint_as_float(r[4 * i + 1]) * v_scale, __uint_as_float(r[4 * i + 2]) * v_scale,
-                                            __uint_as_float(r[4 * i + 3]) * v_scale);
+          for (int u = 0; u < 2; ++u) {
+            const int row = __shfl_sync(0xffffffffu, at, h * 16 + u * 8 + (lane >> 2));
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {                 // r[8 k + 2 u ..]: columns 16 k + 2 (lane % 4) ..; r[8 k + 4 + 2 u ..]: eight further
+              const uint32_t a0 = r[8 * k + 2 * u], a1 = r[8 * k + 2 * u + 1], b0 = r[8 * k + 4 + 2 * u], b1 = r[8 * k + 5 + 2 * u];
+              const bool odd = lane & 1;
+              const uint32_t g0 = __shfl_xor_sync(0xffffffffu, odd ? a0 : b0, 1), g1 = __shfl_xor_sync(0xffffffffu, odd ? a1 : b1, 1);
+              if (row >= 0)
+                *reinterpret_cast<float4*>(a.part_o + (size_t)row * HD + cols * 32 + k * 16 + (odd ? 8 : 0) + (lane & 2) * 2) =
+                    make_float4(__uint_as_float(odd ? g0 : a0) * v_scale, __uint_as_float(odd ? g1 : a1) * v_scale, __uint_as_float(odd ? b0 : g0) * v_scale,
+                                __uint_as_float(odd ? b1 : g1) * v_scale);
+            }
           }
         }
-        if (live) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m, l);
         tc_fence_before();                                // the reads of O are ordered before the next segment's first PV by p_ready
       }
     }
@@ -611,17 +634,6 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         if (left == 1) ++r.seg, r.j = 0;
         moved = true;
       }
-      if (more && (known < 8 || ring[1].seg >= known || (ring[1].seg == known - 1 && ring[1].j > 0))) {
-        ShSegment sg;
-        more = walk.next(sg);
-        const int copies = sh_copies(sg.b.rows * G);
-        if (lane == 0)
-          desc[known & 7] = ShDesc{sg.b.row, sg.b.rows, sg.kvh, (sg.b.page + sg.page) * SH_PAGE, more ? sg.pages : 0, sg.b.part + sg.slot * copies, sg.slots * copies, sg.b.most,
-                                   a.block_table + (size_t)sg.b.seq * a.max_blocks + sg.b.page + sg.page, 0};
-        __syncwarp();
-        ++known;
-        moved = true;
-      }
       if (asked < known && (asked == 0 || all_ok(mbar_test_wait(q_free, (asked - 1) & 1)))) {
         const ShDesc& d = desc[asked & 7];
         const int rows = d.pages != 0 ? d.rows : 0, copies = sh_copies(rows * G), bytes = rows * copies * G * HD * 2;
@@ -660,6 +672,17 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         ++asked;
         moved = true;
       }
+      if (more && (known < 8 || ring[1].seg >= known || (ring[1].seg == known - 1 && ring[1].j > 0))) {
+        ShSegment sg = {};
+        more = walk.next(sg);
+        const int copies = sh_copies(sg.rows * G);
+        if (lane == 0)
+          desc[known & 7] = ShDesc{sg.row, sg.rows, sg.kvh, sg.page * SH_PAGE, more ? sg.pages : 0, sg.part + sg.slot * copies, sg.slots * copies, sg.most,
+                                   a.block_table + (size_t)sg.seq * a.max_blocks + sg.page, 0};
+        __syncwarp();
+        ++known;
+        moved = true;
+      }
       if (moved) {
         idle = 0;
       } else if (++idle > 16) {
@@ -694,18 +717,43 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
       constexpr uint32_t idesc_qk = umma_idesc_f16(SH_PAIRS, SH_PAGE, fmt, fmt);              // both K-major
       constexpr uint32_t idesc_pv = umma_idesc_f16(SH_PAIRS, HD, fmt, fmt) | (1u << 16);      // B (V) is MN-major
       const uint64_t qd = umma_desc_k_sw128(smem_u32(q_sm));
-      int seg_qk = 0, left_qk = 0, seg = 0, left = 0, pages = 1 << 30;      // segments begun, pages left of the segment, of the QKs and of the PVs; all pages, once known
-      bool ok = true;
-      // round n: PV of page n - 2, then QK of page n into the same buffer (a thread's MMAs run in issue order)
+      // Whatever can go on first goes: the next page's QK, up to two pages ahead of the PVs and into the next segment, or the next PV.  (In a fixed order, the PV of a
+      // segment's last page stood behind the next segment's queries.)
+      int n = 0, p = 0, seg_qk = 0, left_qk = 0, seg = 0, left = 0, idle = 0;      // pages with a QK, with a PV; segments begun and pages left of the segment, of each
+      bool more = true;
+      uint64_t since = 0;
 #pragma unroll 1
-      for (int n = 0; n < pages + 2; ++n) {
-        if (n >= 2) {
-          const int p = n - 2, st = p % VS;
+      while (more || p < n) {
+        if (more && n - p < 2) {
+          if (left_qk == 0 && mbar_test_wait(&q_ready[seg_qk & 3], (seg_qk >> 2) & 1)) {
+            left_qk = desc[seg_qk & 7].pages;
+            if (left_qk == 0) {
+              more = false;
+              continue;
+            }
+            ++seg_qk;
+          }
+          const int st = n % KS;
+          if (left_qk != 0 && mbar_test_wait(&k_full[st], (n / KS) & 1)) {
+            tc_fence_after();
+            const uint64_t kd = umma_desc_k_sw128(smem_u32(k_sm + st * TILE));
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; ++kk)
+              tc_mma_f16(tmem_base + (n & 1) * C::S_COLS, qd + (uint64_t)((kk >> 2) * (C::QBOX >> 4) + (kk & 3) * 2), kd + (uint64_t)((kk >> 2) * (8192 >> 4) + (kk & 3) * 2),
+                         idesc_qk, kk != 0);
+            tc_commit(&s_full[n & 1]);                    // (over P(n - 2), which its PV has read: a thread's MMAs run in issue order)
+            tc_commit(&k_empty[st]);
+            if (--left_qk == 0) tc_commit(q_free);
+            ++n;
+            idle = 0;
+            continue;
+          }
+        }
+        const int st = p % VS;
+        if (p < n && mbar_test_wait(&p_ready[p & 1], (p >> 1) & 1) && mbar_test_wait(&v_full[st], (p / VS) & 1)) {
           const bool fresh = left == 0;
           if (fresh) left = desc[seg++ & 7].pages;
           --left;
-          ok = sh_wait(&v_full[st], (p / VS) & 1, abort_flag, a.status, 100) && sh_wait(&p_ready[p & 1], (p >> 1) & 1, abort_flag, a.status, 101);
-          if (!ok) break;
           tc_fence_after();
           const uint64_t vd = sh_desc_v(smem_u32(v_sm + st * TILE), 8192);
 #pragma unroll
@@ -713,30 +761,16 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             tc_mma_f16_ts(tmem_base + C::O, tmem_base + (p & 1) * C::S_COLS + kk * 8, vd + (uint64_t)(kk * (2048 >> 4)), idesc_pv, !fresh || kk != 0);
           tc_commit(&pv_done[p & 1]);
           tc_commit(&v_empty[st]);
+          ++p;
+          idle = 0;
+          continue;
         }
-        if (n >= pages) continue;
-        if (left_qk == 0) {
-          ok = sh_wait(&q_ready[seg_qk & 3], (seg_qk >> 2) & 1, abort_flag, a.status, 99);
-          if (!ok) break;
-          left_qk = desc[seg_qk & 7].pages;
-          if (left_qk == 0) {
-            pages = n;                                    // (the PVs of the last two are left)
-            continue;
-          }
-          ++seg_qk;
+        if ((++idle & 4095) == 0) {                       // (bounded, as mbar_wait is)
+          if (idle == 4096) since = globaltimer_ns();
+          const bool stop = host_abort(a.status), late = globaltimer_ns() - since > wait_limit_ns(a.status);
+          if (stop || late) set_status(a.status, stop ? ST_ABORTED : ST_TIMEOUT, 98, n), *abort_flag = 1;
+          if (*abort_flag != 0) break;
         }
-        const int st = n % KS;
-        ok = sh_wait(&k_full[st], (n / KS) & 1, abort_flag, a.status, 98);
-        if (!ok) break;
-        tc_fence_after();
-        const uint64_t kd = umma_desc_k_sw128(smem_u32(k_sm + st * TILE));
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk)
-          tc_mma_f16(tmem_base + (n & 1) * C::S_COLS, qd + (uint64_t)((kk >> 2) * (C::QBOX >> 4) + (kk & 3) * 2), kd + (uint64_t)((kk >> 2) * (8192 >> 4) + (kk & 3) * 2),
-                     idesc_qk, kk != 0);
-        tc_commit(&s_full[n & 1]);
-        tc_commit(&k_empty[st]);
-        if (--left_qk == 0) tc_commit(q_free);
       }
       // every MMA issued so far has completed when this commit arrives: the columns may then be returned
       tc_commit(drained);
@@ -803,9 +837,9 @@ __global__ void __launch_bounds__(128) attn_shared_merge_kernel(const int* plan,
     const int id = plan[SH_AT_ROWS + 4 * row + u];
     if (id < 0) continue;
     const ShBlock s = blk[id];
-    const int unit = sh_unit(s, kvh, n_kv), copies = sh_copies(s.rows * (n_q / n_kv));
+    const int unit = sh_unit(s, kvh, n_kv), copies = sh_copies((s.rows & 255) * (n_q / n_kv));
     n[u] = ((unit + s.pages - 1) / L - unit / L + 1) * copies;
-    at[u] = (size_t)(s.part + (row - s.row) * sh_slots(s.pages, L) * copies) * n_q + hq;
+    at[u] = (size_t)(s.part + (row - s.row) * (s.rows >> 8) * copies) * n_q + hq;
   }
   auto slot = [&](int s) { return s < n[0] ? at[0] + (size_t)s * n_q : at[1] + (size_t)(s - n[0]) * n_q; };
   const int all = n[0] + n[1];
