@@ -474,7 +474,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
           const float ms = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2;
           // The running maximum moves only by more than 2^8: the probabilities stay below 2^8, harmless in 16-bit operands and fp32 sums.  (A move in a page's second
           // part comes before the first part's product: those probabilities would be of the old maximum.  So they move with O.)
-          const bool moves = ms > m + 8.f;
+          const bool moves = live && ms > m + 8.f;        // (a lane without a pair has another's old queries, or none: its scores may be anything)
           if (__any_sync(0xffffffffu, moves)) {           // all pages but a segment's first few: no
             float alpha = 1.f;
             if (moves) {
