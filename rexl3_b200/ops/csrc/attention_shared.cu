@@ -605,35 +605,38 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
     // Of eight descriptions the one that is overwritten, segment w - 8's, is out of use: V has begun segment w - 1, with a page whose copy waited for the PV of a page
     // two (E4M3: four) earlier, in segment w - 5 or later, and that PV for all softmax warps to leave the segments before.
     ShWalk walk(a.plan, a.n_kv);
-    struct Ring { int seg, j, n; };                       // segment, its next page, pages issued
-    Ring ring[2] = {{0, 0, 0}, {0, 0, 0}};
     int known = 0, asked = 0, queries = 0, idle = 0;      // segments with a description, with queries; the last one whose queries were fetched, + 1
     bool more = true;
     uint64_t since = 0;
-    while (more || asked < known || ring[0].seg < known - 1 || ring[1].seg < known - 1) {
+    // lane 0 brings K, lane 1 V: the ring's place, and the pages that are left of the lane's segment
+    const int S = lane == 0 ? C::KC : C::VC, who = lane & 1;
+    uint64_t *full = F8 ? raw_full + who * C::RS : who ? v_full : k_full, *empty = F8 ? raw_empty + who * C::RS : who ? v_empty : k_empty;
+    uint8_t* to = F8 ? raw + who * C::RS * C::RAW : who ? v_sm : k_sm;
+    const CUtensorMap* map = who ? &tv : &tk;
+    const int* table = nullptr;
+    int at = 0, begun = 0, st = 0, round = 0, left = 0, kvh = 0, copied = 0;      // segments looked at, and begun; the ring's place; pages left of the segment, asked for
+    bool done = lane > 1;
+    while (more || asked < known || __any_sync(0xffffffffu, !done)) {
       bool moved = false;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        constexpr int S[2] = {C::KC, C::VC};
-        Ring& r = ring[u];
-        const int st = r.n % S[u];
-        uint64_t *full = (F8 ? raw_full + u * C::RS : u ? v_full : k_full) + st, *empty = (F8 ? raw_empty + u * C::RS : u ? v_empty : k_empty) + st;
-        if (r.seg >= known) continue;
-        const ShDesc& d = desc[r.seg & 7];
-        const int left = d.pages - r.j;
-        if (left == 0 || (r.n >= S[u] && !all_ok(mbar_test_wait(empty, ((r.n / S[u]) - 1) & 1)))) continue;
-        if (elect_one()) {
-          const int y = (d.table[r.j] * a.n_kv + d.kvh) * SH_PAGE;
-          uint8_t* dst = (F8 ? raw + u * C::RS * C::RAW : u ? v_sm : k_sm) + st * C::COPY;
-          mbar_arrive_expect_tx(full, C::COPY);
-#pragma unroll
-          for (int x = 0; x < (F8 ? 1 : BOXES); ++x) tma_load_2d(dst + x * 8192, u ? &tv : &tk, x * 64, y, full);
+      if (!done) {
+        if (left == 0 && at < known) {
+          const ShDesc& d = desc[at & 7];
+          left = d.pages, table = d.table, kvh = d.kvh;
+          done = left == 0;
+          ++at;
         }
-        __syncwarp();
-        ++r.n, ++r.j;
-        if (left == 1) ++r.seg, r.j = 0;
-        moved = true;
+        if (left != 0 && (round == 0 || mbar_test_wait(&empty[st], (round - 1) & 1))) {
+          const int y = (*table * a.n_kv + kvh) * SH_PAGE;
+          mbar_arrive_expect_tx(&full[st], C::COPY);
+#pragma unroll
+          for (int x = 0; x < (F8 ? 1 : BOXES); ++x) tma_load_2d(to + st * C::COPY + x * 8192, map, x * 64, y, &full[st]);
+          ++table, --left, ++copied;
+          begun = at;
+          if (++st == S) st = 0, ++round;
+          moved = true;
+        }
       }
+      __syncwarp();
       if (asked < known && (asked == 0 || all_ok(mbar_test_wait(q_free, (asked - 1) & 1)))) {
         const ShDesc& d = desc[asked & 7];
         const int rows = d.pages != 0 ? d.rows : 0, copies = sh_copies(rows * G), bytes = rows * copies * G * HD * 2;
@@ -672,7 +675,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         ++asked;
         moved = true;
       }
-      if (more && (known < 8 || ring[1].seg >= known || (ring[1].seg == known - 1 && ring[1].j > 0))) {
+      if (more && (known < 8 || __shfl_sync(0xffffffffu, begun, 1) >= known)) {
         ShSegment sg = {};
         more = walk.next(sg);
         const int copies = sh_copies(sg.rows * G);
@@ -683,12 +686,12 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         ++known;
         moved = true;
       }
-      if (moved) {
+      if (__any_sync(0xffffffffu, moved)) {
         idle = 0;
-      } else if (++idle > 16) {
-        __nanosleep(40);
-        if ((idle & 255) == 0) {                          // (a bounded wait, as mbar_wait's, for whatever can go on first)
-          if (idle == 256) since = globaltimer_ns();
+      } else if (++idle > 64) {
+        __nanosleep(20);
+        if ((idle & 511) == 0) {                          // (a bounded wait, as mbar_wait's, for whatever can go on first)
+          if (idle == 512) since = globaltimer_ns();
           const bool stop = host_abort(a.status), late = globaltimer_ns() - since > wait_limit_ns(a.status);
           if (lane == 0 && (stop || late)) set_status(a.status, stop ? ST_ABORTED : ST_TIMEOUT, 96), *abort_flag = 1;
           __syncwarp();
@@ -696,14 +699,16 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         }
       }
     }
-    if (lane == 0) {
-      ring_landed(F8 ? raw_full : k_full, C::KC, ring[0].n);
-      ring_landed(F8 ? raw_full + C::RS : v_full, C::VC, ring[1].n);
+    __syncwarp();
+    if (lane < 2) {
+      ring_landed(full, S, copied);
       if constexpr (F8) {                                 // the expanding warps learn that there are no more
-        *pages_all = ring[0].n;
-        mbar_arrive(&raw_full[ring[0].n % C::RS]);
-        mbar_arrive(&raw_full[C::RS + ring[1].n % C::RS]);
+        if (lane == 0) *pages_all = copied;
+        __syncwarp(3);
+        mbar_arrive(&full[st]);
       }
+    }
+    if (lane == 0) {
       // (where the others gave up, nobody has waited for the last queries)
       uint64_t* last = F8 ? q_there : &q_ready[(queries - 1) & 3];
       const int parity = (F8 ? queries - 1 : (queries - 1) >> 2) & 1;
@@ -827,7 +832,7 @@ __global__ void __launch_bounds__(128) attn_shared_merge_kernel(const int* plan,
   pdl_wait();
   const int row = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, width = n_q * HD;
   const int b = blockIdx.y * 4 + warp;
-  if (b >= width / 128) return;
+  if (b >= width / 128) return;                           // (a whole warp)
   const int e0 = b * 128 + lane * 4, hq = e0 / HD, d0 = e0 % HD, kvh = hq / (n_q / n_kv), L = plan[1];
   const ShBlock* blk = reinterpret_cast<const ShBlock*>(plan + SH_AT_BLOCKS);
   size_t at[2] = {0, 0};
@@ -843,18 +848,38 @@ __global__ void __launch_bounds__(128) attn_shared_merge_kernel(const int* plan,
   }
   auto slot = [&](int s) { return s < n[0] ? at[0] + (size_t)s * n_q : at[1] + (size_t)(s - n[0]) * n_q; };
   const int all = n[0] + n[1];
-  float m = -INFINITY;
-  for (int s = 0; s < all; ++s) m = fmaxf(m, part_ml[slot(s) * 2]);
-  float acc[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
-#pragma unroll 8
-  for (int s = 0; s < all; ++s) {
-    const size_t i = slot(s);
-    const float2 ml = *reinterpret_cast<const float2*>(part_ml + i * 2);
-    const float4 o = *reinterpret_cast<const float4*>(part_o + i * HD + d0);
-    const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);
-    l += f * ml.y;
-    acc[0] += f * o.x, acc[1] += f * o.y, acc[2] += f * o.z, acc[3] += f * o.w;
+  // A head's GL lanes take GL slots at a time, lane = slot for the maxima and factors, with eight partial outputs on their way at once.  (Two heads of 64 in a warp
+  // may have unlike numbers of slots.)
+  constexpr int GL = HD / 4, U = 8;
+  const int gl = lane % GL, g0 = lane - gl, most = HD == 128 ? all : max(all, __shfl_xor_sync(0xffffffffu, all, 16));
+  float acc[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f, m = -INFINITY;
+  for (int s0 = 0; s0 < most; s0 += GL) {
+    const int here = min(GL, all - s0);                   // (of the other head of the warp, maybe none)
+    const float2 ml = gl < here ? *reinterpret_cast<const float2*>(part_ml + slot(s0 + gl) * 2) : make_float2(-INFINITY, 0.f);
+    float4 o[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (u < here) o[u] = *reinterpret_cast<const float4*>(part_o + slot(s0 + u) * HD + d0);
+    float top = ml.x;
+#pragma unroll
+    for (int w = GL / 2; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+    top = fmaxf(m, top);
+    const float old = m == -INFINITY ? 0.f : exp2f(m - top), f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
+    m = top;
+    l = l * old + f * ml.y;                               // (lane = slot: added up at the end)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] *= old;
+    for (int u0 = 0; u0 < min(GL, most - s0); u0 += U) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float g = __shfl_sync(0xffffffffu, f, g0 + u0 + u);
+        if (u0 + u < here) acc[0] += g * o[u].x, acc[1] += g * o[u].y, acc[2] += g * o[u].z, acc[3] += g * o[u].w;
+        if (u0 + U + u < here) o[u] = *reinterpret_cast<const float4*>(part_o + slot(s0 + u0 + U + u) * HD + d0);
+      }
+    }
   }
+#pragma unroll
+  for (int w = GL / 2; w > 0; w >>= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
   const float inv = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) acc[i] = all > 0 ? acc[i] * inv : 0.f;
@@ -950,6 +975,7 @@ RX_API int rx_attn_shared(const void* tmap_k, const void* tmap_v, const void* q,
   if (hd == 128) e = kv_scale != nullptr ? launch_shared<128, true>(dev, tk, tv, tq, a, st) : launch_shared<128, false>(dev, tk, tv, tq, a, st);
   else e = kv_scale != nullptr ? launch_shared<64, true>(dev, tk, tv, tq, a, st) : launch_shared<64, false>(dev, tk, tv, tq, a, st);
   if (e != cudaSuccess) return (int)e;
-  return (int)rx::launch(hd == 128 ? attn_shared_merge_kernel<128> : attn_shared_merge_kernel<64>, dim3(rows, (n_q * hd / 128 + 3) / 4), dim3(128), 0, st, a.plan, a.part_o,
+  // (early whatever the grid: the kernel before is one wave whose CTAs leave room beside them)
+  return (int)rx::launch_pdl(true, hd == 128 ? attn_shared_merge_kernel<128> : attn_shared_merge_kernel<64>, dim3(rows, (n_q * hd / 128 + 3) / 4), dim3(128), 0, st, a.plan, a.part_o,
                          a.part_ml, n_q, n_kv, (const __half*)suh, (__half*)xr, (uint16_t*)out);
 }
