@@ -538,12 +538,11 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
 #pragma unroll
             for (int o = 1; o < 4; ++o) sh_st_zero<8>(s_addr + 8 * ((copy + o) & 3));
           }
-          // The next page's scores are fetched while the probabilities are on their way.  (They do not wait for these: the QKs are two pages ahead.)
+          // The next page's scores are fetched while the probabilities are on their way, if they are there: where a page's exponentials are quickly done, waiting for
+          // them (they come after the PV before) would be what takes longest.
           const bool last = j + 1 == d.pages;
-          if (!last) {
-            if (!all_ok(sh_wait(&s_full[(n + 1) & 1], ((n + 1) >> 1) & 1, abort_flag, a.status, 102))) return false;
-            scores(n + 1, 0);
-          }
+          const bool early = !last && all_ok(mbar_test_wait(&s_full[(n + 1) & 1], ((n + 1) >> 1) & 1));
+          if (early) scores(n + 1, 0);
           tc_wait_st();
           tc_fence_before();
           if (!tail(j)) return false;
@@ -552,6 +551,10 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
           if (last) {
             ++n;
             return true;
+          }
+          if (!early) {
+            if (!all_ok(sh_wait(&s_full[(n + 1) & 1], ((n + 1) >> 1) & 1, abort_flag, a.status, 102))) return false;
+            scores(n + 1, 0);
           }
         }
       };
