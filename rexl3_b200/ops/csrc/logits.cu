@@ -13,26 +13,26 @@
 namespace rx {
 
 // ------------------------------------------------------------------------------------------------ counts
-constexpr int CNT_THREADS = 512;
-constexpr int CNT_MAX_SLICE = 24576;                       // counters of a CTA: 96 KB of shared memory, two CTAs an SM
-constexpr int CNT_MIN_SLICE = 1024;
+constexpr int CNT_THREADS = 1024;
+constexpr int CNT_MAX_SLICE = 76032;                       // 16-bit words of a CTA: 152 KB of shared memory
+constexpr int CNT_MIN_SLICE = 2048;
 constexpr unsigned CNT_PROMPT = 0x80000000u;
 
-__device__ __forceinline__ uint16_t cnt_word(uint32_t c) {
-  const uint32_t g = c & ~CNT_PROMPT;
-  return (uint16_t)((g < 32767u ? g : 32767u) | (c >> 31 << 15));
-}
-
 // A CTA owns a slice of one slot's vocabulary: it reads the whole history, counts what falls into its slice in shared memory and writes the slice once.  No
-// clearing pass, no atomics on global memory, one launch; what it costs is that a history is read once per slice, from L2 but for the first time.
+// clearing pass, no atomics on global memory, one launch; what it costs is that a history is read once per slice, from L2 but for the first time.  The words are
+// counted as they are stored, two in a 32-bit word of shared memory: with at most 32767 generated tokens no count can stop or carry.  A longer history takes
+// the slice in two halves of 32-bit counters.
 __global__ void __launch_bounds__(CNT_THREADS) token_counts_kernel(uint16_t* __restrict__ counts, const int* __restrict__ slots, const int* __restrict__ starts,
                                                                    const int* __restrict__ prompt, const int* __restrict__ tokens, int n_tokens, int n_slots,
                                                                    int vocab, int slice, int* status) {
   pdl_launch();
-  extern __shared__ uint32_t cnt[];
+  extern __shared__ __align__(16) uint32_t cnt[];
   const int req = blockIdx.y, tid = threadIdx.x;
   const int v0 = blockIdx.x * slice, v1 = min(vocab, v0 + slice);
-  for (int i = tid; i < slice; i += CNT_THREADS) cnt[i] = 0;
+  auto clear = [&]() {
+    for (int i = tid; i < slice / 8; i += CNT_THREADS) reinterpret_cast<uint4*>(cnt)[i] = make_uint4(0u, 0u, 0u, 0u);
+  };
+  clear();
   pdl_wait();
   const int slot = slots[req], begin = starts[req], end = starts[req + 1];
   bool skip = slot < 0 || slot >= n_slots || begin < 0 || end < begin || end > n_tokens;
@@ -42,29 +42,61 @@ __global__ void __launch_bounds__(CNT_THREADS) token_counts_kernel(uint16_t* __r
     return;
   }
   const int p_end = begin + min(max(prompt[req], 0), end - begin);
+  uint16_t* out = counts + (size_t)slot * vocab;
   bool bad = false;
-#pragma unroll 4
-  for (int i = begin + tid; i < end; i += CNT_THREADS) {
-    const int t = tokens[i];
-    bad |= (unsigned)t >= (unsigned)vocab;
-    if (t >= v0 && t < v1) {
-      if (i < p_end) atomicOr(&cnt[t - v0], CNT_PROMPT);
-      else atomicAdd(&cnt[t - v0], 1u);
+  if (end - p_end <= 32767) {
+    // four tokens on their way at once
+    for (int i0 = begin + tid; i0 < end; i0 += 4 * CNT_THREADS) {
+      int t[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) t[u] = i0 + u * CNT_THREADS < end ? tokens[i0 + u * CNT_THREADS] : v0 - 1;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (i0 + u * CNT_THREADS >= end) continue;
+        bad |= (unsigned)t[u] >= (unsigned)vocab;
+        if (t[u] < v0 || t[u] >= v1) continue;
+        const int at = t[u] - v0;
+        if (i0 + u * CNT_THREADS < p_end) atomicOr(&cnt[at >> 1], 0x8000u << (16 * (at & 1)));
+        else atomicAdd(&cnt[at >> 1], 1u << (16 * (at & 1)));
+      }
+    }
+    __syncthreads();
+    // 16-byte stores where the slot's row allows them (rows of an odd vocabulary begin anywhere)
+    const uint16_t* word = reinterpret_cast<const uint16_t*>(cnt);
+    const int skew = (int)(((uintptr_t)(out + v0) >> 1) & 7), head = min(v1 - v0, (8 - skew) & 7), body = (v1 - v0 - head) & ~7;
+    for (int i = tid; i < head; i += CNT_THREADS) out[v0 + i] = word[i];
+    if (skew == 0) {
+      for (int i = 8 * tid; i < body; i += 8 * CNT_THREADS) *reinterpret_cast<uint4*>(out + v0 + i) = *reinterpret_cast<const uint4*>(word + i);
+    } else {
+      for (int i = head + 8 * tid; i < head + body; i += 8 * CNT_THREADS) {
+        uint32_t w[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) w[u] = (uint32_t)word[i + 2 * u] | (uint32_t)word[i + 2 * u + 1] << 16;
+        *reinterpret_cast<uint4*>(out + v0 + i) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+    for (int i = head + body + tid; i < v1 - v0; i += CNT_THREADS) out[v0 + i] = word[i];
+  } else {
+    for (int h0 = v0; h0 < v1; h0 += slice / 2) {
+      const int h1 = min(v1, h0 + slice / 2);
+      for (int i = begin + tid; i < end; i += CNT_THREADS) {
+        const int t = tokens[i];
+        bad |= (unsigned)t >= (unsigned)vocab;
+        if (t < h0 || t >= h1) continue;
+        if (i < p_end) atomicOr(&cnt[t - h0], CNT_PROMPT);
+        else atomicAdd(&cnt[t - h0], 1u);
+      }
+      __syncthreads();
+      for (int i = tid; i < h1 - h0; i += CNT_THREADS) {
+        const uint32_t g = cnt[i] & ~CNT_PROMPT;
+        out[h0 + i] = (uint16_t)((g < 32767u ? g : 32767u) | (cnt[i] >> 31 << 15));
+      }
+      __syncthreads();
+      clear();
+      __syncthreads();
     }
   }
   if (bad && blockIdx.x == 0) set_status(status, ST_BAD_ARG, 93, req);
-  __syncthreads();
-  // 16-byte stores where the slot's row allows them (rows of an odd vocabulary begin anywhere)
-  uint16_t* out = counts + (size_t)slot * vocab;
-  const int skew = (int)(((uintptr_t)(out + v0) >> 1) & 7), head = min(v1 - v0, (8 - skew) & 7), body = (v1 - v0 - head) & ~7;
-  for (int i = tid; i < head; i += CNT_THREADS) out[v0 + i] = cnt_word(cnt[i]);
-  for (int i = head + 8 * tid; i < head + body; i += 8 * CNT_THREADS) {
-    uint32_t w[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) w[u] = (uint32_t)cnt_word(cnt[i + 2 * u]) | (uint32_t)cnt_word(cnt[i + 2 * u + 1]) << 16;
-    *reinterpret_cast<uint4*>(out + v0 + i) = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-  for (int i = head + body + tid; i < v1 - v0; i += CNT_THREADS) out[v0 + i] = cnt_word(cnt[i]);
 }
 
 // counts[slots[i], tokens[i]] += 1 (or the prompt bit).  Compare-and-swap on the 16-bit word: the count stops at 32767, and the order does not matter.
@@ -108,128 +140,235 @@ struct PickArgs {
   int rows, vocab, n_slots, n_bias, n_masks, words, count, nchunks;
 };
 
-// A CTA takes 4096 ids of a row.  VEC: four ids side by side at a time (16-byte loads of logits, 8-byte loads of counts); else one.
-// Masked ids cost neither their logit nor their count.  An id at -inf is no key at all (0): it is a candidate only where a row has fewer than `count` ids above
-// -inf, and the second selection finds those by counting.  (As keys, thousands of equal values would all pass the selection's threshold.)
+// The order of values as that of unsigned words (0: no candidate): every NaN is above +inf, -0 is 0.
+__device__ __forceinline__ uint32_t pick_order(float v) {
+  const uint32_t b = __float_as_uint(v != v ? __uint_as_float(0x7FC00000u) : v + 0.f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t pick_key(uint32_t order, int id) { return (uint64_t)order << 32 | (uint32_t)~id; }
+
+// The rules but for the mask.
+__device__ __forceinline__ float pick_rules(float v, uint32_t word, uint32_t drafts, float rep, float freq, float pres) {
+  const uint32_t gen = (word & 0x7FFFu) + drafts;
+  if (gen != 0 || word != 0) {
+    v = v > 0.f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
+    v = __fsub_rn(v, __fmul_rn(freq, (float)gen));
+    if (gen != 0) v = __fsub_rn(v, pres);
+  }
+  return v;
+}
+
+constexpr int PICK_THREADS = 256, PICK_PER = 32, PICK_CHUNK = PICK_THREADS * PICK_PER, PICK_LIST = 512;
+struct PickShared { uint64_t best[PICK_THREADS], list[PICK_LIST], least; int n; };
+
+// The `count` largest keys of the block, in descending order, to out (0 where there are fewer).  A thread's candidates come by `each(f)`: f(key) for every one above 0,
+// `mine` is the largest of them.
+// The count-th largest of the maxima of groups of threads is no larger than the count-th largest key, so only keys from there on - hardly more than `count`,
+// with 64 groups for up to half as many - can be among the results; each finds its own place by counting the larger ones.  Where more of them pass than the
+// list holds (one group far below the others), and for one or two results, the block's maximum is taken `count` times.
+template <typename Each>
+__device__ __forceinline__ void pick_select(uint64_t mine, Each each, int count, uint64_t* out, PickShared& sm) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (count > 2) {
+    const int per = count > 32 ? 1 : PICK_THREADS / 64, groups = PICK_THREADS / per;
+    uint64_t m = mine;
+    if (per > 1) {
+#pragma unroll
+      for (int o = 1; o < PICK_THREADS / 64; o <<= 1) m = u64_max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    }
+    if (tid % per == 0) sm.best[tid / per] = m;
+    if (tid == 0) sm.n = 0;
+    __syncthreads();
+    if (tid < groups) {
+      const uint64_t own = sm.best[tid];
+      int place = 0;
+#pragma unroll 16
+      for (int j = 0; j < groups; ++j) place += sm.best[j] > own || (sm.best[j] == own && j < tid);
+      if (place == count - 1) sm.least = own;
+    }
+    __syncthreads();
+    const uint64_t least = sm.least;
+    if (mine != 0 && mine >= least)
+      each([&](uint64_t key) {
+        if (key < least) return;
+        const int at = atomicAdd(&sm.n, 1);
+        if (at < PICK_LIST) sm.list[at] = key;
+      });
+    __syncthreads();
+    const int n = sm.n;
+    if (n <= PICK_LIST) {
+      for (int i = tid; i < n; i += PICK_THREADS) {
+        const uint64_t own = sm.list[i];
+        int place = 0;
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) place += sm.list[j] > own;
+        if (place < count) out[place] = own;
+      }
+      for (int r = n + tid; r < count; r += PICK_THREADS) out[r] = 0;
+      __syncthreads();
+      return;
+    }
+  }
+  uint64_t below = ~0ull;                                  // the last maximum
+  for (int r = 0; r < count; ++r) {
+    uint64_t best = mine < below ? mine : 0;
+    if (mine >= below) each([&](uint64_t key) { if (key < below) best = u64_max(best, key); });
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) best = u64_max(best, __shfl_xor_sync(0xffffffffu, best, o));
+    if (lane == 0) sm.best[warp] = best;
+    __syncthreads();
+    below = 0;
+#pragma unroll
+    for (int w = 0; w < PICK_THREADS / 32; ++w) below = u64_max(below, sm.best[w]);
+    if (tid == 0) out[r] = below;
+    __syncthreads();
+  }
+}
+
+// A CTA takes 8192 ids of a row, a thread 32 of them.  VEC: four ids side by side at a time (16-byte loads of logits, 8-byte loads of counts); else one.
+// Masked ids cost neither their logit nor their count.  An id at -inf is no candidate: it is one only where a row has fewer than `count` ids above -inf, and the
+// second selection finds those by counting.  (As keys, thousands of equal values would all pass the selection's threshold.)
+// Bound by the latency of a chain of loads (slot, mask, logits and counts) and barriers; the larger the chunk, the less of it there is.
 template <bool VEC>
-__global__ void __launch_bounds__(TOPK_THREADS) pick_stage1_kernel(const __grid_constant__ PickArgs a) {
+__global__ void __launch_bounds__(PICK_THREADS, 3) pick_stage1_kernel(const __grid_constant__ PickArgs a) {
   pdl_launch();
   pdl_wait();
-  __shared__ TopkShared sm;
-  __shared__ float s_bias[TOPK_CHUNK];
-  __shared__ uint16_t s_fed[TOPK_CHUNK];
-  __shared__ uint32_t s_list[PICK_MAX_BIAS];              // biases inside this chunk: place in the slot's list << 12 | id - base, in no order
+  __shared__ PickShared sm;
+  __shared__ uint32_t s_list[PICK_MAX_BIAS];              // places of the slot's bias list, then rows of the window, whose id is in this chunk
+  __shared__ int s_id[PICK_MAX_BIAS];
+  __shared__ uint32_t s_order[PICK_MAX_BIAS];
   __shared__ int s_listed;
-  constexpr int W = VEC ? 4 : 1, N = TOPK_PER_THREAD / W;
-  const int row = blockIdx.y, tid = threadIdx.x, base = blockIdx.x * TOPK_CHUNK;
+  constexpr int W = VEC ? 4 : 1, N = PICK_PER / W;
+  const int row = blockIdx.y, tid = threadIdx.x, base = blockIdx.x * PICK_CHUNK, ids_here = min(a.vocab - base, PICK_CHUNK);
   const int slot_in = a.row_slot != nullptr ? a.row_slot[row] : -1, slot = slot_in >= 0 && slot_in < a.n_slots ? slot_in : -1;
   const int mrow = a.mask != nullptr ? a.mask_row[row] : -1;
   const bool masked = mrow >= 0 && mrow < a.n_masks;
-  // which of the thread's ids may be taken
+  const float* lr = a.logits + (size_t)row * a.ld + base;
+  const uint16_t* cr = a.counts != nullptr && slot >= 0 ? a.counts + (size_t)slot * a.vocab + base : nullptr;
+  const uint32_t* mr = a.mask + (size_t)(masked ? mrow : 0) * a.words + base / 32;
+  if (tid == 0) s_listed = 0;
+  // which of the thread's ids may be taken: of ids (i * 256 + tid) W .. + W - 1, bits i W ..
   uint32_t ok = 0;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const int id = base + (i * TOPK_THREADS + tid) * W;
-    if (id >= a.vocab) continue;
-    const uint32_t w = masked ? a.mask[(size_t)mrow * a.words + (id >> 5)] >> (id & 31) : 0xFu;
-    ok |= (w & ((1u << W) - 1)) << (i * W);
+    const int at = (i * PICK_THREADS + tid) * W;
+    uint32_t w = at < ids_here ? (1u << W) - 1 : 0u;
+    if (masked && w != 0) w &= mr[at >> 5] >> (at & 31);
+    ok |= w << (i * W);
   }
-  float x[TOPK_PER_THREAD];
-  uint32_t c[TOPK_PER_THREAD];
-  const float* lr = a.logits + (size_t)row * a.ld;
-  const uint16_t* cr = a.counts != nullptr && slot >= 0 ? a.counts + (size_t)slot * a.vocab : nullptr;
+  float x[PICK_PER];
+  uint32_t c[VEC ? PICK_PER / 2 : PICK_PER];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const int id = base + (i * TOPK_THREADS + tid) * W;
+    const int at = (i * PICK_THREADS + tid) * W;
     const bool some = (ok >> (i * W) & ((1u << W) - 1)) != 0;
     if constexpr (VEC) {
-      const float4 v = some ? *reinterpret_cast<const float4*>(lr + id) : make_float4(0.f, 0.f, 0.f, 0.f);
-      const uint2 n = some && cr != nullptr ? *reinterpret_cast<const uint2*>(cr + id) : make_uint2(0u, 0u);
+      const float4 v = some ? *reinterpret_cast<const float4*>(lr + at) : make_float4(0.f, 0.f, 0.f, 0.f);
+      const uint2 n = some && cr != nullptr ? *reinterpret_cast<const uint2*>(cr + at) : make_uint2(0u, 0u);
       x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
-      c[4 * i] = n.x & 0xFFFFu, c[4 * i + 1] = n.x >> 16, c[4 * i + 2] = n.y & 0xFFFFu, c[4 * i + 3] = n.y >> 16;
+      c[2 * i] = n.x, c[2 * i + 1] = n.y;
     } else {
-      x[i] = some ? lr[id] : 0.f;
-      c[i] = some && cr != nullptr ? cr[id] : 0u;
+      x[i] = some ? lr[at] : 0.f;
+      c[i] = some && cr != nullptr ? cr[at] : 0u;
     }
   }
-  // biases and drafts inside this chunk: rare, so the tables that hold them are only made where there are any
-  const int* bid = a.bias_id != nullptr && slot >= 0 ? a.bias_id + (size_t)slot * a.n_bias : nullptr;
-  const int nb = bid != nullptr ? a.n_bias : 0;
-  const int r0 = a.first != nullptr && cr != nullptr ? max(a.first[row], 0) : row;
-  if (tid == 0) s_listed = 0;
-  __syncthreads();
-  const int ids_here = min(a.vocab - base, TOPK_CHUNK);
-  bool drafts = false;
-  for (int e = tid; e < nb; e += TOPK_THREADS) {
-    const int id = bid[e] - base;
-    if (bid[e] >= 0 && id >= 0 && id < ids_here) s_list[atomicAdd(&s_listed, 1)] = (uint32_t)e << 12 | (uint32_t)id;
-  }
-  for (int r = r0 + 1 + tid; r <= row; r += TOPK_THREADS) drafts |= a.fed[r] >= base && a.fed[r] - base < ids_here;
-  const bool any_drafts = __syncthreads_or(drafts);
-  const int listed = s_listed;
-  const bool any_bias = listed > 0;
-  if (any_bias) for (int i = tid; i < TOPK_CHUNK; i += TOPK_THREADS) s_bias[i] = 0.f;
-  if (any_drafts) for (int i = tid; i < TOPK_CHUNK / 2; i += TOPK_THREADS) reinterpret_cast<uint32_t*>(s_fed)[i] = 0u;
-  __syncthreads();
-  for (int i = tid; i < listed; i += TOPK_THREADS) {
-    // an id that stands in the slot's list more than once: its first place adds them up in list order
-    const uint32_t mine = s_list[i], id = mine & 4095u;
-    float sum = a.bias_val[(size_t)slot * a.n_bias + (mine >> 12)];
-    bool lead = true;
-    for (uint32_t at = mine;;) {
-      uint32_t next = ~0u;
-      for (int j = 0; j < listed; ++j) {
-        const uint32_t other = s_list[j];
-        if ((other & 4095u) != id) continue;
-        lead = lead && other >= mine;
-        if (other > at && other < next) next = other;
-      }
-      if (!lead || next == ~0u) break;
-      sum = __fadd_rn(sum, a.bias_val[(size_t)slot * a.n_bias + (next >> 12)]);
-      at = next;
-    }
-    if (lead) s_bias[id] = sum;
-  }
-  if (drafts)
-    for (int r = r0 + 1 + tid; r <= row; r += TOPK_THREADS) {
-      const int id = a.fed[r] - base;
-      if (a.fed[r] >= base && id < ids_here) atomicAdd(reinterpret_cast<uint32_t*>(s_fed) + (id >> 1), 1u << (16 * (id & 1)));
-    }
-  __syncthreads();
   float rep = 1.f, freq = 0.f, pres = 0.f;
   if (cr != nullptr) rep = a.penalties[3 * slot], freq = a.penalties[3 * slot + 1], pres = a.penalties[3 * slot + 2];
-  uint64_t k[TOPK_PER_THREAD];
-#pragma unroll
-  for (int i = 0; i < TOPK_PER_THREAD; ++i) {
-    const int local = ((i / W) * TOPK_THREADS + tid) * W + i % W;
-    float v = x[i];
-    const uint32_t gen = (c[i] & 0x7FFFu) + (any_drafts ? s_fed[local] : 0u);
-    if (gen != 0 || c[i] != 0) {
-      v = v > 0.f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
-      v = __fsub_rn(v, __fmul_rn(freq, (float)gen));
-      if (gen != 0) v = __fsub_rn(v, pres);
+  __syncthreads();
+  // ids with a bias or among the drafts: few, and in few chunks
+  const int* bid = a.bias_id != nullptr && slot >= 0 ? a.bias_id + (size_t)slot * a.n_bias : nullptr;
+  const float* bval = a.bias_val + (size_t)max(slot, 0) * a.n_bias;
+  const int nb = bid != nullptr ? a.n_bias : 0, r0 = a.first != nullptr && cr != nullptr ? max(a.first[row], 0) + 1 : row + 1;
+  for (int e = tid; e < nb; e += PICK_THREADS)
+    if (bid[e] >= base && bid[e] - base < ids_here) {
+      const int at = atomicAdd(&s_listed, 1);
+      if (at < PICK_MAX_BIAS) s_list[at] = e;
     }
-    if (any_bias) v = __fadd_rn(v, s_bias[local]);
-    v = v != v ? __uint_as_float(0x7FC00000u) : v + 0.f;  // every NaN is above +inf, and -0 is 0
-    k[i] = (ok >> i & 1) && v != -INFINITY ? topk_key(v, (uint32_t)(base + local)) : 0;
+  for (int r = r0 + tid; r <= row; r += PICK_THREADS)
+    if (a.fed[r] >= base && a.fed[r] - base < ids_here) {
+      const int at = atomicAdd(&s_listed, 1);
+      if (at < PICK_MAX_BIAS) s_list[at] = PICK_MAX_BIAS + r;
+    }
+  uint32_t u[PICK_PER];
+#pragma unroll
+  for (int i = 0; i < PICK_PER; ++i) {
+    const uint32_t word = VEC ? c[i / 2] >> (16 * (i & 1)) & 0xFFFFu : c[VEC ? 0 : i];
+    const float v = pick_rules(x[i], word, 0, rep, freq, pres);
+    u[i] = (ok >> i & 1) && v != -INFINITY ? pick_order(v) : 0;
   }
-  block_select(k, a.count, a.cand + ((size_t)row * a.nchunks + blockIdx.x) * a.count, sm);
+  __syncthreads();
+  const int listed = s_listed;
+  if (listed > 0) {
+    // Such an id is worked out again by itself, by a thread per place in the list (an id more than once: the same each time), and put in its owner's place.  A
+    // window with more drafts in the chunk than the list holds is gone over whole.
+    const int from = min(listed, PICK_MAX_BIAS), all = listed <= PICK_MAX_BIAS ? from : nb + max(row - r0 + 1, 0);
+    for (int l0 = 0; l0 < all; l0 += PICK_MAX_BIAS) {
+      const int here = min(PICK_MAX_BIAS, all - l0);
+      __syncthreads();
+      for (int l = tid; l < here; l += PICK_THREADS) {
+        const int e = listed <= PICK_MAX_BIAS ? (int)s_list[l] : l0 + l < nb ? l0 + l : PICK_MAX_BIAS + r0 + l0 + l - nb;
+        const int id = e < PICK_MAX_BIAS ? bid[e] : a.fed[e - PICK_MAX_BIAS];
+        s_id[l] = id >= base && id - base < ids_here ? id - base : -1;
+        if (s_id[l] < 0) continue;
+        uint32_t drafts = 0;
+        for (int r = r0; r <= row; ++r) drafts += a.fed[r] == id;
+        float v = pick_rules(lr[id - base], cr != nullptr ? cr[id - base] : 0u, drafts, rep, freq, pres), sum = 0.f;
+        bool any = false;
+        for (int f = 0; f < nb; ++f)
+          if (bid[f] == id) sum = any ? __fadd_rn(sum, bval[f]) : bval[f], any = true;
+        if (any) v = __fadd_rn(v, sum);
+        s_order[l] = v != -INFINITY ? pick_order(v) : 0;
+      }
+      __syncthreads();
+      for (int l = 0; l < here; ++l) {
+        const int at = s_id[l];
+        if (at < 0 || at / W % PICK_THREADS != tid) continue;
+        const int mine = at / W / PICK_THREADS * W + at % W;
+#pragma unroll
+        for (int i = 0; i < PICK_PER; ++i)
+          if (i == mine) u[i] = ok >> i & 1 ? s_order[l] : 0;
+      }
+    }
+  }
+  // the thread's best: the lowest of its ids with the highest order (they ascend with i)
+  uint32_t top = 0;
+  int first = 0;
+#pragma unroll
+  for (int i = 0; i < PICK_PER; ++i)
+    if (u[i] > top) top = u[i], first = i;
+  auto id = [&](int i) { return base + ((i / W) * PICK_THREADS + tid) * W + i % W; };
+  pick_select(top != 0 ? pick_key(top, id(first)) : 0,
+              [&](auto f) {
+#pragma unroll
+                for (int i = 0; i < PICK_PER; ++i)
+                  if (u[i] != 0) f(pick_key(u[i], id(i)));
+              },
+              a.count, a.cand + ((size_t)row * a.nchunks + blockIdx.x) * a.count, sm);
 }
 
-__global__ void __launch_bounds__(TOPK_THREADS) pick_stage2_kernel(const uint64_t* cand, int total, int count, int* __restrict__ ids, float* __restrict__ vals) {
+// total <= PICK_THREADS * 16 candidates a row
+__global__ void __launch_bounds__(PICK_THREADS) pick_stage2_kernel(const uint64_t* cand, int total, int count, int* __restrict__ ids, float* __restrict__ vals) {
   pdl_launch();
   pdl_wait();
-  __shared__ TopkShared sm;
+  __shared__ PickShared sm;
   __shared__ uint64_t outk[64];
   const int row = blockIdx.x;
   const uint64_t* c = cand + (size_t)row * total;
-  uint64_t k[TOPK_PER_THREAD];
+  constexpr int PER = 16;
+  uint64_t k[PER], mine = 0;
 #pragma unroll
-  for (int i = 0; i < TOPK_PER_THREAD; ++i) {
-    const int j = i * TOPK_THREADS + threadIdx.x;
+  for (int i = 0; i < PER; ++i) {
+    const int j = i * PICK_THREADS + threadIdx.x;
     k[i] = j < total ? c[j] : 0;
+    mine = u64_max(mine, k[i]);
   }
-  block_select(k, count, outk, sm);
+  pick_select(mine,
+              [&](auto f) {
+#pragma unroll
+                for (int i = 0; i < PER; ++i)
+                  if (k[i] != 0) f(k[i]);
+              },
+              count, outk, sm);
   __syncthreads();
   if ((int)threadIdx.x >= count) return;
   int id;
@@ -259,20 +398,20 @@ using namespace rx;
 RX_API int rx_token_counts(void* counts, int n_slots, int vocab, const void* slots, const void* starts, const void* prompt, const void* tokens, int n_tokens, int n,
                            int* status, void* stream) {
   if (n < 1 || n > 65535 || n_slots < 1 || vocab < 1 || n_tokens < 0) return (int)cudaErrorInvalidValue;
-  // slices so small that two waves of CTAs have work, so large that a history is not read more often than need be
-  int slice = (vocab + (592 + n - 1) / n - 1) / ((592 + n - 1) / n);
-  slice = slice < CNT_MIN_SLICE ? CNT_MIN_SLICE : slice > CNT_MAX_SLICE ? CNT_MAX_SLICE : (slice + 7) & ~7;
-  const int parts = (vocab + slice - 1) / slice;
+  // One slice per CTA, as few as shared memory allows, but a CTA for every SM; slices of whole 16-byte words and whole halves of those.
+  const int fewest = (vocab + CNT_MAX_SLICE - 1) / CNT_MAX_SLICE, wanted = (148 + n - 1) / n, most = (vocab + CNT_MIN_SLICE - 1) / CNT_MIN_SLICE;
+  const int cut = wanted > most ? most : wanted, into = cut < fewest ? fewest : cut;
+  const int slice = ((vocab + into - 1) / into + 15) & ~15, parts = (vocab + slice - 1) / slice;
   static bool configured[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return (int)e;
   if (dev >= 64 || !configured[dev]) {
-    e = cudaFuncSetAttribute(token_counts_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, CNT_MAX_SLICE * 4);
+    e = cudaFuncSetAttribute(token_counts_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, CNT_MAX_SLICE * 2 + 64);
     if (e != cudaSuccess) return (int)e;
     if (dev < 64) configured[dev] = true;
   }
-  return (int)rx::launch(token_counts_kernel, dim3(parts, n), dim3(CNT_THREADS), (size_t)slice * 4, (cudaStream_t)stream, (uint16_t*)counts, (const int*)slots,
+  return (int)rx::launch(token_counts_kernel, dim3(parts, n), dim3(CNT_THREADS), (size_t)slice * 2, (cudaStream_t)stream, (uint16_t*)counts, (const int*)slots,
                          (const int*)starts, (const int*)prompt, (const int*)tokens, n_tokens, n_slots, vocab, slice, status);
 }
 
@@ -282,12 +421,12 @@ RX_API int rx_token_counts_add(void* counts, int n_slots, int vocab, const void*
                          n_slots, vocab, in_prompt, status);
 }
 
-// scratch: as rx_topk's.  Any of counts (with penalties), bias_id (with bias_val), mask (with mask_row) and first (with fed) may be null.
+// scratch: rx_topk_scratch_bytes (of which half is used).  Any of counts (with penalties), bias_id (with bias_val), mask (with mask_row) and first (with fed) may be null.
 RX_API int rx_topk_adjusted(const void* logits, long long ld, int rows, int vocab, int count, void* scratch, void* ids, void* vals, const void* row_slot,
                             const void* counts, const void* penalties, int n_slots, const void* bias_id, const void* bias_val, int n_bias, const void* mask,
                             const void* mask_row, int n_masks, const void* first, const void* fed, void* stream) {
-  const int nchunks = (vocab + TOPK_CHUNK - 1) / TOPK_CHUNK;
-  if (rows < 1 || rows > 65535 || vocab < 1 || count < 1 || count > 64 || count > vocab || (long long)nchunks * count > TOPK_CHUNK || ld < vocab || n_bias < 0 || n_bias > PICK_MAX_BIAS)
+  const int nchunks = (vocab + PICK_CHUNK - 1) / PICK_CHUNK;
+  if (rows < 1 || rows > 65535 || vocab < 1 || count < 1 || count > 64 || count > vocab || (long long)nchunks * count > PICK_THREADS * 16 || ld < vocab || n_bias < 0 || n_bias > PICK_MAX_BIAS)
     return (int)cudaErrorInvalidValue;
   PickArgs a = {(const float*)logits, (const int*)row_slot, (const uint16_t*)counts, (const float*)penalties, (const int*)bias_id, (const float*)bias_val,
                 (const uint32_t*)mask, (const int*)mask_row, (const int*)first, (const int*)fed, (uint64_t*)scratch, ld, rows, vocab, n_slots, n_bias, n_masks,
@@ -295,7 +434,7 @@ RX_API int rx_topk_adjusted(const void* logits, long long ld, int rows, int voca
   // four ids at a time where every row of logits and counts begins on a 16- and an 8-byte boundary
   const bool vec = vocab % 4 == 0 && ld % 4 == 0 && ((uintptr_t)logits & 15) == 0 && ((uintptr_t)counts & 7) == 0;
   cudaStream_t st = (cudaStream_t)stream;
-  cudaError_t e = rx::launch(vec ? pick_stage1_kernel<true> : pick_stage1_kernel<false>, dim3(nchunks, rows), dim3(TOPK_THREADS), 0, st, a);
+  cudaError_t e = rx::launch(vec ? pick_stage1_kernel<true> : pick_stage1_kernel<false>, dim3(nchunks, rows), dim3(PICK_THREADS), 0, st, a);
   if (e != cudaSuccess) return (int)e;
-  return (int)rx::launch(pick_stage2_kernel, dim3(rows), dim3(TOPK_THREADS), 0, st, (const uint64_t*)scratch, nchunks * count, count, (int*)ids, (float*)vals);
+  return (int)rx::launch(pick_stage2_kernel, dim3(rows), dim3(PICK_THREADS), 0, st, (const uint64_t*)scratch, nchunks * count, count, (int*)ids, (float*)vals);
 }

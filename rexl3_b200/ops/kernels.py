@@ -392,17 +392,28 @@ def topk(logits: torch.Tensor, count: int, scratch, ids: torch.Tensor, vals: tor
     _lib.count(2)
 
 
-def _operand(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, like: "torch.Tensor | None" = None) -> int:
-    """The device pointer of a contiguous operand of the current device; a None in `shape` stands for any extent."""
+def _operand(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device: int) -> int:
+    """The device pointer of a contiguous operand on the current device `device`.  (A call has ten of them: what is in order is seen by few looks.)"""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == device and t.is_contiguous():
+        return t.data_ptr()
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{name}: a CUDA tensor is needed")
-    if t.device.index != (torch.cuda.current_device() if like is None else like.device.index):
-        raise ValueError(f"{name} is on {t.device}" + (f", not on the current device cuda:{torch.cuda.current_device()}" if like is None else f", not on {like.device}"))
-    if t.dtype != dtype or t.ndim != len(shape) or any(want is not None and want != got for want, got in zip(shape, t.shape)):
-        raise ValueError(f"{name}: {dtype} {tuple('any' if x is None else x for x in shape)} is needed, not {t.dtype} {tuple(t.shape)}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name}: must be contiguous")
-    return t.data_ptr()
+    if t.get_device() != device:
+        raise ValueError(f"{name} is on {t.device}, not on the current device cuda:{device}")
+    if t.dtype is not dtype or t.shape != shape:
+        raise ValueError(f"{name}: {dtype} {shape} is needed, not {t.dtype} {tuple(t.shape)}")
+    raise ValueError(f"{name}: must be contiguous")
+
+
+def _extents(t: torch.Tensor, name: str, dims: int) -> tuple:
+    if not isinstance(t, torch.Tensor) or t.dim() != dims:
+        raise ValueError(f"{name}: a CUDA tensor of {dims} dimension{'s' if dims > 1 else ''} is needed")
+    return t.shape
+
+
+def _here(t: torch.Tensor) -> int:
+    """The current device; for a tensor that is on none, what no tensor's device is (a CPU tensor's is -1)."""
+    return torch.cuda.current_device() if t.is_cuda else -2
 
 
 def topk_adjusted(logits: torch.Tensor, count: int, scratch: torch.Tensor, ids: torch.Tensor, vals: torch.Tensor, row_slot: "torch.Tensor | None" = None, *,
@@ -417,48 +428,45 @@ def topk_adjusted(logits: torch.Tensor, count: int, scratch: torch.Tensor, ids: 
     mask = (bits int32 [n, ceil(vocab / 32)], row int32 [rows]): row r may take the ids whose bit of bits[row[r]] is set (id i: bit i % 32 of word i // 32), every
     id where row[r] is outside 0 .. n - 1.  What is masked stands at -inf, whatever its logit.  Where a row has fewer than count ids above -inf, the rest are
     its lowest other ids at -inf.  A NaN that is not masked is above everything.  scratch: `topk_scratch`; calls that may overlap need one each."""
-    if not isinstance(logits, torch.Tensor) or logits.ndim != 2 or logits.dtype != torch.float32 or not logits.is_cuda:
+    if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or logits.dtype is not torch.float32 or not logits.is_cuda:
         raise ValueError("logits: a CUDA float32 [rows, vocab] tensor is needed")
-    rows, vocab = logits.shape
-    if logits.device.index != torch.cuda.current_device():
-        raise ValueError(f"logits is on {logits.device}, not on the current device cuda:{torch.cuda.current_device()}")
-    if rows > 1 and (logits.stride(0) < vocab) or vocab > 1 and logits.stride(1) != 1:
+    L, dev, (rows, vocab), (ld, step) = _lib.load(), _here(logits), logits.shape, logits.stride()
+    if logits.get_device() != dev:
+        raise ValueError(f"logits is on {logits.device}, not on the current device cuda:{dev}")
+    if rows > 1 and ld < vocab or vocab > 1 and step != 1:
         raise ValueError("logits: a row's values must stand side by side, and rows must not overlap")
     if not 1 <= count <= min(64, vocab) or (vocab + 4095) // 4096 * count > 4096:
         raise ValueError(f"count {count}: 1 .. 64, no more than the vocabulary of {vocab}, and ceil(vocab / 4096) * count <= 4096")
     if rows > 65535:
         raise ValueError(f"{rows} rows: at most 65535")
-    p_ids, p_vals = _operand(ids, "ids", torch.int32, (rows, count), logits), _operand(vals, "vals", torch.float32, (rows, count), logits)
+    p_ids, p_vals = _operand(ids, "ids", torch.int32, (rows, count), dev), _operand(vals, "vals", torch.float32, (rows, count), dev)
     if rows == 0:
         return
-    if not scratch.is_cuda or scratch.device != logits.device or not scratch.is_contiguous() or \
-            scratch.numel() * scratch.element_size() < _lib.load().rx_topk_scratch_bytes(rows, vocab, count):
+    if scratch.get_device() != dev or not scratch.is_contiguous() or scratch.numel() * scratch.element_size() < L.rx_topk_scratch_bytes(rows, vocab, count):
         raise ValueError("scratch: too small (see topk_scratch), not contiguous or on another device")
     if (counts is None) != (penalties is None):
         raise ValueError("counts and penalties go together")
     if row_slot is None and (counts is not None or bias is not None):
         raise ValueError("penalties and biases need row_slot")
-    p_slot = None if row_slot is None else _operand(row_slot, "row_slot", torch.int32, (rows,), logits)
+    p_slot = None if row_slot is None else _operand(row_slot, "row_slot", torch.int32, (rows,), dev)
     slots, p_counts, p_pen, p_bid, p_bval, nb, p_mask, p_mrow, nm, p_first, p_fed = 0, None, None, None, None, 0, None, None, 0, None, None
     if counts is not None:
-        p_counts = _operand(counts, "counts", torch.int16, (None, vocab), logits)
-        slots = counts.shape[0]
-        p_pen = _operand(penalties, "penalties", torch.float32, (slots, 3), logits)
+        slots = _extents(counts, "counts", 2)[0]
+        p_counts = _operand(counts, "counts", torch.int16, (slots, vocab), dev)
+        p_pen = _operand(penalties, "penalties", torch.float32, (slots, 3), dev)
     if bias is not None:
-        n_slots = slots if counts is not None else None
-        p_bid = _operand(bias[0], "bias ids", torch.int32, (n_slots, None), logits)
-        slots, nb = bias[0].shape
-        p_bval = _operand(bias[1], "bias values", torch.float32, (slots, nb), logits)
+        n, nb = _extents(bias[0], "bias ids", 2)
+        slots = slots if counts is not None else n
+        p_bid, p_bval = _operand(bias[0], "bias ids", torch.int32, (slots, nb), dev), _operand(bias[1], "bias values", torch.float32, (slots, nb), dev)
         if nb > 1024:
             raise ValueError(f"{nb} biases a slot: at most 1024")
     if mask is not None:
-        p_mask, p_mrow = _operand(mask[0], "mask bits", torch.int32, (None, (vocab + 31) // 32), logits), _operand(mask[1], "mask row", torch.int32, (rows,), logits)
-        nm = mask[0].shape[0]
+        nm = _extents(mask[0], "mask bits", 2)[0]
+        p_mask, p_mrow = _operand(mask[0], "mask bits", torch.int32, (nm, (vocab + 31) // 32), dev), _operand(mask[1], "mask row", torch.int32, (rows,), dev)
     if window is not None:
-        p_first, p_fed = (_operand(t, n, torch.int32, (rows,), logits) for t, n in zip(window, ("window first", "window fed")))
-    _lib.check(_lib.load().rx_topk_adjusted(logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab, count, scratch.data_ptr(),
-                                            p_ids, p_vals, p_slot, p_counts, p_pen, slots, p_bid, p_bval, nb, p_mask, p_mrow, nm, p_first, p_fed, _lib.stream_ptr()),
-               "rx_topk_adjusted")
+        p_first, p_fed = _operand(window[0], "window first", torch.int32, (rows,), dev), _operand(window[1], "window fed", torch.int32, (rows,), dev)
+    _lib.check(L.rx_topk_adjusted(logits.data_ptr(), ld if rows > 1 else vocab, rows, vocab, count, scratch.data_ptr(), p_ids, p_vals, p_slot, p_counts, p_pen, slots,
+                                  p_bid, p_bval, nb, p_mask, p_mrow, nm, p_first, p_fed, _lib.stream_ptr()), "rx_topk_adjusted")
     _lib.count(2)
 
 
@@ -467,28 +475,29 @@ def token_counts(counts: torch.Tensor, slots: torch.Tensor, starts: torch.Tensor
     the id, bits 0 .. 14 = times generated, up to 32767.  Request i's history is tokens[starts[i]:starts[i + 1]], its first prompt_len[i] tokens the prompt; row
     slots[i] of counts is written whole, the others stay.  int32 tensors; starts has one more entry than slots.  A token outside the vocabulary is left out, a slot
     outside the table, a slot's second request and a range outside `tokens` are passed over; each sets the status."""
-    p_counts = _operand(counts, "counts", torch.int16, (None, None))
-    n = slots.numel()
-    p = [_operand(t, name, torch.int32, shape, counts) for t, name, shape in ((slots, "slots", (n,)), (starts, "starts", (n + 1,)), (prompt_len, "prompt_len", (n,)),
-                                                                             (tokens, "tokens", (None,)), (status, "status", (STATUS_WORDS,)))]
+    n_slots, vocab = _extents(counts, "counts", 2)
+    dev, n, n_tokens = _here(counts), _extents(slots, "slots", 1)[0], _extents(tokens, "tokens", 1)[0]
+    p = (_operand(counts, "counts", torch.int16, (n_slots, vocab), dev), _operand(slots, "slots", torch.int32, (n,), dev), _operand(starts, "starts", torch.int32, (n + 1,), dev),
+         _operand(prompt_len, "prompt_len", torch.int32, (n,), dev), _operand(tokens, "tokens", torch.int32, (n_tokens,), dev),
+         _operand(status, "status", torch.int32, (STATUS_WORDS,), dev))
     if n > 65535:
         raise ValueError(f"{n} requests: at most 65535")
-    if n == 0 or counts.numel() == 0:
+    if n == 0 or n_slots * vocab == 0:
         return
-    _lib.check(_lib.load().rx_token_counts(p_counts, counts.shape[0], counts.shape[1], p[0], p[1], p[2], p[3], tokens.numel(), n, p[4], _lib.stream_ptr()), "rx_token_counts")
+    _lib.check(_lib.load().rx_token_counts(p[0], n_slots, vocab, p[1], p[2], p[3], p[4], n_tokens, n, p[5], _lib.stream_ptr()), "rx_token_counts")
     _lib.count()
 
 
 def token_counts_add(counts: torch.Tensor, slots: torch.Tensor, tokens: torch.Tensor, status: torch.Tensor, prompt: bool = False) -> None:
     """counts[slots[i], tokens[i]] takes one more generated token (`prompt`: the prompt bit), for the tokens that a step committed; a pair may stand more than
     once.  int32 [n] each.  A slot or token outside the table is left out and sets the status."""
-    p_counts = _operand(counts, "counts", torch.int16, (None, None))
-    n = slots.numel()
-    p = [_operand(t, name, torch.int32, shape, counts) for t, name, shape in ((slots, "slots", (n,)), (tokens, "tokens", (n,)), (status, "status", (STATUS_WORDS,)))]
-    if n == 0 or counts.numel() == 0:
+    n_slots, vocab = _extents(counts, "counts", 2)
+    dev, n = _here(counts), _extents(slots, "slots", 1)[0]
+    p = (_operand(counts, "counts", torch.int16, (n_slots, vocab), dev), _operand(slots, "slots", torch.int32, (n,), dev), _operand(tokens, "tokens", torch.int32, (n,), dev),
+         _operand(status, "status", torch.int32, (STATUS_WORDS,), dev))
+    if n == 0 or n_slots * vocab == 0:
         return
-    _lib.check(_lib.load().rx_token_counts_add(p_counts, counts.shape[0], counts.shape[1], p[0], p[1], n, 1 if prompt else 0, p[2], _lib.stream_ptr()),
-               "rx_token_counts_add")
+    _lib.check(_lib.load().rx_token_counts_add(p[0], n_slots, vocab, p[1], p[2], n, 1 if prompt else 0, p[3], _lib.stream_ptr()), "rx_token_counts_add")
     _lib.count()
 
 
@@ -502,22 +511,22 @@ def window_rows(seq: torch.Tensor, have: torch.Tensor, new: torch.Tensor, block_
     the new tokens begin, and free_next = free_at + their number (it may be the same tensor as free_at).  Without them the table holds those pages already.
     All or nothing: a length below 0, tokens beyond the table, more rows than cap, more pages than there are, a table row outside the table or
     given twice sets the status and changes nothing else.  A table entry below 0 where a row is to be written gives slot -1 (the row is not cached) and sets the status."""
-    n, cap = seq.numel(), rows.shape[-1] if isinstance(rows, torch.Tensor) and rows.ndim else 0
-    p_table = _operand(block_table, "block_table", torch.int32, (None, None))
-    tables, width = block_table.shape
-    p = [_operand(t, name, torch.int32, shape, block_table) for t, name, shape in (
-        (seq, "seq", (n,)), (have, "have", (n,)), (new, "new", (n,)), (rows, "rows", (5, None)), (starts, "starts", (n + 1,)), (status, "status", (STATUS_WORDS,)))]
-    if not 1 <= n <= _lib.load().rx_window_rows_max():
-        raise ValueError(f"{n} requests: 1 .. {_lib.load().rx_window_rows_max()}")
+    L, (tables, width), n, (five, cap) = _lib.load(), _extents(block_table, "block_table", 2), _extents(seq, "seq", 1)[0], _extents(rows, "rows", 2)
+    dev = _here(block_table)
+    p = (_operand(seq, "seq", torch.int32, (n,), dev), _operand(have, "have", torch.int32, (n,), dev), _operand(new, "new", torch.int32, (n,), dev),
+         _operand(block_table, "block_table", torch.int32, (tables, width), dev), _operand(rows, "rows", torch.int32, (5, cap), dev),
+         _operand(starts, "starts", torch.int32, (n + 1,), dev), _operand(status, "status", torch.int32, (STATUS_WORDS,), dev))
+    if not 1 <= n <= L.rx_window_rows_max():
+        raise ValueError(f"{n} requests: 1 .. {L.rx_window_rows_max()}")
     if not 1 <= tables <= 32768 or not 1 <= width <= 1 << 24 or cap > 1 << 20:
         raise ValueError("block_table: 1 .. 32768 rows of 1 .. 2^24 pages; rows: at most 2^20")
     if (free is None) != (free_at is None) or (free is None) != (free_next is None):
         raise ValueError("free, free_at and free_next go together")
-    f = [None, None, None]
+    f, n_free = (None, None, None), 0
     if free is not None:
-        f = [_operand(t, name, torch.int32, shape, block_table) for t, name, shape in ((free, "free", (None,)), (free_at, "free_at", (1,)), (free_next, "free_next", (1,)))]
-    _lib.check(_lib.load().rx_window_rows(p[0], p[1], p[2], n, p_table, tables, width, f[0], 0 if free is None else free.numel(), f[1], f[2], p[3], cap, p[4], p[5],
-                                          _lib.stream_ptr()), "rx_window_rows")
+        n_free = _extents(free, "free", 1)[0]
+        f = _operand(free, "free", torch.int32, (n_free,), dev), _operand(free_at, "free_at", torch.int32, (1,), dev), _operand(free_next, "free_next", torch.int32, (1,), dev)
+    _lib.check(L.rx_window_rows(p[0], p[1], p[2], n, p[3], tables, width, f[0], n_free, f[1], f[2], p[4], cap, p[5], p[6], _lib.stream_ptr()), "rx_window_rows")
     _lib.count()
 
 
@@ -594,23 +603,22 @@ def attn_shared_plan_buffer(device="cuda") -> torch.Tensor:
 
 
 def _shared_window(block_table, row_seq, ctx_len, common, status, n_q: int, n_kv: int):
-    p_table = _operand(block_table, "block_table", torch.int32, (None, None))
-    rows = row_seq.numel()
-    p = [p_table] + [_operand(t, name, torch.int32, shape, block_table) for t, name, shape in (
-        (row_seq, "row_seq", (rows,)), (ctx_len, "ctx_len", (rows,)), (common, "common", (rows,)), (status, "status", (STATUS_WORDS,)))]
+    (tables, width), rows, dev = _extents(block_table, "block_table", 2), _extents(row_seq, "row_seq", 1)[0], _here(block_table)
+    p = (_operand(block_table, "block_table", torch.int32, (tables, width), dev), _operand(row_seq, "row_seq", torch.int32, (rows,), dev),
+         _operand(ctx_len, "ctx_len", torch.int32, (rows,), dev), _operand(common, "common", torch.int32, (rows,), dev), _operand(status, "status", torch.int32, (STATUS_WORDS,), dev))
     if not 1 <= rows <= 1024 or n_kv < 1 or n_q % n_kv or not 1 <= n_q // n_kv <= 128:
         raise ValueError(f"{rows} rows of {n_q} query and {n_kv} KV heads: 1 .. 1024 rows, n_kv divides n_q, at most 128 query heads share a KV head")
-    if block_table.numel() == 0 or rows * block_table.shape[1] * n_kv >= 1 << 29:
-        raise ValueError("block_table: empty, or rows * pages a sequence * n_kv reaches 2^29")
-    return rows, p
+    if tables * width == 0 or rows * (width + 2) * n_kv >= 1 << 29:
+        raise ValueError("block_table: empty, or rows * (pages a sequence + 2) * n_kv reaches 2^29")
+    return rows, tables, width, dev, p
 
 
 def attn_shared_plan(block_table, row_seq, ctx_len, common, n_q: int, n_kv: int, plan: torch.Tensor, status: torch.Tensor) -> None:
     """The work plan of `attn_shared` for one window: a function of these tensors' values (of block_table only its extents), so one plan serves every layer."""
-    rows, p = _shared_window(block_table, row_seq, ctx_len, common, status, n_q, n_kv)
+    rows, tables, width, dev, p = _shared_window(block_table, row_seq, ctx_len, common, status, n_q, n_kv)
     L = _lib.load()
-    p_plan = _operand(plan, "plan", torch.int32, (L.rx_attn_shared_plan_ints(),), block_table)
-    _lib.check(L.rx_attn_shared_plan(p[1], p[2], p[3], rows, block_table.shape[0], block_table.shape[1], n_q, n_kv, p_plan, p[4], _lib.stream_ptr()), "rx_attn_shared_plan")
+    p_plan = _operand(plan, "plan", torch.int32, (L.rx_attn_shared_plan_ints(),), dev)
+    _lib.check(L.rx_attn_shared_plan(p[1], p[2], p[3], rows, tables, width, n_q, n_kv, p_plan, p[4], _lib.stream_ptr()), "rx_attn_shared_plan")
     _lib.count()
 
 
@@ -624,27 +632,29 @@ def attn_shared(tk: KvTensorMap, tv: KvTensorMap, q, block_table, row_seq, ctx_l
     64 or 128; n_q * hd a multiple of 128.  A row's last bits depend on the rows beside it: the cut of the work follows the whole window.
     A table row or a context outside the table sets the status and stands for a context of 0.
     `plan`: from `attn_shared_plan` for this window (one serves every layer); None: the call plans for itself."""
-    rows, p = _shared_window(block_table, row_seq, ctx_len, common, status, n_q, n_kv)
+    rows, tables, pages, dev, p = _shared_window(block_table, row_seq, ctx_len, common, status, n_q, n_kv)
     if hd not in (64, 128) or n_q * hd % 128:
         raise ValueError(f"heads of {hd}: 64 or 128, and n_q * hd a multiple of 128")
-    for t, name in ((tk, "K"), (tv, "V")):
-        if t.i8 or t.fp8 != (kv_scale is not None) or tuple(t._keep.shape[1:]) != (n_kv, 64, hd) or t._keep.device != block_table.device:
-            raise ValueError(f"{name} cache: bf16, or E4M3 bytes with kv_scale, [pages, {n_kv}, 64, {hd}] on {block_table.device} is needed")
+    for t in (tk, tv):
+        cache = t._keep
+        if t.i8 or t.fp8 != (kv_scale is not None) or cache.shape[1:] != (n_kv, 64, hd) or cache.get_device() != dev:
+            raise ValueError(f"cache: bf16, or E4M3 bytes with kv_scale, [pages, {n_kv}, 64, {hd}] on cuda:{dev} is needed")
     if out is None and xr is None or (suh is None) != (xr is None):
         raise ValueError("out, or suh with xr, or both are needed")
     L, width = _lib.load(), n_q * hd
-    p_q = _operand(q, "q", torch.bfloat16, (rows, width), block_table)
-    p_out = None if out is None else _operand(out, "out", torch.bfloat16, (rows, width), block_table)
-    p_suh, p_xr = (None, None) if xr is None else (_operand(suh, "suh", torch.float16, (width,), block_table), _operand(xr, "xr", torch.float16, (rows, width), block_table))
-    p_scale = None if kv_scale is None else _operand(kv_scale, "kv_scale", torch.float32, (2, n_kv), block_table)
-    p_plan = None if plan is None else _operand(plan, "plan", torch.int32, (L.rx_attn_shared_plan_ints(),), block_table)
-    p_scratch = _operand(scratch, "scratch", torch.float32, (None,), block_table)
-    if scratch.numel() < L.rx_attn_shared_scratch_floats(rows, n_q, n_kv, hd):
+    p_q = _operand(q, "q", torch.bfloat16, (rows, width), dev)
+    p_out = None if out is None else _operand(out, "out", torch.bfloat16, (rows, width), dev)
+    p_suh, p_xr = (None, None) if xr is None else (_operand(suh, "suh", torch.float16, (width,), dev), _operand(xr, "xr", torch.float16, (rows, width), dev))
+    p_scale = None if kv_scale is None else _operand(kv_scale, "kv_scale", torch.float32, (2, n_kv), dev)
+    p_plan = None if plan is None else _operand(plan, "plan", torch.int32, (L.rx_attn_shared_plan_ints(),), dev)
+    floats = _extents(scratch, "scratch", 1)[0]
+    p_scratch = _operand(scratch, "scratch", torch.float32, (floats,), dev)
+    if floats < L.rx_attn_shared_scratch_floats(rows, n_q, n_kv, hd):
         raise ValueError("scratch: too small (see attn_shared_scratch)")
     if (p_q | p_scratch | (p_plan or 0)) & 15 or ((p_out or 0) | (p_xr or 0)) & 7:
         raise ValueError("q, scratch and plan begin on 16-byte boundaries, out and xr on 8-byte ones")
-    _lib.check(L.rx_attn_shared(tk.rows_ptr, tv.rows_ptr, p_q, p[0], block_table.shape[0], block_table.shape[1], p[1], p[2], p[3], p_scratch, rows, n_q, n_kv, hd, scale,
-                                p_scale, p_suh, p_xr, p_out, p_plan, p[4], _lib.stream_ptr()), "rx_attn_shared")
+    _lib.check(L.rx_attn_shared(tk.rows_ptr, tv.rows_ptr, p_q, p[0], tables, pages, p[1], p[2], p[3], p_scratch, rows, n_q, n_kv, hd, scale, p_scale, p_suh, p_xr, p_out,
+                                p_plan, p[4], _lib.stream_ptr()), "rx_attn_shared")
     _lib.count(2 if plan is not None else 3)
 
 

@@ -183,7 +183,10 @@ def ptr(t) -> int:
 
 
 def stream_ptr() -> int:
+    """The current stream of the current device.  (By way of a torch.cuda.Stream object it took 3.4 us a call, as much as a launch.)"""
     import torch
+    if torch.cuda.is_initialized():
+        return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
     return torch.cuda.current_stream().cuda_stream
 
 
