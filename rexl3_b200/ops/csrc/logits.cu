@@ -158,97 +158,117 @@ __device__ __forceinline__ float pick_rules(float v, uint32_t word, uint32_t dra
   return v;
 }
 
-constexpr int PICK_THREADS = 256, PICK_PER = 32, PICK_CHUNK = PICK_THREADS * PICK_PER, PICK_LIST = 512;
-struct PickShared { uint64_t best[PICK_THREADS], list[PICK_LIST], least; int n; };
+constexpr int PICK_THREADS = 256, PICK_CTAS = 5, PICK_LIST = 512;
+struct PickShared { uint32_t best[PICK_THREADS], least; int n; uint64_t list[PICK_LIST], top[PICK_THREADS / 32]; };
 
-// The `count` largest keys of the block, in descending order, to out (0 where there are fewer).  A thread's candidates come by `each(f)`: f(key) for every one above 0,
-// `mine` is the largest of them.
-// The count-th largest of the maxima of groups of threads is no larger than the count-th largest key, so only keys from there on - hardly more than `count`,
-// with 64 groups for up to half as many - can be among the results; each finds its own place by counting the larger ones.  Where more of them pass than the
-// list holds (one group far below the others), and for one or two results, the block's maximum is taken `count` times.
+// The `count` (<= 64) largest keys of the block, in descending order, to out (0 where there are fewer).  `mine` is the order of the thread's best (0: it has
+// none); each(least, f) calls f(key) for the thread's keys whose order is at least `least` (> 0).
+// As many threads as `count` have an order from the count-th largest of the threads' own best on, so no key with a lower order can be among the results.  One warp
+// searches for that threshold by halving the interval between the lowest and the highest best, and takes a lower one that few more threads pass: the steps that
+// are left would cost more than the few keys.  Each key that passes finds its place by counting the larger ones.
+// Where more pass than the list holds (many equal values, or one thread that has most of the high ones), the block's maximum is taken `count` times.
 template <typename Each>
-__device__ __forceinline__ void pick_select(uint64_t mine, Each each, int count, uint64_t* out, PickShared& sm) {
+__device__ __forceinline__ void pick_select(uint32_t mine, Each each, int count, uint64_t* out, PickShared& sm) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (count > 2) {
-    const int per = count > 32 ? 1 : PICK_THREADS / 64, groups = PICK_THREADS / per;
-    uint64_t m = mine;
-    if (per > 1) {
+  sm.best[tid] = mine;
+  if (tid == 0) sm.n = 0;
+  __syncthreads();
+  if (warp == 0) {
+    constexpr int K = PICK_THREADS / 32;
+    uint32_t b[K], lo = ~0u, hi = 0;
 #pragma unroll
-      for (int o = 1; o < PICK_THREADS / 64; o <<= 1) m = u64_max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int i = 0; i < K; ++i) b[i] = sm.best[i * 32 + lane], lo = min(lo, b[i]), hi = max(hi, b[i]);
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    int pass = PICK_THREADS;                               // threads from lo on; from hi on: too few, or hi is the highest
+    while (pass > count + count / 4 + 2 && lo < hi) {
+      const uint32_t mid = hi - (hi - lo) / 2;
+      int c = 0;
+#pragma unroll
+      for (int i = 0; i < K; ++i) c += b[i] >= mid;
+      c = __reduce_add_sync(0xffffffffu, c);
+      if (c >= count) lo = mid, pass = c;
+      else hi = mid - 1;
     }
-    if (tid % per == 0) sm.best[tid / per] = m;
-    if (tid == 0) sm.n = 0;
-    __syncthreads();
-    if (tid < groups) {
-      const uint64_t own = sm.best[tid];
-      int place = 0;
-#pragma unroll 16
-      for (int j = 0; j < groups; ++j) place += sm.best[j] > own || (sm.best[j] == own && j < tid);
-      if (place == count - 1) sm.least = own;
-    }
-    __syncthreads();
-    const uint64_t least = sm.least;
-    if (mine != 0 && mine >= least)
-      each([&](uint64_t key) {
-        if (key < least) return;
-        const int at = atomicAdd(&sm.n, 1);
-        if (at < PICK_LIST) sm.list[at] = key;
-      });
-    __syncthreads();
-    const int n = sm.n;
-    if (n <= PICK_LIST) {
-      for (int i = tid; i < n; i += PICK_THREADS) {
-        const uint64_t own = sm.list[i];
-        int place = 0;
-#pragma unroll 8
-        for (int j = 0; j < n; ++j) place += sm.list[j] > own;
-        if (place < count) out[place] = own;
-      }
-      for (int r = n + tid; r < count; r += PICK_THREADS) out[r] = 0;
-      __syncthreads();
-      return;
-    }
+    if (lane == 0) sm.least = max(lo, 1u);
   }
-  uint64_t below = ~0ull;                                  // the last maximum
+  __syncthreads();
+  const uint32_t least = sm.least;
+  if (mine >= least)
+    each(least, [&](uint64_t key) {
+      const int at = atomicAdd(&sm.n, 1);
+      if (at < PICK_LIST) sm.list[at] = key;
+    });
+  __syncthreads();
+  const int n = sm.n;
+  if (n <= PICK_LIST) {
+    for (int i = tid; i < n; i += PICK_THREADS) {
+      const uint64_t own = sm.list[i];
+      int place = 0;
+#pragma unroll 8
+      for (int j = 0; j < n; ++j) place += sm.list[j] > own;
+      if (place < count) out[place] = own;
+    }
+    for (int r = n + tid; r < count; r += PICK_THREADS) out[r] = 0;
+    return;
+  }
+  uint64_t below = ~0ull, own = 0;                         // the last maximum; the thread's best that is below it
+  bool again = mine != 0;
   for (int r = 0; r < count; ++r) {
-    uint64_t best = mine < below ? mine : 0;
-    if (mine >= below) each([&](uint64_t key) { if (key < below) best = u64_max(best, key); });
+    if (again) {
+      own = 0;
+      each(1u, [&](uint64_t key) { if (key < below) own = u64_max(own, key); });
+    }
+    uint64_t best = own;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) best = u64_max(best, __shfl_xor_sync(0xffffffffu, best, o));
-    if (lane == 0) sm.best[warp] = best;
+    if (lane == 0) sm.top[warp] = best;
     __syncthreads();
     below = 0;
 #pragma unroll
-    for (int w = 0; w < PICK_THREADS / 32; ++w) below = u64_max(below, sm.best[w]);
+    for (int w = 0; w < PICK_THREADS / 32; ++w) below = u64_max(below, sm.top[w]);
+    again = below != 0 && own == below;
     if (tid == 0) out[r] = below;
     __syncthreads();
   }
 }
 
-// A CTA takes 8192 ids of a row, a thread 32 of them.  VEC: four ids side by side at a time (16-byte loads of logits, 8-byte loads of counts); else one.
+// the value that a word stands for (not 0)
+__device__ __forceinline__ float pick_value(uint32_t order) { return __uint_as_float(order & 0x80000000u ? order & 0x7FFFFFFFu : ~order); }
+// the larger value; a NaN is above all
+__device__ __forceinline__ float pick_max(float a, float b) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
+
+// A CTA takes 256 PER ids of a row, a thread PER of them: VEC: four ids side by side at a time (16-byte loads of logits, 8-byte loads of counts); else one.  Their
+// values stand in shared memory, where the few ids that a rule touches are worked out again by themselves.  The kernel is bound by instructions: what is done
+// for every id is a load, a test of its count, a store, a load and a maximum, and its order is worked out only behind the threshold.
 // Masked ids cost neither their logit nor their count.  An id at -inf is no candidate: it is one only where a row has fewer than `count` ids above -inf, and the
-// second selection finds those by counting.  (As keys, thousands of equal values would all pass the selection's threshold.)
-// Bound by the latency of a chain of loads (slot, mask, logits and counts) and barriers; the larger the chunk, the less of it there is.
-template <bool VEC>
-__global__ void __launch_bounds__(PICK_THREADS, 3) pick_stage1_kernel(const __grid_constant__ PickArgs a) {
+// second selection finds those by counting.
+template <bool VEC, int PER>
+__global__ void __launch_bounds__(PICK_THREADS, PICK_CTAS) pick_stage1_kernel(const __grid_constant__ PickArgs a) {
   pdl_launch();
   pdl_wait();
+  constexpr int W = VEC ? 4 : 1, N = PER / W, CHUNK = PICK_THREADS * PER;
   __shared__ PickShared sm;
-  __shared__ uint32_t s_list[PICK_MAX_BIAS];              // places of the slot's bias list, then rows of the window, whose id is in this chunk
-  __shared__ int s_id[PICK_MAX_BIAS];
-  __shared__ uint32_t s_order[PICK_MAX_BIAS];
-  __shared__ int s_listed;
-  constexpr int W = VEC ? 4 : 1, N = PICK_PER / W;
-  const int row = blockIdx.y, tid = threadIdx.x, base = blockIdx.x * PICK_CHUNK, ids_here = min(a.vocab - base, PICK_CHUNK);
+  __shared__ __align__(16) float s_val[CHUNK];
+  const int row = blockIdx.y, tid = threadIdx.x, base = blockIdx.x * CHUNK, ids_here = min(a.vocab - base, CHUNK);
   const int slot_in = a.row_slot != nullptr ? a.row_slot[row] : -1, slot = slot_in >= 0 && slot_in < a.n_slots ? slot_in : -1;
   const int mrow = a.mask != nullptr ? a.mask_row[row] : -1;
   const bool masked = mrow >= 0 && mrow < a.n_masks;
   const float* lr = a.logits + (size_t)row * a.ld + base;
   const uint16_t* cr = a.counts != nullptr && slot >= 0 ? a.counts + (size_t)slot * a.vocab + base : nullptr;
   const uint32_t* mr = a.mask + (size_t)(masked ? mrow : 0) * a.words + base / 32;
-  if (tid == 0) s_listed = 0;
+  // what the rules need is asked for before the ids' values
+  const int* bid = a.bias_id != nullptr && slot >= 0 ? a.bias_id + (size_t)slot * a.n_bias : nullptr;
+  const int nb = bid != nullptr ? a.n_bias : 0, window = a.first != nullptr && cr != nullptr ? a.first[row] : row;
+  const int bias0 = tid < nb ? bid[tid] : -1, fed0 = a.first != nullptr && tid <= row ? a.fed[row - tid] : -1;
+  float rep = 1.f, freq = 0.f, pres = 0.f;
+  if (cr != nullptr) rep = a.penalties[3 * slot], freq = a.penalties[3 * slot + 1], pres = a.penalties[3 * slot + 2];
   // which of the thread's ids may be taken: of ids (i * 256 + tid) W .. + W - 1, bits i W ..
-  uint32_t ok = 0;
+  uint32_t ok = 0, touched = 0;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int at = (i * PICK_THREADS + tid) * W;
@@ -256,92 +276,89 @@ __global__ void __launch_bounds__(PICK_THREADS, 3) pick_stage1_kernel(const __gr
     if (masked && w != 0) w &= mr[at >> 5] >> (at & 31);
     ok |= w << (i * W);
   }
-  float x[PICK_PER];
-  uint32_t c[VEC ? PICK_PER / 2 : PICK_PER];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int at = (i * PICK_THREADS + tid) * W;
-    const bool some = (ok >> (i * W) & ((1u << W) - 1)) != 0;
+    const uint32_t mine = ok >> (i * W) & ((1u << W) - 1);
     if constexpr (VEC) {
-      const float4 v = some ? *reinterpret_cast<const float4*>(lr + at) : make_float4(0.f, 0.f, 0.f, 0.f);
-      const uint2 n = some && cr != nullptr ? *reinterpret_cast<const uint2*>(cr + at) : make_uint2(0u, 0u);
-      x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
-      c[2 * i] = n.x, c[2 * i + 1] = n.y;
+      float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      uint2 c = make_uint2(0u, 0u);
+      if (mine != 0) {
+        v = *reinterpret_cast<const float4*>(lr + at);
+        if (cr != nullptr) c = *reinterpret_cast<const uint2*>(cr + at);
+      }
+      if (masked) {
+        if (!(mine & 1)) v.x = -INFINITY;
+        if (!(mine & 2)) v.y = -INFINITY;
+        if (!(mine & 4)) v.z = -INFINITY;
+        if (!(mine & 8)) v.w = -INFINITY;
+      }
+      if ((c.x | c.y) != 0)
+        touched |= ((c.x & 0xFFFFu ? 1u : 0u) | (c.x >> 16 ? 2u : 0u) | (c.y & 0xFFFFu ? 4u : 0u) | (c.y >> 16 ? 8u : 0u)) << (i * W);
+      *reinterpret_cast<float4*>(s_val + at) = v;
     } else {
-      x[i] = some ? lr[at] : 0.f;
-      c[i] = some && cr != nullptr ? cr[at] : 0u;
+      const float v = mine ? lr[at] : -INFINITY;
+      if (mine && cr != nullptr && cr[at] != 0) touched |= 1u << i;
+      s_val[at] = v;
     }
   }
-  float rep = 1.f, freq = 0.f, pres = 0.f;
-  if (cr != nullptr) rep = a.penalties[3 * slot], freq = a.penalties[3 * slot + 1], pres = a.penalties[3 * slot + 2];
-  __syncthreads();
-  // ids with a bias or among the drafts: few, and in few chunks
-  const int* bid = a.bias_id != nullptr && slot >= 0 ? a.bias_id + (size_t)slot * a.n_bias : nullptr;
-  const float* bval = a.bias_val + (size_t)max(slot, 0) * a.n_bias;
-  const int nb = bid != nullptr ? a.n_bias : 0, r0 = a.first != nullptr && cr != nullptr ? max(a.first[row], 0) + 1 : row + 1;
-  for (int e = tid; e < nb; e += PICK_THREADS)
-    if (bid[e] >= base && bid[e] - base < ids_here) {
-      const int at = atomicAdd(&s_listed, 1);
-      if (at < PICK_MAX_BIAS) s_list[at] = e;
-    }
-  for (int r = r0 + tid; r <= row; r += PICK_THREADS)
-    if (a.fed[r] >= base && a.fed[r] - base < ids_here) {
-      const int at = atomicAdd(&s_listed, 1);
-      if (at < PICK_MAX_BIAS) s_list[at] = PICK_MAX_BIAS + r;
-    }
-  uint32_t u[PICK_PER];
-#pragma unroll
-  for (int i = 0; i < PICK_PER; ++i) {
-    const uint32_t word = VEC ? c[i / 2] >> (16 * (i & 1)) & 0xFFFFu : c[VEC ? 0 : i];
-    const float v = pick_rules(x[i], word, 0, rep, freq, pres);
-    u[i] = (ok >> i & 1) && v != -INFINITY ? pick_order(v) : 0;
+  while (touched != 0) {
+    const int i = __ffs(touched) - 1, at = (i / W * PICK_THREADS + tid) * W + i % W;
+    touched &= touched - 1;
+    const float v = s_val[at];
+    if (v != -INFINITY) s_val[at] = pick_rules(v, cr[at], 0, rep, freq, pres);                     // at -inf it stays, and a masked id is there
   }
-  __syncthreads();
-  const int listed = s_listed;
-  if (listed > 0) {
-    // Such an id is worked out again by itself, by a thread per place in the list (an id more than once: the same each time), and put in its owner's place.  A
-    // window with more drafts in the chunk than the list holds is gone over whole.
-    const int from = min(listed, PICK_MAX_BIAS), all = listed <= PICK_MAX_BIAS ? from : nb + max(row - r0 + 1, 0);
-    for (int l0 = 0; l0 < all; l0 += PICK_MAX_BIAS) {
-      const int here = min(PICK_MAX_BIAS, all - l0);
-      __syncthreads();
-      for (int l = tid; l < here; l += PICK_THREADS) {
-        const int e = listed <= PICK_MAX_BIAS ? (int)s_list[l] : l0 + l < nb ? l0 + l : PICK_MAX_BIAS + r0 + l0 + l - nb;
-        const int id = e < PICK_MAX_BIAS ? bid[e] : a.fed[e - PICK_MAX_BIAS];
-        s_id[l] = id >= base && id - base < ids_here ? id - base : -1;
-        if (s_id[l] < 0) continue;
-        uint32_t drafts = 0;
-        for (int r = r0; r <= row; ++r) drafts += a.fed[r] == id;
-        float v = pick_rules(lr[id - base], cr != nullptr ? cr[id - base] : 0u, drafts, rep, freq, pres), sum = 0.f;
-        bool any = false;
-        for (int f = 0; f < nb; ++f)
-          if (bid[f] == id) sum = any ? __fadd_rn(sum, bval[f]) : bval[f], any = true;
-        if (any) v = __fadd_rn(v, sum);
-        s_order[l] = v != -INFINITY ? pick_order(v) : 0;
-      }
-      __syncthreads();
-      for (int l = 0; l < here; ++l) {
-        const int at = s_id[l];
-        if (at < 0 || at / W % PICK_THREADS != tid) continue;
-        const int mine = at / W / PICK_THREADS * W + at % W;
+  // ids with a bias or among the drafts, where there are any in this chunk
+  const int r0 = max(window, 0) + 1;
+  bool special = bias0 >= base && bias0 - base < ids_here;
+  if (row - tid >= r0) special |= fed0 >= base && fed0 - base < ids_here;
+  for (int e = tid + PICK_THREADS; e < nb; e += PICK_THREADS) special |= bid[e] >= base && bid[e] - base < ids_here;
+  for (int r = row - tid - PICK_THREADS; r >= r0; r -= PICK_THREADS) special |= a.fed[r] >= base && a.fed[r] - base < ids_here;
+  if (__syncthreads_or(special)) {
+    // each such id again, with its drafts and biases (an id more than once: the same each time)
+    const float* bval = a.bias_val + (size_t)slot * a.n_bias;
+    for (int l = tid; l < nb + row - r0 + 1; l += PICK_THREADS) {
+      const int id = l < nb ? bid[l] : a.fed[r0 + l - nb], at = id - base;
+      if (id < base || at >= ids_here || (masked && !(mr[at >> 5] >> (at & 31) & 1))) continue;
+      uint32_t drafts = 0;
+      for (int r = r0; r <= row; ++r) drafts += a.fed[r] == id;
+      float v = pick_rules(lr[at], cr != nullptr ? cr[at] : 0u, drafts, rep, freq, pres), sum = 0.f;
+      bool any = false;
+      for (int f = 0; f < nb; ++f)
+        if (bid[f] == id) sum = any ? __fadd_rn(sum, bval[f]) : bval[f], any = true;
+      s_val[at] = any ? __fadd_rn(v, sum) : v;
+    }
+    __syncthreads();
+  }
+  float top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < PICK_PER; ++i)
-          if (i == mine) u[i] = ok >> i & 1 ? s_order[l] : 0;
-      }
+  for (int i = 0; i < N; ++i) {
+    const int at = (i * PICK_THREADS + tid) * W;
+    if constexpr (VEC) {
+      const float4 v = *reinterpret_cast<const float4*>(s_val + at);
+      top = pick_max(top, pick_max(pick_max(v.x, v.y), pick_max(v.z, v.w)));
+    } else {
+      top = pick_max(top, s_val[at]);
     }
   }
-  // the thread's best: the lowest of its ids with the highest order (they ascend with i)
-  uint32_t top = 0;
-  int first = 0;
-#pragma unroll
-  for (int i = 0; i < PICK_PER; ++i)
-    if (u[i] > top) top = u[i], first = i;
-  auto id = [&](int i) { return base + ((i / W) * PICK_THREADS + tid) * W + i % W; };
-  pick_select(top != 0 ? pick_key(top, id(first)) : 0,
-              [&](auto f) {
-#pragma unroll
-                for (int i = 0; i < PICK_PER; ++i)
-                  if (u[i] != 0) f(pick_key(u[i], id(i)));
+  pick_select(top != -INFINITY ? pick_order(top) : 0u,
+              [&](uint32_t least, auto f) {
+                const float from = pick_value(least);      // a NaN: the values say nothing yet
+#pragma unroll 4
+                for (int i = 0; i < N; ++i) {
+                  const int at = (i * PICK_THREADS + tid) * W;
+                  if constexpr (VEC) {
+                    const float4 v = *reinterpret_cast<const float4*>(s_val + at);
+                    if (pick_max(pick_max(v.x, v.y), pick_max(v.z, v.w)) < from) continue;
+                  }
+#pragma unroll 1
+                  for (int k = 0; k < W; ++k) {
+                    const float v = s_val[at + k];
+                    if (v < from || v == -INFINITY) continue;
+                    const uint32_t order = pick_order(v);
+                    if (order >= least) f(pick_key(order, base + at + k));
+                  }
+                }
               },
               a.count, a.cand + ((size_t)row * a.nchunks + blockIdx.x) * a.count, sm);
 }
@@ -355,18 +372,19 @@ __global__ void __launch_bounds__(PICK_THREADS) pick_stage2_kernel(const uint64_
   const int row = blockIdx.x;
   const uint64_t* c = cand + (size_t)row * total;
   constexpr int PER = 16;
-  uint64_t k[PER], mine = 0;
+  uint64_t k[PER];
+  uint32_t mine = 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int j = i * PICK_THREADS + threadIdx.x;
     k[i] = j < total ? c[j] : 0;
-    mine = u64_max(mine, k[i]);
+    mine = max(mine, (uint32_t)(k[i] >> 32));
   }
   pick_select(mine,
-              [&](auto f) {
+              [&](uint32_t least, auto f) {
 #pragma unroll
                 for (int i = 0; i < PER; ++i)
-                  if (k[i] != 0) f(k[i]);
+                  if ((uint32_t)(k[i] >> 32) >= least) f(k[i]);
               },
               count, outk, sm);
   __syncthreads();
@@ -377,15 +395,17 @@ __global__ void __launch_bounds__(PICK_THREADS) pick_stage2_kernel(const uint64_
     id = (int)(~(uint32_t)outk[threadIdx.x]);
     v = topk_val(outk[threadIdx.x]);
   } else {
-    // fewer ids above -inf than places: the lowest of the other ids, which all stand at -inf, in order
+    // Fewer ids above -inf than places: the lowest of the other ids, which all stand at -inf, in order.  The q-th id that is not among n others is q + (how
+    // many of those are not above it).
     int n = 0;
     while (n < count && outk[n] != 0) ++n;
-    int left = (int)threadIdx.x - n;                       // ids at -inf before this place's
-    for (id = 0;; ++id) {
-      bool taken = false;
-      for (int j = 0; j < n; ++j) taken |= (int)(~(uint32_t)outk[j]) == id;
-      if (!taken && left-- == 0) break;
-    }
+    const int q = (int)threadIdx.x - n;
+    int passed = 0;
+    do {
+      id = q + passed;
+      passed = 0;
+      for (int j = 0; j < n; ++j) passed += (int)(~(uint32_t)outk[j]) <= id;
+    } while (q + passed != id);
   }
   ids[(size_t)row * count + threadIdx.x] = id;
   vals[(size_t)row * count + threadIdx.x] = v;
@@ -425,7 +445,8 @@ RX_API int rx_token_counts_add(void* counts, int n_slots, int vocab, const void*
 RX_API int rx_topk_adjusted(const void* logits, long long ld, int rows, int vocab, int count, void* scratch, void* ids, void* vals, const void* row_slot,
                             const void* counts, const void* penalties, int n_slots, const void* bias_id, const void* bias_val, int n_bias, const void* mask,
                             const void* mask_row, int n_masks, const void* first, const void* fed, void* stream) {
-  const int nchunks = (vocab + PICK_CHUNK - 1) / PICK_CHUNK;
+  const bool small = (long long)rows * ((vocab + 4095) / 4096) <= 148 * PICK_CTAS;
+  const int nchunks = small ? (vocab + 4095) / 4096 : (vocab + 8191) / 8192;
   if (rows < 1 || rows > 65535 || vocab < 1 || count < 1 || count > 64 || count > vocab || (long long)nchunks * count > PICK_THREADS * 16 || ld < vocab || n_bias < 0 || n_bias > PICK_MAX_BIAS)
     return (int)cudaErrorInvalidValue;
   PickArgs a = {(const float*)logits, (const int*)row_slot, (const uint16_t*)counts, (const float*)penalties, (const int*)bias_id, (const float*)bias_val,
@@ -434,7 +455,8 @@ RX_API int rx_topk_adjusted(const void* logits, long long ld, int rows, int voca
   // four ids at a time where every row of logits and counts begins on a 16- and an 8-byte boundary
   const bool vec = vocab % 4 == 0 && ld % 4 == 0 && ((uintptr_t)logits & 15) == 0 && ((uintptr_t)counts & 7) == 0;
   cudaStream_t st = (cudaStream_t)stream;
-  cudaError_t e = rx::launch(vec ? pick_stage1_kernel<true> : pick_stage1_kernel<false>, dim3(nchunks, rows), dim3(PICK_THREADS), 0, st, a);
+  const auto stage1 = small ? (vec ? pick_stage1_kernel<true, 16> : pick_stage1_kernel<false, 16>) : vec ? pick_stage1_kernel<true, 32> : pick_stage1_kernel<false, 32>;
+  cudaError_t e = rx::launch(stage1, dim3(nchunks, rows), dim3(PICK_THREADS), 0, st, a);
   if (e != cudaSuccess) return (int)e;
   return (int)rx::launch(pick_stage2_kernel, dim3(rows), dim3(PICK_THREADS), 0, st, (const uint64_t*)scratch, nchunks * count, count, (int*)ids, (float*)vals);
 }
