@@ -33,8 +33,9 @@ constexpr int SH_MIN_SHARED = 1;                        // pages that a group mu
 constexpr int SH_SEGMENT = 2;                           // what a unit costs beside its pages, in pages: its place in the line is that much longer
 
 // ------------------------------------------------------------------------------------------------ plan
-// Layout (int32): [0] length of the line  [1] a CTA's piece  [2] blocks  [3] n_kv, then the block at which each CTA begins, the blocks, and per row its
-// block over common pages, its block over own pages (-1: none), the keys it sees and nothing.
+// Layout (int32): [0] length of the line  [1] a CTA's piece  [2] blocks  [3] n_kv, then the block at which each CTA begins, the blocks, per row what the merge
+// asks of its block over common pages and of its block over own pages - length of the blocks before, pages (0: no block), the row's partial vectors, copies -,
+// and the keys that each row sees.
 struct ShBlock {
   int row, rows;          // first row; rows, and << 8 how many CTAs a unit can meet
   int seq;                // table row
@@ -46,12 +47,12 @@ struct ShBlock {
 static_assert(sizeof(ShBlock) == 32, "two 16-byte loads");
 constexpr int SH_HEAD = 8, SH_AT_BLOCKS = SH_HEAD + ((SH_CTAS + 7) / 8) * 8;
 constexpr int SH_AT_ROWS = SH_AT_BLOCKS + 2 * SH_MAX_ROWS * 8;
-constexpr int SH_PLAN_INTS = SH_AT_ROWS + 4 * SH_MAX_ROWS + 4;      // (with room to align it)
+constexpr int SH_AT_KEYS = SH_AT_ROWS + 8 * SH_MAX_ROWS, SH_PLAN_INTS = SH_AT_KEYS + SH_MAX_ROWS + 4;      // (with room to align it)
 
 __device__ __forceinline__ int sh_slots(int pages, int L) { return (pages + L - 1) / L + 1; }      // CTAs that a unit of `pages` pages can meet
 __device__ __forceinline__ int sh_copies(int pairs) { return pairs <= 32 ? 4 : pairs <= 64 ? 2 : 1; }
 // where the pages of a unit begin in the line
-__device__ __forceinline__ int sh_unit(const ShBlock& b, int kvh, int n_kv) { return b.before * n_kv + kvh * (b.pages + SH_SEGMENT) + SH_SEGMENT; }
+__device__ __forceinline__ int sh_unit(int before, int pages, int kvh, int n_kv) { return before * n_kv + kvh * (pages + SH_SEGMENT) + SH_SEGMENT; }
 
 // inclusive sum over the block's threads; `all` gets the total
 __device__ __forceinline__ int block_scan(int v, int* s_warp, int& all) {
@@ -135,22 +136,26 @@ __global__ void __launch_bounds__(SH_MAX_ROWS) shared_plan_kernel(const int* __r
   const int all_s = all;
   const int v_o = block_scan(lead_o ? k_o : 0, s_warp, all);
   ShBlock* blk = reinterpret_cast<ShBlock*>(plan + SH_AT_BLOCKS);
-  // (s_seq and s_link are free: the ids of the blocks that begin at a row)
+  // (s_link and s_first, then s_seq and s_gfirst are free: length and partial vectors before the block that begins at a row)
   __syncthreads();
   if (lead_s) {
     const int id = (b_in & 0xFFFF) - 1;
-    s_link[r] = id, s_before[id] = p_s - len_s;
+    s_link[r] = s_before[id] = p_s - len_s, s_first[r] = v_s - k_s;
     blk[id] = ShBlock{r, n_s | sh_slots(shared, L) << 8, s_seq[gfirst], 0, shared, p_s - len_s, v_s - k_s, s_gmost[group]};
   }
   __syncthreads();
   if (lead_o) {
     const int id = nb_s + (b_in >> 16) - 1;
-    s_seq[r] = id, s_before[id] = pages_s + p_o - len_o;
+    s_seq[r] = s_before[id] = pages_s + p_o - len_o, s_gfirst[r] = all_s + v_o - k_o;
     blk[id] = ShBlock{r, n_o | sh_slots(own, L) << 8, seq, shared, own, pages_s + p_o - len_o, all_s + v_o - k_o, s_most[chunk]};
   }
   __syncthreads();
   if (live) {
-    reinterpret_cast<int4*>(plan + SH_AT_ROWS)[r] = make_int4(shared > 0 ? s_link[tile] : -1, own > 0 ? s_seq[chunk] : -1, ctx, 0);
+    const int c_s = sh_copies(n_s * G), c_o = sh_copies(n_o * G);
+    int4* of = reinterpret_cast<int4*>(plan + SH_AT_ROWS) + 2 * r;
+    of[0] = shared > 0 ? make_int4(s_link[tile], shared, s_first[tile] + (r - tile) * sh_slots(shared, L) * c_s, c_s) : make_int4(0, 0, 0, 0);
+    of[1] = own > 0 ? make_int4(s_seq[chunk], own, s_gfirst[chunk] + (r - chunk) * sh_slots(own, L) * c_o, c_o) : make_int4(0, 0, 0, 0);
+    plan[SH_AT_KEYS + r] = ctx;
   }
   for (int c = r; c < SH_CTAS; c += blockDim.x) {
     int lo = 0, hi = nb - 1;
@@ -352,7 +357,8 @@ __device__ __forceinline__ void sh_st_zero(uint32_t taddr) {
   sh_st(taddr, z);
 }
 
-// One row's query heads of a KV head: 64 of their values each, from [rows][n_q][hd]
+// The query heads of a KV head, 64 of their values each, from [rows][n_q][hd]: of as many rows at once as fill a quarter of the pairs
+__host__ __device__ constexpr int sh_box_rows(int G) { return G > 32 ? 1 : 32 / G; }
 __device__ __forceinline__ void sh_load_q(void* dst, const void* tmap, int x, int head, int row, uint64_t* bar) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)), "l"(tmap),
                "r"(smem_u32(bar)), "r"(x), "r"(head), "r"(row)
@@ -440,7 +446,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
       const int rb = pair / G, hq = d.kvh * G + pair % G;
       const bool live = rb < d.rows, some = copies > 1 || warp * 32 < pairs;         // (uniform) the warp holds a pair
       // keys from the segment's first on that the pair sees (a lane without a pair: nothing to mask, nothing comes of it)
-      const int keys = live ? a.plan[SH_AT_ROWS + 4 * (d.row + rb) + 2] - d.key0 : 0x7FFFFFFF;
+      const int keys = live ? a.plan[SH_AT_KEYS + d.row + rb] - d.key0 : 0x7FFFFFFF;
       const float scale_log2 = F8 ? a.scale_log2 * a.kv_scale[d.kvh] : a.scale_log2;
       float m = -INFINITY, l = 0.f;                       // running maximum (log2 units), sum
       // Keys that no row sees yet: their V may hold anything, and 0 * NaN would reach every pair.  (The barrier of V's stage cannot stand a page's use behind: that
@@ -603,12 +609,12 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
   } else if (warp == 4) {
     // ---------------------------------------------------------------- feeder: descriptions and queries of the segments; K and V each at their own pace
     // One warp's ordinary code is slow (some five cycles an instruction), so it does little of it: a segment is looked up once for everybody, and its
-    // queries come by TMA, a row's heads of one KV head per copy (by plain copies, 125 pairs took 25,000 cycles).
+    // queries come by TMA, several rows' heads of one KV head per copy (by plain copies, 125 pairs took 25,000 cycles, by a copy a row 5000).
     // (With K and V in turn, K page n + 2 waited for V page n + 1 and so for PV(n - 1), and a page took as long as a K page's way from memory.)
     // Of eight descriptions the one that is overwritten, segment w - 8's, is out of use: V has begun segment w - 1, with a page whose copy waited for the PV of a page
     // two (E4M3: four) earlier, in segment w - 5 or later, and that PV for all softmax warps to leave the segments before.
     ShWalk walk(a.plan, a.n_kv);
-    int known = 0, asked = 0, queries = 0, idle = 0;      // segments with a description, with queries; the last one whose queries were fetched, + 1
+    int known = 0, asked = 0, queries = 0, converted = 0, idle = 0;      // segments with a description, with queries; the last one whose queries were fetched, + 1
     bool more = true;
     uint64_t since = 0;
     // lane 0 brings K, lane 1 V: the ring's place, and the pages that are left of the lane's segment
@@ -616,33 +622,16 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
     uint64_t *full = F8 ? raw_full + who * C::RS : who ? v_full : k_full, *empty = F8 ? raw_empty + who * C::RS : who ? v_empty : k_empty;
     uint8_t* to = F8 ? raw + who * C::RS * C::RAW : who ? v_sm : k_sm;
     const CUtensorMap* map = who ? &tv : &tk;
-    const int* table = nullptr;
-    int at = 0, begun = 0, st = 0, round = 0, left = 0, kvh = 0, copied = 0;      // segments looked at, and begun; the ring's place; pages left of the segment, asked for
+    const int* table = nullptr;                            // of the lane's segment, behind the page that comes next: that one is known before its place is free
+    int at = 0, next = 0, begun = 0, st = 0, round = 0, left = 0, kvh = 0, copied = 0;      // segments looked at, and begun; the ring's place; pages left of the segment, asked for
     bool done = lane > 1;
-    while (more || asked < known || __any_sync(0xffffffffu, !done)) {
+    while (more || asked < known || (F8 && converted < queries) || __any_sync(0xffffffffu, !done)) {
       bool moved = false;
-      if (!done) {
-        if (left == 0 && at < known) {
-          const ShDesc& d = desc[at & 7];
-          left = d.pages, table = d.table, kvh = d.kvh;
-          done = left == 0;
-          ++at;
-        }
-        if (left != 0 && (round == 0 || mbar_test_wait(&empty[st], (round - 1) & 1))) {
-          const int y = (*table * a.n_kv + kvh) * SH_PAGE;
-          mbar_arrive_expect_tx(&full[st], C::COPY);
-#pragma unroll
-          for (int x = 0; x < (F8 ? 1 : BOXES); ++x) tma_load_2d(to + st * C::COPY + x * 8192, map, x * 64, y, &full[st]);
-          ++table, --left, ++copied;
-          begun = at;
-          if (++st == S) st = 0, ++round;
-          moved = true;
-        }
-      }
-      __syncwarp();
       if (asked < known && (asked == 0 || all_ok(mbar_test_wait(q_free, (asked - 1) & 1)))) {
         const ShDesc& d = desc[asked & 7];
-        const int rows = d.pages != 0 ? d.rows : 0, copies = sh_copies(rows * G), bytes = rows * copies * G * HD * 2;
+        // (the last box of several begins early enough to end with the block; one alone may reach rows behind it, which nothing comes of)
+        const int rows = d.pages != 0 ? d.rows : 0, copies = sh_copies(rows * G), most = sh_box_rows(G), boxes = (rows + most - 1) / most;
+        const int bytes = boxes * most * copies * G * HD * 2;
         uint64_t* bar = F8 ? q_there : &q_ready[asked & 3];
         if (lane == 0) {
           if (bytes != 0) mbar_arrive_expect_tx(bar, bytes);
@@ -650,32 +639,55 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         }
         __syncwarp();
         // 128-byte rows at any multiple of 128 bytes: the swizzle goes by the address, so chunk c of pair p stands at c ^ (p & 7)
-        for (int i = lane; i < rows * copies * BOXES; i += 32) {
-          const int x = i % BOXES, t = i / BOXES % copies, r = i / BOXES / copies;
+        for (int i = lane; i < boxes * copies * BOXES; i += 32) {
+          const int x = i % BOXES, t = i / BOXES & (copies - 1), b = i / BOXES >> (copies >> 1), r = b + 1 < boxes || b == 0 ? b * most : rows - most;
           sh_load_q(q_sm + x * C::QBOX + (t * (SH_PAIRS / copies) + r * G) * 128, &tq, x * 64, d.kvh * G, d.row + r, bar);
         }
         __syncwarp();
         if (rows != 0) queries = asked + 1;
-        if (F8 && rows != 0) {                            // bf16 -> fp16 in place, beside the fp16 values of an E4M3 cache
-          if (!all_ok(sh_wait(q_there, asked & 1, abort_flag, a.status, 112))) break;
-          for (int t = 0; t < copies; ++t)
-#pragma unroll
-            for (int x = 0; x < BOXES; ++x) {
-              const uint32_t at = smem_u32(q_sm + x * C::QBOX + t * (SH_PAIRS / copies) * 128);
-#pragma unroll 4
-              for (int i = lane; i < rows * G * 8; i += 32) {
-                uint4 v = lds128(at + i * 16);
-                uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-                for (int u = 0; u < 4; ++u) w[u] = sh_pack<true>(__uint_as_float(w[u] << 16), __uint_as_float(w[u] & 0xFFFF0000u));
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + i * 16), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-              }
-            }
-          fence_proxy_async();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&q_ready[asked & 3]);
-        }
         ++asked;
+        moved = true;
+      }
+      if (!done) {
+        if (left == 0 && at < known) {
+          const ShDesc& d = desc[at & 7];
+          left = d.pages, table = d.table, kvh = d.kvh;
+          done = left == 0;
+          if (!done) next = *table++;
+          ++at;
+        }
+        if (left != 0 && (round == 0 || mbar_test_wait(&empty[st], (round - 1) & 1))) {
+          const int y = (next * a.n_kv + kvh) * SH_PAGE;
+          mbar_arrive_expect_tx(&full[st], C::COPY);
+#pragma unroll
+          for (int x = 0; x < (F8 ? 1 : BOXES); ++x) tma_load_2d(to + st * C::COPY + x * 8192, map, x * 64, y, &full[st]);
+          if (--left != 0) next = *table++;
+          ++copied;
+          begun = at;
+          if (++st == S) st = 0, ++round;
+          moved = true;
+        }
+      }
+      __syncwarp();
+      if (F8 && converted < queries && all_ok(mbar_test_wait(q_there, converted & 1))) {      // bf16 -> fp16 in place, beside the fp16 values of an E4M3 cache
+        const int rows = desc[converted & 7].rows, copies = sh_copies(rows * G);
+        for (int t = 0; t < copies; ++t)
+#pragma unroll
+          for (int x = 0; x < BOXES; ++x) {
+            const uint32_t at = smem_u32(q_sm + x * C::QBOX + t * (SH_PAIRS / copies) * 128);
+#pragma unroll 4
+            for (int i = lane; i < rows * G * 8; i += 32) {
+              uint4 v = lds128(at + i * 16);
+              uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+              for (int u = 0; u < 4; ++u) w[u] = sh_pack<true>(__uint_as_float(w[u] << 16), __uint_as_float(w[u] & 0xFFFF0000u));
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + i * 16), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+            }
+          }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_ready[converted & 3]);
+        ++converted;
         moved = true;
       }
       if (more && (known < 8 || __shfl_sync(0xffffffffu, begun, 1) >= known)) {
@@ -828,40 +840,40 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
 // ------------------------------------------------------------------------------------------------ merge
 // Joins a row's partial outputs, common pages before own, CTA by CTA: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  A warp per 128 outputs; with
 // `suh` also xr = fp16(H(out * suh)), the input rotation of the output projection.
+// Bound by latency, so all partial outputs of a turn are on their way at once (25 rows of 31 each: 40 -> 37 us of the whole call, against eight at a time; four
+// warps for each 128 outputs and a sum over shared memory: 38 us, but 48 rows of 14 each 86 -> 90 us).
 template <int HD>
 __global__ void __launch_bounds__(128) attn_shared_merge_kernel(const int* plan, const float* part_o, const float* part_ml, int n_q, int n_kv,
                                                                 const __half* __restrict__ suh, __half* __restrict__ xr, uint16_t* __restrict__ out) {
   pdl_launch();
+  const int row = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, width = n_q * HD, b = blockIdx.y * 4 + warp;
+  const int e0 = b * 128 + lane * 4, hq = e0 / HD, d0 = e0 % HD, kvh = hq / (n_q / n_kv);
   pdl_wait();
-  const int row = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, width = n_q * HD;
-  const int b = blockIdx.y * 4 + warp;
   if (b >= width / 128) return;                           // (a whole warp)
-  const int e0 = b * 128 + lane * 4, hq = e0 / HD, d0 = e0 % HD, kvh = hq / (n_q / n_kv), L = plan[1];
-  const ShBlock* blk = reinterpret_cast<const ShBlock*>(plan + SH_AT_BLOCKS);
+  const int L = plan[1];
+  const int4* of = reinterpret_cast<const int4*>(plan + SH_AT_ROWS) + 2 * row;
   size_t at[2] = {0, 0};
   int n[2] = {0, 0};
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    const int id = plan[SH_AT_ROWS + 4 * row + u];
-    if (id < 0) continue;
-    const ShBlock s = blk[id];
-    const int unit = sh_unit(s, kvh, n_kv), copies = sh_copies((s.rows & 255) * (n_q / n_kv));
-    n[u] = ((unit + s.pages - 1) / L - unit / L + 1) * copies;
-    at[u] = (size_t)(s.part + (row - s.row) * (s.rows >> 8) * copies) * n_q + hq;
+    const int4 s = of[u];                                  // before, pages, partial vectors, copies
+    if (s.y == 0) continue;
+    const int unit = sh_unit(s.x, s.y, kvh, n_kv);
+    n[u] = ((unit + s.y - 1) / L - unit / L + 1) * s.w;
+    at[u] = (size_t)s.z * n_q + hq;
   }
   auto slot = [&](int s) { return s < n[0] ? at[0] + (size_t)s * n_q : at[1] + (size_t)(s - n[0]) * n_q; };
   const int all = n[0] + n[1];
-  // A head's GL lanes take GL slots at a time, lane = slot for the maxima and factors, with eight partial outputs on their way at once.  (Two heads of 64 in a warp
-  // may have unlike numbers of slots.)
-  constexpr int GL = HD / 4, U = 8;
+  // A head's GL lanes take GL slots at a time, lane = slot for the maxima and factors.  (Two heads of 64 in a warp may have unlike numbers of slots.)
+  constexpr int GL = HD / 4;
   const int gl = lane % GL, g0 = lane - gl, most = HD == 128 ? all : max(all, __shfl_xor_sync(0xffffffffu, all, 16));
   float acc[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f, m = -INFINITY;
   for (int s0 = 0; s0 < most; s0 += GL) {
     const int here = min(GL, all - s0);                   // (of the other head of the warp, maybe none)
     const float2 ml = gl < here ? *reinterpret_cast<const float2*>(part_ml + slot(s0 + gl) * 2) : make_float2(-INFINITY, 0.f);
-    float4 o[U];
+    float4 o[GL];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < GL; ++u)
       if (u < here) o[u] = *reinterpret_cast<const float4*>(part_o + slot(s0 + u) * HD + d0);
     float top = ml.x;
 #pragma unroll
@@ -872,13 +884,10 @@ __global__ void __launch_bounds__(128) attn_shared_merge_kernel(const int* plan,
     l = l * old + f * ml.y;                               // (lane = slot: added up at the end)
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] *= old;
-    for (int u0 = 0; u0 < min(GL, most - s0); u0 += U) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const float g = __shfl_sync(0xffffffffu, f, g0 + u0 + u);
-        if (u0 + u < here) acc[0] += g * o[u].x, acc[1] += g * o[u].y, acc[2] += g * o[u].z, acc[3] += g * o[u].w;
-        if (u0 + U + u < here) o[u] = *reinterpret_cast<const float4*>(part_o + slot(s0 + u0 + U + u) * HD + d0);
-      }
+    for (int u = 0; u < GL; ++u) {
+      const float g = __shfl_sync(0xffffffffu, f, g0 + u);
+      if (u < here) acc[0] += g * o[u].x, acc[1] += g * o[u].y, acc[2] += g * o[u].z, acc[3] += g * o[u].w;
     }
   }
 #pragma unroll
@@ -906,7 +915,7 @@ static cudaError_t launch_shared(int dev, const CUtensorMap& tk, const CUtensorM
   return rx::launch(attn_shared_kernel<HD, F8>, dim3(SH_CTAS), dim3(Sh<HD, F8>::THREADS), Sh<HD, F8>::SMEM, st, tk, tv, tq, a);
 }
 
-// The queries [rows][n_q][hd] by boxes of one row's G heads, 64 values of each.
+// The queries [rows][n_q][hd] by boxes of some rows' G heads, 64 values of each.
 static bool sh_query_map(CUtensorMap* map, const void* q, int rows, int n_q, int G, int hd) {
   typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
                              CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -918,7 +927,7 @@ static bool sh_query_map(CUtensorMap* map, const void* q, int rows, int n_q, int
     encode = (Encode)p;
   }
   const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)n_q, (cuuint64_t)rows}, strides[2] = {(cuuint64_t)hd * 2, (cuuint64_t)n_q * hd * 2};
-  const cuuint32_t box[3] = {64, (cuuint32_t)G, 1}, steps[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)sh_box_rows(G)}, steps[3] = {1, 1, 1};
   return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                 CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -979,6 +988,6 @@ RX_API int rx_attn_shared(const void* tmap_k, const void* tmap_v, const void* q,
   else e = kv_scale != nullptr ? launch_shared<64, true>(dev, tk, tv, tq, a, st) : launch_shared<64, false>(dev, tk, tv, tq, a, st);
   if (e != cudaSuccess) return (int)e;
   // (early whatever the grid: the kernel before is one wave whose CTAs leave room beside them)
-  return (int)rx::launch_pdl(true, hd == 128 ? attn_shared_merge_kernel<128> : attn_shared_merge_kernel<64>, dim3(rows, (n_q * hd / 128 + 3) / 4), dim3(128), 0, st, a.plan, a.part_o,
-                         a.part_ml, n_q, n_kv, (const __half*)suh, (__half*)xr, (uint16_t*)out);
+  return (int)rx::launch_pdl(true, hd == 128 ? attn_shared_merge_kernel<128> : attn_shared_merge_kernel<64>, dim3(rows, (n_q * hd / 128 + 3) / 4), dim3(128), 0, st, a.plan,
+                             a.part_o, a.part_ml, n_q, n_kv, (const __half*)suh, (__half*)xr, (uint16_t*)out);
 }
