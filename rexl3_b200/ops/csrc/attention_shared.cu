@@ -799,33 +799,48 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
   } else if constexpr (F8) {
     // ---------------------------------------------------------------- expansion of byte pages: E4M3 -> fp16 (exact) in the operand layout
     // A warp takes half of every page of K or of V.  (Straight from global memory, a page ahead in registers, a page took 3300 cycles: the way of plain loads.)
+    // Eight lanes take two keys, of 128-byte rows a half each: neither loads nor stores then meet in a bank.
     const int v = (warp - 6) >> 1, half = warp & 1, S = v ? VS : KS;
     uint64_t *full = v ? v_full : k_full, *empty = v ? v_empty : k_empty, *rfull = raw_full + v * C::RS, *rempty = raw_empty + v * C::RS;
+    // (bytes) lane's first 16 values of a page, of even and - rows of 128 bytes - odd turns; where they go, in two chunks; from turn to turn (pair of turns to pair) both
+    // move by whole groups of eight keys
+    constexpr int TURNS = HD / 16, ODD = HD == 128 ? 2 : 1;
+    const int key = half * 32 + (HD == 128 ? (lane >> 3) * 2 + (lane >> 2 & 1) : lane >> 2);
+    uint32_t from[ODD], into[ODD][2];
+#pragma unroll
+    for (int o = 0; o < ODD; ++o) {
+      const int x = (lane & 3) + (HD == 128 ? 4 * ((lane >> 2 & 1) ^ o) : 0);
+      from[o] = key * HD + x * 16;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int ch = 2 * x + u;                         // 16-byte chunk of the fp16 row
+        into[o][u] = (ch >> 3) * 8192 + key * 128 + (((ch & 7) ^ (key & 7)) << 4);
+      }
+    }
     for (int n = 0;; ++n) {
       const int rs = n % C::RS, st = n % S;
       if (!all_ok(sh_wait(&rfull[rs], (n / C::RS) & 1, abort_flag, a.status, 106)) || n >= *pages_all) break;
+      const uint32_t src = smem_u32(raw + (v * C::RS + rs) * C::RAW), dst = smem_u32((v ? v_sm : k_sm) + st * TILE);
+      uint4 b[TURNS];
+#pragma unroll
+      for (int i = 0; i < TURNS; ++i) b[i] = lds128(src + from[i % ODD] + i / ODD * 8 * HD);
       if (n >= S && !all_ok(sh_wait(&empty[st], ((n / S) - 1) & 1, abort_flag, a.status, 107))) break;
-      const uint32_t src = smem_u32(raw + (v * C::RS + rs) * C::RAW);
-      uint8_t* dst = (v ? v_sm : k_sm) + st * TILE;
-#pragma unroll 4
-      for (int i = 0; i < HD / 16; ++i) {
-        // eight lanes take two keys, of 128-byte rows a half each: neither loads nor stores then meet in a bank
-        const int key = half * 32 + (HD == 128 ? (i >> 1) * 8 + (lane >> 3) * 2 + (lane >> 2 & 1) : i * 8 + (lane >> 2));
-        const int x = (lane & 3) + (HD == 128 ? 4 * ((lane >> 2 & 1) ^ (i & 1)) : 0);
-        const uint4 b = lds128(src + key * HD + x * 16);
-        const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int i = 0; i < TURNS; ++i) {
+        const uint32_t w[4] = {b[i].x, b[i].y, b[i].z, b[i].w};
         uint32_t e[8];
 #pragma unroll
         for (int u = 0; u < 4; ++u)
           asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(e[2 * u]), "=r"(e[2 * u + 1]) : "r"(w[u]));
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int ch = 2 * x + u;                       // 16-byte chunk of the fp16 row
-          *reinterpret_cast<uint4*>(dst + (ch >> 3) * 8192 + key * 128 + (((ch & 7) ^ (key & 7)) << 4)) = make_uint4(e[4 * u], e[4 * u + 1], e[4 * u + 2], e[4 * u + 3]);
-        }
+        for (int u = 0; u < 2; ++u)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + into[i % ODD][u] + i / ODD * 1024), "r"(e[4 * u]), "r"(e[4 * u + 1]), "r"(e[4 * u + 2]),
+                       "r"(e[4 * u + 3])
+                       : "memory");
       }
       fence_proxy_async();
       __syncwarp();
+      // (the bytes' place is given back only here: an arrival does not wait for loads whose values nothing has used yet)
       if (lane == 0) {
         mbar_arrive(&full[st]);
         mbar_arrive(&rempty[rs]);
