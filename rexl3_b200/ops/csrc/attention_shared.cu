@@ -14,13 +14,21 @@
 // its window mates.
 //
 // A page's 64 scores a pair go to tensor memory, come back as exponentials in 16 bits over the same columns, and are the A operand of the product with V.
-// The QKs run two pages ahead of the PVs, also into the next segment.
+// The QKs run two pages ahead of the PVs, also into the next segment.  Scores, maxima, sums and outputs are fp32; the probabilities are rounded to the type that V
+// has as an operand (both operands of an MMA have one), and their sum is that of the unrounded ones: each stands for itself within 2^-9 (bf16) or 2^-12 (fp16),
+// no more than the rounding of the outputs.
 //
 // Warps: 0..3 = softmax, 4 = feeder (descriptions of the segments; TMA), 5 = MMA issuer (owns the tensor memory), for E4M3 caches 6, 7 and 8, 9 = expansion of
 // byte pages of K and of V to fp16 operand tiles.
 // A block of up to 64 or 32 pairs would leave two or three quarters idle and the others bound by one warp's exponentials: its queries
-// stand in the tensor memory two or four times, each copy takes its part of a page's keys - the rest of its P is zero - and leaves its own partial output.
+// stand among the 128 two or four times, each copy takes its part of a page's keys - the rest of its P is zero - and leaves its own partial output.
 // All waits are bounded (status words), no cluster multicast.
+//
+// Whole calls with 40 query and 8 KV heads of 128, plan and merge included (4 and 4 to 5 us):
+//     64 rows behind 8192 common keys, 60 .. 700 keys of their own: 45 us.  134 MB, 20.6 us at the rate of a copy: three blocks a page, a page 0.9 us of an SM - the
+//         chain from scores over 64 exponentials a lane to P and back - and the first pages' way from memory.
+//     48 rows of 500 .. 4000 keys behind 150 common ones: 85 us.  448 MB, 68.6 us: bound by memory, 5.2 TB/s.
+//     32 rows behind 32,700 common keys, E4M3: 69 us.  104 MB, 16 us: bound by instructions, the expansion's beside the softmax's (bf16: 208 MB, 61 us).
 #include <cuda.h>
 #include <cuda_fp8.h>
 #include <type_traits>
@@ -29,8 +37,13 @@
 namespace rx {
 
 constexpr int SH_PAGE = 64, SH_PAIRS = 128, SH_CTAS = 296, SH_MAX_ROWS = 1024;
-constexpr int SH_MIN_SHARED = 1;                        // pages that a group must have in common
-constexpr int SH_SEGMENT = 2;                           // what a unit costs beside its pages, in pages: its place in the line is that much longer
+// Pages that a group must have in common.  (64 rows of 40 heads and 100 .. 700 keys: of one common page nothing comes either way, 3 pages 37.1 against 38.5 us where
+// each sequence reads them for itself, 6 pages 37.4 against 40.6; 256 rows of 8 heads and up to 60 keys behind 3 pages 23.5 against 27 us.)
+constexpr int SH_MIN_SHARED = 1;
+// What a unit costs beside its pages, in pages: its place in the line is that much longer.  (One, two, three, four: 64 rows behind 8192 common keys 47, 45, 46, 48 us;
+// 16 sequences of five rows behind 4001 28, 26, 25, 25; 48 E4M3 rows of 500 .. 4000 keys 98, 78, 76, 76.  Pages weighted by the copies of their block's pairs, 8 : 7 : 6,
+// changed as much for the worse as for the better.)
+constexpr int SH_SEGMENT = 2;
 
 // ------------------------------------------------------------------------------------------------ plan
 // Layout (int32): [0] length of the line  [1] a CTA's piece  [2] blocks  [3] n_kv, then the block at which each CTA begins, the blocks, per row what the merge
@@ -200,8 +213,7 @@ __device__ __forceinline__ uint64_t sh_desc_v(uint32_t smem_addr, uint32_t box) 
   return (uint64_t)((smem_addr & 0x3FFFF) >> 4) | (uint64_t)(box >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
 
-// mbar_wait reads the clock and the host's limit before it polls again: some 1000 cycles, of 2100 that a page took where every wait of its chain
-// (scores, softmax, products) was met a little early.  Here that begins after polls that a page's work never outlasts.
+// One poll.  (mbar_wait's loop in line at every wait was half of the kernel's code, and the five programs of two CTAs outgrew the instruction cache.)
 __device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
@@ -220,7 +232,7 @@ __device__ __noinline__ bool sh_wait_long(uint64_t* bar, uint32_t parity, volati
   return mbar_wait(bar, parity, abort_flag, status, site);
 }
 __device__ __forceinline__ bool sh_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int site) {
-  return mbar_try_wait(bar, parity) || sh_wait_long(bar, parity, abort_flag, status, site);      // (a call: in line, the waits were half of the kernel's code)
+  return mbar_try_wait(bar, parity) || sh_wait_long(bar, parity, abort_flag, status, site);
 }
 
 struct ShArgs {
@@ -290,10 +302,9 @@ struct ShWalk {
 };
 
 // What the warps know of a segment; the eight last are in shared memory.  pages == 0: there are no more.
-struct ShDesc {
+struct alignas(16) ShDesc {
   int row, rows, kvh, key0, pages, part, stride, most;
   const int* table;       // its page ids
-  long long pad;
 };
 
 // N columns of the thread's lane, once they are there (load and wait in one statement: no copy of a register comes between them)
@@ -401,9 +412,8 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
   uint64_t* q_free = q_ready + 4;                         // commit after a segment's last QK
   uint64_t* drained = q_free + 1;
   uint64_t* q_there = drained + 1;                        // (E4M3 caches) the queries as they are
-  uint64_t* spare = q_there + 1;
-  uint64_t* p_ready = spare + 1;                          // [2] the 4 softmax warps
-  ShDesc* desc = (ShDesc*)(p_ready + 2);                  // [8] (behind an even number of words: on a 16-byte boundary)
+  uint64_t* p_ready = q_there + 1;                        // [2] the 4 softmax warps
+  ShDesc* desc = (ShDesc*)(((uintptr_t)(p_ready + 2) + 15) & ~(uintptr_t)15);      // [8]
   uint32_t* tmem_slot = (uint32_t*)(desc + 8);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
   volatile int* pages_all = abort_flag + 1;               // (E4M3 caches) pages of the CTA's piece, once the last has been asked for
@@ -696,7 +706,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         const int copies = sh_copies(sg.rows * G);
         if (lane == 0)
           desc[known & 7] = ShDesc{sg.row, sg.rows, sg.kvh, sg.page * SH_PAGE, more ? sg.pages : 0, sg.part + sg.slot * copies, sg.slots * copies, sg.most,
-                                   a.block_table + (size_t)sg.seq * a.max_blocks + sg.page, 0};
+                                   a.block_table + (size_t)sg.seq * a.max_blocks + sg.page};
         __syncwarp();
         ++known;
         moved = true;

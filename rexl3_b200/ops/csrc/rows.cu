@@ -9,8 +9,9 @@
 //
 // All or nothing: every CTA checks all requests (a few KB) and works out their sums for itself, and a request that cannot be served leaves every
 // output as it was.  Bound by latency (a chain of the loads of lengths, two scans of up to 1024 values, a table entry, a store), not by the 20 bytes a row
-// that it writes: the host's numpy loop over the requests and the upload of five arrays are what it replaces.  One launch: with `free_next` in the place of
-// `free_at` a CTA would overwrite what another has yet to read, so the CTAs are one cluster that meets between the reading and the writing.
+// that it writes: 64 requests of a row each 4.1 us, 23 prompts of 8000 rows together 4.9 us.  One launch: with `free_next` in the place of
+// `free_at` a CTA would overwrite what another has yet to read, so the CTAs are one cluster that meets between the reading and the writing.  (One CTA instead
+// of the eight: eight requests of up to five rows 3.3 against 3.1 us, 40 of them 4.9 against 4.0 us, 256 13.5 against 4.7 us.)
 #include "common.cuh"
 
 namespace rx {
@@ -40,7 +41,8 @@ __global__ void __launch_bounds__(ROWS_THREADS) window_rows_kernel(const RowsArg
   __shared__ uint32_t s_used[ROWS_MAX_TABLE / 32];
   __shared__ int s_sum[3][ROWS_WARPS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.n;
-  const int cta = blockIdx.x, ctas = gridDim.x;
+  constexpr int ctas = ROWS_CLUSTER;
+  const int cta = blockIdx.x;
   for (int i = tid; i < (a.n_tables + 31) / 32; i += ROWS_THREADS) s_used[i] = 0;
   pdl_wait();
   const int at0 = a.free_at != nullptr ? *a.free_at : 0;
@@ -154,13 +156,11 @@ RX_API int rx_window_rows(const void* seq, const void* have, const void* fed, in
   if ((free_at == nullptr) != (free_next == nullptr) || ((free_ids == nullptr || free_at == nullptr) && n_free != 0)) return (int)cudaErrorInvalidValue;
   const RowsArgs a = {(const int*)seq, (const int*)have, (const int*)fed, (const int*)free_ids, (const int*)free_at, (int*)table, (int*)rows, (int*)starts,
                       (int*)free_next, status, n, n_tables, width, cap, n_free};
-  // one CTA has a warp for each of 16 requests and a thread for each of 512 rows
-  const int ctas = n <= ROWS_WARPS && cap <= ROWS_THREADS ? 1 : ROWS_CLUSTER;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas); cfg.blockDim = dim3(ROWS_THREADS); cfg.stream = (cudaStream_t)stream;
+  cfg.gridDim = dim3(ROWS_CLUSTER); cfg.blockDim = dim3(ROWS_THREADS); cfg.stream = (cudaStream_t)stream;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = ctas; at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[0].val.clusterDim.x = ROWS_CLUSTER; at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
