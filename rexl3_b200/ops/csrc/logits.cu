@@ -8,7 +8,7 @@
 //     x    = x - frequency * c;   x = x - (c > 0 ? presence : 0);   x = x + bias
 //     x    = -inf where the row's grammar mask has no bit
 // then the `count` best (value, then lower id).
-#include "topk.cuh"
+#include "common.cuh"
 
 namespace rx {
 
@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(256) token_counts_add_kernel(uint16_t* counts,
 }
 
 // ------------------------------------------------------------------------------------------------ rules + first selection
-constexpr int PICK_MAX_BIAS = 1024;
+constexpr int PICK_MAX_BIAS = 1024, PICK_MAX_WINDOW = 4096;      // (a row looks through its slot's biases and its window's rows before it)
 struct PickArgs {
   const float* logits;                // row r at logits + r * ld
   const int* row_slot;                // [rows]; a value that is no slot: the row is under no penalties and no biases
@@ -217,16 +217,16 @@ __device__ __forceinline__ void pick_select(uint32_t mine, Each each, int count,
   for (int r = 0; r < count; ++r) {
     if (again) {
       own = 0;
-      each(1u, [&](uint64_t key) { if (key < below) own = u64_max(own, key); });
+      each(1u, [&](uint64_t key) { if (key < below) own = max(own, key); });
     }
     uint64_t best = own;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) best = u64_max(best, __shfl_xor_sync(0xffffffffu, best, o));
+    for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
     if (lane == 0) sm.top[warp] = best;
     __syncthreads();
     below = 0;
 #pragma unroll
-    for (int w = 0; w < PICK_THREADS / 32; ++w) below = u64_max(below, sm.top[w]);
+    for (int w = 0; w < PICK_THREADS / 32; ++w) below = max(below, sm.top[w]);
     again = below != 0 && own == below;
     if (tid == 0) out[r] = below;
     __syncthreads();
@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(PICK_THREADS) pick_stage2_kernel(const uint64_
   float v = -INFINITY;
   if (outk[threadIdx.x] != 0) {
     id = (int)(~(uint32_t)outk[threadIdx.x]);
-    v = topk_val(outk[threadIdx.x]);
+    v = pick_value((uint32_t)(outk[threadIdx.x] >> 32));
   } else {
     // Fewer ids above -inf than places: the lowest of the other ids, which all stand at -inf, in order.  The q-th id that is not among n others is q + (how
     // many of those are not above it).
@@ -420,7 +420,7 @@ using namespace rx;
 
 RX_API int rx_token_counts(void* counts, int n_slots, int vocab, const void* slots, const void* starts, const void* prompt, const void* tokens, int n_tokens, int n,
                            int* status, void* stream) {
-  if (n < 1 || n > 65535 || n_slots < 1 || vocab < 1 || n_tokens < 0) return (int)cudaErrorInvalidValue;
+  if (n < 1 || n > 65535 || n_slots < 1 || vocab < 1 || vocab > (1 << 30) || n_tokens < 0 || n_tokens > (1 << 30)) return (int)cudaErrorInvalidValue;
   // As many slices as give every SM at most one CTA, but no more than shared memory asks for where that is not enough: one history of 151,936 ids in 75 slices 2.4 us, in
   // two 4.7 us; 64 histories in two slices each 6.6 us, in three - more CTAs than SMs - 8.2 us.  Slices of whole 16-byte words and whole halves of those.
   const int fewest = (vocab + CNT_MAX_SLICE - 1) / CNT_MAX_SLICE, wanted = 148 / n, most = (vocab + CNT_MIN_SLICE - 1) / CNT_MIN_SLICE;
@@ -440,12 +440,12 @@ RX_API int rx_token_counts(void* counts, int n_slots, int vocab, const void* slo
 }
 
 RX_API int rx_token_counts_add(void* counts, int n_slots, int vocab, const void* slots, const void* tokens, int n, int in_prompt, int* status, void* stream) {
-  if (n < 1 || n_slots < 1 || vocab < 1) return (int)cudaErrorInvalidValue;
+  if (n < 1 || n > (1 << 30) || n_slots < 1 || vocab < 1) return (int)cudaErrorInvalidValue;
   return (int)rx::launch(token_counts_add_kernel, dim3((n + 255) / 256), dim3(256), 0, (cudaStream_t)stream, (uint16_t*)counts, (const int*)slots, (const int*)tokens, n,
                          n_slots, vocab, in_prompt, status);
 }
 
-// scratch: rx_topk_scratch_bytes (of which half is used).  Any of counts (with penalties), bias_id (with bias_val), mask (with mask_row) and first (with fed) may be null.
+// scratch: rx_topk_scratch_bytes.  Any of counts (with penalties), bias_id (with bias_val), mask (with mask_row) and first (with fed) may be null.
 RX_API int rx_topk_adjusted(const void* logits, long long ld, int rows, int vocab, int count, void* scratch, void* ids, void* vals, const void* row_slot,
                             const void* counts, const void* penalties, int n_slots, const void* bias_id, const void* bias_val, int n_bias, const void* mask,
                             const void* mask_row, int n_masks, const void* first, const void* fed, void* stream) {
@@ -453,7 +453,8 @@ RX_API int rx_topk_adjusted(const void* logits, long long ld, int rows, int voca
   // 8192: half as many selections (64 rows of 151,936 ids 30 -> 26 us).
   const bool small = (long long)rows * ((vocab + 4095) / 4096) <= 148 * PICK_CTAS;
   const int nchunks = small ? (vocab + 4095) / 4096 : (vocab + 8191) / 8192;
-  if (rows < 1 || rows > 65535 || vocab < 1 || count < 1 || count > 64 || count > vocab || (long long)nchunks * count > PICK_THREADS * 16 || ld < vocab || n_bias < 0 || n_bias > PICK_MAX_BIAS)
+  if (rows < 1 || rows > 65535 || vocab < 1 || count < 1 || count > 64 || count > vocab || (long long)nchunks * count > PICK_THREADS * 16 || ld < vocab || n_bias < 0 || n_bias > PICK_MAX_BIAS ||
+      (first != nullptr && rows > PICK_MAX_WINDOW))
     return (int)cudaErrorInvalidValue;
   PickArgs a = {(const float*)logits, (const int*)row_slot, (const uint16_t*)counts, (const float*)penalties, (const int*)bias_id, (const float*)bias_val,
                 (const uint32_t*)mask, (const int*)mask_row, (const int*)first, (const int*)fed, (uint64_t*)scratch, ld, rows, vocab, n_slots, n_bias, n_masks,
