@@ -46,7 +46,7 @@ constexpr int SH_MIN_SHARED = 1;
 constexpr int SH_SEGMENT = 2;
 
 // ------------------------------------------------------------------------------------------------ plan
-// Layout (int32): [0] length of the line  [1] a CTA's piece  [2] blocks  [3] n_kv, then the block at which each CTA begins, the blocks, per row what the merge
+// Layout (int32): [0] length of the line  [1] a CTA's piece  [2] blocks  [3] n_kv  [4] n_q  [5] rows  [6] table rows  [7] pages of one, then the block at which each CTA begins, the blocks, per row what the merge
 // asks of its block over common pages and of its block over own pages - length of the blocks before, pages (0: no block), the row's partial vectors, copies -,
 // and the keys that each row sees.
 struct ShBlock {
@@ -66,6 +66,13 @@ __device__ __forceinline__ int sh_slots(int pages, int L) { return (pages + L - 
 __device__ __forceinline__ int sh_copies(int pairs) { return pairs <= 32 ? 4 : pairs <= 64 ? 2 : 1; }
 // where the pages of a unit begin in the line
 __device__ __forceinline__ int sh_unit(int before, int pages, int kvh, int n_kv) { return before * n_kv + kvh * (pages + SH_SEGMENT) + SH_SEGMENT; }
+
+// the plan is one of this shape of window: its blocks, pages and partial vectors are in bounds
+__device__ __forceinline__ bool sh_fits(const int* plan, int n_kv, int n_q, int rows, int n_tables, int max_blocks) {
+  const int4* head = reinterpret_cast<const int4*>(plan);
+  const int4 x = head[0], y = head[1];
+  return x.w == n_kv && y.x == n_q && y.y == rows && y.z == n_tables && y.w == max_blocks;
+}
 
 // inclusive sum over the block's threads; `all` gets the total
 __device__ __forceinline__ int block_scan(int v, int* s_warp, int& all) {
@@ -178,7 +185,7 @@ __global__ void __launch_bounds__(SH_MAX_ROWS) shared_plan_kernel(const int* __r
     }
     plan[SH_HEAD + c] = lo;
   }
-  if (r == 0) plan[0] = total, plan[1] = L, plan[2] = nb, plan[3] = n_kv;
+  if (r == 0) plan[0] = total, plan[1] = L, plan[2] = nb, plan[3] = n_kv, plan[4] = n_kv * G, plan[5] = rows, plan[6] = n_tables, plan[7] = width;
 }
 
 // ------------------------------------------------------------------------------------------------ attention
@@ -242,7 +249,7 @@ struct ShArgs {
   float* part_o;
   float* part_ml;
   int* status;
-  int max_blocks, n_q, n_kv;
+  int max_blocks, n_q, n_kv, rows, n_tables;
   float scale_log2;
 };
 
@@ -271,12 +278,12 @@ struct ShWalk {
     const int at = min(b + 1, last) * 2;
     nx = blk[at], ny = blk[at + 1];
   }
-  __device__ __forceinline__ ShWalk(const int* plan, int n_kv_) : n_kv(n_kv_) {
-    const int total = plan[0];
+  __device__ __forceinline__ ShWalk(const int* plan, int n_kv_, bool fits) : n_kv(n_kv_) {
+    const int all = plan[0], total = fits ? all : 0;
     L = plan[1], last = plan[2] - 1;
+    b = plan[SH_HEAD + blockIdx.x];
     blk = reinterpret_cast<const int4*>(plan + SH_AT_BLOCKS);
     pos = (int)min((long long)total, (long long)blockIdx.x * L), end = (int)min((long long)total, (long long)pos + L);
-    b = plan[SH_HEAD + blockIdx.x];
     if (pos >= end) return;
     x = blk[2 * b], y = blk[2 * b + 1];
     fetch();
@@ -623,7 +630,9 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
     // (With K and V in turn, K page n + 2 waited for V page n + 1 and so for PV(n - 1), and a page took as long as a K page's way from memory.)
     // Of eight descriptions the one that is overwritten, segment w - 8's, is out of use: V has begun segment w - 1, with a page whose copy waited for the PV of a page
     // two (E4M3: four) earlier, in segment w - 5 or later, and that PV for all softmax warps to leave the segments before.
-    ShWalk walk(a.plan, a.n_kv);
+    const bool fits = sh_fits(a.plan, a.n_kv, a.n_q, a.rows, a.n_tables, a.max_blocks);      // (else there is nothing to do, and the merge gives zeros)
+    if (!fits && blockIdx.x == 0 && lane == 0) set_status(a.status, ST_BAD_ARG, 97, a.plan[5]);
+    ShWalk walk(a.plan, a.n_kv, fits);
     int known = 0, asked = 0, queries = 0, converted = 0, idle = 0;      // segments with a description, with queries; the last one whose queries were fetched, + 1
     bool more = true;
     uint64_t since = 0;
@@ -868,13 +877,14 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
 // Bound by latency, so all partial outputs of a turn are on their way at once (25 rows of 31 each: 40 -> 37 us of the whole call, against eight at a time; four
 // warps for each 128 outputs and a sum over shared memory: 38 us, but 48 rows of 14 each 86 -> 90 us).
 template <int HD>
-__global__ void __launch_bounds__(128) attn_shared_merge_kernel(const int* plan, const float* part_o, const float* part_ml, int n_q, int n_kv,
-                                                                const __half* __restrict__ suh, __half* __restrict__ xr, uint16_t* __restrict__ out) {
+__global__ void __launch_bounds__(128) attn_shared_merge_kernel(const int* plan, const float* part_o, const float* part_ml, int n_q, int n_kv, int n_tables,
+                                                                int max_blocks, const __half* __restrict__ suh, __half* __restrict__ xr, uint16_t* __restrict__ out) {
   pdl_launch();
   const int row = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, width = n_q * HD, b = blockIdx.y * 4 + warp;
   const int e0 = b * 128 + lane * 4, hq = e0 / HD, d0 = e0 % HD, kvh = hq / (n_q / n_kv);
   pdl_wait();
   if (b >= width / 128) return;                           // (a whole warp)
+  const bool fits = sh_fits(plan, n_kv, n_q, gridDim.x, n_tables, max_blocks);
   const int L = plan[1];
   const int4* of = reinterpret_cast<const int4*>(plan + SH_AT_ROWS) + 2 * row;
   size_t at[2] = {0, 0};
@@ -882,7 +892,7 @@ __global__ void __launch_bounds__(128) attn_shared_merge_kernel(const int* plan,
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int4 s = of[u];                                  // before, pages, partial vectors, copies
-    if (s.y == 0) continue;
+    if (s.y == 0 || !fits) continue;
     const int unit = sh_unit(s.x, s.y, kvh, n_kv);
     n[u] = ((unit + s.y - 1) / L - unit / L + 1) * s.w;
     at[u] = (size_t)s.z * n_q + hq;
@@ -972,7 +982,7 @@ RX_API long long rx_attn_shared_scratch_floats(int rows, int n_q, int n_kv, int 
 }
 
 static bool sh_takes(int rows, int n_q, int n_kv, int n_tables, int max_blocks) {
-  return rows >= 1 && rows <= SH_MAX_ROWS && n_kv >= 1 && n_q >= n_kv && n_q % n_kv == 0 && n_q / n_kv <= SH_PAIRS && n_tables >= 1 && max_blocks >= 1 &&
+  return rows >= 1 && rows <= SH_MAX_ROWS && n_kv >= 1 && n_q <= 65536 && n_q >= n_kv && n_q % n_kv == 0 && n_q / n_kv <= SH_PAIRS && n_tables >= 1 && max_blocks >= 1 &&
          (long long)rows * (max_blocks + SH_SEGMENT) * n_kv < (1ll << 29) && max_blocks < (1 << 24);
 }
 
@@ -1001,7 +1011,8 @@ RX_API int rx_attn_shared(const void* tmap_k, const void* tmap_v, const void* q,
   int* own_plan = (int*)(a.part_ml + vectors * 2);
   own_plan = (int*)(((uintptr_t)own_plan + 15) & ~(uintptr_t)15);
   a.block_table = (const int*)block_table; a.plan = plan != nullptr ? (const int*)plan : own_plan;
-  a.kv_scale = (const float*)kv_scale; a.status = status; a.max_blocks = max_blocks; a.n_q = n_q; a.n_kv = n_kv; a.scale_log2 = scale * 1.4426950408889634f;
+  a.kv_scale = (const float*)kv_scale; a.status = status; a.max_blocks = max_blocks; a.n_q = n_q; a.n_kv = n_kv; a.rows = rows;
+  a.n_tables = n_tables; a.scale_log2 = scale * 1.4426950408889634f;
   if (plan == nullptr) {
     const int r = rx_attn_shared_plan(row_seq, ctx_len, common, rows, n_tables, max_blocks, n_q, n_kv, own_plan, status, stream);
     if (r != 0) return r;
@@ -1014,5 +1025,5 @@ RX_API int rx_attn_shared(const void* tmap_k, const void* tmap_v, const void* q,
   if (e != cudaSuccess) return (int)e;
   // (early whatever the grid: the kernel before is one wave whose CTAs leave room beside them)
   return (int)rx::launch_pdl(true, hd == 128 ? attn_shared_merge_kernel<128> : attn_shared_merge_kernel<64>, dim3(rows, (n_q * hd / 128 + 3) / 4), dim3(128), 0, st, a.plan,
-                             a.part_o, a.part_ml, n_q, n_kv, (const __half*)suh, (__half*)xr, (uint16_t*)out);
+                             a.part_o, a.part_ml, n_q, n_kv, n_tables, max_blocks, (const __half*)suh, (__half*)xr, (uint16_t*)out);
 }

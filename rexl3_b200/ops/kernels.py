@@ -4,6 +4,8 @@ from __future__ import annotations
 
 from dataclasses import dataclass
 
+import math
+
 import numpy as np
 import torch
 
@@ -423,7 +425,8 @@ def topk_adjusted(logits: torch.Tensor, count: int, scratch: torch.Tensor, ids: 
     (-1): no penalties, no biases.  Each step rounds to f32:
     counts (int16 [slots, vocab], see `token_counts`) with penalties (f32 [slots, 3]: repetition > 0, frequency, presence): an id that the prompt holds or
     that was generated is divided by repetition (multiplied where it is <= 0); then frequency * (times generated) and, where that is not 0, presence go off.
-    window = (first, fed), int32 [rows] each: rows first[r] .. r feed the tokens fed of a verify window; those after first[r] count as generated for row r.
+    window = (first, fed), int32 [rows] each: rows first[r] .. r feed the tokens fed of a verify window; those after first[r] count as generated for row r
+    (up to 4096 rows).
     bias = (ids int32 [slots, n], values f32 [slots, n]), n up to 1024: added; an id outside the vocabulary (-1) is an unused place, equal ids add up in order.
     mask = (bits int32 [n, ceil(vocab / 32)], row int32 [rows]): row r may take the ids whose bit of bits[row[r]] is set (id i: bit i % 32 of word i // 32), every
     id where row[r] is outside 0 .. n - 1.  What is masked stands at -inf, whatever its logit.  Where a row has fewer than count ids above -inf, the rest are
@@ -442,8 +445,8 @@ def topk_adjusted(logits: torch.Tensor, count: int, scratch: torch.Tensor, ids: 
     p_ids, p_vals = _operand(ids, "ids", torch.int32, (rows, count), dev), _operand(vals, "vals", torch.float32, (rows, count), dev)
     if rows == 0:
         return
-    if scratch.get_device() != dev or not scratch.is_contiguous() or scratch.numel() * scratch.element_size() < L.rx_topk_scratch_bytes(rows, vocab, count):
-        raise ValueError("scratch: too small (see topk_scratch), not contiguous or on another device")
+    if scratch.get_device() != dev or not scratch.is_contiguous() or scratch.data_ptr() & 7 or scratch.numel() * scratch.element_size() < L.rx_topk_scratch_bytes(rows, vocab, count):
+        raise ValueError("scratch: too small (see topk_scratch), not contiguous, not on an 8-byte boundary or on another device")
     if (counts is None) != (penalties is None):
         raise ValueError("counts and penalties go together")
     if row_slot is None and (counts is not None or bias is not None):
@@ -464,6 +467,8 @@ def topk_adjusted(logits: torch.Tensor, count: int, scratch: torch.Tensor, ids: 
         nm = _extents(mask[0], "mask bits", 2)[0]
         p_mask, p_mrow = _operand(mask[0], "mask bits", torch.int32, (nm, (vocab + 31) // 32), dev), _operand(mask[1], "mask row", torch.int32, (rows,), dev)
     if window is not None:
+        if rows > 4096:
+            raise ValueError(f"{rows} rows of windows: at most 4096")
         p_first, p_fed = _operand(window[0], "window first", torch.int32, (rows,), dev), _operand(window[1], "window fed", torch.int32, (rows,), dev)
     _lib.check(L.rx_topk_adjusted(logits.data_ptr(), ld if rows > 1 else vocab, rows, vocab, count, scratch.data_ptr(), p_ids, p_vals, p_slot, p_counts, p_pen, slots,
                                   p_bid, p_bval, nb, p_mask, p_mrow, nm, p_first, p_fed, _lib.stream_ptr()), "rx_topk_adjusted")
@@ -480,8 +485,8 @@ def token_counts(counts: torch.Tensor, slots: torch.Tensor, starts: torch.Tensor
     p = (_operand(counts, "counts", torch.int16, (n_slots, vocab), dev), _operand(slots, "slots", torch.int32, (n,), dev), _operand(starts, "starts", torch.int32, (n + 1,), dev),
          _operand(prompt_len, "prompt_len", torch.int32, (n,), dev), _operand(tokens, "tokens", torch.int32, (n_tokens,), dev),
          _operand(status, "status", torch.int32, (STATUS_WORDS,), dev))
-    if n > 65535:
-        raise ValueError(f"{n} requests: at most 65535")
+    if n > 65535 or n_tokens > 1 << 30:
+        raise ValueError(f"{n} requests of {n_tokens} tokens together: at most 65535, and 2^30 tokens")
     if n == 0 or n_slots * vocab == 0:
         return
     _lib.check(_lib.load().rx_token_counts(p[0], n_slots, vocab, p[1], p[2], p[3], p[4], n_tokens, n, p[5], _lib.stream_ptr()), "rx_token_counts")
@@ -618,6 +623,8 @@ def attn_shared_plan(block_table, row_seq, ctx_len, common, n_q: int, n_kv: int,
     rows, tables, width, dev, p = _shared_window(block_table, row_seq, ctx_len, common, status, n_q, n_kv)
     L = _lib.load()
     p_plan = _operand(plan, "plan", torch.int32, (L.rx_attn_shared_plan_ints(),), dev)
+    if p_plan & 15:
+        raise ValueError("plan begins on a 16-byte boundary")
     _lib.check(L.rx_attn_shared_plan(p[1], p[2], p[3], rows, tables, width, n_q, n_kv, p_plan, p[4], _lib.stream_ptr()), "rx_attn_shared_plan")
     _lib.count()
 
@@ -630,11 +637,16 @@ def attn_shared(tk: KvTensorMap, tv: KvTensorMap, q, block_table, row_seq, ctx_l
     it; sequences whose pages agree should stand side by side, and 0 is always right.  `window_rows` writes all three.
     out bf16 [rows, n_q * hd] or None; with suh also xr fp16, `attn_decode`'s rotated output.  bf16 caches, or E4M3 ones with kv_scale (f32 [2, n_kv]); heads of
     64 or 128; n_q * hd a multiple of 128.  A row's last bits depend on the rows beside it: the cut of the work follows the whole window.
-    A table row or a context outside the table sets the status and stands for a context of 0.
-    `plan`: from `attn_shared_plan` for this window (one serves every layer); None: the call plans for itself."""
+    A table row or a context outside the table sets the status and stands for a context of 0.  What stands behind the last key that any row of a sequence or group
+    sees may be anything; of an infinite or NaN value of V at a key before it, the rows that do not see that key may get NaN too.  With an E4M3 cache the queries
+    are taken in fp16 (up to 65504).
+    `plan`: from `attn_shared_plan` for this window (one serves every layer); None: the call plans for itself.  One for another shape of window sets the status and
+    gives zeros."""
     rows, tables, pages, dev, p = _shared_window(block_table, row_seq, ctx_len, common, status, n_q, n_kv)
     if hd not in (64, 128) or n_q * hd % 128:
         raise ValueError(f"heads of {hd}: 64 or 128, and n_q * hd a multiple of 128")
+    if not 0 < scale < math.inf:
+        raise ValueError(f"scale {scale}: a positive number is needed")
     for t in (tk, tv):
         cache = t._keep
         if t.i8 or t.fp8 != (kv_scale is not None) or cache.shape[1:] != (n_kv, 64, hd) or cache.get_device() != dev:

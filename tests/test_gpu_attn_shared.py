@@ -199,6 +199,40 @@ def test_again_and_again_the_same_bits():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("seqs,shared,heads", [
+    ([(0, 8200 + 9 * i, 1) for i in range(64)], 128, (40, 8, 128)),
+    ([(0, 600 + 67 * i, 1) for i in range(48)], 2, (40, 8, 128)),
+    ([(i // 8, 4100 + 11 * i, 5) for i in range(16)], 62, (32, 4, 128)),
+    ([(i // 8, 4100 + 11 * i, 5) for i in range(16)], 62, (16, 4, 64)),
+])
+def test_a_full_device_gives_the_same_bits(seqs, shared, heads, fp8):
+    """What one warp hands to another too early shows itself in some of many calls."""
+    w = Window(seqs, shared, *heads, fp8=fp8, seed=17)
+    first = w.check() and w.run()
+    for _ in range(60):
+        assert torch.equal(w.run(), first)
+
+
+@pytest.mark.gpu
+def test_a_plan_of_another_window_sets_the_status_and_gives_zeros():
+    w = Window([(0, 500 + 31 * i, 2) for i in range(6)], 7, 10, 2, 128, seed=18)
+    other = Window([(0, 500 + 31 * i, 1) for i in range(5)], 7, 10, 2, 128, seed=18)
+    plans = [K.attn_shared_plan_buffer()]                     # none at all, of fewer rows, of other heads, of a wider table
+    for a in ((other.table, other.row_seq, other.ctx, other.common, 10, 2), (w.table, w.row_seq, w.ctx, w.common, 20, 2),
+              (torch.cat([w.table, w.table], 1).contiguous(), w.row_seq, w.ctx, w.common, 10, 2)):
+        plans.append(K.attn_shared_plan_buffer())
+        K.attn_shared_plan(*a, plans[-1], K.new_status())
+    for plan in plans:
+        out, st = torch.ones_like(w.q), K.new_status()
+        K.attn_shared(*w.maps, w.q, w.table, w.row_seq, w.ctx, w.common, K.attn_shared_scratch(12, 10, 2, 128), 10, 2, 128, 0.1, out, st, plan=plan)
+        assert int(out.abs().sum()) == 0
+        with pytest.raises(RuntimeError):
+            K.check_status(st)
+    w.check()
+
+
+@pytest.mark.gpu
 def test_two_graphs_with_one_workspace_and_another_stream():
     """Two captured windows over one scratch, replayed in turn; the lengths change between replays."""
     a, b = Window([(0, 300 + i, 1) for i in range(8)], 4, 10, 2, 128, seed=11, width=40), Window([(-1, 900, 3), (0, 500, 1), (0, 600, 1)], 2, 10, 2, 128, seed=12, width=40)
@@ -309,11 +343,14 @@ def test_refusals():
                dict(ctx_len=w.ctx.long()), dict(common=None), dict(n_q=11), dict(n_kv=3), dict(hd=96), dict(hd=64), dict(scratch=torch.empty(100, device="cuda")), dict(out=None),
                dict(out=torch.empty(2, 1280, device="cuda")), dict(status=t([0])), dict(tk=f8, tv=f8), dict(tk=i8, tv=i8), dict(kv_scale=scales), dict(tk=half, tv=half, kv_scale=scales),
                dict(tk=f8, tv=f8, kv_scale=scales[:1]), dict(suh=suh), dict(xr=xr), dict(plan=t([0])), dict(block_table=w.table[:, :0]),
-               dict(scratch=torch.empty(ok["scratch"].numel() + 1, device="cuda")[1:])):
+               dict(scratch=torch.empty(ok["scratch"].numel() + 1, device="cuda")[1:]), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf"))):
         with pytest.raises(ValueError):
             K.attn_shared(**{**ok, **kw})
     big = t([1]).expand(1025).contiguous()
     with pytest.raises(ValueError):
         K.attn_shared_plan(w.table, big, big, big, 10, 2, K.attn_shared_plan_buffer(), K.new_status())
+    n = K.attn_shared_plan_buffer().numel()
+    with pytest.raises(ValueError):
+        K.attn_shared_plan(w.table, w.row_seq, w.ctx, w.common, 10, 2, torch.zeros(n + 1, dtype=torch.int32, device="cuda")[1:], K.new_status())
     K.attn_shared(**ok)
     K.check_status(ok["status"])

@@ -249,6 +249,11 @@ def test_refusals():
             K.topk_adjusted(**a)
     with pytest.raises(ValueError):
         K.topk_adjusted(torch.randn(1, 5, device="cuda"), 8, sc, ids[:1], vals[:1])
+    many, zero = torch.zeros(4097, 8, device="cuda"), torch.zeros(4097, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="4096"):
+        K.topk_adjusted(many, 1, K.topk_scratch(4097, 8, 1), zero[:, None], many[:, :1].contiguous(), window=(zero, zero))
+    with pytest.raises(ValueError, match="boundary"):
+        K.topk_adjusted(x, 8, torch.empty(4096, dtype=torch.uint8, device="cuda")[4:], ids, vals)
     K.topk_adjusted(torch.empty(0, V, device="cuda"), 8, sc, ids[:0], vals[:0])
     for a in ((counts.int(), slot, t([0, 1, 2]), slot, slot, st), (counts, slot, slot, slot, slot, st), (counts, slot, t([0, 1, 2]), slot[:1], slot, st), (counts, slot.long(), t([0, 1, 2]), slot, slot, st),
               (counts[:, ::2], slot, t([0, 1, 2]), slot, slot, st), (counts, slot, t([0, 1, 2]), slot, slot.cpu(), st)):
