@@ -4,6 +4,7 @@ from __future__ import annotations
 
 from dataclasses import dataclass
 
+import functools
 import math
 
 import numpy as np
@@ -394,28 +395,58 @@ def topk(logits: torch.Tensor, count: int, scratch, ids: torch.Tensor, vals: tor
     _lib.count(2)
 
 
-def _operand(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device: int) -> int:
-    """The device pointer of a contiguous operand on the current device `device`.  (A call has ten of them: what is in order is seen by few looks.)"""
-    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == device and t.is_contiguous():
-        return t.data_ptr()
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+# A call below has about ten operands, and looking at them costs as much as a launch: what is in order is seen by few looks (a name for each type, elements before
+# shapes), and only what is not is looked at again for its error.
+_Tensor, _I16, _I32, _F16, _BF16, _F32 = torch.Tensor, torch.int16, torch.int32, torch.float16, torch.bfloat16, torch.float32
+
+
+def _refuse(t, name: str, dtype: torch.dtype, shape: tuple, device: int) -> int:
+    if not isinstance(t, _Tensor) or not t.is_cuda:
         raise ValueError(f"{name}: a CUDA tensor is needed")
     if t.get_device() != device:
         raise ValueError(f"{name} is on {t.device}, not on the current device cuda:{device}")
-    if t.dtype is not dtype or t.shape != shape:
-        raise ValueError(f"{name}: {dtype} {shape} is needed, not {t.dtype} {tuple(t.shape)}")
-    raise ValueError(f"{name}: must be contiguous")
+    if t.dtype is not dtype or len(t.shape) != len(shape) or any(b is not None and a != b for a, b in zip(t.shape, shape)):
+        raise ValueError(f"{name}: {dtype} [{', '.join('any' if b is None else str(b) for b in shape)}] is needed, not {t.dtype} {list(t.shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: must be contiguous")
+    return t.data_ptr()                                    # (a subclass of Tensor)
 
 
-def _extents(t: torch.Tensor, name: str, dims: int) -> tuple:
-    if not isinstance(t, torch.Tensor) or t.dim() != dims:
-        raise ValueError(f"{name}: a CUDA tensor of {dims} dimension{'s' if dims > 1 else ''} is needed")
-    return t.shape
+def _vector(t, name: str, dtype: torch.dtype, n: int, device: int) -> int:
+    """The device pointer of a contiguous operand of n values on the current device `device`."""
+    if t.__class__ is _Tensor and t.dtype is dtype and t.numel() == n and t.get_device() == device and t.is_contiguous():
+        return t.data_ptr()
+    return _refuse(t, name, dtype, (n,), device)
 
 
-def _here(t: torch.Tensor) -> int:
-    """The current device; for a tensor that is on none, what no tensor's device is (a CPU tensor's is -1)."""
-    return torch.cuda.current_device() if t.is_cuda else -2
+def _matrix(t, name: str, dtype: torch.dtype, shape: tuple, device: int) -> int:
+    """... of a contiguous operand of two dimensions"""
+    if t.__class__ is _Tensor and t.dtype is dtype and t.shape == shape and t.get_device() == device and t.is_contiguous():
+        return t.data_ptr()
+    return _refuse(t, name, dtype, shape, device)
+
+
+def _table(t, name: str, dtype: torch.dtype, device: int) -> tuple:
+    """... of one whose extents say the sizes of the others, with those"""
+    if t.__class__ is _Tensor and t.dtype is dtype and t.get_device() == device and t.is_contiguous():
+        shape = t.shape
+        if len(shape) == 2:
+            return t.data_ptr(), shape[0], shape[1]
+    p = _refuse(t, name, dtype, (None, None), device)
+    return p, t.shape[0], t.shape[1]
+
+
+def _length(t, name: str) -> int:
+    if not isinstance(t, _Tensor) or len(t.shape) != 1:
+        raise ValueError(f"{name}: a CUDA tensor of one dimension is needed")
+    return t.numel()
+
+
+def _here(t, name: str) -> int:
+    """The current device; the call's first operand is on one"""
+    if not isinstance(t, _Tensor) or not t.is_cuda:
+        raise ValueError(f"{name}: a CUDA tensor is needed")
+    return torch._C._cuda_getDevice()
 
 
 def topk_adjusted(logits: torch.Tensor, count: int, scratch: torch.Tensor, ids: torch.Tensor, vals: torch.Tensor, row_slot: "torch.Tensor | None" = None, *,
@@ -431,9 +462,10 @@ def topk_adjusted(logits: torch.Tensor, count: int, scratch: torch.Tensor, ids: 
     mask = (bits int32 [n, ceil(vocab / 32)], row int32 [rows]): row r may take the ids whose bit of bits[row[r]] is set (id i: bit i % 32 of word i // 32), every
     id where row[r] is outside 0 .. n - 1.  What is masked stands at -inf, whatever its logit.  Where a row has fewer than count ids above -inf, the rest are
     its lowest other ids at -inf.  A NaN that is not masked is above everything.  scratch: `topk_scratch`; calls that may overlap need one each."""
-    if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or logits.dtype is not torch.float32 or not logits.is_cuda:
+    dev = _here(logits, "logits")
+    if logits.dtype is not _F32 or logits.dim() != 2:
         raise ValueError("logits: a CUDA float32 [rows, vocab] tensor is needed")
-    L, dev, (rows, vocab), (ld, step) = _lib.load(), _here(logits), logits.shape, logits.stride()
+    (rows, vocab), (ld, step) = logits.shape, logits.stride()
     if logits.get_device() != dev:
         raise ValueError(f"logits is on {logits.device}, not on the current device cuda:{dev}")
     if rows > 1 and ld < vocab or vocab > 1 and step != 1:
@@ -442,36 +474,41 @@ def topk_adjusted(logits: torch.Tensor, count: int, scratch: torch.Tensor, ids: 
         raise ValueError(f"count {count}: 1 .. 64, no more than the vocabulary of {vocab}, and ceil(vocab / 4096) * count <= 4096")
     if rows > 65535:
         raise ValueError(f"{rows} rows: at most 65535")
-    p_ids, p_vals = _operand(ids, "ids", torch.int32, (rows, count), dev), _operand(vals, "vals", torch.float32, (rows, count), dev)
+    p_ids, p_vals = _matrix(ids, "ids", _I32, (rows, count), dev), _matrix(vals, "vals", _F32, (rows, count), dev)
     if rows == 0:
         return
-    if scratch.get_device() != dev or not scratch.is_contiguous() or scratch.data_ptr() & 7 or scratch.numel() * scratch.element_size() < L.rx_topk_scratch_bytes(rows, vocab, count):
+    p_scratch = scratch.data_ptr()
+    if p_scratch & 7 or scratch.get_device() != dev or not scratch.is_contiguous() or scratch.nbytes < rows * ((vocab + 4095) // 4096) * count * 8:
         raise ValueError("scratch: too small (see topk_scratch), not contiguous, not on an 8-byte boundary or on another device")
     if (counts is None) != (penalties is None):
         raise ValueError("counts and penalties go together")
     if row_slot is None and (counts is not None or bias is not None):
         raise ValueError("penalties and biases need row_slot")
-    p_slot = None if row_slot is None else _operand(row_slot, "row_slot", torch.int32, (rows,), dev)
+    p_slot = None if row_slot is None else _vector(row_slot, "row_slot", _I32, rows, dev)
     slots, p_counts, p_pen, p_bid, p_bval, nb, p_mask, p_mrow, nm, p_first, p_fed = 0, None, None, None, None, 0, None, None, 0, None, None
     if counts is not None:
-        slots = _extents(counts, "counts", 2)[0]
-        p_counts = _operand(counts, "counts", torch.int16, (slots, vocab), dev)
-        p_pen = _operand(penalties, "penalties", torch.float32, (slots, 3), dev)
+        p_counts, slots, ids_of = _table(counts, "counts", _I16, dev)
+        if ids_of != vocab:
+            raise ValueError(f"counts: {ids_of} ids a slot, the vocabulary has {vocab}")
+        p_pen = _matrix(penalties, "penalties", _F32, (slots, 3), dev)
     if bias is not None:
-        n, nb = _extents(bias[0], "bias ids", 2)
-        slots = slots if counts is not None else n
-        p_bid, p_bval = _operand(bias[0], "bias ids", torch.int32, (slots, nb), dev), _operand(bias[1], "bias values", torch.float32, (slots, nb), dev)
+        p_bid, n, nb = _table(bias[0], "bias ids", _I32, dev)
+        if counts is not None and n != slots:
+            raise ValueError(f"bias ids: of {n} slots, counts is of {slots}")
+        slots, p_bval = n, _matrix(bias[1], "bias values", _F32, (n, nb), dev)
         if nb > 1024:
             raise ValueError(f"{nb} biases a slot: at most 1024")
     if mask is not None:
-        nm = _extents(mask[0], "mask bits", 2)[0]
-        p_mask, p_mrow = _operand(mask[0], "mask bits", torch.int32, (nm, (vocab + 31) // 32), dev), _operand(mask[1], "mask row", torch.int32, (rows,), dev)
+        p_mask, nm, words = _table(mask[0], "mask bits", _I32, dev)
+        if words != (vocab + 31) // 32:
+            raise ValueError(f"mask bits: {words} words a row, the vocabulary needs {(vocab + 31) // 32}")
+        p_mrow = _vector(mask[1], "mask row", _I32, rows, dev)
     if window is not None:
         if rows > 4096:
             raise ValueError(f"{rows} rows of windows: at most 4096")
-        p_first, p_fed = _operand(window[0], "window first", torch.int32, (rows,), dev), _operand(window[1], "window fed", torch.int32, (rows,), dev)
-    _lib.check(L.rx_topk_adjusted(logits.data_ptr(), ld if rows > 1 else vocab, rows, vocab, count, scratch.data_ptr(), p_ids, p_vals, p_slot, p_counts, p_pen, slots,
-                                  p_bid, p_bval, nb, p_mask, p_mrow, nm, p_first, p_fed, _lib.stream_ptr()), "rx_topk_adjusted")
+        p_first, p_fed = _vector(window[0], "window first", _I32, rows, dev), _vector(window[1], "window fed", _I32, rows, dev)
+    _lib.check(_lib.load().rx_topk_adjusted(logits.data_ptr(), ld if rows > 1 else vocab, rows, vocab, count, p_scratch, p_ids, p_vals, p_slot, p_counts, p_pen, slots,
+                                            p_bid, p_bval, nb, p_mask, p_mrow, nm, p_first, p_fed, _lib.stream_ptr()), "rx_topk_adjusted")
     _lib.count(2)
 
 
@@ -480,29 +517,27 @@ def token_counts(counts: torch.Tensor, slots: torch.Tensor, starts: torch.Tensor
     the id, bits 0 .. 14 = times generated, up to 32767.  Request i's history is tokens[starts[i]:starts[i + 1]], its first prompt_len[i] tokens the prompt; row
     slots[i] of counts is written whole, the others stay.  int32 tensors; starts has one more entry than slots.  A token outside the vocabulary is left out, a slot
     outside the table, a slot's second request and a range outside `tokens` are passed over; each sets the status."""
-    n_slots, vocab = _extents(counts, "counts", 2)
-    dev, n, n_tokens = _here(counts), _extents(slots, "slots", 1)[0], _extents(tokens, "tokens", 1)[0]
-    p = (_operand(counts, "counts", torch.int16, (n_slots, vocab), dev), _operand(slots, "slots", torch.int32, (n,), dev), _operand(starts, "starts", torch.int32, (n + 1,), dev),
-         _operand(prompt_len, "prompt_len", torch.int32, (n,), dev), _operand(tokens, "tokens", torch.int32, (n_tokens,), dev),
-         _operand(status, "status", torch.int32, (STATUS_WORDS,), dev))
+    dev, n, n_tokens = _here(counts, "counts"), _length(slots, "slots"), _length(tokens, "tokens")
+    p_counts, n_slots, vocab = _table(counts, "counts", _I16, dev)
+    p = (_vector(slots, "slots", _I32, n, dev), _vector(starts, "starts", _I32, n + 1, dev), _vector(prompt_len, "prompt_len", _I32, n, dev),
+         _vector(tokens, "tokens", _I32, n_tokens, dev), _vector(status, "status", _I32, STATUS_WORDS, dev))
     if n > 65535 or n_tokens > 1 << 30:
         raise ValueError(f"{n} requests of {n_tokens} tokens together: at most 65535, and 2^30 tokens")
     if n == 0 or n_slots * vocab == 0:
         return
-    _lib.check(_lib.load().rx_token_counts(p[0], n_slots, vocab, p[1], p[2], p[3], p[4], n_tokens, n, p[5], _lib.stream_ptr()), "rx_token_counts")
+    _lib.check(_lib.load().rx_token_counts(p_counts, n_slots, vocab, p[0], p[1], p[2], p[3], n_tokens, n, p[4], _lib.stream_ptr()), "rx_token_counts")
     _lib.count()
 
 
 def token_counts_add(counts: torch.Tensor, slots: torch.Tensor, tokens: torch.Tensor, status: torch.Tensor, prompt: bool = False) -> None:
     """counts[slots[i], tokens[i]] takes one more generated token (`prompt`: the prompt bit), for the tokens that a step committed; a pair may stand more than
     once.  int32 [n] each.  A slot or token outside the table is left out and sets the status."""
-    n_slots, vocab = _extents(counts, "counts", 2)
-    dev, n = _here(counts), _extents(slots, "slots", 1)[0]
-    p = (_operand(counts, "counts", torch.int16, (n_slots, vocab), dev), _operand(slots, "slots", torch.int32, (n,), dev), _operand(tokens, "tokens", torch.int32, (n,), dev),
-         _operand(status, "status", torch.int32, (STATUS_WORDS,), dev))
+    dev, n = _here(counts, "counts"), _length(slots, "slots")
+    p_counts, n_slots, vocab = _table(counts, "counts", _I16, dev)
+    p = _vector(slots, "slots", _I32, n, dev), _vector(tokens, "tokens", _I32, n, dev), _vector(status, "status", _I32, STATUS_WORDS, dev)
     if n == 0 or n_slots * vocab == 0:
         return
-    _lib.check(_lib.load().rx_token_counts_add(p[0], n_slots, vocab, p[1], p[2], n, 1 if prompt else 0, p[3], _lib.stream_ptr()), "rx_token_counts_add")
+    _lib.check(_lib.load().rx_token_counts_add(p_counts, n_slots, vocab, p[0], p[1], n, 1 if prompt else 0, p[2], _lib.stream_ptr()), "rx_token_counts_add")
     _lib.count()
 
 
@@ -516,22 +551,22 @@ def window_rows(seq: torch.Tensor, have: torch.Tensor, new: torch.Tensor, block_
     the new tokens begin, and free_next = free_at + their number (it may be the same tensor as free_at).  Without them the table holds those pages already.
     All or nothing: a length below 0, tokens beyond the table, more rows than cap, more pages than there are, a table row outside the table or
     given twice sets the status and changes nothing else.  A table entry below 0 where a row is to be written gives slot -1 (the row is not cached) and sets the status."""
-    L, (tables, width), n, (five, cap) = _lib.load(), _extents(block_table, "block_table", 2), _extents(seq, "seq", 1)[0], _extents(rows, "rows", 2)
-    dev = _here(block_table)
-    p = (_operand(seq, "seq", torch.int32, (n,), dev), _operand(have, "have", torch.int32, (n,), dev), _operand(new, "new", torch.int32, (n,), dev),
-         _operand(block_table, "block_table", torch.int32, (tables, width), dev), _operand(rows, "rows", torch.int32, (5, cap), dev),
-         _operand(starts, "starts", torch.int32, (n + 1,), dev), _operand(status, "status", torch.int32, (STATUS_WORDS,), dev))
-    if not 1 <= n <= L.rx_window_rows_max():
-        raise ValueError(f"{n} requests: 1 .. {L.rx_window_rows_max()}")
+    dev, n = _here(block_table, "block_table"), _length(seq, "seq")
+    p_table, tables, width = _table(block_table, "block_table", _I32, dev)
+    p_rows, five, cap = _table(rows, "rows", _I32, dev)
+    p = (_vector(seq, "seq", _I32, n, dev), _vector(have, "have", _I32, n, dev), _vector(new, "new", _I32, n, dev), _vector(starts, "starts", _I32, n + 1, dev),
+         _vector(status, "status", _I32, STATUS_WORDS, dev))
+    if not 1 <= n <= 1024 or five != 5:
+        raise ValueError(f"{n} requests: 1 .. 1024; rows: [5, rows]")
     if not 1 <= tables <= 32768 or not 1 <= width <= 1 << 24 or cap > 1 << 20:
         raise ValueError("block_table: 1 .. 32768 rows of 1 .. 2^24 pages; rows: at most 2^20")
     if (free is None) != (free_at is None) or (free is None) != (free_next is None):
         raise ValueError("free, free_at and free_next go together")
     f, n_free = (None, None, None), 0
     if free is not None:
-        n_free = _extents(free, "free", 1)[0]
-        f = _operand(free, "free", torch.int32, (n_free,), dev), _operand(free_at, "free_at", torch.int32, (1,), dev), _operand(free_next, "free_next", torch.int32, (1,), dev)
-    _lib.check(L.rx_window_rows(p[0], p[1], p[2], n, p[3], tables, width, f[0], n_free, f[1], f[2], p[4], cap, p[5], p[6], _lib.stream_ptr()), "rx_window_rows")
+        n_free = _length(free, "free")
+        f = _vector(free, "free", _I32, n_free, dev), _vector(free_at, "free_at", _I32, 1, dev), _vector(free_next, "free_next", _I32, 1, dev)
+    _lib.check(_lib.load().rx_window_rows(p[0], p[1], p[2], n, p_table, tables, width, f[0], n_free, f[1], f[2], p_rows, cap, p[3], p[4], _lib.stream_ptr()), "rx_window_rows")
     _lib.count()
 
 
@@ -544,6 +579,7 @@ class KvTensorMap:
         assert page == 64 and cache.dtype in (torch.bfloat16, torch.uint8, torch.int8) and cache.is_contiguous()
         self.buf = self.buf_rows = np.zeros(128, dtype=np.uint8)
         self._keep = cache
+        self.held = (n_kv, hd, cache.get_device(), cache.dtype)      # (of a call's own heads and device)
         self.fp8 = cache.dtype == torch.uint8          # E4M3 bytes
         self.i8 = cache.dtype == torch.int8            # int8 with one scale per (token, KV head), kept beside the cache
         L = _lib.load()
@@ -607,10 +643,17 @@ def attn_shared_plan_buffer(device="cuda") -> torch.Tensor:
     return torch.zeros(_lib.load().rx_attn_shared_plan_ints(), dtype=torch.int32, device=device)
 
 
+@functools.lru_cache(maxsize=None)
+def _attn_shared_sizes(rows: int, n_q: int, n_kv: int, hd: int) -> tuple:
+    """scratch floats and plan words"""
+    return _lib.load().rx_attn_shared_scratch_floats(rows, n_q, n_kv, hd), _lib.load().rx_attn_shared_plan_ints()
+
+
 def _shared_window(block_table, row_seq, ctx_len, common, status, n_q: int, n_kv: int):
-    (tables, width), rows, dev = _extents(block_table, "block_table", 2), _extents(row_seq, "row_seq", 1)[0], _here(block_table)
-    p = (_operand(block_table, "block_table", torch.int32, (tables, width), dev), _operand(row_seq, "row_seq", torch.int32, (rows,), dev),
-         _operand(ctx_len, "ctx_len", torch.int32, (rows,), dev), _operand(common, "common", torch.int32, (rows,), dev), _operand(status, "status", torch.int32, (STATUS_WORDS,), dev))
+    dev, rows = _here(block_table, "block_table"), _length(row_seq, "row_seq")
+    p_table, tables, width = _table(block_table, "block_table", _I32, dev)
+    p = (p_table, _vector(row_seq, "row_seq", _I32, rows, dev), _vector(ctx_len, "ctx_len", _I32, rows, dev), _vector(common, "common", _I32, rows, dev),
+         _vector(status, "status", _I32, STATUS_WORDS, dev))
     if not 1 <= rows <= 1024 or n_kv < 1 or n_q % n_kv or not 1 <= n_q // n_kv <= 128:
         raise ValueError(f"{rows} rows of {n_q} query and {n_kv} KV heads: 1 .. 1024 rows, n_kv divides n_q, at most 128 query heads share a KV head")
     if tables * width == 0 or rows * (width + 2) * n_kv >= 1 << 29:
@@ -621,11 +664,10 @@ def _shared_window(block_table, row_seq, ctx_len, common, status, n_q: int, n_kv
 def attn_shared_plan(block_table, row_seq, ctx_len, common, n_q: int, n_kv: int, plan: torch.Tensor, status: torch.Tensor) -> None:
     """The work plan of `attn_shared` for one window: a function of these tensors' values (of block_table only its extents), so one plan serves every layer."""
     rows, tables, width, dev, p = _shared_window(block_table, row_seq, ctx_len, common, status, n_q, n_kv)
-    L = _lib.load()
-    p_plan = _operand(plan, "plan", torch.int32, (L.rx_attn_shared_plan_ints(),), dev)
+    p_plan = _vector(plan, "plan", _I32, _attn_shared_sizes(rows, n_q, n_kv, 128)[1], dev)
     if p_plan & 15:
         raise ValueError("plan begins on a 16-byte boundary")
-    _lib.check(L.rx_attn_shared_plan(p[1], p[2], p[3], rows, tables, width, n_q, n_kv, p_plan, p[4], _lib.stream_ptr()), "rx_attn_shared_plan")
+    _lib.check(_lib.load().rx_attn_shared_plan(p[1], p[2], p[3], rows, tables, width, n_q, n_kv, p_plan, p[4], _lib.stream_ptr()), "rx_attn_shared_plan")
     _lib.count()
 
 
@@ -647,26 +689,25 @@ def attn_shared(tk: KvTensorMap, tv: KvTensorMap, q, block_table, row_seq, ctx_l
         raise ValueError(f"heads of {hd}: 64 or 128, and n_q * hd a multiple of 128")
     if not 0 < scale < math.inf:
         raise ValueError(f"scale {scale}: a positive number is needed")
-    for t in (tk, tv):
-        cache = t._keep
-        if t.i8 or t.fp8 != (kv_scale is not None) or cache.shape[1:] != (n_kv, 64, hd) or cache.get_device() != dev:
-            raise ValueError(f"cache: bf16, or E4M3 bytes with kv_scale, [pages, {n_kv}, 64, {hd}] on cuda:{dev} is needed")
+    held = (n_kv, hd, dev, _BF16 if kv_scale is None else torch.uint8)
+    if tk.held != held or tv.held != held:
+        raise ValueError(f"cache: bf16, or E4M3 bytes with kv_scale, [pages, {n_kv}, 64, {hd}] on cuda:{dev} is needed")
     if out is None and xr is None or (suh is None) != (xr is None):
         raise ValueError("out, or suh with xr, or both are needed")
-    L, width = _lib.load(), n_q * hd
-    p_q = _operand(q, "q", torch.bfloat16, (rows, width), dev)
-    p_out = None if out is None else _operand(out, "out", torch.bfloat16, (rows, width), dev)
-    p_suh, p_xr = (None, None) if xr is None else (_operand(suh, "suh", torch.float16, (width,), dev), _operand(xr, "xr", torch.float16, (rows, width), dev))
-    p_scale = None if kv_scale is None else _operand(kv_scale, "kv_scale", torch.float32, (2, n_kv), dev)
-    p_plan = None if plan is None else _operand(plan, "plan", torch.int32, (L.rx_attn_shared_plan_ints(),), dev)
-    floats = _extents(scratch, "scratch", 1)[0]
-    p_scratch = _operand(scratch, "scratch", torch.float32, (floats,), dev)
-    if floats < L.rx_attn_shared_scratch_floats(rows, n_q, n_kv, hd):
+    width, (floats, plan_words) = n_q * hd, _attn_shared_sizes(rows, n_q, n_kv, hd)
+    p_q = _matrix(q, "q", _BF16, (rows, width), dev)
+    p_out = None if out is None else _matrix(out, "out", _BF16, (rows, width), dev)
+    p_suh, p_xr = (None, None) if xr is None else (_vector(suh, "suh", _F16, width, dev), _matrix(xr, "xr", _F16, (rows, width), dev))
+    p_scale = None if kv_scale is None else _matrix(kv_scale, "kv_scale", _F32, (2, n_kv), dev)
+    p_plan = None if plan is None else _vector(plan, "plan", _I32, plan_words, dev)
+    held_floats = _length(scratch, "scratch")
+    p_scratch = _vector(scratch, "scratch", _F32, held_floats, dev)
+    if held_floats < floats:
         raise ValueError("scratch: too small (see attn_shared_scratch)")
     if (p_q | p_scratch | (p_plan or 0)) & 15 or ((p_out or 0) | (p_xr or 0)) & 7:
         raise ValueError("q, scratch and plan begin on 16-byte boundaries, out and xr on 8-byte ones")
-    _lib.check(L.rx_attn_shared(tk.rows_ptr, tv.rows_ptr, p_q, p[0], tables, pages, p[1], p[2], p[3], p_scratch, rows, n_q, n_kv, hd, scale, p_scale, p_suh, p_xr, p_out,
-                                p_plan, p[4], _lib.stream_ptr()), "rx_attn_shared")
+    _lib.check(_lib.load().rx_attn_shared(tk.rows_ptr, tv.rows_ptr, p_q, p[0], tables, pages, p[1], p[2], p[3], p_scratch, rows, n_q, n_kv, hd, scale, p_scale, p_suh, p_xr, p_out,
+                                          p_plan, p[4], _lib.stream_ptr()), "rx_attn_shared")
     _lib.count(2 if plan is not None else 3)
 
 

@@ -23,6 +23,8 @@ class KernelError(RuntimeError):
 
 def load(build_if_missing: bool = True):
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib
@@ -31,8 +33,9 @@ def load(build_if_missing: bool = True):
                 raise KernelError(f"{LIB_PATH} is missing: run python -m rexl3_b200.ops.build")
             from . import build as _b
             _b.build()
-        _lib = ctypes.CDLL(LIB_PATH)
-        _declare(_lib)
+        lib = ctypes.CDLL(LIB_PATH)
+        _declare(lib)
+        _lib = lib                                         # (only now: who looks without the lock finds it whole)
         return _lib
 
 
@@ -182,12 +185,19 @@ def ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+_raw_stream = None
+
+
 def stream_ptr() -> int:
     """The current stream of the current device.  (By way of a torch.cuda.Stream object it took 3.4 us a call, as much as a launch.)"""
-    import torch
-    if torch.cuda.is_initialized():
-        return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
-    return torch.cuda.current_stream().cuda_stream
+    global _raw_stream
+    if _raw_stream is None:
+        import torch
+        if not torch.cuda.is_initialized():
+            return torch.cuda.current_stream().cuda_stream
+        _raw_stream = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+    stream, device = _raw_stream
+    return stream(device())
 
 
 def count(n: int = 1) -> None:
