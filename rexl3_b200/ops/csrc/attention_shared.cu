@@ -74,27 +74,34 @@ __device__ __forceinline__ bool sh_fits(const int* plan, int n_kv, int n_q, int 
   return x.w == n_kv && y.x == n_q && y.y == rows && y.z == n_tables && y.w == max_blocks;
 }
 
-// inclusive sum over the block's threads; `all` gets the total
-__device__ __forceinline__ int block_scan(int v, int* s_warp, int& all) {
+// inclusive sums over the block's threads, of N values each; `all` gets the totals
+template <int N>
+__device__ __forceinline__ void block_scan(int (&v)[N], int (*s_warp)[32], int (&all)[N]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int p = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += p;
-  }
-  if (lane == 31) s_warp[warp] = v;
-  __syncthreads();
-  int w = lane < nw ? s_warp[lane] : 0;
-  const int mine = w;
+  for (int o = 1; o < 32; o <<= 1)
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int p = __shfl_up_sync(0xffffffffu, w, o);
-    if (lane >= o) w += p;
-  }
-  all = __shfl_sync(0xffffffffu, w, 31);
-  v += __shfl_sync(0xffffffffu, w - mine, warp);
+    for (int i = 0; i < N; ++i) {
+      const int p = __shfl_up_sync(0xffffffffu, v[i], o);
+      if (lane >= o) v[i] += p;
+    }
+  if (lane == 31)
+#pragma unroll
+    for (int i = 0; i < N; ++i) s_warp[i][warp] = v[i];
   __syncthreads();
-  return v;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    int w = lane < nw ? s_warp[i][lane] : 0;
+    const int mine = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int p = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += p;
+    }
+    all[i] = __shfl_sync(0xffffffffu, w, 31);
+    v[i] += __shfl_sync(0xffffffffu, w - mine, warp);
+  }
+  __syncthreads();
 }
 
 // Thread = row.  A run is the adjacent rows of one sequence.  Runs are joined into a group where their link (the pages that a run has in common with the one
@@ -104,7 +111,7 @@ __global__ void __launch_bounds__(SH_MAX_ROWS) shared_plan_kernel(const int* __r
                                                                   int rows, int n_tables, int width, int G, int n_kv, int* __restrict__ plan, int* status) {
   pdl_launch();
   __shared__ int s_seq[SH_MAX_ROWS], s_first[SH_MAX_ROWS + 1], s_link[SH_MAX_ROWS + 1], s_group[SH_MAX_ROWS], s_shared[SH_MAX_ROWS], s_gfirst[SH_MAX_ROWS + 1],
-      s_gmost[SH_MAX_ROWS], s_most[SH_MAX_ROWS], s_before[2 * SH_MAX_ROWS], s_warp[32];
+      s_gmost[SH_MAX_ROWS], s_most[SH_MAX_ROWS], s_before[2 * SH_MAX_ROWS], s_warp[3][32];
   pdl_wait();
   const int r = threadIdx.x, rt = SH_PAIRS / G;
   const bool live = r < rows;
@@ -117,15 +124,18 @@ __global__ void __launch_bounds__(SH_MAX_ROWS) shared_plan_kernel(const int* __r
   }
   if (live) s_seq[r] = seq, s_shared[r] = 0x7FFFFFFF, s_gmost[r] = s_most[r] = 0;
   __syncthreads();
-  int runs, groups, all;
   const bool head = live && (r == 0 || s_seq[r - 1] != seq);
-  const int run = block_scan(head, s_warp, runs) - 1;
+  int heads[1] = {head}, all_runs[1];
+  block_scan(heads, s_warp, all_runs);
+  const int run = heads[0] - 1, runs = all_runs[0];
   if (head) s_first[run] = r, s_link[run] = r == 0 || seq < 0 || s_seq[r - 1] < 0 ? 0 : link;
   if (r == 0) s_first[runs] = rows, s_link[runs] = 0;
   __syncthreads();
   const int mine = r < runs ? s_link[r] : 0;               // (thread = run)
   const bool joined = r > 0 && r < runs && mine >= SH_MIN_SHARED && 2 * (long long)mine >= s_link[r - 1] && 2 * (long long)mine >= s_link[r + 1];
-  const int g_of_run = block_scan(r < runs && !joined, s_warp, groups) - 1;
+  int leaders[1] = {r < runs && !joined}, all_groups[1];
+  block_scan(leaders, s_warp, all_groups);
+  const int g_of_run = leaders[0] - 1, groups = all_groups[0];
   if (r < runs) {
     s_group[r] = g_of_run;
     if (!joined) s_gfirst[g_of_run] = s_first[r];
@@ -144,17 +154,17 @@ __global__ void __launch_bounds__(SH_MAX_ROWS) shared_plan_kernel(const int* __r
   const int gfirst = live ? s_gfirst[group] : 0, tile = gfirst + (r - gfirst) / rt * rt;
   const int own = live ? max((s_most[chunk] + SH_PAGE - 1) / SH_PAGE - shared, 0) : 0;
   const bool lead_s = live && shared > 0 && r == tile, lead_o = live && own > 0 && r == chunk;
-  int pages_s, pages_o, blocks;
-  const int b_in = block_scan((lead_s ? 1 : 0) | (lead_o ? 1 << 16 : 0), s_warp, blocks);
   const int len_s = shared + SH_SEGMENT, len_o = own + SH_SEGMENT;
-  const int p_s = block_scan(lead_s ? len_s : 0, s_warp, pages_s), p_o = block_scan(lead_o ? len_o : 0, s_warp, pages_o);
+  int sum[3] = {(lead_s ? 1 : 0) | (lead_o ? 1 << 16 : 0), lead_s ? len_s : 0, lead_o ? len_o : 0}, sums[3];
+  block_scan(sum, s_warp, sums);
+  const int b_in = sum[0], p_s = sum[1], p_o = sum[2], blocks = sums[0], pages_s = sums[1], pages_o = sums[2];
   const int nb_s = blocks & 0xFFFF, nb = nb_s + (blocks >> 16);
   const int total = (pages_s + pages_o) * n_kv, L = max((total + SH_CTAS - 1) / SH_CTAS, 1);
   const int n_s = live ? min(rt, s_gfirst[group + 1] - tile) : 0, n_o = live ? min(rt, s_first[run + 1] - chunk) : 0;
   const int k_s = n_s * sh_slots(shared, L) * sh_copies(n_s * G), k_o = n_o * sh_slots(own, L) * sh_copies(n_o * G);
-  const int v_s = block_scan(lead_s ? k_s : 0, s_warp, all);
-  const int all_s = all;
-  const int v_o = block_scan(lead_o ? k_o : 0, s_warp, all);
+  int vec[2] = {lead_s ? k_s : 0, lead_o ? k_o : 0}, vecs[2];
+  block_scan(vec, s_warp, vecs);
+  const int v_s = vec[0], v_o = vec[1], all_s = vecs[0];
   ShBlock* blk = reinterpret_cast<ShBlock*>(plan + SH_AT_BLOCKS);
   // (s_link and s_first, then s_seq and s_gfirst are free: length and partial vectors before the block that begins at a row)
   __syncthreads();
@@ -989,7 +999,7 @@ static bool sh_takes(int rows, int n_q, int n_kv, int n_tables, int max_blocks) 
 RX_API int rx_attn_shared_plan(const void* row_seq, const void* ctx_len, const void* common, int rows, int n_tables, int max_blocks, int n_q, int n_kv, void* plan,
                                int* status, void* stream) {
   if (!sh_takes(rows, n_q, n_kv, n_tables, max_blocks)) return (int)cudaErrorInvalidValue;
-  const int threads = rows <= 128 ? 128 : (rows + 31) / 32 * 32;
+  const int threads = rows <= 320 ? 320 : (rows + 31) / 32 * 32;      // (a thread looks up a CTA's first block, too)
   return (int)rx::launch(shared_plan_kernel, dim3(1), dim3(threads), 0, (cudaStream_t)stream, (const int*)row_seq, (const int*)ctx_len, (const int*)common, rows,
                          n_tables, max_blocks, n_q / n_kv, n_kv, (int*)plan, status);
 }
