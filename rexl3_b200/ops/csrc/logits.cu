@@ -161,14 +161,14 @@ __device__ __forceinline__ float pick_rules(float v, uint32_t word, uint32_t dra
 constexpr int PICK_THREADS = 256, PICK_CTAS = 5, PICK_LIST = 512;
 struct PickShared { uint32_t best[PICK_THREADS], least; int n; uint64_t list[PICK_LIST], top[PICK_THREADS / 32]; };
 
-// The `count` (<= 64) largest keys of the block, in descending order, to out (0 where there are fewer).  `mine` is the order of the thread's best (0: it has
+// The `count` (<= 64) largest keys of the block, in descending order, to out, `apart` from one another (0 where there are fewer).  `mine` is the order of the thread's best (0: it has
 // none); each(least, f) calls f(key) for the thread's keys whose order is at least `least` (> 0).
 // As many threads as `count` have an order from the count-th largest of the threads' own best on, so no key with a lower order can be among the results.  One warp
 // searches for that threshold by halving the interval between the lowest and the highest best, and takes a lower one that few more threads pass: the steps that
 // are left would cost more than the few keys.  Each key that passes finds its place by counting the larger ones.
 // Where more pass than the list holds (many equal values, or one thread that has most of the high ones), the block's maximum is taken `count` times.
 template <typename Each>
-__device__ __forceinline__ void pick_select(uint32_t mine, Each each, int count, uint64_t* out, PickShared& sm) {
+__device__ __forceinline__ void pick_select(uint32_t mine, Each each, int count, uint64_t* out, int apart, PickShared& sm) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   sm.best[tid] = mine;
   if (tid == 0) sm.n = 0;
@@ -207,9 +207,9 @@ __device__ __forceinline__ void pick_select(uint32_t mine, Each each, int count,
       int place = 0;
 #pragma unroll 8
       for (int j = 0; j < n; ++j) place += sm.list[j] > own;
-      if (place < count) out[place] = own;
+      if (place < count) out[place * apart] = own;
     }
-    for (int r = n + tid; r < count; r += PICK_THREADS) out[r] = 0;
+    for (int r = n + tid; r < count; r += PICK_THREADS) out[r * apart] = 0;
     return;
   }
   uint64_t below = ~0ull, own = 0;                         // the last maximum; the thread's best that is below it
@@ -228,7 +228,7 @@ __device__ __forceinline__ void pick_select(uint32_t mine, Each each, int count,
 #pragma unroll
     for (int w = 0; w < PICK_THREADS / 32; ++w) below = max(below, sm.top[w]);
     again = below != 0 && own == below;
-    if (tid == 0) out[r] = below;
+    if (tid == 0) out[r * apart] = below;
     __syncthreads();
   }
 }
@@ -246,7 +246,7 @@ __device__ __forceinline__ float pick_max(float a, float b) {
 // values stand in shared memory, where the few ids that a rule touches are worked out again by themselves.  What is done for every id is a load, a test of its
 // count, a store, a load and a maximum, and its order is worked out only behind the threshold.  (With the rules and orders of all ids in registers, a division
 // inlined for each, 64 rows of 151,936 ids took 36 us, both stages; now 26 us, 59 MB or 9 us at the rate of a copy.  Bound by the chain of a CTA's phases -
-// loads, rules, threshold, list - with barriers between, at 40 % of the issue slots.  80 rows of 32,003 ids and 64 candidates 20 us, one row of 151,936 ids 9.7 us:
+// loads, rules, threshold, list - with barriers between, at 40 % of the issue slots.  80 rows of 32,003 ids and 64 candidates 18 us, one row of 151,936 ids 10 us:
 // two kernels of one CTA's latency each.)
 // Masked ids cost neither their logit nor their count.  An id at -inf is no candidate: it is one only where a row has fewer than `count` ids above -inf, and the
 // second selection finds those by counting.
@@ -318,18 +318,69 @@ __global__ void __launch_bounds__(PICK_THREADS, PICK_CTAS) pick_stage1_kernel(co
   for (int e = tid + PICK_THREADS; e < nb; e += PICK_THREADS) special |= bid[e] >= base && bid[e] - base < ids_here;
   for (int r = row - tid - PICK_THREADS; r >= r0; r -= PICK_THREADS) special |= a.fed[r] >= base && a.fed[r] - base < ids_here;
   if (__syncthreads_or(special)) {
-    // each such id again, with its drafts and biases (an id more than once: the same each time)
+    // Each such id again, with its drafts and biases.  Those of the chunk are listed first, with their places among the slot's biases (drafts: behind those); the first
+    // of an id adds up all of it in the order of the places.
     const float* bval = a.bias_val + (size_t)slot * a.n_bias;
-    for (int l = tid; l < nb + row - r0 + 1; l += PICK_THREADS) {
-      const int id = l < nb ? bid[l] : a.fed[r0 + l - nb], at = id - base;
-      if (id < base || at >= ids_here || (masked && !(mr[at >> 5] >> (at & 31) & 1))) continue;
+    if (tid == 0) sm.n = 0;
+    __syncthreads();
+    auto take = [&](int id, uint32_t place) {
+      if (id < base || id - base >= ids_here) return;
+      const int at = atomicAdd(&sm.n, 1);
+      if (at < PICK_LIST) sm.list[at] = (uint64_t)id << 32 | place;
+    };
+    for (int e = tid; e < nb; e += PICK_THREADS) take(bid[e], e);
+    for (int r = row - tid; r >= r0; r -= PICK_THREADS) take(a.fed[r], PICK_MAX_BIAS);
+    __syncthreads();
+    auto again = [&](int id, auto biases) {
+      const int at = id - base;
+      if (masked && !(mr[at >> 5] >> (at & 31) & 1)) return;
       uint32_t drafts = 0;
       for (int r = r0; r <= row; ++r) drafts += a.fed[r] == id;
-      float v = pick_rules(lr[at], cr != nullptr ? cr[at] : 0u, drafts, rep, freq, pres), sum = 0.f;
-      bool any = false;
-      for (int f = 0; f < nb; ++f)
-        if (bid[f] == id) sum = any ? __fadd_rn(sum, bval[f]) : bval[f], any = true;
+      const float v = pick_rules(lr[at], cr != nullptr ? cr[at] : 0u, drafts, rep, freq, pres);
+      float sum = 0.f;
+      const bool any = biases(sum);
       s_val[at] = any ? __fadd_rn(v, sum) : v;
+    };
+    const int listed = sm.n;
+    if (listed <= PICK_LIST) {
+      for (int l = tid; l < listed; l += PICK_THREADS) {
+        const uint64_t own = sm.list[l];
+        const int id = (int)(own >> 32);
+        uint64_t next = ~0ull;                             // the id's next place
+        bool first = true;
+        for (int j = 0; j < listed; ++j) {
+          const uint64_t other = sm.list[j];
+          if ((int)(other >> 32) != id) continue;
+          if (other < own) first = false;
+          else if (other > own) next = min(next, other);
+        }
+        if (!first) continue;                              // (a draft given twice: each the same)
+        again(id, [&](float& sum) {
+          uint32_t place = (uint32_t)own;
+          if (place >= PICK_MAX_BIAS) return false;
+          sum = bval[place];
+          for (uint64_t to = next; to != ~0ull && (uint32_t)to < PICK_MAX_BIAS;) {
+            place = (uint32_t)to;
+            sum = __fadd_rn(sum, bval[place]);
+            to = ~0ull;
+            for (int j = 0; j < listed; ++j)
+              if ((int)(sm.list[j] >> 32) == id && (uint32_t)sm.list[j] > place) to = min(to, sm.list[j]);
+          }
+          return true;
+        });
+      }
+    } else {
+      // more than the list holds: each for itself, an id more than once the same each time
+      for (int l = tid; l < nb + row - r0 + 1; l += PICK_THREADS) {
+        const int id = l < nb ? bid[l] : a.fed[r0 + l - nb];
+        if (id < base || id - base >= ids_here) continue;
+        again(id, [&](float& sum) {
+          bool any = false;
+          for (int f = 0; f < nb; ++f)
+            if (bid[f] == id) sum = any ? __fadd_rn(sum, bval[f]) : bval[f], any = true;
+          return any;
+        });
+      }
     }
     __syncthreads();
   }
@@ -363,15 +414,18 @@ __global__ void __launch_bounds__(PICK_THREADS, PICK_CTAS) pick_stage1_kernel(co
                   }
                 }
               },
-              a.count, a.cand + ((size_t)row * a.nchunks + blockIdx.x) * a.count, sm);
+              a.count, a.cand + (size_t)row * a.nchunks * a.count + blockIdx.x, a.nchunks, sm);
 }
 
-// total <= PICK_THREADS * 16 candidates a row
+// total <= PICK_THREADS * 16 candidates a row, the chunks' best first, then their second best and so on: the best of all are then those of different threads.  (Chunk
+// by chunk a few threads had most of them, the threshold let through more than the list holds, and four rows of 151,936 ids with 64 candidates took 37 us, now 11.)
 __global__ void __launch_bounds__(PICK_THREADS) pick_stage2_kernel(const uint64_t* cand, int total, int count, int* __restrict__ ids, float* __restrict__ vals) {
   pdl_launch();
   pdl_wait();
   __shared__ PickShared sm;
   __shared__ uint64_t outk[64];
+  __shared__ uint32_t taken[4];                            // of the ids below 128, those among the results
+  if (threadIdx.x < 4) taken[threadIdx.x] = 0;
   const int row = blockIdx.x;
   const uint64_t* c = cand + (size_t)row * total;
   constexpr int PER = 16;
@@ -389,7 +443,12 @@ __global__ void __launch_bounds__(PICK_THREADS) pick_stage2_kernel(const uint64_
                 for (int i = 0; i < PER; ++i)
                   if ((uint32_t)(k[i] >> 32) >= least) f(k[i]);
               },
-              count, outk, sm);
+              count, outk, 1, sm);
+  __syncthreads();
+  if ((int)threadIdx.x < count && outk[threadIdx.x] != 0) {
+    const uint32_t own = ~(uint32_t)outk[threadIdx.x];
+    if (own < 128) atomicOr(&taken[own >> 5], 1u << (own & 31));
+  }
   __syncthreads();
   if ((int)threadIdx.x >= count) return;
   int id;
@@ -398,17 +457,11 @@ __global__ void __launch_bounds__(PICK_THREADS) pick_stage2_kernel(const uint64_
     id = (int)(~(uint32_t)outk[threadIdx.x]);
     v = pick_value((uint32_t)(outk[threadIdx.x] >> 32));
   } else {
-    // Fewer ids above -inf than places: the lowest of the other ids, which all stand at -inf, in order.  The q-th id that is not among n others is q + (how
-    // many of those are not above it).
-    int n = 0;
-    while (n < count && outk[n] != 0) ++n;
-    const int q = (int)threadIdx.x - n;
-    int passed = 0;
-    do {
-      id = q + passed;
-      passed = 0;
-      for (int j = 0; j < n; ++j) passed += (int)(~(uint32_t)outk[j]) <= id;
-    } while (q + passed != id);
+    // Fewer ids above -inf than places: the lowest of the other ids, which all stand at -inf, in order.  With at most 64 ids to leave out they are below 128.
+    int q = threadIdx.x, w = 0;
+    for (int r = 0; r < count; ++r) q -= outk[r] != 0;
+    while (q >= __popc(~taken[w])) q -= __popc(~taken[w]), ++w;
+    id = w * 32 + __fns(~taken[w], 0, q + 1);
   }
   ids[(size_t)row * count + threadIdx.x] = id;
   vals[(size_t)row * count + threadIdx.x] = v;
@@ -449,8 +502,8 @@ RX_API int rx_token_counts_add(void* counts, int n_slots, int vocab, const void*
 RX_API int rx_topk_adjusted(const void* logits, long long ld, int rows, int vocab, int count, void* scratch, void* ids, void* vals, const void* row_slot,
                             const void* counts, const void* penalties, int n_slots, const void* bias_id, const void* bias_val, int n_bias, const void* mask,
                             const void* mask_row, int n_masks, const void* first, const void* fed, void* stream) {
-  // Chunks of 4096 ids where all of them run at once: twice as many CTAs, each done sooner (80 rows of 32,003 ids 24 -> 20 us, one row of 151,936 10.7 -> 9.7 us).  Else of
-  // 8192: half as many selections (64 rows of 151,936 ids 30 -> 26 us).
+  // Chunks of 4096 ids where all of them run at once: twice as many CTAs, each done sooner (with 8192: 80 rows of 32,003 ids 24 against 20 us, one row of 151,936 ids
+  // 10.7 against 9.7 us).  Else of 8192: half as many selections (64 rows of 151,936 ids 30 against 26 us).
   const bool small = (long long)rows * ((vocab + 4095) / 4096) <= 148 * PICK_CTAS;
   const int nchunks = small ? (vocab + 4095) / 4096 : (vocab + 8191) / 8192;
   if (rows < 1 || rows > 65535 || vocab < 1 || count < 1 || count > 64 || count > vocab || (long long)nchunks * count > PICK_THREADS * 16 || ld < vocab || n_bias < 0 || n_bias > PICK_MAX_BIAS ||

@@ -117,6 +117,14 @@ def test_few_ids_left(allowed):
     same(x, 28, mask=((words - (words >> 31 << 32)).int().contiguous(), t([0, 1, 2])))
 
 
+@pytest.mark.parametrize("allowed", [[], [0], list(range(63)), list(range(64)), list(range(0, 126, 2)), list(range(63, 127)), [0, 500] + list(range(64, 125)), [8999]])
+def test_places_without_a_candidate_take_the_lowest_ids(allowed):
+    V = 9001
+    x = torch.full((1, V), NEG, device="cuda")
+    x[0, allowed] = torch.randn(len(allowed), device="cuda")
+    same(x, 64)
+
+
 def test_infinities_nan_and_masked_nan():
     V = 5000
     x = torch.randn(4, V, device="cuda")
@@ -149,6 +157,14 @@ def test_a_bias_given_more_than_once_adds_up_in_order():
     vals = (10.0 ** torch.linspace(-6, 6, nb, device="cuda") * torch.where(torch.arange(nb, device="cuda") % 2 == 0, 1.0, -0.999))[None].contiguous()
     same(torch.randn(1, V, device="cuda"), 28, t([0]), bias=(ids, vals))
     same(torch.randn(1, V, device="cuda"), 28, t([0]), bias=(torch.full((1, 1024), 5, dtype=torch.int32, device="cuda"), torch.randn(1, 1024, device="cuda")))
+
+
+@pytest.mark.parametrize("V,nb", [(2048, 200), (2048, 1024), (9000, 1024), (40, 1000)])
+def test_many_biases_and_drafts(V, nb):
+    kw = rules(12, V, 2, V + nb, nb=nb)
+    kw["bias"][0].remainder_(max(V // 4, 30))                            # most ids more than once, some of them among the drafts
+    kw["window"] = (kw["window"][0], kw["window"][1].remainder(max(V // 4, 30)))
+    same(torch.randn(12, V, device="cuda"), 28, kw.pop("row_slot"), **kw)
 
 
 def test_drafts_of_a_window_count_for_the_rows_behind_them():
