@@ -28,7 +28,7 @@
 //     64 rows behind 8192 common keys, 60 .. 700 keys of their own: 45 us.  134 MB, 20.6 us at the rate of a copy: three blocks a page, a page 0.9 us of an SM - the
 //         chain from scores over 64 exponentials a lane to P and back - and the first pages' way from memory.
 //     48 rows of 500 .. 4000 keys behind 150 common ones: 85 us.  448 MB, 68.6 us: bound by memory, 5.2 TB/s.
-//     32 rows behind 32,700 common keys, E4M3: 69 us.  104 MB, 16 us: bound by instructions, the expansion's beside the softmax's (bf16: 208 MB, 61 us).
+//     32 rows behind 32,700 common keys, E4M3: 65 us.  104 MB, 16 us: bound by instructions, the expansion's beside the softmax's (bf16: 208 MB, 61 us).
 #include <cuda.h>
 #include <cuda_fp8.h>
 #include <type_traits>
@@ -44,6 +44,11 @@ constexpr int SH_MIN_SHARED = 1;
 // 16 sequences of five rows behind 4001 28, 26, 25, 25; 48 E4M3 rows of 500 .. 4000 keys 98, 78, 76, 76.  Pages weighted by the copies of their block's pairs, 8 : 7 : 6,
 // changed as much for the worse as for the better.)
 constexpr int SH_SEGMENT = 2;
+// A CTA's piece has no least length: one of two or four pages leaves fewer partial outputs, but on 57 drawn windows of all sizes it gained nothing, or lost 7 %.
+// Few warps of the merge would join many partial outputs one after the other, so up to 148 blocks of 128 outputs go by 16 warps each where a row may have more than 64,
+// up to 1480 by four, more by one: two rows of five heads behind 31,637 keys, 992 partial outputs each, 90 -> 26 us of the whole call; 32 rows of 40 heads behind 32,700
+// (1280 blocks of some 30) 70 -> 65 us; but 1728 blocks of few 24 -> 27 us by four, and four blocks of few 11.0 -> 12.7 us by 16.
+constexpr int SH_SPLIT16 = 148, SH_SPLIT16_OF = 64, SH_SPLIT4 = 1480;
 
 // ------------------------------------------------------------------------------------------------ plan
 // Layout (int32): [0] length of the line  [1] a CTA's piece  [2] blocks  [3] n_kv  [4] n_q  [5] rows  [6] table rows  [7] pages of one, then the block at which each CTA begins, the blocks, per row what the merge
@@ -882,18 +887,19 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
 }
 
 // ------------------------------------------------------------------------------------------------ merge
-// Joins a row's partial outputs, common pages before own, CTA by CTA: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  A warp per 128 outputs; with
-// `suh` also xr = fp16(H(out * suh)), the input rotation of the output projection.
-// Bound by latency, so all partial outputs of a turn are on their way at once (25 rows of 31 each: 40 -> 37 us of the whole call, against eight at a time; four
-// warps for each 128 outputs and a sum over shared memory: 38 us, but 48 rows of 14 each 86 -> 90 us).
-template <int HD>
-__global__ void __launch_bounds__(128) attn_shared_merge_kernel(const int* plan, const float* part_o, const float* part_ml, int n_q, int n_kv, int n_tables,
-                                                                int max_blocks, const __half* __restrict__ suh, __half* __restrict__ xr, uint16_t* __restrict__ out) {
+// Joins a row's partial outputs, common pages before own, CTA by CTA: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  128 outputs by SPLIT warps, each
+// with every SPLIT-th slot, and U partial outputs of a warp on their way at once; with `suh` also xr = fp16(H(out * suh)), the input rotation of the output projection.
+template <int HD, int SPLIT, int U>
+__global__ void __launch_bounds__(SPLIT > 4 ? 32 * SPLIT : 128) attn_shared_merge_kernel(const int* plan, const float* part_o, const float* part_ml, int n_q, int n_kv,
+                                                                                         int n_tables, int max_blocks, const __half* __restrict__ suh,
+                                                                                         __half* __restrict__ xr, uint16_t* __restrict__ out) {
   pdl_launch();
-  const int row = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, width = n_q * HD, b = blockIdx.y * 4 + warp;
-  const int e0 = b * 128 + lane * 4, hq = e0 / HD, d0 = e0 % HD, kvh = hq / (n_q / n_kv);
+  __shared__ float4 s_acc[SPLIT][32];
+  __shared__ float2 s_ml[SPLIT][32];
+  const int row = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, width = n_q * HD, who = SPLIT > 1 ? warp : 0;
+  const int b = SPLIT > 1 ? blockIdx.y : blockIdx.y * 4 + warp, e0 = b * 128 + lane * 4, hq = e0 / HD, d0 = e0 % HD, kvh = hq / (n_q / n_kv);
   pdl_wait();
-  if (b >= width / 128) return;                           // (a whole warp)
+  if (b >= width / 128) return;                           // (a whole warp; with SPLIT none)
   const bool fits = sh_fits(plan, n_kv, n_q, gridDim.x, n_tables, max_blocks);
   const int L = plan[1];
   const int4* of = reinterpret_cast<const int4*>(plan + SH_AT_ROWS) + 2 * row;
@@ -907,18 +913,22 @@ __global__ void __launch_bounds__(128) attn_shared_merge_kernel(const int* plan,
     n[u] = ((unit + s.y - 1) / L - unit / L + 1) * s.w;
     at[u] = (size_t)s.z * n_q + hq;
   }
-  auto slot = [&](int s) { return s < n[0] ? at[0] + (size_t)s * n_q : at[1] + (size_t)(s - n[0]) * n_q; };
-  const int all = n[0] + n[1];
+  auto slot = [&](int i) {
+    const int s = i * SPLIT + who;
+    return s < n[0] ? at[0] + (size_t)s * n_q : at[1] + (size_t)(s - n[0]) * n_q;
+  };
+  const int all = (n[0] + n[1] - who + SPLIT - 1) / SPLIT;      // the warp's slots
   // A head's GL lanes take GL slots at a time, lane = slot for the maxima and factors.  (Two heads of 64 in a warp may have unlike numbers of slots.)
   constexpr int GL = HD / 4;
+  static_assert(GL % U == 0, "whole turns");
   const int gl = lane % GL, g0 = lane - gl, most = HD == 128 ? all : max(all, __shfl_xor_sync(0xffffffffu, all, 16));
   float acc[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f, m = -INFINITY;
   for (int s0 = 0; s0 < most; s0 += GL) {
     const int here = min(GL, all - s0);                   // (of the other head of the warp, maybe none)
     const float2 ml = gl < here ? *reinterpret_cast<const float2*>(part_ml + slot(s0 + gl) * 2) : make_float2(-INFINITY, 0.f);
-    float4 o[GL];
+    float4 o[U];
 #pragma unroll
-    for (int u = 0; u < GL; ++u)
+    for (int u = 0; u < U; ++u)
       if (u < here) o[u] = *reinterpret_cast<const float4*>(part_o + slot(s0 + u) * HD + d0);
     float top = ml.x;
 #pragma unroll
@@ -930,16 +940,46 @@ __global__ void __launch_bounds__(128) attn_shared_merge_kernel(const int* plan,
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] *= old;
 #pragma unroll
-    for (int u = 0; u < GL; ++u) {
-      const float g = __shfl_sync(0xffffffffu, f, g0 + u);
-      if (u < here) acc[0] += g * o[u].x, acc[1] += g * o[u].y, acc[2] += g * o[u].z, acc[3] += g * o[u].w;
+    for (int u0 = 0; u0 < GL; u0 += U) {
+      if (u0 > 0) {
+        if (u0 >= min(GL, most - s0)) break;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (u0 + u < here) o[u] = *reinterpret_cast<const float4*>(part_o + slot(s0 + u0 + u) * HD + d0);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float g = __shfl_sync(0xffffffffu, f, g0 + u0 + u);
+        if (u0 + u < here) acc[0] += g * o[u].x, acc[1] += g * o[u].y, acc[2] += g * o[u].z, acc[3] += g * o[u].w;
+      }
     }
   }
 #pragma unroll
   for (int w = GL / 2; w > 0; w >>= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
+  if constexpr (SPLIT > 1) {
+    s_acc[who][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    s_ml[who][lane] = make_float2(m, l);
+    __syncthreads();
+    if (who != 0) return;
+    float top = m;
+#pragma unroll
+    for (int w = 1; w < SPLIT; ++w) top = fmaxf(top, s_ml[w][lane].x);
+    const float own = m == -INFINITY ? 0.f : exp2f(m - top);
+    l *= own;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] *= own;
+#pragma unroll 4
+    for (int w = 1; w < SPLIT; ++w) {
+      const float2 ml = s_ml[w][lane];
+      const float4 o = s_acc[w][lane];
+      const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
+      l += f * ml.y;
+      acc[0] += f * o.x, acc[1] += f * o.y, acc[2] += f * o.z, acc[3] += f * o.w;
+    }
+  }
   const float inv = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) acc[i] = all > 0 ? acc[i] * inv : 0.f;
+  for (int i = 0; i < 4; ++i) acc[i] = n[0] + n[1] > 0 ? acc[i] * inv : 0.f;
   if (out != nullptr) *reinterpret_cast<uint2*>(out + (size_t)row * width + e0) = make_uint2(sh_pack<false>(acc[0], acc[1]), sh_pack<false>(acc[2], acc[3]));
   if (xr != nullptr) {
 #pragma unroll
@@ -1034,6 +1074,10 @@ RX_API int rx_attn_shared(const void* tmap_k, const void* tmap_v, const void* q,
   else e = kv_scale != nullptr ? launch_shared<64, true>(dev, tk, tv, tq, a, st) : launch_shared<64, false>(dev, tk, tv, tq, a, st);
   if (e != cudaSuccess) return (int)e;
   // (early whatever the grid: the kernel before is one wave whose CTAs leave room beside them)
-  return (int)rx::launch_pdl(true, hd == 128 ? attn_shared_merge_kernel<128> : attn_shared_merge_kernel<64>, dim3(rows, (n_q * hd / 128 + 3) / 4), dim3(128), 0, st, a.plan,
-                             a.part_o, a.part_ml, n_q, n_kv, n_tables, max_blocks, (const __half*)suh, (__half*)xr, (uint16_t*)out);
+  const long long blocks = n_q * hd / 128, merges = rows * blocks;
+  const int split = merges <= SH_SPLIT16 && 4ll * max_blocks > SH_SPLIT16_OF ? 16 : merges <= SH_SPLIT4 ? 4 : 1;      // (each page may leave four)
+  const auto merge = hd == 128 ? (split == 16 ? attn_shared_merge_kernel<128, 16, 16> : split == 4 ? attn_shared_merge_kernel<128, 4, 8> : attn_shared_merge_kernel<128, 1, 32>)
+                               : (split == 16 ? attn_shared_merge_kernel<64, 16, 16> : split == 4 ? attn_shared_merge_kernel<64, 4, 8> : attn_shared_merge_kernel<64, 1, 16>);
+  return (int)rx::launch_pdl(true, merge, dim3(rows, (unsigned)(split > 1 ? blocks : (blocks + 3) / 4)), dim3(split > 4 ? 32 * split : 128), 0, st, a.plan, a.part_o, a.part_ml, n_q, n_kv,
+                             n_tables, max_blocks, (const __half*)suh, (__half*)xr, (uint16_t*)out);
 }
