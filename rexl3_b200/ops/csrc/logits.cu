@@ -164,7 +164,7 @@ struct PickShared { uint32_t best[PICK_THREADS], least; int n; uint64_t list[PIC
 // The `count` (<= 64) largest keys of the block, in descending order, to out, `apart` from one another (0 where there are fewer).  `mine` is the order of the thread's best (0: it has
 // none); each(least, f) calls f(key) for the thread's keys whose order is at least `least` (> 0).
 // As many threads as `count` have an order from the count-th largest of the threads' own best on, so no key with a lower order can be among the results.  One warp
-// searches for that threshold by halving the interval between the lowest and the highest best, and takes a lower one that few more threads pass: the steps that
+// searches for that threshold by quartering the interval between the lowest and the highest best, and takes a lower one that few more threads pass: the steps that
 // are left would cost more than the few keys.  Each key that passes finds its place by counting the larger ones.
 // Where more pass than the list holds (many equal values, or one thread that has most of the high ones), the block's maximum is taken `count` times.
 template <typename Each>
@@ -176,21 +176,28 @@ __device__ __forceinline__ void pick_select(uint32_t mine, Each each, int count,
   if (warp == 0) {
     constexpr int K = PICK_THREADS / 32;
     uint32_t b[K], lo = ~0u, hi = 0;
+    int pass = 0;                                          // threads from lo on; from hi + 1 on too few
 #pragma unroll
-    for (int i = 0; i < K; ++i) b[i] = sm.best[i * 32 + lane], lo = min(lo, b[i]), hi = max(hi, b[i]);
-    lo = __reduce_min_sync(0xffffffffu, lo);
+    for (int i = 0; i < K; ++i) b[i] = sm.best[i * 32 + lane], lo = min(lo, b[i] - 1), hi = max(hi, b[i]), pass += b[i] != 0;
+    lo = __reduce_min_sync(0xffffffffu, lo) + 1;           // (of those that have any)
     hi = __reduce_max_sync(0xffffffffu, hi);
-    int pass = PICK_THREADS;                               // threads from lo on; from hi on: too few, or hi is the highest
+    pass = __reduce_add_sync(0xffffffffu, pass);
+    if (pass < count) lo = hi = 1;                         // all
     while (pass > count + count / 4 + 2 && lo < hi) {
-      const uint32_t mid = hi - (hi - lo) / 2;
-      int c = 0;
+      // three probes at once: a step's time is that of its chain
+      const uint32_t q = (hi - lo) / 4, m1 = lo + q + 1, m3 = hi - q, m2 = m1 + (m3 - m1) / 2;
+      int c1 = 0, c2 = 0, c3 = 0;
 #pragma unroll
-      for (int i = 0; i < K; ++i) c += b[i] >= mid;
-      c = __reduce_add_sync(0xffffffffu, c);
-      if (c >= count) lo = mid, pass = c;
-      else hi = mid - 1;
+      for (int i = 0; i < K; ++i) c1 += b[i] >= m1, c2 += b[i] >= m2, c3 += b[i] >= m3;
+      c1 = __reduce_add_sync(0xffffffffu, c1);
+      c2 = __reduce_add_sync(0xffffffffu, c2);
+      c3 = __reduce_add_sync(0xffffffffu, c3);
+      if (c3 >= count) lo = m3, pass = c3;
+      else if (c2 >= count) lo = m2, pass = c2, hi = m3 - 1;
+      else if (c1 >= count) lo = m1, pass = c1, hi = m2 - 1;
+      else hi = m1 - 1;
     }
-    if (lane == 0) sm.least = max(lo, 1u);
+    if (lane == 0) sm.least = lo;
   }
   __syncthreads();
   const uint32_t least = sm.least;
@@ -305,13 +312,16 @@ __global__ void __launch_bounds__(PICK_THREADS, PICK_CTAS) pick_stage1_kernel(co
       s_val[at] = v;
     }
   }
+  // two at a time: their counts come from L2 once more
   while (touched != 0) {
-    const int i = __ffs(touched) - 1, at = (i / W * PICK_THREADS + tid) * W + i % W;
-    touched &= touched - 1;
-    const float v = s_val[at];
-    if (v != -INFINITY) s_val[at] = pick_rules(v, cr[at], 0, rep, freq, pres);                     // at -inf it stays, and a masked id is there
+    const int i = __ffs(touched) - 1, rest = touched & (touched - 1), k = rest != 0 ? __ffs(rest) - 1 : i;
+    touched = rest & (rest - 1);
+    const int at = (i / W * PICK_THREADS + tid) * W + i % W, to = (k / W * PICK_THREADS + tid) * W + k % W;
+    const uint32_t word = cr[at], other = cr[to];
+    const float v = s_val[at], u = s_val[to];
+    if (v != -INFINITY) s_val[at] = pick_rules(v, word, 0, rep, freq, pres);                       // at -inf it stays, and a masked id is there
+    if (k != i && u != -INFINITY) s_val[to] = pick_rules(u, other, 0, rep, freq, pres);
   }
-  // ids with a bias or among the drafts, where there are any in this chunk
   const int r0 = max(window, 0) + 1;
   bool special = bias0 >= base && bias0 - base < ids_here;
   if (row - tid >= r0) special |= fed0 >= base && fed0 - base < ids_here;
@@ -397,21 +407,24 @@ __global__ void __launch_bounds__(PICK_THREADS, PICK_CTAS) pick_stage1_kernel(co
   }
   pick_select(top != -INFINITY ? pick_order(top) : 0u,
               [&](uint32_t least, auto f) {
-                const float from = pick_value(least);      // a NaN: the values say nothing yet
-#pragma unroll 4
+                const float from = pick_value(least);      // (a NaN: the values say nothing yet)
+                uint32_t hits = 0;
+#pragma unroll
                 for (int i = 0; i < N; ++i) {
                   const int at = (i * PICK_THREADS + tid) * W;
                   if constexpr (VEC) {
                     const float4 v = *reinterpret_cast<const float4*>(s_val + at);
-                    if (pick_max(pick_max(v.x, v.y), pick_max(v.z, v.w)) < from) continue;
+                    hits |= ((v.x < from ? 0u : 1u) | (v.y < from ? 0u : 2u) | (v.z < from ? 0u : 4u) | (v.w < from ? 0u : 8u)) << (i * W);
+                  } else {
+                    hits |= (s_val[at] < from ? 0u : 1u) << i;
                   }
-#pragma unroll 1
-                  for (int k = 0; k < W; ++k) {
-                    const float v = s_val[at + k];
-                    if (v < from || v == -INFINITY) continue;
-                    const uint32_t order = pick_order(v);
-                    if (order >= least) f(pick_key(order, base + at + k));
-                  }
+                }
+                while (hits != 0) {
+                  const int i = __ffs(hits) - 1, at = (i / W * PICK_THREADS + tid) * W + i % W;
+                  hits &= hits - 1;
+                  const float v = s_val[at];
+                  const uint32_t order = pick_order(v);
+                  if (v != -INFINITY && order >= least) f(pick_key(order, base + at));
                 }
               },
               a.count, a.cand + (size_t)row * a.nchunks * a.count + blockIdx.x, a.nchunks, sm);
