@@ -407,7 +407,8 @@ __global__ void __launch_bounds__(PICK_THREADS, PICK_CTAS) pick_stage1_kernel(co
   }
   pick_select(top != -INFINITY ? pick_order(top) : 0u,
               [&](uint32_t least, auto f) {
-                const float from = pick_value(least);      // (a NaN: the values say nothing yet)
+                // from the lowest finite value on where all may pass, else -inf would be looked at one by one (a NaN: the values say nothing yet)
+                const float lowest = -3.402823466e+38f, from = least < pick_order(lowest) ? lowest : pick_value(least);
                 uint32_t hits = 0;
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
