@@ -252,18 +252,20 @@ __device__ __forceinline__ float pick_max(float a, float b) {
 // A CTA takes 256 PER ids of a row, a thread PER of them: VEC: four ids side by side at a time (16-byte loads of logits, 8-byte loads of counts); else one.  Their
 // values stand in shared memory, where the few ids that a rule touches are worked out again by themselves.  What is done for every id is a load, a test of its
 // count, a store, a load and a maximum, and its order is worked out only behind the threshold.  (With the rules and orders of all ids in registers, a division
-// inlined for each, 64 rows of 151,936 ids took 36 us, both stages; now 26 us, 59 MB or 9 us at the rate of a copy.  Bound by the chain of a CTA's phases -
-// loads, rules, threshold, list - with barriers between, at 40 % of the issue slots.  80 rows of 32,003 ids and 64 candidates 18 us, one row of 151,936 ids 10 us:
-// two kernels of one CTA's latency each.)
+// inlined for each, 64 rows of 151,936 ids took 36 us, both stages.)  Now 20.5 us, 59 MB or 9 us at the rate of a copy: bound by the chain of a CTA's phases -
+// slot and masks, ids, rules, biases, threshold, list - with barriers between.  80 rows of 32,003 ids and 64 candidates 13.5 us, one row of 151,936 ids 6.4 us: two
+// kernels of one CTA's latency each.
 // Masked ids cost neither their logit nor their count.  An id at -inf is no candidate: it is one only where a row has fewer than `count` ids above -inf, and the
 // second selection finds those by counting.
 template <bool VEC, int PER>
 __global__ void __launch_bounds__(PICK_THREADS, PICK_CTAS) pick_stage1_kernel(const __grid_constant__ PickArgs a) {
   pdl_launch();
-  pdl_wait();
   constexpr int W = VEC ? 4 : 1, N = PER / W, CHUNK = PICK_THREADS * PER;
   __shared__ PickShared sm;
   __shared__ __align__(16) float s_val[CHUNK];
+  if (threadIdx.x == 0) sm.n = 0;
+  pdl_wait();
+  __syncthreads();
   const int row = blockIdx.y, tid = threadIdx.x, base = blockIdx.x * CHUNK, ids_here = min(a.vocab - base, CHUNK);
   const int slot_in = a.row_slot != nullptr ? a.row_slot[row] : -1, slot = slot_in >= 0 && slot_in < a.n_slots ? slot_in : -1;
   const int mrow = a.mask != nullptr ? a.mask_row[row] : -1;
@@ -323,24 +325,21 @@ __global__ void __launch_bounds__(PICK_THREADS, PICK_CTAS) pick_stage1_kernel(co
     if (k != i && u != -INFINITY) s_val[to] = pick_rules(u, other, 0, rep, freq, pres);
   }
   const int r0 = max(window, 0) + 1;
-  bool special = bias0 >= base && bias0 - base < ids_here;
-  if (row - tid >= r0) special |= fed0 >= base && fed0 - base < ids_here;
-  for (int e = tid + PICK_THREADS; e < nb; e += PICK_THREADS) special |= bid[e] >= base && bid[e] - base < ids_here;
-  for (int r = row - tid - PICK_THREADS; r >= r0; r -= PICK_THREADS) special |= a.fed[r] >= base && a.fed[r] - base < ids_here;
-  if (__syncthreads_or(special)) {
-    // Each such id again, with its drafts and biases.  Those of the chunk are listed first, with their places among the slot's biases (drafts: behind those); the first
-    // of an id adds up all of it in the order of the places.
+  // Ids of the chunk with a bias or among the drafts are listed, with their places among the slot's biases (drafts: behind those).
+  auto take = [&](int id, uint32_t place) {
+    if (id < base || id - base >= ids_here) return;
+    const int at = atomicAdd(&sm.n, 1);
+    if (at < PICK_LIST) sm.list[at] = (uint64_t)id << 32 | place;
+  };
+  take(bias0, tid);
+  if (row - tid >= r0) take(fed0, PICK_MAX_BIAS);
+  for (int e = tid + PICK_THREADS; e < nb; e += PICK_THREADS) take(bid[e], e);
+  for (int r = row - tid - PICK_THREADS; r >= r0; r -= PICK_THREADS) take(a.fed[r], PICK_MAX_BIAS);
+  __syncthreads();
+  const int listed = sm.n;
+  if (listed > 0) {
+    // Each such id again, with its drafts and biases; the first of an id adds up all of it in the order of the places.
     const float* bval = a.bias_val + (size_t)slot * a.n_bias;
-    if (tid == 0) sm.n = 0;
-    __syncthreads();
-    auto take = [&](int id, uint32_t place) {
-      if (id < base || id - base >= ids_here) return;
-      const int at = atomicAdd(&sm.n, 1);
-      if (at < PICK_LIST) sm.list[at] = (uint64_t)id << 32 | place;
-    };
-    for (int e = tid; e < nb; e += PICK_THREADS) take(bid[e], e);
-    for (int r = row - tid; r >= r0; r -= PICK_THREADS) take(a.fed[r], PICK_MAX_BIAS);
-    __syncthreads();
     auto again = [&](int id, auto biases) {
       const int at = id - base;
       if (masked && !(mr[at >> 5] >> (at & 31) & 1)) return;
@@ -351,7 +350,6 @@ __global__ void __launch_bounds__(PICK_THREADS, PICK_CTAS) pick_stage1_kernel(co
       const bool any = biases(sum);
       s_val[at] = any ? __fadd_rn(v, sum) : v;
     };
-    const int listed = sm.n;
     if (listed <= PICK_LIST) {
       for (int l = tid; l < listed; l += PICK_THREADS) {
         const uint64_t own = sm.list[l];
@@ -432,7 +430,7 @@ __global__ void __launch_bounds__(PICK_THREADS, PICK_CTAS) pick_stage1_kernel(co
 }
 
 // total <= PICK_THREADS * 16 candidates a row, the chunks' best first, then their second best and so on: the best of all are then those of different threads.  (Chunk
-// by chunk a few threads had most of them, the threshold let through more than the list holds, and four rows of 151,936 ids with 64 candidates took 37 us, now 11.)
+// by chunk a few threads had most of them, the threshold let through more than the list holds, and four rows of 151,936 ids with 64 candidates took 37 us, then 11.)
 __global__ void __launch_bounds__(PICK_THREADS) pick_stage2_kernel(const uint64_t* cand, int total, int count, int* __restrict__ ids, float* __restrict__ vals) {
   pdl_launch();
   pdl_wait();
@@ -516,8 +514,8 @@ RX_API int rx_token_counts_add(void* counts, int n_slots, int vocab, const void*
 RX_API int rx_topk_adjusted(const void* logits, long long ld, int rows, int vocab, int count, void* scratch, void* ids, void* vals, const void* row_slot,
                             const void* counts, const void* penalties, int n_slots, const void* bias_id, const void* bias_val, int n_bias, const void* mask,
                             const void* mask_row, int n_masks, const void* first, const void* fed, void* stream) {
-  // Chunks of 4096 ids where all of them run at once: twice as many CTAs, each done sooner (with 8192: 80 rows of 32,003 ids 24 against 20 us, one row of 151,936 ids
-  // 10.7 against 9.7 us).  Else of 8192: half as many selections (64 rows of 151,936 ids 30 against 26 us).
+  // Chunks of 4096 ids where all of them run at once: twice as many CTAs, each done sooner (with 8192: 80 rows of 32,003 ids 15.2 against 13.6 us, one row of 151,936
+  // ids 10.3 against 8.0 us).  Else of 8192: half as many selections (64 rows of 151,936 ids 25.0 against 22.4 us).
   const bool small = (long long)rows * ((vocab + 4095) / 4096) <= 148 * PICK_CTAS;
   const int nchunks = small ? (vocab + 4095) / 4096 : (vocab + 8191) / 8192;
   if (rows < 1 || rows > 65535 || vocab < 1 || count < 1 || count > 64 || count > vocab || (long long)nchunks * count > PICK_THREADS * 16 || ld < vocab || n_bias < 0 || n_bias > PICK_MAX_BIAS ||
