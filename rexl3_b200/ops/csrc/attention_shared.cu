@@ -1074,7 +1074,7 @@ RX_API int rx_attn_shared(const void* tmap_k, const void* tmap_v, const void* q,
   if (hd == 128) e = kv_scale != nullptr ? launch_shared<128, true>(dev, tk, tv, tq, a, st) : launch_shared<128, false>(dev, tk, tv, tq, a, st);
   else e = kv_scale != nullptr ? launch_shared<64, true>(dev, tk, tv, tq, a, st) : launch_shared<64, false>(dev, tk, tv, tq, a, st);
   if (e != cudaSuccess) return (int)e;
-  // (early whatever the grid: the kernel before is one wave whose CTAs leave room beside them)
+  // (early whatever the grid: the kernel before is one wave of CTAs that do not wait for one another, and where one has ended the merge's next is there already)
   const long long blocks = n_q * hd / 128, merges = rows * blocks;
   const int split = merges <= SH_SPLIT16 && 4ll * max_blocks > SH_SPLIT16_OF ? 16 : merges <= SH_SPLIT4 ? 4 : 1;      // (each page may leave four)
   const auto merge = hd == 128 ? (split == 16 ? attn_shared_merge_kernel<128, 16, 16> : split == 4 ? attn_shared_merge_kernel<128, 4, 8> : attn_shared_merge_kernel<128, 1, 32>)
