@@ -37,7 +37,7 @@
 
 namespace rx {
 
-constexpr int SH_PAGE = 64, SH_PAIRS = 128, SH_CTAS = 296, SH_MAX_ROWS = 1024;
+constexpr int SH_PAGE = 64, SH_PAIRS = 128, SH_CTAS = 296, SH_MAX_ROWS = 1024, SH_FUSED_ROWS = 64;
 // Pages that a group must have in common.  (64 rows of 40 heads and 100 .. 700 keys: of one common page nothing comes either way, 3 pages 37.1 against 38.5 us where
 // each sequence reads them for itself, 6 pages 37.4 against 40.6; 256 rows of 8 heads and up to 60 keys behind 3 pages 23.5 against 27 us.)
 constexpr int SH_MIN_SHARED = 1;
@@ -113,18 +113,23 @@ __device__ __forceinline__ void block_scan(int (&v)[N], int (*s_warp)[32], int (
 // Thread = row.  A run is the adjacent rows of one sequence.  Runs are joined into a group where their link (the pages that a run has in common with the one
 // before it) is at least SH_MIN_SHARED pages and at least half of each neighbouring link: a group shares its smallest link, and one pair of
 // strangers with nothing but a first page in common must not take a long prompt away from the pairs on both sides.
-__global__ void __launch_bounds__(SH_MAX_ROWS) shared_plan_kernel(const int* __restrict__ row_seq, const int* __restrict__ ctx_len, const int* __restrict__ common,
-                                                                  int rows, int n_tables, int width, int G, int n_kv, int* __restrict__ plan, int* status) {
-  pdl_launch();
-  __shared__ int s_seq[SH_MAX_ROWS], s_first[SH_MAX_ROWS + 1], s_link[SH_MAX_ROWS + 1], s_group[SH_MAX_ROWS], s_shared[SH_MAX_ROWS], s_gfirst[SH_MAX_ROWS + 1],
-      s_gmost[SH_MAX_ROWS], s_most[SH_MAX_ROWS], s_before[2 * SH_MAX_ROWS], s_warp[3][32];
-  pdl_wait();
+// Of up to MAX rows, by all threads of the block, at least as many; its thread `r` looks up the first blocks of the CTAs cta, cta + cta_step ...;
+// `all`: what the merge asks, and the status, too.
+template <int MAX>
+struct ShPlan {
+  int seq[MAX], first[MAX + 1], link[MAX + 1], group[MAX], shared[MAX], gfirst[MAX + 1], gmost[MAX], most[MAX], before[2 * MAX], warp[3][32];
+};
+template <int MAX>
+__device__ __forceinline__ void sh_plan(ShPlan<MAX>& sh, const int* row_seq, const int* ctx_len, const int* common, int rows, int n_tables, int width, int G, int n_kv,
+                                        int* plan, int* status, bool all, int cta, int cta_step) {
+  int *s_seq = sh.seq, *s_first = sh.first, *s_link = sh.link, *s_group = sh.group, *s_shared = sh.shared, *s_gfirst = sh.gfirst, *s_gmost = sh.gmost, *s_most = sh.most,
+      *s_before = sh.before, (*s_warp)[32] = sh.warp;
   const int r = threadIdx.x, rt = SH_PAIRS / G;
   const bool live = r < rows;
   int seq = live ? row_seq[r] : -1, ctx = live ? ctx_len[r] : 0;
   const int link = live ? min(max(common[r], 0), width) : 0;
   if (live && (seq < 0 || seq >= n_tables || ctx < 0 || ctx > (long long)width * SH_PAGE)) {
-    set_status(status, ST_BAD_ARG, 95, r);
+    if (all) set_status(status, ST_BAD_ARG, 95, r);
     ctx = 0;                                               // a row that sees nothing; without a table row it is a run of its own that nobody is linked to
     if (seq < 0 || seq >= n_tables) seq = -1 - r;
   }
@@ -188,12 +193,14 @@ __global__ void __launch_bounds__(SH_MAX_ROWS) shared_plan_kernel(const int* __r
   __syncthreads();
   if (live) {
     const int c_s = sh_copies(n_s * G), c_o = sh_copies(n_o * G);
-    int4* of = reinterpret_cast<int4*>(plan + SH_AT_ROWS) + 2 * r;
-    of[0] = shared > 0 ? make_int4(s_link[tile], shared, s_first[tile] + (r - tile) * sh_slots(shared, L) * c_s, c_s) : make_int4(0, 0, 0, 0);
-    of[1] = own > 0 ? make_int4(s_seq[chunk], own, s_gfirst[chunk] + (r - chunk) * sh_slots(own, L) * c_o, c_o) : make_int4(0, 0, 0, 0);
+    if (all) {
+      int4* of = reinterpret_cast<int4*>(plan + SH_AT_ROWS) + 2 * r;
+      of[0] = shared > 0 ? make_int4(s_link[tile], shared, s_first[tile] + (r - tile) * sh_slots(shared, L) * c_s, c_s) : make_int4(0, 0, 0, 0);
+      of[1] = own > 0 ? make_int4(s_seq[chunk], own, s_gfirst[chunk] + (r - chunk) * sh_slots(own, L) * c_o, c_o) : make_int4(0, 0, 0, 0);
+    }
     plan[SH_AT_KEYS + r] = ctx;
   }
-  for (int c = r; c < SH_CTAS; c += blockDim.x) {
+  for (int c = cta; c < SH_CTAS; c += cta_step) {
     int lo = 0, hi = nb - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
@@ -202,6 +209,22 @@ __global__ void __launch_bounds__(SH_MAX_ROWS) shared_plan_kernel(const int* __r
     plan[SH_HEAD + c] = lo;
   }
   if (r == 0) plan[0] = total, plan[1] = L, plan[2] = nb, plan[3] = n_kv, plan[4] = n_kv * G, plan[5] = rows, plan[6] = n_tables, plan[7] = width;
+}
+__global__ void __launch_bounds__(SH_MAX_ROWS) shared_plan_kernel(const int* __restrict__ row_seq, const int* __restrict__ ctx_len, const int* __restrict__ common,
+                                                                  int rows, int n_tables, int width, int G, int n_kv, int* __restrict__ plan, int* status) {
+  pdl_launch();
+  __shared__ ShPlan<SH_MAX_ROWS> sh;
+  pdl_wait();
+  sh_plan(sh, row_seq, ctx_len, common, rows, n_tables, width, G, n_kv, plan, status, true, threadIdx.x, blockDim.x);
+}
+// The plan of a window of few rows, by each CTA of the attention for itself: all write the same words to the same places, and read what they have written.  (What only
+// the merge reads is written by one.)
+__device__ __noinline__ void sh_plan_here(void* smem, const int* row_seq, const int* ctx_len, const int* common, int rows, int n_tables, int width, int G, int n_kv, int* plan,
+                                          int* status) {
+  sh_plan(*reinterpret_cast<ShPlan<SH_FUSED_ROWS>*>(smem), row_seq, ctx_len, common, rows, n_tables, width, G, n_kv, plan, status, blockIdx.x == 0,
+          threadIdx.x == 0 ? (int)blockIdx.x : SH_CTAS, SH_CTAS);
+  fence_proxy_async();                                     // (the copies' places were the plan's)
+  __syncthreads();
 }
 
 // ------------------------------------------------------------------------------------------------ attention
@@ -259,6 +282,8 @@ __device__ __forceinline__ bool sh_wait(uint64_t* bar, uint32_t parity, volatile
 }
 
 struct ShArgs {
+  const int *row_seq, *ctx_len, *common;      // of a window that the kernel plans, to `planned`; else nullptr
+  int* planned;
   const int* block_table;
   const int* plan;
   const float* kv_scale;
@@ -463,6 +488,8 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
   pdl_wait();                                             // the plan, q and the caches were written by the previous kernels
   const uint32_t tmem_base = *tmem_slot;
   const int G = a.n_q / a.n_kv;
+  if (a.row_seq != nullptr)
+    sh_plan_here(smem, a.row_seq, a.ctx_len, a.common, a.rows, a.n_tables, a.max_blocks, G, a.n_kv, a.planned, a.status);
 
   if (warp < 4) {
     // ---------------------------------------------------------------- softmax warps: thread = (row, head) pair or a copy of it = TMEM lane
@@ -1064,7 +1091,12 @@ RX_API int rx_attn_shared(const void* tmap_k, const void* tmap_v, const void* q,
   a.block_table = (const int*)block_table; a.plan = plan != nullptr ? (const int*)plan : own_plan;
   a.kv_scale = (const float*)kv_scale; a.status = status; a.max_blocks = max_blocks; a.n_q = n_q; a.n_kv = n_kv; a.rows = rows;
   a.n_tables = n_tables; a.scale_log2 = scale * 1.4426950408889634f;
-  if (plan == nullptr) {
+  // Up to 64 rows are planned by every CTA of the attention for itself, which saves a launch (2.7 us of the host's 17.3 for a call) and the step from one kernel to the
+  // next (64 rows behind 8192 common keys 45.1 -> 44.3 us, 57 drawn windows 18.3 -> 18.0 us); with more, the words that 296 CTAs write cost more (80 rows 26.0 against
+  // 27.0 us, 182 rows 31 against 35 us).
+  const bool here = plan == nullptr && rows <= SH_FUSED_ROWS;
+  a.row_seq = here ? (const int*)row_seq : nullptr; a.ctx_len = (const int*)ctx_len; a.common = (const int*)common; a.planned = own_plan;
+  if (plan == nullptr && !here) {
     const int r = rx_attn_shared_plan(row_seq, ctx_len, common, rows, n_tables, max_blocks, n_q, n_kv, own_plan, status, stream);
     if (r != 0) return r;
   }

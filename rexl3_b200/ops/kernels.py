@@ -708,7 +708,7 @@ def attn_shared(tk: KvTensorMap, tv: KvTensorMap, q, block_table, row_seq, ctx_l
         raise ValueError("q, scratch and plan begin on 16-byte boundaries, out and xr on 8-byte ones")
     _lib.check(_lib.load().rx_attn_shared(tk.rows_ptr, tv.rows_ptr, p_q, p[0], tables, pages, p[1], p[2], p[3], p_scratch, rows, n_q, n_kv, hd, scale, p_scale, p_suh, p_xr, p_out,
                                           p_plan, p[4], _lib.stream_ptr()), "rx_attn_shared")
-    _lib.count(2 if plan is not None else 3)
+    _lib.count(2 if plan is not None or rows <= 64 else 3)
 
 
 def kv_move_rows(tensor_ptrs, row_bytes: int, n_kv: int, moves, n_moves: int) -> None:
