@@ -136,6 +136,8 @@ struct PickArgs {
   const int* first;                   // [rows] or nullptr: first row of the row's window
   const int* fed;                     // [rows]: token fed at the row
   uint64_t* cand;
+  int* ids;                           // of a vocabulary of one chunk of 4096: the results, without a second kernel; else nullptr
+  float* vals;
   long long ld;
   int rows, vocab, n_slots, n_bias, n_masks, words, count, nchunks;
 };
@@ -249,6 +251,30 @@ __device__ __forceinline__ float pick_max(float a, float b) {
   return m;
 }
 
+// A row's results, from its best keys (in order, 0 behind the last); taken[4] is 0
+__device__ __forceinline__ void pick_finish(const uint64_t* outk, uint32_t* taken, int row, int count, int* ids, float* vals) {
+  if ((int)threadIdx.x < count && outk[threadIdx.x] != 0) {
+    const uint32_t own = ~(uint32_t)outk[threadIdx.x];
+    if (own < 128) atomicOr(&taken[own >> 5], 1u << (own & 31));
+  }
+  __syncthreads();
+  if ((int)threadIdx.x >= count) return;
+  int id;
+  float v = -INFINITY;
+  if (outk[threadIdx.x] != 0) {
+    id = (int)(~(uint32_t)outk[threadIdx.x]);
+    v = pick_value((uint32_t)(outk[threadIdx.x] >> 32));
+  } else {
+    // Fewer ids above -inf than places: the lowest of the other ids, which all stand at -inf, in order.  With at most 64 ids to leave out they are below 128.
+    int q = threadIdx.x, w = 0;
+    for (int r = 0; r < count; ++r) q -= outk[r] != 0;
+    while (q >= __popc(~taken[w])) q -= __popc(~taken[w]), ++w;
+    id = w * 32 + __fns(~taken[w], 0, q + 1);
+  }
+  ids[(size_t)row * count + threadIdx.x] = id;
+  vals[(size_t)row * count + threadIdx.x] = v;
+}
+
 // A CTA takes 256 PER ids of a row, a thread PER of them: VEC: four ids side by side at a time (16-byte loads of logits, 8-byte loads of counts); else one.  Their
 // values stand in shared memory, where the few ids that a rule touches are worked out again by themselves.  What is done for every id is a load, a test of its
 // count, a store, a load and a maximum, and its order is worked out only behind the threshold.  (With the rules and orders of all ids in registers, a division
@@ -263,7 +289,11 @@ __global__ void __launch_bounds__(PICK_THREADS, PICK_CTAS) pick_stage1_kernel(co
   constexpr int W = VEC ? 4 : 1, N = PER / W, CHUNK = PICK_THREADS * PER;
   __shared__ PickShared sm;
   __shared__ __align__(16) float s_val[CHUNK];
+  constexpr bool FINAL = PER == 16;                        // (the results' code in the other cost rows of many chunks 5 to 10 %)
+  __shared__ uint64_t s_out[FINAL ? 64 : 1];
+  __shared__ uint32_t s_taken[4];
   if (threadIdx.x == 0) sm.n = 0;
+  if (FINAL && threadIdx.x < 4) s_taken[threadIdx.x] = 0;
   pdl_wait();
   __syncthreads();
   const int row = blockIdx.y, tid = threadIdx.x, base = blockIdx.x * CHUNK, ids_here = min(a.vocab - base, CHUNK);
@@ -426,7 +456,11 @@ __global__ void __launch_bounds__(PICK_THREADS, PICK_CTAS) pick_stage1_kernel(co
                   if (v != -INFINITY && order >= least) f(pick_key(order, base + at));
                 }
               },
-              a.count, a.cand + (size_t)row * a.nchunks * a.count + blockIdx.x, a.nchunks, sm);
+              a.count, FINAL && a.ids != nullptr ? s_out : a.cand + (size_t)row * a.nchunks * a.count + blockIdx.x, a.nchunks, sm);
+  if (FINAL && a.ids != nullptr) {
+    __syncthreads();
+    pick_finish(s_out, s_taken, row, a.count, a.ids, a.vals);
+  }
 }
 
 // total <= PICK_THREADS * 16 candidates a row, the chunks' best first, then their second best and so on: the best of all are then those of different threads.  (Chunk
@@ -457,26 +491,7 @@ __global__ void __launch_bounds__(PICK_THREADS) pick_stage2_kernel(const uint64_
               },
               count, outk, 1, sm);
   __syncthreads();
-  if ((int)threadIdx.x < count && outk[threadIdx.x] != 0) {
-    const uint32_t own = ~(uint32_t)outk[threadIdx.x];
-    if (own < 128) atomicOr(&taken[own >> 5], 1u << (own & 31));
-  }
-  __syncthreads();
-  if ((int)threadIdx.x >= count) return;
-  int id;
-  float v = -INFINITY;
-  if (outk[threadIdx.x] != 0) {
-    id = (int)(~(uint32_t)outk[threadIdx.x]);
-    v = pick_value((uint32_t)(outk[threadIdx.x] >> 32));
-  } else {
-    // Fewer ids above -inf than places: the lowest of the other ids, which all stand at -inf, in order.  With at most 64 ids to leave out they are below 128.
-    int q = threadIdx.x, w = 0;
-    for (int r = 0; r < count; ++r) q -= outk[r] != 0;
-    while (q >= __popc(~taken[w])) q -= __popc(~taken[w]), ++w;
-    id = w * 32 + __fns(~taken[w], 0, q + 1);
-  }
-  ids[(size_t)row * count + threadIdx.x] = id;
-  vals[(size_t)row * count + threadIdx.x] = v;
+  pick_finish(outk, taken, row, count, ids, vals);
 }
 
 }  // namespace rx
@@ -522,13 +537,13 @@ RX_API int rx_topk_adjusted(const void* logits, long long ld, int rows, int voca
       (first != nullptr && rows > PICK_MAX_WINDOW))
     return (int)cudaErrorInvalidValue;
   PickArgs a = {(const float*)logits, (const int*)row_slot, (const uint16_t*)counts, (const float*)penalties, (const int*)bias_id, (const float*)bias_val,
-                (const uint32_t*)mask, (const int*)mask_row, (const int*)first, (const int*)fed, (uint64_t*)scratch, ld, rows, vocab, n_slots, n_bias, n_masks,
+                (const uint32_t*)mask, (const int*)mask_row, (const int*)first, (const int*)fed, (uint64_t*)scratch, small && nchunks == 1 ? (int*)ids : nullptr, (float*)vals, ld, rows, vocab, n_slots, n_bias, n_masks,
                 (vocab + 31) / 32, count, nchunks};
   // four ids at a time where every row of logits and counts begins on a 16- and an 8-byte boundary
   const bool vec = vocab % 4 == 0 && ld % 4 == 0 && ((uintptr_t)logits & 15) == 0 && ((uintptr_t)counts & 7) == 0;
   cudaStream_t st = (cudaStream_t)stream;
   const auto stage1 = small ? (vec ? pick_stage1_kernel<true, 16> : pick_stage1_kernel<false, 16>) : vec ? pick_stage1_kernel<true, 32> : pick_stage1_kernel<false, 32>;
   cudaError_t e = rx::launch(stage1, dim3(nchunks, rows), dim3(PICK_THREADS), 0, st, a);
-  if (e != cudaSuccess) return (int)e;
+  if (e != cudaSuccess || a.ids != nullptr) return (int)e;      // (2048 ids: 7.4 -> 5.5 us)
   return (int)rx::launch(pick_stage2_kernel, dim3(rows), dim3(PICK_THREADS), 0, st, (const uint64_t*)scratch, nchunks * count, count, (int*)ids, (float*)vals);
 }

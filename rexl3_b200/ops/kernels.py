@@ -509,7 +509,7 @@ def topk_adjusted(logits: torch.Tensor, count: int, scratch: torch.Tensor, ids: 
         p_first, p_fed = _vector(window[0], "window first", _I32, rows, dev), _vector(window[1], "window fed", _I32, rows, dev)
     _lib.check(_lib.load().rx_topk_adjusted(logits.data_ptr(), ld if rows > 1 else vocab, rows, vocab, count, p_scratch, p_ids, p_vals, p_slot, p_counts, p_pen, slots,
                                             p_bid, p_bval, nb, p_mask, p_mrow, nm, p_first, p_fed, _lib.stream_ptr()), "rx_topk_adjusted")
-    _lib.count(2)
+    _lib.count(1 if vocab <= 4096 and rows <= 740 else 2)
 
 
 def token_counts(counts: torch.Tensor, slots: torch.Tensor, starts: torch.Tensor, prompt_len: torch.Tensor, tokens: torch.Tensor, status: torch.Tensor) -> None:

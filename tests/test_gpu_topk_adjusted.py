@@ -159,6 +159,12 @@ def test_a_bias_given_more_than_once_adds_up_in_order():
     same(torch.randn(1, V, device="cuda"), 28, t([0]), bias=(torch.full((1, 1024), 5, dtype=torch.int32, device="cuda"), torch.randn(1, 1024, device="cuda")))
 
 
+@pytest.mark.parametrize("rows,V", [(740, 100), (741, 100), (741, 5000), (371, 8192), (150, 20000)])
+def test_more_rows_than_run_at_once(rows, V):
+    kw = rules(rows, V, 9, rows + V, hist=50)
+    same(torch.randn(rows, V, device="cuda"), 5, kw.pop("row_slot"), **kw)
+
+
 @pytest.mark.parametrize("V,nb", [(2048, 200), (2048, 1024), (9000, 1024), (40, 1000)])
 def test_many_biases_and_drafts(V, nb):
     kw = rules(12, V, 2, V + nb, nb=nb)
