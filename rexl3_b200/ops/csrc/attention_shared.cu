@@ -24,8 +24,8 @@
 // stand among the 128 two or four times, each copy takes its part of a page's keys - the rest of its P is zero - and leaves its own partial output.
 // All waits are bounded (status words), no cluster multicast.
 //
-// Whole calls with 40 query and 8 KV heads of 128, plan and merge included (4 and 4 to 5 us):
-//     64 rows behind 8192 common keys, 60 .. 700 keys of their own: 45 us.  134 MB, 20.6 us at the rate of a copy.  Three blocks read each common page, so L2 gives 200 MB:
+// Whole calls with 40 query and 8 KV heads of 128, plan and merge included (3 to 4 and 4 to 5 us):
+//     64 rows behind 8192 common keys, 60 .. 700 keys of their own: 44 us.  134 MB, 20.6 us at the rate of a copy.  Three blocks read each common page, so L2 gives 200 MB:
 //         a page comes 3100 cycles after it is asked for and five are on their way to each CTA, 37 bytes a clock and SM or 9.7 TB/s of them all; the rest is the first
 //         pages' way, the last CTAs' and the merge.
 //     48 rows of 500 .. 4000 keys behind 150 common ones: 85 us.  448 MB, 68.6 us: bound by memory, 5.2 TB/s.
