@@ -782,7 +782,8 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
       if constexpr (F8) {                                 // the expanding warps learn that there are no more
         if (lane == 0) *pages_all = copied;
         __syncwarp(3);
-        mbar_arrive(&full[st]);
+        // (The place must be free, as for a copy: else the barrier could go on by two phases while a warp still waits for the first, of the page before last.)
+        if (round == 0 || sh_wait(&empty[st], (round - 1) & 1, abort_flag, a.status, 111)) mbar_arrive(&full[st]);
       }
     }
     if (lane == 0) {
