@@ -627,8 +627,8 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
       if (!some) {
         for (int j = 0; j < d.pages && ok; ++j, ++n) {
           ok = all_ok(sh_wait(&s_full[n & 1], (n >> 1) & 1, abort_flag, a.status, 102)) && tail(j);
+          __syncwarp();                                   // (the tail's zeros are all lanes')
           if (ok && lane == 0) mbar_arrive(&p_ready[n & 1]);
-          __syncwarp();
         }
       } else {
         // 64 / copies = NC * parts
