@@ -133,7 +133,7 @@ struct PickArgs {
   const float* bias_val;
   const uint32_t* mask;               // [n_masks][words] or nullptr; bit i of word w = id 32 w + i may be taken
   const int* mask_row;                // [rows]; a value that is no mask: every id may
-  const int* first;                   // [rows] or nullptr: first row of the row's window
+  const int* first;                   // [rows] or nullptr: first row of the row's window (below 0: 0; behind the row: the row)
   const int* fed;                     // [rows]: token fed at the row
   uint64_t* cand;
   int* ids;                           // of a vocabulary of one chunk of 4096: the results, without a second kernel; else nullptr
@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(PICK_THREADS, PICK_CTAS) pick_stage1_kernel(co
     if (v != -INFINITY) s_val[at] = pick_rules(v, word, 0, rep, freq, pres);                       // at -inf it stays, and a masked id is there
     if (k != i && u != -INFINITY) s_val[to] = pick_rules(u, other, 0, rep, freq, pres);
   }
-  const int r0 = max(window, 0) + 1;
+  const int r0 = min(max(window, 0), row) + 1;             // the row's drafts: rows r0 .. row
   // Ids of the chunk with a bias or among the drafts are listed, with their places among the slot's biases (drafts: behind those).
   auto take = [&](int id, uint32_t place) {
     if (id < base || id - base >= ids_here) return;

@@ -457,7 +457,7 @@ def topk_adjusted(logits: torch.Tensor, count: int, scratch: torch.Tensor, ids: 
     counts (int16 [slots, vocab], see `token_counts`) with penalties (f32 [slots, 3]: repetition > 0, frequency, presence): an id that the prompt holds or
     that was generated is divided by repetition (multiplied where it is <= 0); then frequency * (times generated) and, where that is not 0, presence go off.
     window = (first, fed), int32 [rows] each: rows first[r] .. r feed the tokens fed of a verify window; those after first[r] count as generated for row r
-    (up to 4096 rows).
+    (up to 4096 rows; a first[r] below 0 is taken as 0, one behind r as r: no drafts).
     bias = (ids int32 [slots, n], values f32 [slots, n]), n up to 1024: added; an id outside the vocabulary (-1) is an unused place, equal ids add up in order.
     mask = (bits int32 [n, ceil(vocab / 32)], row int32 [rows]): row r may take the ids whose bit of bits[row[r]] is set (id i: bit i % 32 of word i // 32), every
     id where row[r] is outside 0 .. n - 1.  What is masked stands at -inf, whatever its logit.  Where a row has fewer than count ids above -inf, the rest are
