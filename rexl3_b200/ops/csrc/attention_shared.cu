@@ -210,8 +210,8 @@ __device__ __forceinline__ void sh_plan(ShPlan<MAX>& sh, const int* row_seq, con
   }
   if (r == 0) plan[0] = total, plan[1] = L, plan[2] = nb, plan[3] = n_kv, plan[4] = n_kv * G, plan[5] = rows, plan[6] = n_tables, plan[7] = width;
 }
-__global__ void __launch_bounds__(SH_MAX_ROWS) shared_plan_kernel(const int* __restrict__ row_seq, const int* __restrict__ ctx_len, const int* __restrict__ common,
-                                                                  int rows, int n_tables, int width, int G, int n_kv, int* __restrict__ plan, int* status) {
+__global__ void __launch_bounds__(SH_MAX_ROWS) shared_plan_kernel(const int* row_seq, const int* ctx_len, const int* common, int rows, int n_tables, int width,
+                                                                  int G, int n_kv, int* plan, int* status) {
   pdl_launch();
   __shared__ ShPlan<SH_MAX_ROWS> sh;
   pdl_wait();

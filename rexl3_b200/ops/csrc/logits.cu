@@ -22,9 +22,8 @@ constexpr unsigned CNT_PROMPT = 0x80000000u;
 // clearing pass, no atomics on global memory, one launch; what it costs is that a history is read once per slice, from L2 but for the first time.  The words are
 // counted as they are stored, two in a 32-bit word of shared memory: with at most 32767 generated tokens no count can stop or carry.  A longer history takes
 // the slice in two halves of 32-bit counters.
-__global__ void __launch_bounds__(CNT_THREADS) token_counts_kernel(uint16_t* __restrict__ counts, const int* __restrict__ slots, const int* __restrict__ starts,
-                                                                   const int* __restrict__ prompt, const int* __restrict__ tokens, int n_tokens, int n_slots,
-                                                                   int vocab, int slice, int* status) {
+__global__ void __launch_bounds__(CNT_THREADS) token_counts_kernel(uint16_t* counts, const int* slots, const int* starts, const int* prompt,
+                                                                   const int* tokens, int n_tokens, int n_slots, int vocab, int slice, int* status) {
   pdl_launch();
   extern __shared__ __align__(16) uint32_t cnt[];
   const int req = blockIdx.y, tid = threadIdx.x;
@@ -100,8 +99,8 @@ __global__ void __launch_bounds__(CNT_THREADS) token_counts_kernel(uint16_t* __r
 }
 
 // counts[slots[i], tokens[i]] += 1 (or the prompt bit).  Compare-and-swap on the 16-bit word: the count stops at 32767, and the order does not matter.
-__global__ void __launch_bounds__(256) token_counts_add_kernel(uint16_t* counts, const int* __restrict__ slots, const int* __restrict__ tokens, int n, int n_slots,
-                                                               int vocab, int in_prompt, int* status) {
+__global__ void __launch_bounds__(256) token_counts_add_kernel(uint16_t* counts, const int* slots, const int* tokens, int n, int n_slots, int vocab,
+                                                               int in_prompt, int* status) {
   pdl_launch();
   pdl_wait();
   const int i = blockIdx.x * 256 + threadIdx.x;
