@@ -15,8 +15,8 @@
 //
 // A page's 64 scores a pair go to tensor memory, come back as exponentials in 16 bits over the same columns, and are the A operand of the product with V.
 // The QKs run two pages ahead of the PVs, also into the next segment.  Scores, maxima, sums and outputs are fp32; the probabilities are rounded to the type that V
-// has as an operand (both operands of an MMA have one), and their sum is that of the unrounded ones: each stands for itself within 2^-9 (bf16) or 2^-12 (fp16),
-// no more than the rounding of the outputs.
+// has as an operand (both operands of an MMA have one), and their sum is that of the unrounded ones: each stands for itself within 2^-8 (bf16) or 2^-11 (fp16; in
+// the range where that is exact to 11 bits, else within 2^-32 of the row's largest: see UP), no more than the rounding of the outputs.
 //
 // Warps: 0..3 = softmax, 4 = feeder (descriptions of the segments; TMA), 5 = MMA issuer (owns the tensor memory), for E4M3 caches 6, 7 and 8, 9 = expansion of
 // byte pages of K and of V to fp16 operand tiles.
@@ -303,6 +303,9 @@ struct Sh {
   static constexpr int SMEM = (KS + VS) * TILE + 2 * RS * RAW + HD / 64 * QBOX + 1024;    // two CTAs an SM: 115,712 bytes at most
   static_assert(SMEM <= 115712, "two CTAs an SM");
   static constexpr int THREADS = 32 * (F8 ? 10 : 6);
+  // fp16 has no values below 2^-24 and few below 2^-14: its operands are the probabilities times 2^7 (at most 2^15), so that what is lost of a key is at most 2^-32 of the
+  // row's largest.  (As they are, 2^-25: 30,000 keys of that size, in the row's sum but not in its outputs, were a thousandth of it.)
+  static constexpr float UP = F8 ? 7.f : 0.f;
   static constexpr int S_COLS = 64, O = 128, COLS = 256;                    // tensor memory: two buffers of S (P over the first 32 columns of one) | O
 };
 
@@ -538,7 +541,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
 #pragma unroll
           for (int i = 0; i < NC; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[i]));
           const float ms = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2;
-          // The running maximum moves only by more than 2^8: the probabilities stay below 2^8, harmless in 16-bit operands and fp32 sums.  (A move in a page's second
+          // The running maximum moves only by more than 2^8: the probabilities stay below 2^8 (2^15 with UP), harmless in 16-bit operands and fp32 sums.  (A move in a page's second
           // part comes before the first part's product: those probabilities would be of the old maximum.  So they move with O.)
           const bool moves = live && ms > m + 8.f;        // (a lane without a pair has another's old queries, or none: its scores may be anything)
           if (__any_sync(0xffffffffu, moves)) {           // all pages but a segment's first few: no
@@ -575,7 +578,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
               }
             }
           }
-          const float m_use = (m == -INFINITY) ? 0.f : m;
+          const float m_use = (m == -INFINITY) ? 0.f : m - Sh<HD, F8>::UP;      // (sum and outputs are 2^UP times as large alike: nothing is to be undone)
           float lsum[4] = {0.f, 0.f, 0.f, 0.f};
           uint32_t pk[NC / 2];
 #pragma unroll
