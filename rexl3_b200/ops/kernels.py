@@ -5,7 +5,6 @@ from __future__ import annotations
 from dataclasses import dataclass
 
 import functools
-import math
 
 import numpy as np
 import torch
@@ -687,8 +686,8 @@ def attn_shared(tk: KvTensorMap, tv: KvTensorMap, q, block_table, row_seq, ctx_l
     rows, tables, pages, dev, p = _shared_window(block_table, row_seq, ctx_len, common, status, n_q, n_kv)
     if hd not in (64, 128) or n_q * hd % 128:
         raise ValueError(f"heads of {hd}: 64 or 128, and n_q * hd a multiple of 128")
-    if not 0 < scale < math.inf:
-        raise ValueError(f"scale {scale}: a positive number is needed")
+    if not 2.0 ** -126 <= scale <= 2.0 ** 126:             # (float32, times log2(e): 0 or infinity would make NaN of what is masked)
+        raise ValueError(f"scale {scale}: a positive number is needed, 2^-126 .. 2^126")
     held = (n_kv, hd, dev, _BF16 if kv_scale is None else torch.uint8)
     if tk.held != held or tv.held != held:
         raise ValueError(f"cache: bf16, or E4M3 bytes with kv_scale, [pages, {n_kv}, 64, {hd}] on cuda:{dev} is needed")
