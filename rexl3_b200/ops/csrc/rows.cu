@@ -8,7 +8,8 @@
 // what `attn_shared` groups rows by.
 //
 // All or nothing: every CTA checks all requests (a few KB) and works out their sums for itself, and a request that cannot be served leaves every
-// output as it was.  Bound by latency (a chain of the loads of lengths, two scans of up to 1024 values, a table entry, a store), not by the 20 bytes a row
+// output as it was.  (But a row whose table entry is no page - below 0, or of 2^25 and more, whose slots int32 cannot hold - gets slot -1, and the others are written.)
+// Bound by latency (a chain of the loads of lengths, two scans of up to 1024 values, a table entry, a store), not by the 20 bytes a row
 // that it writes: 64 requests of a row each 4.1 us, 23 prompts of 8000 rows together 4.9 us.  One launch: with `free_next` in the place of
 // `free_at` a CTA would overwrite what another has yet to read, so the CTAs are one cluster that meets between the reading and the writing.  (One CTA instead
 // of the eight: eight requests of up to five rows 3.3 against 3.1 us, 40 of them 4.9 against 4.0 us, 256 13.5 against 4.7 us.)
@@ -106,7 +107,8 @@ __global__ void __launch_bounds__(ROWS_THREADS) window_rows_kernel(const RowsArg
   for (int r = gtid; r < rows_all; r += all) {
     const int i = rows_owner(s_row, n, r);
     const int seq = s_seq[i], have = s_have[i], pos = have + (r - s_row[i]), b = pos / ROWS_PAGE, held = (have + ROWS_PAGE - 1) / ROWS_PAGE;
-    const int id = a.free_at != nullptr && b >= held ? a.free_ids[at0 + s_page[i] + (b - held)] : a.table[(size_t)seq * a.width + b];
+    const int entry = a.free_at != nullptr && b >= held ? a.free_ids[at0 + s_page[i] + (b - held)] : a.table[(size_t)seq * a.width + b];
+    const int id = entry <= 0x7FFFFFFF / ROWS_PAGE ? entry : -1;      // (a slot past int32)
     if (id < 0) set_status(a.status, ST_BAD_ARG, 91, r);
     a.rows[r] = pos;
     a.rows[(size_t)a.cap + r] = id < 0 ? -1 : id * ROWS_PAGE + pos % ROWS_PAGE;

@@ -549,7 +549,8 @@ def window_rows(seq: torch.Tensor, have: torch.Tensor, new: torch.Tensor, block_
     free (int32 [m]) with free_at, free_next (int32 [1] each): page ids free[free_at:], in request order, become the table entries of the pages that
     the new tokens begin, and free_next = free_at + their number (it may be the same tensor as free_at).  Without them the table holds those pages already.
     All or nothing: a length below 0, tokens beyond the table, more rows than cap, more pages than there are, a table row outside the table or
-    given twice sets the status and changes nothing else.  A table entry below 0 where a row is to be written gives slot -1 (the row is not cached) and sets the status."""
+    given twice sets the status and changes nothing else.  A table entry below 0, or of 2^25 and more (its slots are past int32), where a row is to be written gives slot -1
+    (the row is not cached) and sets the status."""
     dev, n = _here(block_table, "block_table"), _length(seq, "seq")
     p_table, tables, width = _table(block_table, "block_table", _I32, dev)
     p_rows, five, cap = _table(rows, "rows", _I32, dev)
