@@ -687,6 +687,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
     uint64_t *full = F8 ? raw_full + who * C::RS : who ? v_full : k_full, *empty = F8 ? raw_empty + who * C::RS : who ? v_empty : k_empty;
     uint8_t* to = F8 ? raw + who * C::RS * C::RAW : who ? v_sm : k_sm;
     const CUtensorMap* map = who ? &tv : &tk;
+    const unsigned pages_end = (1u << 31) / SH_PAGE / a.n_kv;      // page ids whose rows int32 can count
     const int* table = nullptr;                            // of the lane's segment, behind the page that comes next: that one is known before its place is free
     int at = 0, next = 0, begun = 0, st = 0, round = 0, left = 0, kvh = 0, copied = 0;      // segments looked at, and begun; the ring's place; pages left of the segment, asked for
     bool done = lane > 1;
@@ -722,7 +723,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
           ++at;
         }
         if (left != 0 && (round == 0 || mbar_test_wait(&empty[st], (round - 1) & 1))) {
-          const int y = (next * a.n_kv + kvh) * SH_PAGE;
+          const int y = (unsigned)next < pages_end ? (next * a.n_kv + kvh) * SH_PAGE : -SH_PAGE;      // (outside the cache: zeros)
           mbar_arrive_expect_tx(&full[st], C::COPY);
 #pragma unroll
           for (int x = 0; x < (F8 ? 1 : BOXES); ++x) tma_load_2d(to + st * C::COPY + x * 8192, map, x * 64, y, &full[st]);
