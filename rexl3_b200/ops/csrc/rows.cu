@@ -148,8 +148,6 @@ __global__ void __launch_bounds__(ROWS_THREADS) window_rows_kernel(const RowsArg
 
 using namespace rx;
 
-RX_API int rx_window_rows_max() { return ROWS_MAX_REQ; }
-
 // rows: int32 [5][cap].  free_at == nullptr: every page is in the table already.
 RX_API int rx_window_rows(const void* seq, const void* have, const void* fed, int n, void* table, int n_tables, int width, const void* free_ids, int n_free,
                           const void* free_at, void* free_next, void* rows, int cap, void* starts, int* status, void* stream) {

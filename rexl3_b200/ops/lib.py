@@ -139,7 +139,6 @@ def _declare(lib):
                                      c_void, c_int, c_void, c_void, c_void]),
         "rx_token_counts": (c_int, [c_void, c_int, c_int, c_void, c_void, c_void, c_void, c_int, c_int, c_void, c_void]),
         "rx_token_counts_add": (c_int, [c_void, c_int, c_int, c_void, c_void, c_int, c_int, c_void, c_void]),
-        "rx_window_rows_max": (c_int, []),
         "rx_window_rows": (c_int, [c_void, c_void, c_void, c_int, c_void, c_int, c_int, c_void, c_int, c_void, c_void, c_void, c_int, c_void, c_void, c_void]),
         "rx_attn_shared_plan_ints": (c_int, []),
         "rx_attn_shared_scratch_floats": (c_ll, [c_int, c_int, c_int, c_int]),
