@@ -24,12 +24,13 @@
 // stand among the 128 two or four times, each copy takes its part of a page's keys - the rest of its P is zero - and leaves its own partial output.
 // All waits are bounded (status words), no cluster multicast.
 //
-// Whole calls with 40 query and 8 KV heads of 128, plan and merge included (3 to 4 and 4 to 5 us):
+// Whole calls with 40 query and 8 KV heads of 128, one after the other over the same cache, the plan (inside the kernel for up to 64 rows: 1.5 to 3 us) and the merge
+// (4 to 5 us) included:
 //     64 rows behind 8192 common keys, 60 .. 700 keys of their own: 44 us.  134 MB, 20.6 us at the rate of a copy.  Three blocks read each common page, so L2 gives 200 MB:
 //         a page comes 3100 cycles after it is asked for and five are on their way to each CTA, 37 bytes a clock and SM or 9.7 TB/s of them all; the rest is the first
 //         pages' way, the last CTAs' and the merge.
-//     48 rows of 500 .. 4000 keys behind 150 common ones: 85 us.  448 MB, 68.6 us: bound by memory, 5.2 TB/s.
-//     32 rows behind 32,700 common keys, E4M3: 65 us.  104 MB, 16 us: bound by instructions, the expansion's beside the softmax's (bf16: 208 MB, 61 us).
+//     48 rows of 500 .. 4000 keys behind 150 common ones: 84 us.  448 MB, 68.6 us: bound by memory, 5.3 TB/s.
+//     32 rows behind 32,700 common keys, E4M3: 65 us.  104 MB, 16 us: bound by instructions, the expansion's beside the softmax's (bf16: 208 MB, 60 us).
 #include <cuda.h>
 #include <cuda_fp8.h>
 #include <type_traits>
@@ -41,12 +42,14 @@ constexpr int SH_PAGE = 64, SH_PAIRS = 128, SH_CTAS = 296, SH_MAX_ROWS = 1024, S
 // Pages that a group must have in common.  (64 rows of 40 heads and 100 .. 700 keys: of one common page nothing comes either way, 3 pages 37.1 against 38.5 us where
 // each sequence reads them for itself, 6 pages 37.4 against 40.6; 256 rows of 8 heads and up to 60 keys behind 3 pages 23.5 against 27 us.)
 constexpr int SH_MIN_SHARED = 1;
-// What a unit costs beside its pages, in pages: its place in the line is that much longer.  (One, two, three, four: 64 rows behind 8192 common keys 47, 45, 46, 48 us;
-// 16 sequences of five rows behind 4001 28, 26, 25, 25; 48 E4M3 rows of 500 .. 4000 keys 98, 78, 76, 76.  Pages weighted by the copies of their block's pairs, 8 : 7 : 6,
-// changed as much for the worse as for the better.)
+// What a unit costs beside its pages, in pages: its place in the line is that much longer.  (One, two, three, four: 64 rows behind 8192 common keys 46.6, 44.2, 45.3,
+// 47.5 us; 16 sequences of five rows behind 4001 28.7, 26.1, 25.6, 25.6; 32 E4M3 rows behind 32,700 69.4, 65.3, 65.7, 65.9; 48 rows of 500 .. 4000 keys 86.6, 84.4, 84.2, 85.1,
+// of E4M3 112, 92, 81, 75: two is best for long common prompts, and E4M3 rows that share nothing would take more.  Pages weighted by the copies of their block's pairs,
+// 8 : 7 : 6, changed as much for the worse as for the better.)
 constexpr int SH_SEGMENT = 2;
 // A CTA's piece has no least length: one of two or four pages leaves fewer partial outputs, but on 57 drawn windows of all sizes it gained nothing, or lost 7 %.
-// Few warps of the merge would join many partial outputs one after the other, so up to 148 blocks of 128 outputs go by 16 warps each where a row may have more than 64,
+// Few warps of the merge would join many partial outputs one after the other, so up to 148 blocks of 128 outputs go by 16 warps each where a row may have more than 64
+// (by the width of the table, the only bound that the host knows: a small window in a wide table takes 11.5 us by 16 warps, 10.4 in a narrow one by four),
 // up to 1480 by four, more by one: two rows of five heads behind 31,637 keys, 992 partial outputs each, 90 -> 26 us of the whole call; 32 rows of 40 heads behind 32,700
 // (1280 blocks of some 30) 70 -> 65 us; but 1728 blocks of few 24 -> 27 us by four, and four blocks of few 11.0 -> 12.7 us by 16.
 constexpr int SH_SPLIT16 = 148, SH_SPLIT16_OF = 64, SH_SPLIT4 = 1480;

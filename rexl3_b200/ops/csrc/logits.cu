@@ -277,8 +277,8 @@ __device__ __forceinline__ void pick_finish(const uint64_t* outk, uint32_t* take
 // A CTA takes 256 PER ids of a row, a thread PER of them: VEC: four ids side by side at a time (16-byte loads of logits, 8-byte loads of counts); else one.  Their
 // values stand in shared memory, where the few ids that a rule touches are worked out again by themselves.  What is done for every id is a load, a test of its
 // count, a store, a load and a maximum, and its order is worked out only behind the threshold.  (With the rules and orders of all ids in registers, a division
-// inlined for each, 64 rows of 151,936 ids took 36 us, both stages.)  Now 20.5 us, 59 MB or 9 us at the rate of a copy: bound by the chain of a CTA's phases -
-// slot and masks, ids, rules, biases, threshold, list - with barriers between.  80 rows of 32,003 ids and 64 candidates 13.5 us, one row of 151,936 ids 6.4 us: two
+// inlined for each, 64 rows of 151,936 ids took 36 us, both stages.)  Now 20.7 us, 59 MB or 9 us at the rate of a copy: bound by the chain of a CTA's phases -
+// slot and masks, ids, rules, biases, threshold, list - with barriers between.  80 rows of 32,003 ids and 64 candidates 13.7 us, one row of 151,936 ids 6.5 us: two
 // kernels of one CTA's latency each.
 // Masked ids cost neither their logit nor their count.  An id at -inf is no candidate: it is one only where a row has fewer than `count` ids above -inf, and the
 // second selection finds those by counting.
@@ -528,8 +528,8 @@ RX_API int rx_token_counts_add(void* counts, int n_slots, int vocab, const void*
 RX_API int rx_topk_adjusted(const void* logits, long long ld, int rows, int vocab, int count, void* scratch, void* ids, void* vals, const void* row_slot,
                             const void* counts, const void* penalties, int n_slots, const void* bias_id, const void* bias_val, int n_bias, const void* mask,
                             const void* mask_row, int n_masks, const void* first, const void* fed, void* stream) {
-  // Chunks of 4096 ids where all of them run at once: twice as many CTAs, each done sooner (with 8192: 80 rows of 32,003 ids 15.2 against 13.6 us, one row of 151,936
-  // ids 10.3 against 8.0 us).  Else of 8192: half as many selections (64 rows of 151,936 ids 25.0 against 22.4 us).
+  // Chunks of 4096 ids where all of them run at once: twice as many CTAs, each done sooner (with 8192: 80 rows of 32,003 ids 16.3 against 13.7 us, one row of 151,936
+  // ids 7.2 against 6.6 us).  Else of 8192: half as many selections (64 rows of 151,936 ids 24.0 against 20.7 us; 54 rows, one candidate each, 19 against 20 us, though).
   const bool small = (long long)rows * ((vocab + 4095) / 4096) <= 148 * PICK_CTAS;
   const int nchunks = small ? (vocab + 4095) / 4096 : (vocab + 8191) / 8192;
   if (rows < 1 || rows > 65535 || vocab < 1 || count < 1 || count > 64 || count > vocab || (long long)nchunks * count > PICK_THREADS * 16 || ld < vocab || n_bias < 0 || n_bias > PICK_MAX_BIAS ||

@@ -674,10 +674,11 @@ def attn_shared_plan(block_table, row_seq, ctx_len, common, n_q: int, n_kv: int,
 def attn_shared(tk: KvTensorMap, tv: KvTensorMap, q, block_table, row_seq, ctx_len, common, scratch, n_q: int, n_kv: int, hd: int, scale: float, out, status, *,
                 suh=None, xr=None, kv_scale=None, plan=None) -> None:
     """Decode / verify-window attention that reads the pages neighbouring sequences have in common once for all of them (`attn_decode` reads them once per
-    sequence).  q bf16 [rows, n_q * hd]; row r sees the first ctx_len[r] keys of table row row_seq[r] (0: its output is 0); the rows of a sequence are
+    sequence).  It is the faster one where many rows share long contexts, and for windows of many long rows altogether; for a few rows `attn_decode` is as fast or faster.
+    q bf16 [rows, n_q * hd]; row r sees the first ctx_len[r] keys of table row row_seq[r] (0: its output is 0); the rows of a sequence are
     adjacent.  common (int32 [rows], read at the first row of each sequence): how many leading page ids of its table row are also those of the sequence before
     it; sequences whose pages agree should stand side by side, and 0 is always right.  `window_rows` writes all three.
-    out bf16 [rows, n_q * hd] or None; with suh also xr fp16, `attn_decode`'s rotated output.  bf16 caches, or E4M3 ones with kv_scale (f32 [2, n_kv]); heads of
+    out bf16 [rows, n_q * hd] or None; with suh also xr fp16, `attn_decode`'s rotated output.  bf16 caches, or E4M3 ones with kv_scale (f32 [2, n_kv], above 0); heads of
     64 or 128; n_q * hd a multiple of 128.  A row's last bits depend on the rows beside it: the cut of the work follows the whole window.
     A table row or a context outside the table sets the status and stands for a context of 0.  What stands behind the last key that any row of a sequence or group
     sees may be anything; of an infinite or NaN value of V at a key before it, the rows that do not see that key may get NaN too.  With an E4M3 cache the queries
