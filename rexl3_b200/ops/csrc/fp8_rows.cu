@@ -1,0 +1,243 @@
+// Rows of E4M3 with a float32 scale for each block of 128 columns, for the products of fp8_block.cu (sm_100a).
+//
+//   add_norm     h += x (or + sum_t w_t x_t);  y = h * rsqrt(mean(h^2) + eps) * norm_w   (or y = h)
+//   swiglu       y = silu(g) * u
+//   both         s = max(max|y|, 2^-100) / 448 over a row's block,  q = e4m3(y / s):  q [rows][d] bytes, s [blocks][rows]
+//
+// All steps are float32; y is formed of the sum before that is rounded to h's type, and is rounded once, to its byte.  A thread holds eight neighbouring columns,
+// so a block is 16 lanes: its largest magnitude is four shuffles.  Magnitudes are compared as integers: a NaN is above infinity, reaches the scale and so the block.
+// Scales stand block by block, rows side by side: the products read one block's scales of many rows at once, and a warp of them is one line.
+#include <cuda_fp8.h>
+#include "common.cuh"
+
+namespace rx {
+
+enum : int { F8R_BF16 = 0, F8R_F16 = 1, F8R_F32 = 2 };
+
+// eight values from 16 (32) bytes at p + i
+template <int T>
+__device__ __forceinline__ void load8(const void* p, size_t i, float (&v)[8]) {
+  if constexpr (T == F8R_F32) {
+    const float4 a = *reinterpret_cast<const float4*>((const float*)p + i), b = *reinterpret_cast<const float4*>((const float*)p + i + 4);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  } else {
+    const uint4 a = *reinterpret_cast<const uint4*>((const uint16_t*)p + i);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (T == F8R_BF16) {
+        v[2 * j] = __uint_as_float(w[j] << 16), v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+        v[2 * j] = f.x, v[2 * j + 1] = f.y;
+      }
+    }
+  }
+}
+__device__ __forceinline__ uint4 pack8_bf16(const float (&v)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+    w[j] = *reinterpret_cast<const uint32_t*>(&b);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <int T>
+__device__ __forceinline__ void store8(void* p, size_t i, const float (&v)[8]) {
+  if constexpr (T == F8R_F32) {
+    *reinterpret_cast<float4*>((float*)p + i) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>((float*)p + i + 4) = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+    *reinterpret_cast<uint4*>((uint16_t*)p + i) = pack8_bf16(v);
+  }
+}
+
+// The bytes of a thread's eight columns and, in `scale`, their block's scale.  The 16 lanes of a block call together (with zeros where the row has ended).
+__device__ __forceinline__ uint2 to_e4m3(const float (&y)[8], float& scale) {
+  int m = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) m = max(m, __float_as_int(y[j]) & 0x7FFFFFFF);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const float amax = __int_as_float(max(m, 0x0D800000));           // 2^-100: 448 / amax stays finite
+  scale = amax / 448.f;
+  const float inv = 448.f / amax;
+  uint32_t w[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[4 * j] * inv, y[4 * j + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[4 * j + 2] * inv, y[4 * j + 3] * inv), __NV_SATFINITE, __NV_E4M3);
+    w[j] = lo | hi << 16;
+  }
+  return make_uint2(w[0], w[1]);
+}
+
+struct NormArgs {
+  const void* x;             // [rows][terms][d], rows ldx apart; nullptr: nothing is added
+  const float* weights;      // [rows][terms], nullptr: one term of weight 1
+  void* h;
+  const uint16_t* norm_w;    // bf16 [d], nullptr: no norm
+  uint8_t* q;
+  float* s;
+  uint16_t* xn;              // bf16 y, or nullptr
+  long long ldx, ldh, ldq, lds, ldn;
+  float eps;
+  int rows, terms, d;
+};
+
+// One CTA a row, NV vectors of eight columns a thread, kept in registers from the load to the bytes.
+template <int TX, int TH, int NV>
+__global__ void __launch_bounds__(1024) add_norm_fp8_kernel(const __grid_constant__ NormArgs a) {
+  pdl_launch();
+  pdl_wait();
+  __shared__ float sums[32];
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, nw = blockDim.x >> 5;
+  const long long row = blockIdx.x;
+  float nwv[NV][8];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int c = (v * (int)blockDim.x + t) * 8;
+    if (a.norm_w != nullptr && c < a.d) load8<F8R_BF16>(a.norm_w, c, nwv[v]);
+  }
+  float y[NV][8];
+  float sq = 0.f;
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int c = (v * (int)blockDim.x + t) * 8;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[v][j] = 0.f;
+    if (c < a.d) {
+      load8<TH>(a.h, row * a.ldh + c, y[v]);
+      if (a.weights != nullptr) {
+        for (int k = 0; k < a.terms; ++k) {
+          const float w = a.weights[row * a.terms + k];
+          if (w == 0.f) continue;
+          float x[8];
+          load8<TX>(a.x, row * a.ldx + (long long)k * a.d + c, x);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) y[v][j] = fmaf(w, x[j], y[v][j]);
+        }
+        store8<TH>(a.h, row * a.ldh + c, y[v]);
+      } else if (a.x != nullptr) {
+        float x[8];
+        load8<TX>(a.x, row * a.ldx + c, x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[v][j] += x[j];
+        store8<TH>(a.h, row * a.ldh + c, y[v]);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sq = fmaf(y[v][j], y[v][j], sq);
+    }
+  }
+  if (a.norm_w != nullptr) {
+    sq = warp_sum(sq);
+    if (lane == 0) sums[warp] = sq;
+    __syncthreads();
+    sq = warp_sum(lane < nw ? sums[lane] : 0.f);
+    const float r = rsqrtf(sq / (float)a.d + a.eps);
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = (v * (int)blockDim.x + t) * 8;
+      if (c < a.d) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[v][j] = y[v][j] * r * nwv[v][j];
+      }
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int c = (v * (int)blockDim.x + t) * 8;
+    float scale;
+    const uint2 b = to_e4m3(y[v], scale);
+    if (c < a.d) {
+      *reinterpret_cast<uint2*>(a.q + row * a.ldq + c) = b;
+      if ((t & 15) == 0) a.s[(long long)(c >> 7) * a.lds + row] = scale;
+      if (a.xn != nullptr) *reinterpret_cast<uint4*>(a.xn + row * a.ldn + c) = pack8_bf16(y[v]);
+    }
+  }
+}
+
+struct SwigluArgs {
+  const void* x;             // [rows][gate F | up F], rows ldx apart
+  const int* total;          // rows that hold something, nullptr: all
+  uint8_t* q;
+  float* s;
+  long long ldx, ldq, lds;
+  int rows, F, blocks;
+};
+
+// 16 lanes a block of 128 outputs; a CTA takes 16 blocks of one row
+template <int TX>
+__global__ void __launch_bounds__(256) swiglu_fp8_kernel(const __grid_constant__ SwigluArgs a) {
+  pdl_launch();
+  pdl_wait();
+  const long long row = blockIdx.x;
+  if (a.total != nullptr && row >= *a.total) return;
+  const int block = blockIdx.y * 16 + (threadIdx.x >> 4), c = block * 128 + (threadIdx.x & 15) * 8;
+  float y[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) y[j] = 0.f;
+  if (c < a.F) {
+    float g[8], u[8];
+    load8<TX>(a.x, row * a.ldx + c, g);
+    load8<TX>(a.x, row * a.ldx + a.F + c, u);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = __fdividef(g[j], 1.f + __expf(-g[j])) * u[j];
+  }
+  float scale;
+  const uint2 b = to_e4m3(y, scale);
+  if (c < a.F) {
+    *reinterpret_cast<uint2*>(a.q + row * a.ldq + c) = b;
+    if ((threadIdx.x & 15) == 0) a.s[(long long)block * a.lds + row] = scale;
+  }
+}
+
+template <int TX, int TH>
+static int launch_norm(const NormArgs& a, cudaStream_t st) {
+  const int vecs = a.d / 8;
+  const int nv = vecs <= 1024 ? 1 : vecs <= 2048 ? 2 : 4;
+  const int threads = ((vecs + nv - 1) / nv + 31) / 32 * 32;
+  if (nv == 1) return (int)rx::launch(add_norm_fp8_kernel<TX, TH, 1>, dim3(a.rows), dim3(threads), 0, st, a);
+  if (nv == 2) return (int)rx::launch(add_norm_fp8_kernel<TX, TH, 2>, dim3(a.rows), dim3(threads), 0, st, a);
+  return (int)rx::launch(add_norm_fp8_kernel<TX, TH, 4>, dim3(a.rows), dim3(threads), 0, st, a);
+}
+
+}  // namespace rx
+
+using namespace rx;
+
+// x [rows][terms][d] (type x_type: 0 bf16, 1 fp16, 2 fp32) or nullptr, weights f32 [rows][terms] or nullptr (then terms = 1), h bf16 or fp32 (h_type 0 or 2),
+// q bytes, s f32 [ceil(d / 128)][lds], xn bf16 or nullptr.  d a multiple of 16 up to 32768; every row begins on 16 bytes.
+RX_API int rx_add_norm_fp8(const void* x, int x_type, long long ldx, const void* weights, int terms, void* h, int h_type, long long ldh, const void* norm_w, float eps,
+                           void* q, long long ldq, void* s, long long lds, void* xn, long long ldn, int rows, int d, void* stream) {
+  if (rows < 1 || d < 16 || d % 16 != 0 || d > 32768 || terms < 1 || (terms > 1 && (weights == nullptr || x == nullptr))) return (int)cudaErrorInvalidValue;
+  if (x_type < 0 || x_type > 2 || (h_type != F8R_BF16 && h_type != F8R_F32) || h == nullptr || q == nullptr || s == nullptr) return (int)cudaErrorInvalidValue;
+  if (x != nullptr && ldx < (long long)terms * d || ldh < d || ldq < d || lds < rows || (xn != nullptr && ldn < d)) return (int)cudaErrorInvalidValue;
+  if (((uintptr_t)x | (uintptr_t)h | (uintptr_t)q | (uintptr_t)xn | (uintptr_t)norm_w) & 15) return (int)cudaErrorMisalignedAddress;
+  if (ldx * (x_type == F8R_F32 ? 4 : 2) % 16 || ldh * (h_type == F8R_F32 ? 4 : 2) % 16 || ldq % 16 || (xn != nullptr && ldn % 8)) return (int)cudaErrorMisalignedAddress;
+  const NormArgs a = {x, (const float*)weights, h, (const uint16_t*)norm_w, (uint8_t*)q, (float*)s, (uint16_t*)xn, ldx, ldh, ldq, lds, ldn, eps, rows, terms, d};
+  cudaStream_t st = (cudaStream_t)stream;
+  if (h_type == F8R_BF16) {
+    if (x_type == F8R_BF16) return launch_norm<F8R_BF16, F8R_BF16>(a, st);
+    if (x_type == F8R_F16) return launch_norm<F8R_F16, F8R_BF16>(a, st);
+    return launch_norm<F8R_F32, F8R_BF16>(a, st);
+  }
+  if (x_type == F8R_BF16) return launch_norm<F8R_BF16, F8R_F32>(a, st);
+  if (x_type == F8R_F16) return launch_norm<F8R_F16, F8R_F32>(a, st);
+  return launch_norm<F8R_F32, F8R_F32>(a, st);
+}
+
+// x [rows][2 F] (gate | up; type as above), q bytes [rows][F], s f32 [ceil(F / 128)][lds]; total: device int32, rows from it on are left as they are, or nullptr.
+RX_API int rx_swiglu_fp8(const void* x, int x_type, long long ldx, void* q, long long ldq, void* s, long long lds, const void* total, int rows, int F, void* stream) {
+  if (rows < 1 || F < 16 || F % 16 != 0 || F > (1 << 20) || x_type < 0 || x_type > 2 || x == nullptr || q == nullptr || s == nullptr) return (int)cudaErrorInvalidValue;
+  if (ldx < 2ll * F || ldq < F || lds < rows) return (int)cudaErrorInvalidValue;
+  if (((uintptr_t)x | (uintptr_t)q) & 15 || ldx * (x_type == F8R_F32 ? 4 : 2) % 16 || ldq % 16) return (int)cudaErrorMisalignedAddress;
+  const int blocks = (F + 127) / 128;
+  const SwigluArgs a = {x, (const int*)total, (uint8_t*)q, (float*)s, ldx, ldq, lds, rows, F, blocks};
+  const dim3 grid(rows, (blocks + 15) / 16), threads(256);
+  cudaStream_t st = (cudaStream_t)stream;
+  if (x_type == F8R_BF16) return (int)rx::launch(swiglu_fp8_kernel<F8R_BF16>, grid, threads, 0, st, a);
+  if (x_type == F8R_F16) return (int)rx::launch(swiglu_fp8_kernel<F8R_F16>, grid, threads, 0, st, a);
+  return (int)rx::launch(swiglu_fp8_kernel<F8R_F32>, grid, threads, 0, st, a);
+}

@@ -570,6 +570,198 @@ def window_rows(seq: torch.Tensor, have: torch.Tensor, new: torch.Tensor, block_
     _lib.count()
 
 
+# ------------------------------------------------------------------------------------------------ rows and weights of E4M3 with scales for blocks of 128
+_E4M3, _U8 = torch.float8_e4m3fn, torch.uint8
+_FLOATS = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def fp8_rows(rows: int, width: int, device="cuda") -> tuple:
+    """Buffers for `rows` rows of E4M3 with a scale for each 128 columns, as the operators below write and read them: (q float8_e4m3fn [rows, width],
+    s float32 [ceil(width / 128), rows]); row r stands for q[r, c] * s[c // 128, r]."""
+    return torch.empty(rows, width, dtype=_E4M3, device=device), torch.empty((width + 127) // 128, rows, dtype=torch.float32, device=device)
+
+
+def _rows2(t, name: str, dtypes, rows, width: int, device: int) -> tuple:
+    """The pointer of rows of `width` values side by side, and how far apart the rows are"""
+    if not isinstance(t, _Tensor) or not t.is_cuda:
+        raise ValueError(f"{name}: a CUDA tensor is needed")
+    if t.get_device() != device:
+        raise ValueError(f"{name} is on {t.device}, not on the current device cuda:{device}")
+    shape = t.shape
+    if t.dtype not in dtypes or len(shape) != 2 or shape[1] != width or rows is not None and shape[0] != rows:
+        raise ValueError(f"{name}: {' or '.join(str(d) for d in dtypes)} [{'rows' if rows is None else rows}, {width}] is needed, not {t.dtype} {list(shape)}")
+    ld, step = t.stride()
+    if shape[0] <= 1:
+        ld = width
+    if width > 1 and step != 1 or ld < width:
+        raise ValueError(f"{name}: a row's values must stand side by side, and rows must not overlap")
+    return t.data_ptr(), ld
+
+
+def _on16(name: str, p: int, ld_bytes: int) -> None:
+    if (p | ld_bytes) & 15:
+        raise ValueError(f"{name}: every row must begin on a 16-byte boundary")
+
+
+def _scales(s, name: str, rows: int, width: int, device: int) -> tuple:
+    """... of the scales of such rows: [blocks, rows], blocks may be further apart"""
+    return _rows2(s, name, (_F32,), (width + 127) // 128, rows, device)
+
+
+def add_norm_fp8(x: "torch.Tensor | None", h: torch.Tensor, norm_w: "torch.Tensor | None", eps: float, q: torch.Tensor, s: torch.Tensor, *, weights=None,
+                 xn: "torch.Tensor | None" = None) -> None:
+    """h += x, and the root-mean-square norm of the sum as E4M3 rows: y = h * rsqrt(mean(h^2) + eps) * norm_w, over each 128 columns of a row s = max(max|y|, 2^-100) / 448
+    and q = e4m3(y / s) (`fp8_rows`).  h bf16 or float32 [rows, d], in place; y is formed of the sum before it is rounded to h's type.  All steps are float32.
+    x: bf16, fp16 or float32 [rows, d]; None: nothing is added.  With weights (float32 [rows, n]) x is [rows, n, d], contiguous, the outputs of a row's n routed experts:
+    h += sum of weights[r, i] * x[r, i], in that order; what has the weight 0 is not read.  norm_w bf16 [d]; None: no norm, y is the sum.
+    xn (bf16 [rows, d]): y for who needs it unquantised (a router).  d: a multiple of 16, up to 32768; rows may be further apart than d, and begin on 16-byte boundaries.
+    An infinity or NaN in y makes its block's scale one, so the whole block reads as NaN."""
+    dev = _here(h, "h")
+    if h.dim() != 2:
+        raise ValueError("h: a CUDA tensor [rows, d] is needed")
+    rows, d = h.shape
+    if d % 16 or not 16 <= d <= 32768:
+        raise ValueError(f"rows of {d}: a multiple of 16, 16 .. 32768")
+    p_h, ldh = _rows2(h, "h", (_BF16, _F32), rows, d, dev)
+    p_q, ldq = _rows2(q, "q", (_E4M3, _U8), rows, d, dev)
+    p_s, lds = _scales(s, "s", rows, d, dev)
+    p_x, ldx, x_type, terms, p_w = None, 0, 0, 1, None
+    if weights is not None:
+        if x is None:
+            raise ValueError("weights need x")
+        p_w, n, terms = _table(weights, "weights", _F32, dev)
+        if n != rows or not 1 <= terms <= 1024:
+            raise ValueError(f"weights: [{rows}, 1 .. 1024] is needed, not {list(weights.shape)}")
+        if not isinstance(x, _Tensor) or x.dtype not in _FLOATS or x.shape != (rows, terms, d) or x.get_device() != dev or not x.is_contiguous():
+            raise ValueError(f"x: a contiguous bf16, fp16 or float32 [{rows}, {terms}, {d}] on cuda:{dev} is needed")
+        p_x, ldx, x_type = x.data_ptr(), terms * d, _FLOATS[x.dtype]
+    elif x is not None:
+        p_x, ldx = _rows2(x, "x", tuple(_FLOATS), rows, d, dev)
+        x_type = _FLOATS[x.dtype]
+    p_nw = None if norm_w is None else _vector(norm_w, "norm_w", _BF16, d, dev)
+    p_xn, ldn = (None, 0) if xn is None else _rows2(xn, "xn", (_BF16,), rows, d, dev)
+    if rows == 0:
+        return
+    _on16("h", p_h, ldh * h.element_size())
+    _on16("q", p_q, ldq)
+    if p_x is not None:
+        _on16("x", p_x, ldx * x.element_size())
+    _on16("norm_w", p_nw or 0, 0)
+    _on16("xn", p_xn or 0, ldn * 2)
+    _lib.check(_lib.load().rx_add_norm_fp8(p_x, x_type, ldx, p_w, terms, p_h, _FLOATS[h.dtype], ldh, p_nw, float(eps), p_q, ldq, p_s, lds, p_xn, ldn, rows, d,
+                                           _lib.stream_ptr()), "rx_add_norm_fp8")
+    _lib.count()
+
+
+def swiglu_fp8(x: torch.Tensor, q: torch.Tensor, s: torch.Tensor, *, total: "torch.Tensor | None" = None) -> None:
+    """SwiGLU as E4M3 rows: y = silu(gate) * up of x = [gate | up], bf16, fp16 or float32 [rows, 2 * ffn], q and s as `add_norm_fp8` writes them ([rows, ffn]).  ffn: a
+    multiple of 16, up to 2^20; rows may be further apart, and begin on 16-byte boundaries.  total (int32 [1], on the device): only the first total rows hold
+    something (routed pairs); the others' q and s stay as they are."""
+    dev = _here(x, "x")
+    if x.dim() != 2 or x.shape[1] % 32 or not 32 <= x.shape[1] <= 1 << 21:
+        raise ValueError(f"x: [rows, 2 * ffn] with ffn a multiple of 16, 16 .. 2^20, not {list(x.shape)}")
+    rows, F = x.shape[0], x.shape[1] // 2
+    p_x, ldx = _rows2(x, "x", tuple(_FLOATS), rows, 2 * F, dev)
+    p_q, ldq = _rows2(q, "q", (_E4M3, _U8), rows, F, dev)
+    p_s, lds = _scales(s, "s", rows, F, dev)
+    p_total = None if total is None else _vector(total, "total", _I32, 1, dev)
+    if rows == 0:
+        return
+    _on16("x", p_x, ldx * x.element_size())
+    _on16("q", p_q, ldq)
+    _lib.check(_lib.load().rx_swiglu_fp8(p_x, _FLOATS[x.dtype], ldx, p_q, ldq, p_s, lds, p_total, rows, F, _lib.stream_ptr()), "rx_swiglu_fp8")
+    _lib.count()
+
+
+class Fp8BlockWeight:
+    """A linear layer's E4M3 matrix with a float32 scale for each 128 x 128 block: `w` (float8_e4m3fn or its bytes, uint8) [N, K], `scales` [ceil(N / 128), ceil(K / 128)],
+    optional float32 bias [N]; w[n, k] stands for w * scales[n // 128, k // 128].  Or as many such matrices as there are experts, [experts, N, K] and
+    [experts, ...], without a bias (`fp8_block_experts`).  K: a multiple of 16.  A product may begin to read the matrix before the kernel ahead of it has
+    ended: a kernel of this library that writes it must be followed by another one, or by a synchronisation."""
+
+    def __init__(self, w: torch.Tensor, scales: torch.Tensor, bias: "torch.Tensor | None" = None):
+        if w.dtype not in (_E4M3, _U8) or w.dim() not in (2, 3) or min(w.shape) < 1 or w.shape[-1] % 16 or w.shape[-1] > 1 << 24 or w.shape[-2] > 1 << 22:
+            raise ValueError(f"w: E4M3 [N, K] or [experts, N, K] with K a multiple of 16 (up to 2^24, N up to 2^22), not {w.dtype} {list(w.shape)}")
+        self.experts, self.N, self.K = (w.shape[0] if w.dim() == 3 else None), w.shape[-2], w.shape[-1]
+        blocks = (*w.shape[:-2], (self.N + 127) // 128, (self.K + 127) // 128)
+        if scales.dtype != torch.float32 or tuple(scales.shape) != blocks or scales.device != w.device:
+            raise ValueError(f"scales: float32 {list(blocks)} on {w.device} is needed, not {scales.dtype} {list(scales.shape)} on {scales.device}")
+        if bias is not None and (self.experts is not None or bias.dtype != torch.float32 or tuple(bias.shape) != (self.N,) or bias.device != w.device):
+            raise ValueError(f"bias: float32 [{self.N}] on {w.device}, and none for experts")
+        if self.experts is not None and (self.experts > 4096 or self.experts * self.N > (1 << 31) - 128):
+            raise ValueError(f"{self.experts} experts of {self.N} columns: at most 4096, and 2^31 columns")
+        self.w, self.scales, self.bias = w.contiguous(), scales.contiguous(), None if bias is None else bias.contiguous()
+        if self.w.data_ptr() & 15:
+            raise ValueError("w: must begin on a 16-byte boundary")
+
+    @staticmethod
+    def quantize(dense: torch.Tensor, bias=None) -> "Fp8BlockWeight":
+        """dense float [N, K] or [experts, N, K] -> every block scaled so that its largest magnitude is 448, values rounded to E4M3."""
+        N, Kd = dense.shape[-2:]
+        nb, kb = (N + 127) // 128, (Kd + 127) // 128
+        t = torch.nn.functional.pad(dense.float(), (0, kb * 128 - Kd, 0, nb * 128 - N)).view(*dense.shape[:-2], nb, 128, kb, 128)
+        scales = t.abs().amax(dim=(-3, -1)).clamp_min(2.0 ** -100) / 448.0
+        q = (t / scales[..., :, None, :, None]).clamp(-448, 448).view(*dense.shape[:-2], nb * 128, kb * 128)[..., :N, :Kd]
+        return Fp8BlockWeight(q.to(_E4M3).contiguous(), scales, bias)
+
+    def dense(self) -> torch.Tensor:
+        """The float32 matrix that the bytes stand for (oracle side)."""
+        s = self.scales.repeat_interleave(128, -2)[..., :self.N, :].repeat_interleave(128, -1)[..., :self.K]
+        return self.w.view(_E4M3).float() * s
+
+
+def _product(q, s, w, out, status, experts: bool):
+    dev = _here(q, "q")
+    if not isinstance(w, Fp8BlockWeight) or (w.experts is not None) != experts:
+        raise ValueError("w: an Fp8BlockWeight " + ("of experts" if experts else "of one matrix") + " is needed")
+    if q.dim() != 2 or q.shape[1] != w.K:
+        raise ValueError(f"q: [rows, {w.K}] is needed, not {list(q.shape)}")
+    if w.w.get_device() != dev:
+        raise ValueError(f"w is on {w.w.device}, not on the current device cuda:{dev}")
+    rows = q.shape[0]
+    p_q, ldq = _rows2(q, "q", (_E4M3, _U8), rows, w.K, dev)
+    p_s, lds = _scales(s, "s", rows, w.K, dev)
+    p_out, ldo = _rows2(out, "out", tuple(_FLOATS), None if experts else rows, w.N, dev)
+    _on16("q", p_q, ldq)
+    return dev, rows, p_q, ldq, p_s, lds, p_out, ldo, _vector(status, "status", _I32, STATUS_WORDS, dev)
+
+
+def fp8_block_linear(q: torch.Tensor, s: torch.Tensor, w: Fp8BlockWeight, out: torch.Tensor, status: torch.Tensor) -> None:
+    """out = (q under s) @ (w under its scales)^T (+ bias), both operands E4M3 on the tensor cores: q float8_e4m3fn (or its bytes) [rows, K], s float32 [ceil(K / 128), rows]
+    (`fp8_rows`, written by `add_norm_fp8` or `swiglu_fp8`), out bf16, fp16 or float32 [rows, N].  A block's products are summed in float32, the blocks' sums take their scales
+    and are summed in float32; out is rounded once.  Rows of q begin on 16-byte boundaries; rows of q and out and blocks of s may be further apart.  A row's last
+    bits depend on the number of rows, which decides how the sum over K is cut.  (`fp8_linear` takes bf16 activations and scales of 32 x 32 tiles.)"""
+    dev, rows, p_q, ldq, p_s, lds, p_out, ldo, p_status = _product(q, s, w, out, status, False)
+    if rows == 0:
+        return
+    _lib.check(_lib.load().rx_fp8_block_linear(p_q, ldq, p_s, lds, rows, w.K, w.w.data_ptr(), w.scales.data_ptr(), _lib.ptr(w.bias), w.N, p_out, _FLOATS[out.dtype], ldo,
+                                               p_status, _lib.stream_ptr()), "rx_fp8_block_linear")
+    _lib.count()
+
+
+def fp8_block_experts(q: torch.Tensor, s: torch.Tensor, w: Fp8BlockWeight, offs: torch.Tensor, out: torch.Tensor, status: torch.Tensor, *, src=None, src_div: int = 1,
+                      dst=None) -> None:
+    """`fp8_block_linear` through routed experts.  Positions offs[e] .. offs[e + 1] (int32 [experts + 1], ascending from 0 and more) belong to expert e's matrix, as
+    `rx_moe_plan` sorts (row, pick) pairs.  Position p takes row src[p] // src_div of q (int32; the up product: src = the plan's pair_of_pos, src_div = picks a row) and
+    writes row dst[p] of out (int32; the down product: dst = pair_of_pos).  Without them it is row p; positions beyond offs[experts] are not looked at, and rows of out
+    that no position writes stay as they are.  No two positions write the same row.  Offsets that descend or leave the positions, a row outside q (its output is
+    0) or outside out (nothing is written) set the status."""
+    dev, rows, p_q, ldq, p_s, lds, p_out, ldo, p_status = _product(q, s, w, out, status, True)
+    cap = _length(src, "src") if src is not None else _length(dst, "dst") if dst is not None else rows
+    p_offs = _vector(offs, "offs", _I32, w.experts + 1, dev)
+    p_src = None if src is None else _vector(src, "src", _I32, cap, dev)
+    p_dst = None if dst is None else _vector(dst, "dst", _I32, cap, dev)
+    if src is None and cap > rows or dst is None and cap > out.shape[0]:
+        raise ValueError(f"{cap} positions: more than rows of q ({rows}) or of out ({out.shape[0]})")
+    if src_div < 1 or src_div != 1 and src is None:
+        raise ValueError(f"src_div {src_div}: 1 and more, with src")
+    if cap == 0 or rows == 0 or out.shape[0] == 0:
+        return
+    _lib.check(_lib.load().rx_fp8_block_experts(p_q, ldq, p_s, lds, rows, w.K, w.w.data_ptr(), w.scales.data_ptr(), w.experts, w.N, p_offs, p_src, int(src_div), p_dst, cap,
+                                                p_out, _FLOATS[out.dtype], ldo, out.shape[0], p_status, _lib.stream_ptr()), "rx_fp8_block_experts")
+    _lib.count()
+
+
 class KvTensorMap:
     """Host-side TMA descriptors of one layer's K or V cache (bf16 or bytes [pages, n_kv, 64, hd]): `ptr` for decode attention, `rows_ptr` for prefill
     (they differ for E4M3 bytes, whose decode kernel takes its pages swizzled)."""

@@ -107,6 +107,11 @@ def _declare(lib):
         "rx_tp_coll_combine": (c_int, [c_void, c_ll, c_int, c_void, c_void, c_void]),
         "rx_fp8_linear_scratch_floats": (c_ll, [c_int, c_int, c_int]),
         "rx_fp8_linear": (c_int, [c_void, c_int, c_int, c_void, c_void, c_int, c_void, c_int, c_int, c_void, c_void, c_int, c_void, c_void]),
+        "rx_add_norm_fp8": (c_int, [c_void, c_int, c_ll, c_void, c_int, c_void, c_int, c_ll, c_void, c_f, c_void, c_ll, c_void, c_ll, c_void, c_ll, c_int, c_int, c_void]),
+        "rx_swiglu_fp8": (c_int, [c_void, c_int, c_ll, c_void, c_ll, c_void, c_ll, c_void, c_int, c_int, c_void]),
+        "rx_fp8_block_linear": (c_int, [c_void, c_ll, c_void, c_ll, c_int, c_int, c_void, c_void, c_void, c_int, c_void, c_int, c_ll, c_void, c_void]),
+        "rx_fp8_block_experts": (c_int, [c_void, c_ll, c_void, c_ll, c_int, c_int, c_void, c_void, c_int, c_int, c_void, c_void, c_int, c_void, c_int, c_void, c_int, c_ll,
+                                         c_int, c_void, c_void]),
         "rx_dsa_gather": (c_int, [c_void, c_void, c_int, c_void, c_void, c_int, c_void, c_void, c_void, c_int, c_int, c_void]),
         "rx_mxfp4_gemm_grouped": (c_int, [c_void, c_int, c_int, c_void, c_void, c_int, c_int, c_void, c_int, c_void, c_int, c_int, c_void, c_void]),
         "rx_moe_combine": (c_int, [c_void, c_int, c_int, c_int, c_int, c_int, c_void, c_void, c_void, c_void, c_void, c_void, c_void]),
