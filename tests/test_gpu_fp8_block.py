@@ -159,7 +159,7 @@ def check_experts(q, s, w, offs, out, before, src=None, div=1, dst=None):
     near(out[written], want[written], size[written], w.K, out.dtype)
 
 
-@pytest.mark.parametrize("rows,picks,experts,held", [(1, 1, 1, 1), (1, 2, 8, 8), (16, 8, 128, 128), (5, 3, 300, 300), (40, 2, 6, 4), (130, 4, 16, 3), (333, 2, 5, 5), (700, 2, 3, 2), (64, 8, 40, 1)])
+@pytest.mark.parametrize("rows,picks,experts,held", [(1, 1, 1, 1), (2000, 2, 600, 600), (90, 8, 20, 20), (1, 2, 8, 8), (16, 8, 128, 128), (5, 3, 300, 300), (40, 2, 6, 4), (130, 4, 16, 3), (333, 2, 5, 5), (700, 2, 3, 2), (64, 8, 40, 1)])
 @pytest.mark.parametrize("Kd,N", [(128, 128), (688, 300), (272, 17), (1024, 256)])
 def test_experts_up_and_down(rows, picks, experts, held, Kd, N):
     g = gen(rows + experts + Kd)
