@@ -1070,10 +1070,8 @@ static int fb_launch_wide(const void* q, long long ldq, const void* w, const FbA
 // How many clusters of `size` CTAs of the kernel the current device holds at once with one CTA an SM.  (Clusters stay within a GPC: of six CTAs there is room for 22, of
 // seven for 15.)
 template <auto KERN>
-static int fb_at_once(int size, int threads, int smem) {
+static int fb_at_once(int dev, int size, int threads, int smem) {
   static int known[64][9];
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return 0;
   if (known[dev][size] == 0) {
     if (fb_allow<KERN>(smem) != 0) return 0;
     cudaLaunchConfig_t cfg = {};
@@ -1093,13 +1091,13 @@ static int fb_at_once(int size, int threads, int smem) {
 // read again; a start 3 and 7 us (the larger kernel has its SM alone, so it cannot begin under the kernel before), a cluster's sums 1.3 and 3.
 struct FbChoice { int cg, T, parts; double us; };
 template <int T>
-static void fb_consider_step(const FbArgs& a, FbChoice& best) {
+static void fb_consider_step(int dev, const FbArgs& a, FbChoice& best) {
   using L = FbStep<T>;
   const long long row_tiles = (a.rows + T - 1) / T, strips = (a.N + 127) / 128, tiles = row_tiles * strips;
   if (row_tiles > 65535) return;
   const double dram = (double)a.N * a.K, all = (double)tiles * a.kblocks * (FB_A + (a.rows < T ? a.rows : T) * FB_K), mem = dram / 6.6e6 + (all - dram) / 10e6;
   for (int parts = 1; parts <= 8 && parts <= a.kblocks; ++parts) {
-    const int slots = L::PER_SM * fb_at_once<fp8_block_step_kernel<T, false>>(parts, L::THREADS, L::SMEM);
+    const int slots = L::PER_SM * fb_at_once<fp8_block_step_kernel<T, false>>(dev, parts, L::THREADS, L::SMEM);
     if (slots <= 0) continue;
     const double waves = (double)((tiles + slots - 1) / slots), blocks = (a.kblocks + parts - 1) / parts, k = waves * blocks * (T == 16 ? 0.24 : T == 32 ? 0.27 : 0.29);
     const double us = 3.0 * waves + sqrt(k * k + mem * mem) + (parts > 1 ? 1.3 : 0);
@@ -1107,12 +1105,12 @@ static void fb_consider_step(const FbArgs& a, FbChoice& best) {
   }
 }
 template <int CG>
-static void fb_consider_wide(const FbArgs& a, FbChoice& best) {
+static void fb_consider_wide(int dev, const FbArgs& a, FbChoice& best) {
   using L = FbWide<CG>;
   const long long row_tiles = (a.rows + 128 * CG - 1) / (128 * CG), tiles = row_tiles * ((a.N + 255) / 256);
   const double dram = (double)a.N * a.K, all = (double)tiles * CG * a.kblocks * ((a.rows < 128 ? a.rows : 128) * FB_K + L::B), mem = dram / 6.6e6 + (all - dram) / 10e6;
   for (int parts = 1; parts * CG <= 8 && parts <= a.kblocks; ++parts) {
-    const int slots = fb_at_once<fp8_block_wide_kernel<CG, false>>(CG * parts, L::THREADS, L::SMEM);
+    const int slots = fb_at_once<fp8_block_wide_kernel<CG, false>>(dev, CG * parts, L::THREADS, L::SMEM);
     if (slots <= 0 || (parts > 1 && tiles > slots)) continue;      // (a cluster with parts has one tile)
     const double waves = (double)((tiles + slots - 1) / slots), blocks = (a.kblocks + parts - 1) / parts, k = waves * (blocks * (CG == 2 ? 0.46 : 0.47) + 0.4);
     const double us = 7.0 + sqrt(k * k + mem * mem) + (parts > 1 ? 3.0 : 0);
@@ -1141,13 +1139,16 @@ RX_API int rx_fp8_block_linear(const void* q, long long ldq, const void* s, long
   a.q = (const uint8_t*)q, a.ldq = ldq, a.s = (const float*)s, a.ws = (const float*)ws, a.bias = (const float*)bias, a.out = out, a.status = status;
   a.lds = lds, a.ldo = ldo, a.rows = rows, a.K = K, a.N = N, a.kblocks = (K + 127) / 128, a.out_type = out_type, a.experts = 1, a.out_rows = rows, a.src_div = 1;
   if (const int e = fb_check(q, ldq, a, w)) return e;
+  int dev = 0;
+  if (const cudaError_t e = cudaGetDevice(&dev)) return (int)e;
+  if (dev >= 64) return (int)cudaErrorInvalidDevice;
   FbChoice c = {-1, 0, 0, 1e300};
-  if (rows <= 16) fb_consider_step<16>(a, c);
-  else if (rows <= 32) fb_consider_step<32>(a, c);
-  else if (rows <= 512) fb_consider_step<64>(a, c);
+  if (rows <= 16) fb_consider_step<16>(dev, a, c);
+  else if (rows <= 32) fb_consider_step<32>(dev, a, c);
+  else if (rows <= 512) fb_consider_step<64>(dev, a, c);
   if (rows > 16) {
-    fb_consider_wide<1>(a, c);
-    fb_consider_wide<2>(a, c);
+    fb_consider_wide<1>(dev, a, c);
+    fb_consider_wide<2>(dev, a, c);
   }
   cudaStream_t st = (cudaStream_t)stream;
   if (c.cg == 1) return fb_launch_wide<1, false>(q, ldq, w, a, c.parts, st);

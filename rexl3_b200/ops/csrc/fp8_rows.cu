@@ -60,9 +60,12 @@ __device__ __forceinline__ uint2 to_e4m3(const float (&y)[8], float& scale) {
   for (int j = 0; j < 8; ++j) m = max(m, __float_as_int(y[j]) & 0x7FFFFFFF);
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const float amax = __int_as_float(max(m, 0x0D800000));           // 2^-100: 448 / amax stays finite
-  scale = amax / 448.f;
-  const float inv = 448.f / amax;
+  const float amax = __int_as_float(max(m, 0x0D800000));           // 2^-100: 1 / scale stays finite
+  constexpr float R = 1.f / 448.f;                                 // (a quotient by it, corrected by its remainder: as a division rounds)
+  scale = amax * R;
+  scale = fmaf(fmaf(-448.f, scale, amax), R, scale);
+  scale = m >= 0x7F800000 ? amax : scale;                          // infinity, NaN: the remainder would be NaN
+  const float inv = __frcp_rn(scale);
   uint32_t w[2];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
@@ -82,72 +85,96 @@ struct NormArgs {
   float* s;
   uint16_t* xn;              // bf16 y, or nullptr
   long long ldx, ldh, ldq, lds, ldn;
-  float eps;
+  float eps, per_d;          // per_d: 1 / d
   int rows, terms, d;
 };
 
-// One CTA a row, NV vectors of eight columns a thread, kept in registers from the load to the bytes.
-template <int TX, int TH, int NV>
-__global__ void __launch_bounds__(1024) add_norm_fp8_kernel(const __grid_constant__ NormArgs a) {
+// NV vectors of eight columns a thread, kept in registers from the load to the bytes.  THREADS = 0: eight warps with a row each (narrow rows); otherwise one CTA a row.
+enum : int { NORM_FIRST = 0, NORM_ADD = 1, NORM_EXPERTS = 2 };
+template <int TX, int TH, int MODE, int NV, int THREADS, int CTAS>
+__global__ void __launch_bounds__(THREADS ? THREADS : 256, CTAS) add_norm_fp8_kernel(const __grid_constant__ NormArgs a) {
   pdl_launch();
   pdl_wait();
-  __shared__ float sums[32];
-  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, nw = blockDim.x >> 5;
-  const long long row = blockIdx.x;
-  float nwv[NV][8];
-#pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    const int c = (v * (int)blockDim.x + t) * 8;
-    if (a.norm_w != nullptr && c < a.d) load8<F8R_BF16>(a.norm_w, c, nwv[v]);
-  }
+  __shared__ float sums[THREADS ? 32 : 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = THREADS ? (int)threadIdx.x : lane, threads = THREADS ? (int)blockDim.x : 32;
+  const long long row = THREADS ? (long long)blockIdx.x : (long long)blockIdx.x * 8 + warp;
+  if (row >= a.rows) return;
   float y[NV][8];
-  float sq = 0.f;
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
-    const int c = (v * (int)blockDim.x + t) * 8;
+    const int c = (v * threads + t) * 8;
 #pragma unroll
     for (int j = 0; j < 8; ++j) y[v][j] = 0.f;
-    if (c < a.d) {
-      load8<TH>(a.h, row * a.ldh + c, y[v]);
-      if (a.weights != nullptr) {
-        for (int k = 0; k < a.terms; ++k) {
-          const float w = a.weights[row * a.terms + k];
-          if (w == 0.f) continue;
-          float x[8];
-          load8<TX>(a.x, row * a.ldx + (long long)k * a.d + c, x);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) y[v][j] = fmaf(w, x[j], y[v][j]);
-        }
-        store8<TH>(a.h, row * a.ldh + c, y[v]);
-      } else if (a.x != nullptr) {
-        float x[8];
-        load8<TX>(a.x, row * a.ldx + c, x);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) y[v][j] += x[j];
-        store8<TH>(a.h, row * a.ldh + c, y[v]);
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) sq = fmaf(y[v][j], y[v][j], sq);
-    }
+    if (c < a.d) load8<TH>(a.h, row * a.ldh + c, y[v]);
   }
-  if (a.norm_w != nullptr) {
-    sq = warp_sum(sq);
-    if (lane == 0) sums[warp] = sq;
-    __syncthreads();
-    sq = warp_sum(lane < nw ? sums[lane] : 0.f);
-    const float r = rsqrtf(sq / (float)a.d + a.eps);
+  if constexpr (MODE == NORM_ADD) {
+    float x[NV][8];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int c = (v * (int)blockDim.x + t) * 8;
-      if (c < a.d) {
+      const int c = (v * threads + t) * 8;
+      if (c < a.d) load8<TX>(a.x, row * a.ldx + c, x[v]);
+    }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[v][j] = y[v][j] * r * nwv[v][j];
+    for (int v = 0; v < NV; ++v) {
+      const int c = (v * threads + t) * 8;
+      if (c >= a.d) continue;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[v][j] += x[v][j];
+      store8<TH>(a.h, row * a.ldh + c, y[v]);
+    }
+  } else if constexpr (MODE == NORM_EXPERTS) {
+    constexpr int AT_ONCE = 4;                     // experts' outputs under way together
+    for (int k0 = 0; k0 < a.terms; k0 += AT_ONCE) {
+      float w[AT_ONCE];
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; ++k) w[k] = k0 + k < a.terms ? a.weights[row * a.terms + k0 + k] : 0.f;
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        const int c = (v * threads + t) * 8;
+        if (c >= a.d) continue;
+        float x[AT_ONCE][8];
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[k][j] = 0.f;
+          if (w[k] != 0.f) load8<TX>(a.x, row * a.ldx + (long long)(k0 + k) * a.d + c, x[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) y[v][j] = fmaf(w[k], x[k][j], y[v][j]);
       }
     }
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = (v * threads + t) * 8;
+      if (c < a.d) store8<TH>(a.h, row * a.ldh + c, y[v]);
+    }
+  }
+  float r = 1.f;
+  if (a.norm_w != nullptr) {
+    float sq = 0.f;
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sq = fmaf(y[v][j], y[v][j], sq);
+    sq = warp_sum(sq);
+    if constexpr (THREADS != 0) {
+      if (lane == 0) sums[warp] = sq;
+      __syncthreads();
+      sq = warp_sum(lane < threads / 32 ? sums[lane] : 0.f);
+    }
+    r = rsqrtf(sq * a.per_d + a.eps);
   }
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
-    const int c = (v * (int)blockDim.x + t) * 8;
+    const int c = (v * threads + t) * 8;
+    if (a.norm_w != nullptr && c < a.d) {
+      float w[8];
+      load8<F8R_BF16>(a.norm_w, c, w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[v][j] = y[v][j] * r * w[j];
+    }
     float scale;
     const uint2 b = to_e4m3(y[v], scale);
     if (c < a.d) {
@@ -164,21 +191,23 @@ struct SwigluArgs {
   uint8_t* q;
   float* s;
   long long ldx, ldq, lds;
-  int rows, F, blocks;
+  int rows, F, blocks;       // blocks of a row
+  uint32_t magic, shift;     // n / blocks = (umulhi(n, magic) + n) >> shift
 };
 
-// 16 lanes a block of 128 outputs; a CTA takes 16 blocks of one row
+// 16 lanes a block of 128 outputs, blocks row after row
 template <int TX>
 __global__ void __launch_bounds__(256) swiglu_fp8_kernel(const __grid_constant__ SwigluArgs a) {
   pdl_launch();
   pdl_wait();
-  const long long row = blockIdx.x;
-  if (a.total != nullptr && row >= *a.total) return;
-  const int block = blockIdx.y * 16 + (threadIdx.x >> 4), c = block * 128 + (threadIdx.x & 15) * 8;
+  const uint32_t n = blockIdx.x * 16 + (threadIdx.x >> 4), row32 = (__umulhi(n, a.magic) + n) >> a.shift;
+  const long long row = row32;
+  const int block = (int)(n - row32 * (uint32_t)a.blocks), c = block * 128 + (threadIdx.x & 15) * 8;
+  const bool live = row < (a.total == nullptr ? a.rows : min(a.rows, *a.total)) && c < a.F;
   float y[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) y[j] = 0.f;
-  if (c < a.F) {
+  if (live) {
     float g[8], u[8];
     load8<TX>(a.x, row * a.ldx + c, g);
     load8<TX>(a.x, row * a.ldx + a.F + c, u);
@@ -187,20 +216,33 @@ __global__ void __launch_bounds__(256) swiglu_fp8_kernel(const __grid_constant__
   }
   float scale;
   const uint2 b = to_e4m3(y, scale);
-  if (c < a.F) {
+  if (live) {
     *reinterpret_cast<uint2*>(a.q + row * a.ldq + c) = b;
     if ((threadIdx.x & 15) == 0) a.s[(long long)block * a.lds + row] = scale;
   }
 }
 
+template <int TX, int TH, int MODE, int NV, int THREADS, int CTAS>
+static int launch_norm_as(const NormArgs& a, cudaStream_t st) {
+  if (THREADS == 0) return (int)rx::launch(add_norm_fp8_kernel<TX, TH, MODE, NV, THREADS, CTAS>, dim3((a.rows + 7) / 8), dim3(256), 0, st, a);
+  const int threads = ((a.d / 8 + NV - 1) / NV + 31) / 32 * 32;
+  return (int)rx::launch(add_norm_fp8_kernel<TX, TH, MODE, NV, THREADS, CTAS>, dim3(a.rows), dim3(threads), 0, st, a);
+}
+template <int TX, int TH, int MODE>
+static int launch_norm_mode(const NormArgs& a, cudaStream_t st) {
+  if (a.d <= 256) return launch_norm_as<TX, TH, MODE, 1, 0, 1>(a, st);
+  if (a.d <= 512) return launch_norm_as<TX, TH, MODE, 2, 0, 1>(a, st);
+  if (a.d <= 1024 && a.rows > 148) return launch_norm_as<TX, TH, MODE, 4, 0, 1>(a, st);
+  if (a.d > 16384) return launch_norm_as<TX, TH, MODE, 4, 1024, 1>(a, st);
+  if (a.d > 8192) return launch_norm_as<TX, TH, MODE, 2, 1024, 1>(a, st);
+  if (a.rows > 1500) return launch_norm_as<TX, TH, MODE, 2, 512, MODE == NORM_EXPERTS ? 2 : 3>(a, st);
+  return launch_norm_as<TX, TH, MODE, 1, 1024, 1>(a, st);
+}
 template <int TX, int TH>
 static int launch_norm(const NormArgs& a, cudaStream_t st) {
-  const int vecs = a.d / 8;
-  const int nv = vecs <= 1024 ? 1 : vecs <= 2048 ? 2 : 4;
-  const int threads = ((vecs + nv - 1) / nv + 31) / 32 * 32;
-  if (nv == 1) return (int)rx::launch(add_norm_fp8_kernel<TX, TH, 1>, dim3(a.rows), dim3(threads), 0, st, a);
-  if (nv == 2) return (int)rx::launch(add_norm_fp8_kernel<TX, TH, 2>, dim3(a.rows), dim3(threads), 0, st, a);
-  return (int)rx::launch(add_norm_fp8_kernel<TX, TH, 4>, dim3(a.rows), dim3(threads), 0, st, a);
+  if (a.x == nullptr) return launch_norm_mode<F8R_BF16, TH, NORM_FIRST>(a, st);
+  if (a.weights == nullptr) return launch_norm_mode<TX, TH, NORM_ADD>(a, st);
+  return launch_norm_mode<TX, TH, NORM_EXPERTS>(a, st);
 }
 
 }  // namespace rx
@@ -216,7 +258,7 @@ RX_API int rx_add_norm_fp8(const void* x, int x_type, long long ldx, const void*
   if (x != nullptr && ldx < (long long)terms * d || ldh < d || ldq < d || lds < rows || (xn != nullptr && ldn < d)) return (int)cudaErrorInvalidValue;
   if (((uintptr_t)x | (uintptr_t)h | (uintptr_t)q | (uintptr_t)xn | (uintptr_t)norm_w) & 15) return (int)cudaErrorMisalignedAddress;
   if (ldx * (x_type == F8R_F32 ? 4 : 2) % 16 || ldh * (h_type == F8R_F32 ? 4 : 2) % 16 || ldq % 16 || (xn != nullptr && ldn % 8)) return (int)cudaErrorMisalignedAddress;
-  const NormArgs a = {x, (const float*)weights, h, (const uint16_t*)norm_w, (uint8_t*)q, (float*)s, (uint16_t*)xn, ldx, ldh, ldq, lds, ldn, eps, rows, terms, d};
+  const NormArgs a = {x, (const float*)weights, h, (const uint16_t*)norm_w, (uint8_t*)q, (float*)s, (uint16_t*)xn, ldx, ldh, ldq, lds, ldn, eps, 1.f / (float)d, rows, terms, d};
   cudaStream_t st = (cudaStream_t)stream;
   if (h_type == F8R_BF16) {
     if (x_type == F8R_BF16) return launch_norm<F8R_BF16, F8R_BF16>(a, st);
@@ -234,8 +276,12 @@ RX_API int rx_swiglu_fp8(const void* x, int x_type, long long ldx, void* q, long
   if (ldx < 2ll * F || ldq < F || lds < rows) return (int)cudaErrorInvalidValue;
   if (((uintptr_t)x | (uintptr_t)q) & 15 || ldx * (x_type == F8R_F32 ? 4 : 2) % 16 || ldq % 16) return (int)cudaErrorMisalignedAddress;
   const int blocks = (F + 127) / 128;
-  const SwigluArgs a = {x, (const int*)total, (uint8_t*)q, (float*)s, ldx, ldq, lds, rows, F, blocks};
-  const dim3 grid(rows, (blocks + 15) / 16), threads(256);
+  if ((long long)rows * blocks > 0x7FFFFFF0ll) return (int)cudaErrorInvalidValue;
+  uint32_t shift = 0;
+  while ((1u << shift) < (uint32_t)blocks) ++shift;
+  const uint32_t magic = (uint32_t)((((1ull << shift) - blocks) << 32) / blocks + 1);
+  const SwigluArgs a = {x, (const int*)total, (uint8_t*)q, (float*)s, ldx, ldq, lds, rows, F, blocks, magic, shift};
+  const dim3 grid((uint32_t)(((long long)rows * blocks + 15) / 16)), threads(256);
   cudaStream_t st = (cudaStream_t)stream;
   if (x_type == F8R_BF16) return (int)rx::launch(swiglu_fp8_kernel<F8R_BF16>, grid, threads, 0, st, a);
   if (x_type == F8R_F16) return (int)rx::launch(swiglu_fp8_kernel<F8R_F16>, grid, threads, 0, st, a);

@@ -583,6 +583,8 @@ def fp8_rows(rows: int, width: int, device="cuda") -> tuple:
 
 def _rows2(t, name: str, dtypes, rows, width: int, device: int) -> tuple:
     """The pointer of rows of `width` values side by side, and how far apart the rows are"""
+    if t.__class__ is _Tensor and t.dtype in dtypes and t.shape == (rows, width) and t.get_device() == device and t.is_contiguous():
+        return t.data_ptr(), width
     if not isinstance(t, _Tensor) or not t.is_cuda:
         raise ValueError(f"{name}: a CUDA tensor is needed")
     if t.get_device() != device:
