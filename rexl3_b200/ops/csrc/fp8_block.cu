@@ -65,26 +65,6 @@ __device__ __forceinline__ bool fb_wait(uint64_t* bar, uint32_t parity, volatile
       : "memory");
   return ok != 0;
 }
-// ... for two barriers at once: both are asked before either answers
-__device__ __forceinline__ bool fb_wait_both(uint64_t* x, uint32_t x_parity, uint64_t* y, uint32_t y_parity, volatile int* abort_flag) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p, q, r;\n\t.reg .u32 f;\n\t"
-      "POLL:\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 r, [%3], %4;\n\t"
-      "and.pred p, p, r;\n\t"
-      "@p bra OVER;\n\t"
-      "ld.volatile.shared.u32 f, [%5];\n\t"
-      "setp.eq.u32 q, f, 0;\n\t"
-      "@q bra POLL;\n\t"
-      "OVER:\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(x)), "r"(x_parity), "r"(smem_u32(y)), "r"(y_parity), "r"(smem_u32((const void*)abort_flag))
-      : "memory");
-  return ok != 0;
-}
 // One thread of the CTA, until `drained` (its last phase's end): puts the abort flag up when the host does, or when the copies have not come on for as long as a wait may last.
 __device__ __forceinline__ void fb_watch(uint64_t* drained, const volatile int* progress, volatile int* abort_flag, int* status, int site) {
   const uint64_t limit = wait_limit_ns(status);
@@ -506,7 +486,8 @@ struct FbWide {
   static constexpr int A = 128 * FB_K, B = 256 / CG * FB_K;
   static constexpr int STAGE = A + B, STAGES = CG == 2 ? 6 : 4;
   static constexpr int SG = 8, SC = 2;             // blocks of scales that are fetched and given back together; that many times
-  static constexpr int SC_ROW = 132, SC_BUF = SG * SC_ROW;    // of a block: 128 rows', two strips'
+  static constexpr int SC_ROW = 132;               // of a block: 128 rows', two strips'
+  static constexpr int SC_BUF = SG * SC_ROW + 260; // and, with a tile's first blocks, what the sums know of it: where each row goes, its row of q, the column tile, its rows
   static constexpr int MAX_EXPERTS = 512;
   static constexpr int SMEM = 1024 + STAGES * STAGE + SC * SC_BUF * 4 + 512;
   static constexpr int SMEM_EXPERTS = SMEM + (MAX_EXPERTS + 1) * 4;
@@ -629,7 +610,7 @@ fp8_block_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::STAGES; ++i) { mbar_init(&full[i], EXPERTS && a.src != nullptr ? 2 : 1); mbar_init(&empty[i], 1); }
     for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], CG * L::EW); }
-    for (int i = 0; i < L::SC; ++i) { mbar_init(&sc_full[i], 32); mbar_init(&sc_empty[i], L::EW); }
+    for (int i = 0; i < L::SC; ++i) { mbar_init(&sc_full[i], 32 + 1); mbar_init(&sc_empty[i], L::EW); }   // the scales' copies, the tile's rows
     mbar_init(drained, 1);
     *abort_flag = 0;
     *n_sent = 0;
@@ -786,7 +767,7 @@ fp8_block_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
         bool ok = true;
         for (int t = unit; t < tiles && ok; t += units)
           for (int b = 0; b < nb; ++b, ++it) {
-            ok = fb_wait_both(&full[s], phase, &acc_empty[buf], acc_phase, abort_flag);
+            ok = fb_wait(&full[s], phase, abort_flag) && fb_wait(&acc_empty[buf], acc_phase, abort_flag);
             if (!ok) break;
             tc_fence_after();
             const uint32_t ad = (uint32_t)desc0 + s * (L::STAGE >> 4);
@@ -803,7 +784,8 @@ fp8_block_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
     } else if (warp == 11) {
       if (lane == 0) fb_watch(drained, n_sent, abort_flag, a.status, 190);
     } else if (warp == 10) {
-      // ---- scales: four rows a lane, and the tile's two strips'.  (Rows that the tile lacks: whatever stands there, their sums go nowhere.)
+      // ---- scales: four rows a lane, and the tile's two strips'.  (Rows that the tile lacks: whatever stands there, their sums go nowhere.)  And the tile's rows: the sums
+      // would wait for their numbers with nothing else to do.
       int at = 0, it = 0;
       uint32_t phase = 1;
       bool ok = true;
@@ -812,14 +794,28 @@ fp8_block_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
         const FbTile f = tile_of(t);
         const int mine = min(128, f.rows - 128 * half), row0 = f.row0 + 128 * half;
         const float* from[4];
+        int in[4], out[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          int r = 32 * j + lane < mine ? row0 + 32 * j + lane : -1;
-          if (EXPERTS && a.src != nullptr && r >= 0) {
-            const int p = a.src[r];
-            r = p < 0 ? -1 : p / a.src_div;
+          const int n = 32 * j + lane;
+          int r = n < mine ? row0 + n : -1, o = r;
+          if (EXPERTS && r >= 0) {
+            if (a.src != nullptr) {
+              const int p = a.src[r];
+              r = p < 0 ? -1 : p / a.src_div;
+            }
+            if (a.dst != nullptr) o = a.dst[o];
+            if (r < 0 || r >= a.rows) {
+              set_status(a.status, ST_BAD_ARG, 181, r);
+              r = -1;
+            }
+            if (o < 0 || o >= a.out_rows) {
+              set_status(a.status, ST_BAD_ARG, 182, o);
+              o = -1;
+            }
           }
-          from[j] = r < 0 || r >= a.rows ? nullptr : a.s + (long long)b0 * a.lds + r;
+          in[j] = r, out[j] = o;
+          from[j] = r < 0 ? nullptr : a.s + (long long)b0 * a.lds + r;
         }
         const float* ws = a.ws + ((long long)f.expert * strips + 2 * f.ct + lane) * a.kblocks + b0;
         const bool strip = lane < 2 && 2 * f.ct + lane < strips;
@@ -828,6 +824,14 @@ fp8_block_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
             ok = false;
             break;
           }
+          if (b0g == 0) {
+            int* tile = (int*)(scales + at * L::SC_BUF + L::SG * L::SC_ROW);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) tile[32 * j + lane] = out[j], tile[128 + 32 * j + lane] = in[j];
+            if (lane == 0) tile[256] = f.ct, tile[257] = mine;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sc_full[at]);
           const uint32_t slot = smem_u32(scales + at * L::SC_BUF + lane);
           for (int b = b0g; b < min(b0g + L::SG, nb); ++b) {
             const uint32_t to = slot + (b - b0g) * L::SC_ROW * 4;
@@ -852,32 +856,15 @@ fp8_block_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
     uint32_t acc_phase = 0, sc_phase = 0;
     bool ok = true;
     for (int t = unit; t < tiles && ok; t += units) {
-      const FbTile f = tile_of(t);
-      const int mine = min(128, f.rows - 128 * half);
-      int r = -1, o = -1;
-      if (at_row < mine) {
-        r = o = f.row0 + 128 * half + at_row;
-        if (EXPERTS) {
-          if (a.src != nullptr) {
-            const int p = a.src[r];
-            r = p < 0 ? -1 : p / a.src_div;
-          }
-          if (a.dst != nullptr) o = a.dst[o];
-          if (r < 0 || r >= a.rows) {
-            set_status(a.status, ST_BAD_ARG, 181, r);
-            r = -1;
-          }
-          if (o < 0 || o >= a.out_rows) {
-            set_status(a.status, ST_BAD_ARG, 182, o);
-            o = -1;
-          }
-        }
-      }
+      ok = fb_wait_warp(&sc_full[at], sc_phase, abort_flag);
+      if (!ok) break;
+      const int* tile = (const int*)(scales + at * L::SC_BUF + L::SG * L::SC_ROW);
+      const int o = tile[at_row], r = tile[128 + at_row], ct = tile[256], mine = tile[257];
       float acc[128];
 #pragma unroll
       for (int j = 0; j < 128; ++j) acc[j] = 0.f;
       for (int b = 0; b < nb; ++b) {
-        if (b % L::SG == 0) {
+        if (b % L::SG == 0 && b > 0) {
           ok = fb_wait_warp(&sc_full[at], sc_phase, abort_flag);
           if (!ok) break;
         }
@@ -906,7 +893,7 @@ fp8_block_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
         }
       }
       if (!ok) break;
-      const int n = f.ct * 256 + 128 * side;
+      const int n = ct * 256 + 128 * side;
       if (wa.parts == 1) {
         if (o >= 0 && n < a.N) fb_store_row(a, o, n, acc, r < 0, wa.vec);
       } else {

@@ -5,7 +5,7 @@
 //   both         s = max(max|y|, 2^-100) / 448 over a row's block,  q = e4m3(y / s):  q [rows][d] bytes, s [blocks][rows]
 //
 // All steps are float32; y is formed of the sum before that is rounded to h's type, and is rounded once, to its byte.  A thread holds eight neighbouring columns,
-// so a block is 16 lanes: its largest magnitude is four shuffles.  Magnitudes are compared as integers: a NaN is above infinity, reaches the scale and so the block.
+// so a block is 16 lanes: its largest magnitude is four shuffles, by maxima that keep a NaN, which so reaches the scale and the block.
 // Scales stand block by block, rows side by side: the products read one block's scales of many rows at once, and a warp of them is one line.
 #include <cuda_fp8.h>
 #include "common.cuh"
@@ -14,14 +14,15 @@ namespace rx {
 
 enum : int { F8R_BF16 = 0, F8R_F16 = 1, F8R_F32 = 2 };
 
-// eight values from 16 (32) bytes at p + i
-template <int T>
+// eight values from 16 (32) bytes at p + i; STREAM: they will not be read again
+template <int T, bool STREAM = false>
 __device__ __forceinline__ void load8(const void* p, size_t i, float (&v)[8]) {
   if constexpr (T == F8R_F32) {
     const float4 a = *reinterpret_cast<const float4*>((const float*)p + i), b = *reinterpret_cast<const float4*>((const float*)p + i + 4);
     v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
   } else {
-    const uint4 a = *reinterpret_cast<const uint4*>((const uint16_t*)p + i);
+    const uint4* from = reinterpret_cast<const uint4*>((const uint16_t*)p + i);
+    const uint4 a = STREAM ? __ldcs(from) : *from;
     const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -53,19 +54,29 @@ __device__ __forceinline__ void store8(void* p, size_t i, const float (&v)[8]) {
   }
 }
 
+__device__ __forceinline__ float max_nan(float a, float b) {         // NaN if either is
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
+__device__ __forceinline__ float silu_mul(float g, float u) {        // g u / (1 + e^-g)
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + __expf(-g)));
+  return g * r * u;
+}
 // The bytes of a thread's eight columns and, in `scale`, their block's scale.  The 16 lanes of a block call together (with zeros where the row has ended).
 __device__ __forceinline__ uint2 to_e4m3(const float (&y)[8], float& scale) {
-  int m = 0;
+  float m = 7.888609052210118e-31f;                                // 2^-100: 1 / scale stays finite
 #pragma unroll
-  for (int j = 0; j < 8; ++j) m = max(m, __float_as_int(y[j]) & 0x7FFFFFFF);
+  for (int j = 0; j < 8; ++j) m = max_nan(m, fabsf(y[j]));
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const float amax = __int_as_float(max(m, 0x0D800000));           // 2^-100: 1 / scale stays finite
+  for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
   constexpr float R = 1.f / 448.f;                                 // (a quotient by it, corrected by its remainder: as a division rounds)
-  scale = amax * R;
-  scale = fmaf(fmaf(-448.f, scale, amax), R, scale);
-  scale = m >= 0x7F800000 ? amax : scale;                          // infinity, NaN: the remainder would be NaN
-  const float inv = __frcp_rn(scale);
+  scale = m * R;
+  scale = fmaf(fmaf(-448.f, scale, m), R, scale);
+  scale = m < __int_as_float(0x7F800000) ? scale : m;              // infinity, NaN: the remainder would be NaN
+  float inv;                                                       // (within a step: of 448, the largest byte, what comes out above saturates)
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));
   uint32_t w[2];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
@@ -137,7 +148,7 @@ __global__ void __launch_bounds__(THREADS ? THREADS : 256, CTAS) add_norm_fp8_ke
         for (int k = 0; k < AT_ONCE; ++k) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) x[k][j] = 0.f;
-          if (w[k] != 0.f) load8<TX>(a.x, row * a.ldx + (long long)(k0 + k) * a.d + c, x[k]);
+          if (w[k] != 0.f) load8<TX, true>(a.x, row * a.ldx + (long long)(k0 + k) * a.d + c, x[k]);
         }
 #pragma unroll
         for (int k = 0; k < AT_ONCE; ++k)
@@ -212,7 +223,7 @@ __global__ void __launch_bounds__(256) swiglu_fp8_kernel(const __grid_constant__
     load8<TX>(a.x, row * a.ldx + c, g);
     load8<TX>(a.x, row * a.ldx + a.F + c, u);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = __fdividef(g[j], 1.f + __expf(-g[j])) * u[j];
+    for (int j = 0; j < 8; ++j) y[j] = silu_mul(g[j], u[j]);
   }
   float scale;
   const uint2 b = to_e4m3(y, scale);
