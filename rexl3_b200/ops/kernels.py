@@ -663,6 +663,8 @@ def swiglu_fp8(x: torch.Tensor, q: torch.Tensor, s: torch.Tensor, *, total: "tor
     if x.dim() != 2 or x.shape[1] % 32 or not 32 <= x.shape[1] <= 1 << 21:
         raise ValueError(f"x: [rows, 2 * ffn] with ffn a multiple of 16, 16 .. 2^20, not {list(x.shape)}")
     rows, F = x.shape[0], x.shape[1] // 2
+    if rows * ((F + 127) // 128) > 0x7FFFFFF0:
+        raise ValueError(f"{rows} rows of {F}: up to 2^31 - 16 blocks")
     p_x, ldx = _rows2(x, "x", tuple(_FLOATS), rows, 2 * F, dev)
     p_q, ldq = _rows2(q, "q", (_E4M3, _U8), rows, F, dev)
     p_s, lds = _scales(s, "s", rows, F, dev)

@@ -75,3 +75,12 @@ def test_entry_points_refuse_what_does_not_fit():
     exp = dict(q=p, ldq=256, s=p, lds=4, rows=4, K=256, w=p, ws=p, experts=2, N=128, offs=p, src=None, src_div=1, dst=None, cap=4, out=p, out_type=0, ldo=128, out_rows=4, status=p, stream=None)
     for bad in (*common, dict(experts=0), dict(experts=5000), dict(offs=None), dict(cap=0), dict(cap=5), dict(cap=5, src=p), dict(cap=5, dst=p), dict(src_div=0), dict(out_rows=0), dict(out_rows=3)):
         assert lib.rx_fp8_block_experts(*{**exp, **bad}.values()) != 0, bad
+
+
+def test_entry_points_refuse_what_their_numbers_cannot_hold():
+    lib, p, many = L.load(), 4096, (1 << 30) + 1
+    assert lib.rx_add_norm_fp8(p, 0, 16, None, 1, p, 0, 16, p, 1e-6, p, 16, p, many, None, 0, many, 16, None) != 0
+    assert lib.rx_swiglu_fp8(p, 0, 1 << 21, p, 1 << 20, p, 1 << 18, None, 1 << 18, 1 << 20, None) != 0        # 2^31 blocks
+    assert lib.rx_fp8_block_linear(p, 16, p, many, many, 16, p, p, None, 16, p, 0, 16, p, None) != 0
+    for rows, cap, experts, N, ldq in ((many, 4, 1, 16, 16), (4, many, 1, 16, 16), (4, 4, 4096, 1 << 20, 16), (1 << 20, 4, 1, 16, 1 << 17)):
+        assert lib.rx_fp8_block_experts(p, ldq, p, rows, rows, 16, p, p, experts, N, p, p, 1, p, cap, p, 0, N, 4, p, None) != 0, (rows, cap, experts, N, ldq)

@@ -179,6 +179,18 @@ def test_bad_gates_read_as_nan():
     assert bool(torch.isnan(got[1]).all()) and bool(torch.isfinite(got[0]).all())
 
 
+def test_small_gates_of_large_values():
+    """1 / (1 + e^90) is below the normal numbers of float32 (there in steps of 2^-149, 2^-19 of it), but a value of 2^120 brings it back."""
+    x = torch.zeros(2, 256, device="cuda")
+    x[0, :3], x[0, 128:] = torch.tensor([-88.0, -87.5, -80.0]), 2.0 ** 120
+    x[1, 0], x[1, 128:] = -90.0, 2.0 ** 120
+    q, s = K.fp8_rows(2, 128)
+    K.swiglu_fp8(x, q, s)
+    g = x[:, :128].double()
+    y = g * torch.sigmoid(g) * x[:, 128:].double()
+    check_rows(q.view(torch.uint8), s, y, y.abs() * ((12 + 2 * 90) * 2 * U + 2.0 ** -19))
+
+
 def test_no_rows_and_captured_calls():
     K.add_norm_fp8(None, torch.zeros(0, 128, device="cuda"), None, 1e-6, *K.fp8_rows(0, 128))
     K.swiglu_fp8(torch.zeros(0, 256, device="cuda"), *K.fp8_rows(0, 128))
