@@ -162,6 +162,39 @@ __device__ __forceinline__ void fb_store(const FbArgs& a, long long row, int n, 
   else ((float*)a.out)[i] = v;
 }
 
+// A warp counts the experts' tiles of ROWS rows up, four experts a lane (their offsets arrive together): each(expert, tiles before its, its tiles, its positions) of those
+// that there are; all tiles.  An expert whose offsets descend or leave the positions has none.
+template <int ROWS, typename F>
+__device__ __forceinline__ int fb_count_tiles(const FbArgs& a, int lane, F&& each) {
+  int before = 0;
+  for (int e0 = 0; e0 < a.experts; e0 += 128) {
+    int o[5], tiles[4], mine = 0;
+#pragma unroll
+    for (int u = 0; u < 5; ++u) o[u] = a.offs[min(e0 + 4 * lane + u, a.experts)];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const bool good = o[u] >= 0 && o[u + 1] >= o[u] && o[u + 1] <= a.cap;
+      if (!good && e0 + 4 * lane + u < a.experts) set_status(a.status, ST_BAD_ARG, 180, e0 + 4 * lane + u);
+      tiles[u] = good ? (o[u + 1] - o[u] + ROWS - 1) / ROWS : 0;
+      mine += tiles[u];
+    }
+    int sum = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += v;
+    }
+    int at = before + sum - mine;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (e0 + 4 * lane + u < a.experts) each(e0 + 4 * lane + u, at, tiles[u], o[u], o[u + 1]);
+      at += tiles[u];
+    }
+    before += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return before;
+}
+
 // Few rows.  The weights are the M side: a CTA has a strip of 128 output columns (TMEM lanes) and T rows (TMEM columns), and the CTAs of a cluster share the
 // strip's blocks of k; their sums are added in the order of the CTAs through distributed shared memory.
 template <int T>
@@ -223,27 +256,11 @@ fp8_block_step_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
   if (EXPERTS) {
     pdl_wait();                                    // the plan comes from a kernel before
     if (warp == 0) {
-      // the expert whose rows hold the row_tile-th tile: experts' tiles counted up, 32 experts a step
-      int before = 0, e = -1, pos = 0, n = 0;
-      for (int e0 = 0; e0 < a.experts; e0 += 32) {
-        const int i = e0 + lane;
-        int lo = i < a.experts ? a.offs[i] : 0, hi = i < a.experts ? a.offs[i + 1] : 0;
-        if (lo < 0 || hi < lo || hi > a.cap) {
-          set_status(a.status, ST_BAD_ARG, 180, i);
-          lo = hi = 0;
-        }
-        const int tiles = (hi - lo + T - 1) / T;
-        int sum = tiles;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int u = __shfl_up_sync(0xffffffffu, sum, o);
-          if (lane >= o) sum += u;
-        }
-        const int at = row_tile - before - (sum - tiles);         // which of the expert's tiles
+      int e = -1, pos = 0, n = 0;                  // the expert whose rows hold the row_tile-th tile
+      fb_count_tiles<T>(a, lane, [&](int i, int before, int tiles, int lo, int hi) {
+        const int at = row_tile - before;
         if (at >= 0 && at < tiles) e = i, pos = lo + at * T, n = min(T, hi - pos);
-        before += __shfl_sync(0xffffffffu, sum, 31);
-        if (before > row_tile) break;
-      }
+      });
       const unsigned found = __ballot_sync(0xffffffffu, e >= 0);
       const int who = found ? __ffs(found) - 1 : 0;
       e = __shfl_sync(0xffffffffu, e, who), pos = __shfl_sync(0xffffffffu, pos, who), n = __shfl_sync(0xffffffffu, n, who);
@@ -488,7 +505,7 @@ struct FbWide {
   static constexpr int SG = 8, SC = 2;             // blocks of scales that are fetched and given back together; that many times
   static constexpr int SC_ROW = 132;               // of a block: 128 rows', two strips'
   static constexpr int SC_BUF = SG * SC_ROW + 260; // and, with a tile's first blocks, what the sums know of it: where each row goes, its row of q, the column tile, its rows
-  static constexpr int MAX_EXPERTS = 512;
+  static constexpr int MAX_EXPERTS = 4096;
   static constexpr int SMEM = 1024 + STAGES * STAGE + SC * SC_BUF * 4 + 512;
   static constexpr int SMEM_EXPERTS = SMEM + (MAX_EXPERTS + 1) * 4;
 };
@@ -597,7 +614,7 @@ fp8_block_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
   uint32_t* tmem_slot = (uint32_t*)(drained + 1);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
   volatile int* n_sent = (volatile int*)(tmem_slot + 2);          // stages that this CTA's copies were issued for
-  int* sent = (int*)(tmem_slot + 3);                              // [STAGES] their bytes
+  int* sent = (int*)(tmem_slot + 3);                              // [STAGES] the bytes that the pair's second CTA copies for them
   int* first = (int*)(smem + L::SMEM - 1024);                     // experts: row tiles before each expert's
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t rank = 0;
@@ -629,25 +646,8 @@ fp8_block_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
   }
   pdl_wait();
   if (EXPERTS && warp == 0) {
-    int before = 0;
-    for (int e0 = 0; e0 < a.experts; e0 += 32) {
-      const int i = e0 + lane;
-      int lo = i < a.experts ? a.offs[i] : 0, hi = i < a.experts ? a.offs[i + 1] : 0;
-      if (lo < 0 || hi < lo || hi > a.cap) {
-        set_status(a.status, ST_BAD_ARG, 180, i);
-        lo = hi = 0;
-      }
-      const int tiles = (hi - lo + ROWS - 1) / ROWS;
-      int sum = tiles;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += u;
-      }
-      if (i < a.experts) first[i] = before + sum - tiles;
-      before += __shfl_sync(0xffffffffu, sum, 31);
-    }
-    if (lane == 0) first[a.experts] = before;
+    const int all = fb_count_tiles<ROWS>(a, lane, [&](int i, int before, int, int, int) { first[i] = before; });
+    if (lane == 0) first[a.experts] = all;
   }
   tc_fence_before();
   __syncthreads();
@@ -715,7 +715,6 @@ fp8_block_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
             }
             uint8_t* st = smem + s * L::STAGE;
             if (elect_one()) {
-              sent[s] = L::B;
               *n_sent = it + 1;
               mbar_arrive_expect_tx(&full[s], L::B);
               fb_load<CG>(st + L::A, &tmap_w, (b0 + b) * FB_K, wrow, smem_u32(&full[s]));
@@ -744,7 +743,7 @@ fp8_block_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
             uint8_t* st = smem + s * L::STAGE;
             const uint32_t bar = CG == 2 ? mapa_u32(smem_u32(&full[s]), lead) : smem_u32(&full[s]);
             if (elect_one()) {
-              sent[s] = (int)bytes;
+              if (CG == 2) sent[s] = (int)(half == 0 ? both - bytes : bytes);
               *n_sent = it + 1;
               if (half == 0) mbar_arrive_expect_tx(&full[s], both);
               if (mine > 0) fb_load<CG>(st, &tmap_x, (b0 + b) * FB_K, row0, bar);
@@ -1106,7 +1105,7 @@ static void fb_consider_wide(int dev, const FbArgs& a, FbChoice& best) {
 }
 
 static int fb_check(const void* q, long long ldq, const FbArgs& a, const void* w) {
-  if (a.rows < 1 || a.K < 16 || a.K % 16 != 0 || a.K > (1 << 24) || a.N < 1 || a.N > (1 << 22) || ldq < a.K || a.lds < a.rows || a.ldo < a.N) return (int)cudaErrorInvalidValue;
+  if (a.rows < 1 || a.rows > (1 << 30) || a.K < 16 || a.K % 16 != 0 || a.K > (1 << 24) || a.N < 1 || a.N > (1 << 22) || ldq < a.K || a.lds < a.rows || a.ldo < a.N) return (int)cudaErrorInvalidValue;
   if (q == nullptr || w == nullptr || a.s == nullptr || a.ws == nullptr || a.out == nullptr || a.out_type < 0 || a.out_type > 2) return (int)cudaErrorInvalidValue;
   if (((uintptr_t)q | (uintptr_t)w) & 15 || ldq % 16 || ((uintptr_t)a.s | (uintptr_t)a.ws | (uintptr_t)a.bias) & 3 ||
       (uintptr_t)a.out & (a.out_type == FB_F32 ? 3 : 1))
@@ -1156,14 +1155,13 @@ RX_API int rx_fp8_block_experts(const void* q, long long ldq, const void* s, lon
   a.lds = lds, a.ldo = ldo, a.rows = rows, a.K = K, a.N = N, a.kblocks = (K + 127) / 128, a.out_type = out_type, a.experts = experts, a.cap = cap;
   a.src_div = src_div, a.out_rows = out_rows;
   if (const int e = fb_check(q, ldq, a, w)) return e;
-  if (experts < 1 || experts > 4096 || (long long)experts * N > (1ll << 31) - 128 || cap < 1 || src_div < 1 || out_rows < 1 || offs == nullptr) return (int)cudaErrorInvalidValue;
+  if (experts < 1 || experts > FbWide<1>::MAX_EXPERTS || (long long)experts * N > (1ll << 31) - 128 || cap < 1 || cap > (1 << 30) || src_div < 1 || out_rows < 1 || offs == nullptr) return (int)cudaErrorInvalidValue;
   if ((src == nullptr && cap > rows) || (dst == nullptr && cap > out_rows)) return (int)cudaErrorInvalidValue;
   if (src != nullptr && (long long)rows * (ldq / 16) > 0xFFFFFFFFll) return (int)cudaErrorInvalidValue;      // a row's place is held in 32 bits, of 16 bytes
   cudaStream_t st = (cudaStream_t)stream;
   // Up to six positions an expert: tiles of 16 rows, whose CTAs begin sooner (8 of 128 experts, a row each 10 us and 17, 800 positions 65 and 67; 2000 positions 88 and 70).
-  if (experts <= FbWide<1>::MAX_EXPERTS && cap > 6 * experts) return fb_launch_wide<1, true>(q, ldq, w, a, 1, st);
+  if (cap > 6 * experts) return fb_launch_wide<1, true>(q, ldq, w, a, 1, st);
   const int some = experts < cap ? experts : cap;
   const long long row_tiles = ((long long)cap + (long long)some * 15) / 16;          // the most tiles that `cap` rows of `some` experts can make
-  if (row_tiles > 65535) return (int)cudaErrorInvalidValue;
   return fb_launch_step<16, true>(q, ldq, w, a, (int)row_tiles, 1, st);
 }

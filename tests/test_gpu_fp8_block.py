@@ -1,4 +1,8 @@
 """Products of E4M3 rows and weights under scales for blocks of 128, dense and through routed experts, against the formula in 64 bits."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -358,3 +362,142 @@ def test_refusals():
               dict(out=out[:3]), dict(src=idx[None]), dict(dst=idx.cpu())):
         with pytest.raises(ValueError):
             K.fp8_block_experts(**{**ok, **b})
+
+
+# ------------------------------------------------------------------------------------------------ what else a call may meet
+@pytest.mark.parametrize("first", [1, 2])
+@pytest.mark.parametrize("rows,picks", [(5000, 2), (13000, 2)])
+def test_as_many_experts_as_there_may_be(rows, picks, first):
+    g = gen(rows)
+    w, status = weight_of(16 * first, 16, g, experts=4096), K.new_status()
+    q, s = rows_of(rows, 16 * first, g)
+    ids = torch.randint(0, 4096, (rows * picks,), device="cuda", generator=g)
+    pairs = torch.sort(ids, stable=True).indices.int()
+    offs = torch.cat([ids.new_zeros(1), torch.bincount(ids, minlength=4096).cumsum(0)]).int()
+    before = torch.full((rows * picks, 16), 7.0, device="cuda")
+    out = before.clone()
+    K.fp8_block_experts(q, s, w, offs, out, status, src=pairs, src_div=picks)
+    K.check_status(status)
+    check_experts(q, s, w, offs, out, before, src=pairs, div=picks)
+
+
+@pytest.mark.parametrize("rows,picks", [(9, 2), (70, 3)])
+def test_experts_with_rows_and_places_of_their_own(rows, picks):
+    """src and dst in one call, rows of q and out and blocks of s further apart than they need be."""
+    g = gen(rows)
+    _, offs, pairs = plan(rows, picks, 4, 3, g)
+    P = rows * picks
+    w, status = weight_of(400, 264, g, experts=3), K.new_status()
+    q, s = rows_of(rows, 400, g)
+    qq, ss = torch.full((rows, 448), 0x7F, dtype=torch.uint8, device="cuda"), torch.full((4, rows + 5), float("nan"), device="cuda")
+    qq[:, :400], ss[:, :rows] = q.view(torch.uint8), s
+    dst = torch.randperm(P + 4, device="cuda", generator=g)[:P].int()
+    for dtype in (BF16, F16, F32):
+        room = torch.full((P + 4, 264 + 8), 7.0, device="cuda", dtype=dtype)
+        K.fp8_block_experts(qq[:, :400], ss[:, :rows], w, offs, room[:, :264], status, src=pairs, src_div=picks, dst=dst)
+        K.check_status(status)
+        assert bool((room[:, 264:] == 7).all())
+        check_experts(q, s, w, offs, room[:, :264], torch.full_like(room[:, :264], 7.0), src=pairs, div=picks, dst=dst)
+
+
+@pytest.mark.parametrize("o", [[0, 1, 0], [0] * 300 + [1, 0], [0] * 200 + [1] * 200 + [0]])
+def test_bad_offsets_behind_the_last_tile_set_the_status(o):
+    """One position: as many tiles as a call of that size is cut for, and the fault stands behind them."""
+    g = gen(6)
+    w, status = weight_of(128, 128, g, experts=len(o) - 1), K.new_status()
+    q, s = rows_of(1, 128, g)
+    out = torch.zeros(1, 128, device="cuda")
+    K.fp8_block_experts(q, s, w, torch.tensor(o, dtype=torch.int32, device="cuda"), out, status)
+    torch.cuda.synchronize()
+    assert int(status[0]) == K.ST_BAD_ARG
+
+
+@pytest.mark.parametrize("rows", [4, 150])
+def test_a_captured_call_follows_the_routing(rows):
+    """The offsets and pairs are read when the graph runs: two graphs side by side, with new routing before every replay."""
+    g = gen(rows)
+    w, jobs = weight_of(256, 136, g, experts=8), []
+    for _ in range(2):
+        q, s = rows_of(rows, 256, g)
+        _, offs, pairs = plan(rows, 3, 8, 8, g)
+        out, status, graph, stream = torch.zeros(rows * 3, 136, device="cuda"), K.new_status(), torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        K.fp8_block_experts(q, s, w, offs, out, status, src=pairs, src_div=3)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            K.fp8_block_experts(q, s, w, offs, out, status, src=pairs, src_div=3)
+        jobs.append((q, s, offs, pairs, out, status, graph, stream))
+    for held in (8, 2, 5):
+        for q, s, offs, pairs, out, status, graph, stream in jobs:
+            _, o, p = plan(rows, 3, 8, held, g)
+            offs.fill_(int(o[-1])), pairs.copy_(p), out.fill_(7.0)
+            offs[:held + 1] = o
+        torch.cuda.synchronize()
+        for *_, graph, stream in jobs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for q, s, offs, pairs, out, status, graph, stream in jobs:
+            K.check_status(status)
+            check_experts(q, s, w, offs, out, torch.full_like(out, 7.0), src=pairs, div=3)
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    code = """
+import torch
+from rexl3_b200.ops import kernels as K
+q = torch.ones(M, 256, device="cuda").to(torch.float8_e4m3fn)
+s, st, out = torch.ones(2, M, device="cuda"), K.new_status(), torch.zeros(M, 384, device="cuda")
+w = K.Fp8BlockWeight(torch.ones(384, 256, device="cuda").to(torch.float8_e4m3fn), torch.ones(3, 2, device="cuda"))
+we = K.Fp8BlockWeight(w.w[None], w.scales[None])
+offs, oe = torch.tensor([0, M], dtype=torch.int32, device="cuda"), torch.zeros(M, 384, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    K.fp8_block_linear(q, s, w, out, st)
+    K.fp8_block_experts(q, s, we, offs, oe, st)
+g.replay()
+torch.cuda.synchronize()
+K.check_status(st)
+assert bool((out == 256).all()) and bool((oe == 256).all())
+"""
+    for M in (3, 300):
+        subprocess.run([sys.executable, "-c", f"M = {M}\n" + code], check=True, timeout=300, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+
+
+def gives_up(call, like):
+    """`call(out, status)` under short limits and the abort word, with plain calls after each: it returns, says so if a wait gave up, and the next call is right."""
+    want, st = torch.full_like(like, float("nan")), K.new_status()
+    call(want, st)
+    K.check_status(st)
+    for us in ("abort", 1, 2, 5, 10, 20, 40, 100, "abort"):
+        st = K.new_status()
+        K.set_abort(st) if us == "abort" else K.set_wait_limit(st, us)
+        got = torch.full_like(like, float("nan"))
+        call(got, st)
+        code = st.tolist()[0]
+        assert code in (0, K.ST_ABORTED if us == "abort" else K.ST_TIMEOUT)
+        assert code != 0 or torch.equal(got, want)
+        for _ in range(2):
+            st, got = K.new_status(), torch.full_like(like, float("nan"))
+            call(got, st)
+            K.check_status(st)
+            assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("M,Kd,N", [(1, 16384, 256), (24, 8192, 512), (64, 8192, 4096), (40, 2048, 20000), (333, 7168, 2112), (1000, 2048, 1000), (2404, 8192, 4096), (4000, 512, 8192)])
+def test_waits_that_give_up(M, Kd, N):
+    g = gen(M)
+    q, s = rows_of(M, Kd, g)
+    w = weight_of(Kd, N, g)
+    gives_up(lambda out, st: K.fp8_block_linear(q, s, w, out, st), torch.zeros(M, N, device="cuda"))
+
+
+@pytest.mark.parametrize("rows,picks,experts", [(16, 2, 32), (700, 4, 32)])
+def test_experts_waits_that_give_up(rows, picks, experts):
+    g = gen(rows)
+    _, offs, pairs = plan(rows, picks, experts, experts, g)
+    w = weight_of(2048, 512, g, experts=experts)
+    q, s = rows_of(rows, 2048, g)
+    gives_up(lambda out, st: K.fp8_block_experts(q, s, w, offs, out, st, src=pairs, src_div=picks), torch.zeros(rows * picks, 512, device="cuda"))
+    q, s = rows_of(rows * picks, 2048, g)
+    gives_up(lambda out, st: K.fp8_block_experts(q, s, w, offs, out, st, dst=pairs), torch.zeros(rows * picks, 512, device="cuda"))
