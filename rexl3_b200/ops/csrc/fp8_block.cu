@@ -541,60 +541,81 @@ __device__ __forceinline__ void fb_load(void* dst, const void* tmap, int x, int 
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)), "l"(tmap), "r"(bar), "r"(x), "r"(y)
                  : "memory");
 }
-// neighbouring columns of a row from n on, `vec` bytes (32, 16 or 0: one by one) a store
+// Neighbouring columns of a row from n on.  A thread has a row, so value by value a warp would send 32 sectors for 64 bytes (200 x 4096 -> 2867: 24 us): WIDE, 32 bytes a store where every
+// row begins on such a boundary; otherwise 16 bytes from the row's first 16-byte boundary on, shifted into place by selects, and what lies before it and behind the last one by itself.
 template <int COLS>
-__device__ __forceinline__ void fb_store_row(const FbArgs& a, long long row, int n, float (&acc)[COLS], bool zero, int vec) {
+__device__ __forceinline__ void fb_store_row(const FbArgs& a, long long row, int n, float (&acc)[COLS], bool zero, bool wide) {
   if (zero)
 #pragma unroll
     for (int j = 0; j < COLS; ++j) acc[j] = 0.f;
+  const int left = min(COLS, a.N - n);
+  if (a.bias != nullptr) {
+    const float* bias = a.bias + n;
 #pragma unroll
-  for (int c = 0; c < COLS; c += 16) {
-    float v[16];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = acc[c + j];
-    if (a.bias != nullptr)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) v[j] += n + c + j < a.N ? __ldg(a.bias + n + c + j) : 0.f;
-    const long long i = row * a.ldo + n + c;
-    if (vec == 0 || n + c + 16 > a.N) {
-#pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (n + c + j < a.N) fb_store(a, row, n + c + j, v[j]);
-      continue;
-    }
-    uint32_t w[16];
-    if (a.out_type == FB_F32) {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(v[j]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (a.out_type == FB_BF16) {
-          const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-          w[j] = *reinterpret_cast<const uint32_t*>(&h);
-        } else {
-          const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-          w[j] = *reinterpret_cast<const uint32_t*>(&h);
-        }
-      }
-    }
-    char* p = (char*)a.out + i * (a.out_type == FB_F32 ? 4 : 2);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (h == 1 && a.out_type != FB_F32) break;
-      if (vec == 32) {
-        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p + 32 * h), "r"(w[8 * h]), "r"(w[8 * h + 1]), "r"(w[8 * h + 2]), "r"(w[8 * h + 3]), "r"(w[8 * h + 4]),
-                     "r"(w[8 * h + 5]), "r"(w[8 * h + 6]), "r"(w[8 * h + 7])
-                     : "memory");
-      } else {
-        *reinterpret_cast<uint4*>(p + 32 * h) = make_uint4(w[8 * h], w[8 * h + 1], w[8 * h + 2], w[8 * h + 3]);
-        *reinterpret_cast<uint4*>(p + 32 * h + 16) = make_uint4(w[8 * h + 4], w[8 * h + 5], w[8 * h + 6], w[8 * h + 7]);
-      }
-    }
+    for (int j = 0; j < COLS; ++j)
+      if (j < left) acc[j] += __ldg(bias + j);
   }
+  const auto store = [&](auto type) {
+    constexpr int TYPE = decltype(type)::value, SIZE = TYPE == FB_F32 ? 4 : 2, WORDS = COLS * SIZE / 4;
+    const auto word = [&](int i) -> uint32_t {
+      if (i >= WORDS) return 0u;
+      if constexpr (TYPE == FB_F32) {
+        return __float_as_uint(acc[i]);
+      } else if constexpr (TYPE == FB_BF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(acc[2 * i], acc[2 * i + 1]);
+        return *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __half2 h = __floats2half2_rn(acc[2 * i], acc[2 * i + 1]);
+        return *reinterpret_cast<const uint32_t*>(&h);
+      }
+    };
+    char* p = (char*)a.out + (row * a.ldo + n) * SIZE;
+    if ((SIZE == 2 || COLS < 128) && wide && left == COLS) {      // (of 128 float32 columns: the build would spill)
+#pragma unroll
+      for (int i = 0; i < WORDS; i += 8)
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p + 4 * i), "r"(word(i)), "r"(word(i + 1)), "r"(word(i + 2)), "r"(word(i + 3)), "r"(word(i + 4)),
+                     "r"(word(i + 5)), "r"(word(i + 6)), "r"(word(i + 7))
+                     : "memory");
+      return;
+    }
+    const int before = (int)(-(uintptr_t)p & 15), end = left * SIZE - before;             // bytes; end: from the boundary on
+    p += before;
+    const auto some = [&](const uint32_t (&x)[4], int at, int from, int to) {      // of 16 bytes, the first of which is byte `at`, those from .. to
+#pragma unroll
+      for (int j = 0; j < 16 / SIZE; ++j) {
+        const int b = at + SIZE * j;
+        if (b < from || b >= to) continue;
+        if constexpr (SIZE == 4) *reinterpret_cast<uint32_t*>(p + b) = x[j];
+        else *reinterpret_cast<uint16_t*>(p + b) = (uint16_t)(j & 1 ? x[j / 2] >> 16 : x[j / 2]);
+      }
+    };
+    if (before != 0) {
+      const uint32_t x[4] = {word(0), word(1), word(2), word(3)};
+      some(x, -before, -before, min(0, end));
+    }
+#pragma unroll
+    for (int i = 0; i < WORDS; i += 4) {
+      uint32_t x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = word(i + j);
+#pragma unroll
+      for (int j = 0; j < 6; ++j) x[j] = before & 8 ? x[j + 2] : x[j];
+#pragma unroll
+      for (int j = 0; j < 5; ++j) x[j] = before & 4 ? x[j + 1] : x[j];
+      if constexpr (SIZE == 2)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = __funnelshift_r(x[j], x[j + 1], before & 2 ? 16 : 0);
+      const uint32_t y[4] = {x[0], x[1], x[2], x[3]};
+      if (4 * i + 16 <= end) *reinterpret_cast<uint4*>(p + 4 * i) = make_uint4(y[0], y[1], y[2], y[3]);
+      else if (4 * i < end) some(y, 4 * i, 4 * i, end);
+    }
+  };
+  if (a.out_type == FB_BF16) store(std::integral_constant<int, FB_BF16>());
+  else if (a.out_type == FB_F16) store(std::integral_constant<int, FB_F16>());
+  else store(std::integral_constant<int, FB_F32>());
 }
 
-struct FbWideArgs { int parts, row_tiles, col_tiles, band, vec; };
+struct FbWideArgs { int parts, row_tiles, col_tiles, band, wide; };           // wide: every row of out begins on a 32-byte boundary
 
 template <int CG, bool EXPERTS>
 __global__ void __launch_bounds__(FbWide<CG>::THREADS, 1)
@@ -894,7 +915,7 @@ fp8_block_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
       if (!ok) break;
       const int n = ct * 256 + 128 * side;
       if (wa.parts == 1) {
-        if (o >= 0 && n < a.N) fb_store_row(a, o, n, acc, r < 0, wa.vec);
+        if (o >= 0 && n < a.N) fb_store_row(a, o, n, acc, EXPERTS && r < 0, wa.wide != 0);
       } else {
         // one tile a cluster: the ring has been read to its end.  [256 columns][128 rows]
         float* red = (float*)smem + 128 * side * 128 + at_row;
@@ -922,22 +943,22 @@ fp8_block_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
   } else if (wa.parts > 1 && unit < tiles) {
     // each of the parts adds up its share of the columns, a thread 16 neighbouring ones of a row at a time
     const FbTile f = tile_of(unit);
-    const int mine = min(128, f.rows - 128 * half), c0 = 16 * (16 * part / wa.parts), c1 = 16 * (16 * (part + 1) / wa.parts), row = threadIdx.x & 127;
+    const int row = threadIdx.x & 127, out_row = f.row0 + 128 * half + row, n0 = f.ct * 256;
+    const int c1 = row < f.rows - 128 * half ? min(16 * (16 * (part + 1) / wa.parts), a.N - n0) : 0;
     const uint32_t base = smem_u32(smem) + row * 4;
-    for (int c = c0 + (threadIdx.x >> 7) * 16; c < c1; c += L::THREADS / 128 * 16) {
-      if (row >= mine || f.ct * 256 + c >= a.N) continue;
+    for (int c = 16 * (16 * part / wa.parts) + (threadIdx.x >> 7) * 16; c < c1; c += L::THREADS / 128 * 16) {
       float v[16];
 #pragma unroll
       for (int u = 0; u < 16; ++u) v[u] = 0.f;
       for (int p = 0; p < wa.parts; ++p) {
-        const uint32_t from = mapa_u32(base, CG * p + half);
+        const uint32_t from = mapa_u32(base, CG * p + half) + c * 512;
         float x[16];
 #pragma unroll
-        for (int u = 0; u < 16; ++u) x[u] = ld_cluster_f(from + (c + u) * 512);
+        for (int u = 0; u < 16; ++u) x[u] = ld_cluster_f(from + u * 512);
 #pragma unroll
         for (int u = 0; u < 16; ++u) v[u] += x[u];
       }
-      fb_store_row(a, f.row0 + 128 * half + row, f.ct * 256 + c, v, false, wa.vec);
+      fb_store_row(a, out_row, n0 + c, v, false, wa.wide != 0);
     }
   }
   if (CG == 2 || wa.parts > 1) cluster_sync();
@@ -1036,8 +1057,7 @@ static int fb_launch_wide(const void* q, long long ldq, const void* w, const FbA
   const int bands = (wa.row_tiles + 8 / CG * 2 - 1) / (8 / CG * 2);
   wa.band = (wa.row_tiles + bands - 1) / bands;
   const int size = a.out_type == FB_F32 ? 4 : 2;
-  const uintptr_t low = (uintptr_t)a.out | (uintptr_t)(a.ldo * size);
-  wa.vec = low % 32 == 0 ? 32 : low % 16 == 0 ? 16 : 0;
+  wa.wide = ((uintptr_t)a.out | (uintptr_t)(a.ldo * size)) % 32 == 0;
   const long long tiles = (long long)wa.row_tiles * wa.col_tiles;
   if (tiles > (1 << 30)) return (int)cudaErrorInvalidValue;
   const int units = parts > 1 || tiles < 148 / CG ? (int)tiles : 148 / CG;
@@ -1072,21 +1092,22 @@ static int fb_at_once(int dev, int size, int threads, int smem) {
   return known[dev][size];
 }
 
-// Which kernel a dense product takes, and how many parts of k: by an estimate of each one's microseconds, fitted to the times of 11 matrices (256 to 34,816 wide) at 11 row
-// counts from 1 to 4096.  A block of k takes a CTA of the few rows' kernel 0.24 to 0.29 us and one of the other 0.47; memory gives 6.6 TB/s of weights and L2 10 TB/s of what tiles
-// read again; a start 3 and 7 us (the larger kernel has its SM alone, so it cannot begin under the kernel before), a cluster's sums 1.3 and 3.
+// Which kernel a dense product takes, and how many parts of k: by an estimate of each one's microseconds, fitted to the times of all of them for 11 matrices (256 to 34,816 wide) at
+// 18 row counts from 1 to 8192.  What it picks takes 0.9% longer than the fastest, on average (128 x 5120 -> 5120 the most: 18.2 us, 16.2).  A block of k takes a CTA of the few rows' kernel 0.19
+// (T 16) to 0.28 us (T 64) and one of the other 0.41; memory gives 8 TB/s of weights and L2 22 of what tiles read again (parts of which other terms hide); a wave of the first starts in 4.4 us,
+// the second in 4, and takes 1.8 a tile to begin and store; a cluster's sums cost 0.1 + 0.12 a part, and 2.2 + 0.9.
 struct FbChoice { int cg, T, parts; double us; };
 template <int T>
 static void fb_consider_step(int dev, const FbArgs& a, FbChoice& best) {
   using L = FbStep<T>;
   const long long row_tiles = (a.rows + T - 1) / T, strips = (a.N + 127) / 128, tiles = row_tiles * strips;
   if (row_tiles > 65535) return;
-  const double dram = (double)a.N * a.K, all = (double)tiles * a.kblocks * (FB_A + (a.rows < T ? a.rows : T) * FB_K), mem = dram / 6.6e6 + (all - dram) / 10e6;
+  const double dram = (double)a.N * a.K, all = (double)tiles * a.kblocks * (FB_A + (a.rows < T ? a.rows : T) * FB_K), mem = dram / 8e6 + (all - dram) / 22e6;
   for (int parts = 1; parts <= 8 && parts <= a.kblocks; ++parts) {
     const int slots = L::PER_SM * fb_at_once<fp8_block_step_kernel<T, false>>(dev, parts, L::THREADS, L::SMEM);
     if (slots <= 0) continue;
-    const double waves = (double)((tiles + slots - 1) / slots), blocks = (a.kblocks + parts - 1) / parts, k = waves * blocks * (T == 16 ? 0.24 : T == 32 ? 0.27 : 0.29);
-    const double us = 3.0 * waves + sqrt(k * k + mem * mem) + (parts > 1 ? 1.3 : 0);
+    const double waves = (double)((tiles + slots - 1) / slots), blocks = (a.kblocks + parts - 1) / parts, k = waves * blocks * (T == 16 ? 0.19 : T == 32 ? 0.205 : 0.28);
+    const double us = 4.4 * waves + sqrt(k * k + mem * mem) + (parts > 1 ? 0.1 + 0.12 * parts : 0);
     if (us < best.us) best = {0, T, parts, us};
   }
 }
@@ -1094,12 +1115,12 @@ template <int CG>
 static void fb_consider_wide(int dev, const FbArgs& a, FbChoice& best) {
   using L = FbWide<CG>;
   const long long row_tiles = (a.rows + 128 * CG - 1) / (128 * CG), tiles = row_tiles * ((a.N + 255) / 256);
-  const double dram = (double)a.N * a.K, all = (double)tiles * CG * a.kblocks * ((a.rows < 128 ? a.rows : 128) * FB_K + L::B), mem = dram / 6.6e6 + (all - dram) / 10e6;
+  const double dram = (double)a.N * a.K, all = (double)tiles * CG * a.kblocks * ((a.rows < 128 ? a.rows : 128) * FB_K + L::B), mem = dram / 8e6 + (all - dram) / 22e6;
   for (int parts = 1; parts * CG <= 8 && parts <= a.kblocks; ++parts) {
     const int slots = fb_at_once<fp8_block_wide_kernel<CG, false>>(dev, CG * parts, L::THREADS, L::SMEM);
     if (slots <= 0 || (parts > 1 && tiles > slots)) continue;      // (a cluster with parts has one tile)
-    const double waves = (double)((tiles + slots - 1) / slots), blocks = (a.kblocks + parts - 1) / parts, k = waves * (blocks * (CG == 2 ? 0.46 : 0.47) + 0.4);
-    const double us = 7.0 + sqrt(k * k + mem * mem) + (parts > 1 ? 3.0 : 0);
+    const double waves = (double)((tiles + slots - 1) / slots), blocks = (a.kblocks + parts - 1) / parts, k = waves * (blocks * 0.41 + 1.8);
+    const double us = 4.0 + sqrt(k * k + mem * mem) + (parts > 1 ? 2.2 + 0.9 * parts : 0);
     if (us < best.us) best = {CG, 0, parts, us};
   }
 }

@@ -78,6 +78,23 @@ def test_linear_of_models_sizes(M, Kd, N, dtype):
     check_linear(M, Kd, N, dtype, bias=True)
 
 
+@pytest.mark.parametrize("M,Kd,N", [(300, 1024, 517), (2000, 256, 1031), (700, 2048, 255), (1500, 128, 300)])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_rows_of_out_that_begin_anywhere(M, Kd, N, dtype):
+    """Columns of a larger tensor from any of 9 on, of odd and even row lengths: what stands beside them stays."""
+    g = gen(M)
+    q, s = rows_of(M, Kd, g)
+    w, status = weight_of(Kd, N, g, bias=True), K.new_status()
+    x, m = values(q, s), dense64(w)
+    want, size = x @ m.T + w.bias.double(), x.abs() @ m.abs().T + w.bias.double().abs()
+    for at, spare in ((0, 0), (1, 0), (2, 1), (3, 0), (4, 3), (5, 2), (6, 0), (7, 1), (8, 5)):
+        room = torch.full((M, N + at + spare), 7.0, device="cuda", dtype=dtype)
+        K.fp8_block_linear(q, s, w, room[:, at:at + N], status)
+        K.check_status(status)
+        assert bool((room[:, :at] == 7).all()) and bool((room[:, at + N:] == 7).all())
+        near(room[:, at:at + N], want, size, Kd, dtype)
+
+
 @pytest.mark.parametrize("M,Kd,N", [(1, 2048, 256), (40, 688, 300), (200, 4096, 256), (900, 1024, 1024)])
 def test_calls_repeat_to_the_bit(M, Kd, N):
     q, s, w, out = check_linear(M, Kd, N)
