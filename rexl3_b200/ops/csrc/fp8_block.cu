@@ -120,6 +120,10 @@ __device__ __forceinline__ float ld_cluster_f(uint32_t addr) {         // of an 
   return v;
 }
 
+__device__ __forceinline__ void st_cluster_f4(uint32_t addr, float a, float b, float c, float d) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
+}
+
 // 16 or 32 columns of a thread's tensor memory lane
 __device__ __forceinline__ void fb_ld(uint32_t taddr, uint32_t (&r)[16]) { tc_ld_32x32b_x16(taddr, r); }
 __device__ __forceinline__ void fb_ld(uint32_t taddr, uint32_t (&r)[32]) {
@@ -504,7 +508,7 @@ struct FbWide {
   static constexpr int STAGE = A + B, STAGES = CG == 2 ? 6 : 4;
   static constexpr int SG = 8, SC = 2;             // blocks of scales that are fetched and given back together; that many times
   static constexpr int SC_ROW = 132;               // of a block: 128 rows', two strips'
-  static constexpr int SC_BUF = SG * SC_ROW + 260; // and, with a tile's first blocks, what the sums know of it: where each row goes, its row of q, the column tile, its rows
+  static constexpr int SC_BUF = SG * SC_ROW + 260; // and, with a tile's first blocks, what the sums know of it: where each row goes, its row of q, the column tile
   static constexpr int MAX_EXPERTS = 4096;
   static constexpr int SMEM = 1024 + STAGES * STAGE + SC * SC_BUF * 4 + 512;
   static constexpr int SMEM_EXPERTS = SMEM + (MAX_EXPERTS + 1) * 4;
@@ -617,10 +621,20 @@ __device__ __forceinline__ void fb_store_row(const FbArgs& a, long long row, int
 
 struct FbWideArgs { int parts, row_tiles, col_tiles, band, wide; };           // wide: every row of out begins on a 32-byte boundary
 
-template <int CG, bool EXPERTS>
+// Registers of a thread: what the block is launched with, and what the sums' warps and the others have then.  (Single CTAs that join their parts need a few more after the sums.)
+constexpr int FB_WIDE_REGS = 168;
+template <int CG, bool PARTS>
+struct FbRegs {
+  static constexpr int OTHERS = CG == 1 && PARTS ? 104 : 88, SUMS = CG == 1 && PARTS ? 200 : 208;
+  static_assert(8 * SUMS + 4 * OTHERS <= 12 * FB_WIDE_REGS, "more registers than the block is launched with");
+};
+
+// PARTS: clusters of several parts, a tile each; otherwise a CTA (pair) goes from tile to tile.  (Both in one build: the sums' loop came out up to a quarter slower.)
+template <int CG, bool EXPERTS, bool PARTS>
 __global__ void __launch_bounds__(FbWide<CG>::THREADS, 1)
 fp8_block_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ FbArgs a, const __grid_constant__ FbWideArgs wa) {
   using L = FbWide<CG>;
+  const int parts = PARTS ? wa.parts : 1;
   pdl_launch();
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -639,9 +653,9 @@ fp8_block_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
   int* first = (int*)(smem + L::SMEM - 1024);                     // experts: row tiles before each expert's
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t rank = 0;
-  if (CG == 2 || wa.parts > 1) asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(rank));
-  const int half = CG == 2 ? rank & 1 : 0, part = rank / CG, units = gridDim.x / (CG * wa.parts), unit = blockIdx.x / (CG * wa.parts);
-  const int b0 = (int)((long long)a.kblocks * part / wa.parts), nb = (int)((long long)a.kblocks * (part + 1) / wa.parts) - b0;
+  if (CG == 2 || PARTS) asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(rank));
+  const int half = CG == 2 ? rank & 1 : 0, part = rank / CG, units = gridDim.x / (CG * parts), unit = blockIdx.x / (CG * parts);
+  const int b0 = (int)((long long)a.kblocks * part / parts), nb = (int)((long long)a.kblocks * (part + 1) / parts) - b0;
   const uint32_t lead = CG == 2 ? rank & ~1u : rank;              // the pair's first CTA
   constexpr int ROWS = 128 * CG;
 
@@ -672,7 +686,7 @@ fp8_block_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
   }
   tc_fence_before();
   __syncthreads();
-  if (CG == 2 || wa.parts > 1) cluster_sync();
+  if (CG == 2 || PARTS) cluster_sync();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int tiles = (EXPERTS ? first[a.experts] : wa.row_tiles) * wa.col_tiles;
@@ -706,7 +720,7 @@ fp8_block_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
   };
   // a group's registers are changed by all its four warps
   if (warp >= L::EW) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(FbRegs<CG, PARTS>::OTHERS));
     if (warp == 8) {
       // ---- copies: this CTA's rows and its share of the tile's columns
       int s = 0, it = 0;
@@ -848,7 +862,7 @@ fp8_block_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
             int* tile = (int*)(scales + at * L::SC_BUF + L::SG * L::SC_ROW);
 #pragma unroll
             for (int j = 0; j < 4; ++j) tile[32 * j + lane] = out[j], tile[128 + 32 * j + lane] = in[j];
-            if (lane == 0) tile[256] = f.ct, tile[257] = mine;
+            if (lane == 0) tile[256] = f.ct;
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(&sc_full[at]);
@@ -866,8 +880,10 @@ fp8_block_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
     }
+    __syncwarp();
+    if (PARTS) cluster_sync();
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(FbRegs<CG, PARTS>::SUMS));
     // ---- sums: lane = row, warps 0-3 the tile's first 128 columns, 4-7 the others
     const int q = warp & 3, side = warp >> 2, at_row = 32 * q + lane;
     const uint32_t src = tmem + ((uint32_t)(q * 32) << 16) + 128 * side;
@@ -879,7 +895,7 @@ fp8_block_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
       ok = fb_wait_warp(&sc_full[at], sc_phase, abort_flag);
       if (!ok) break;
       const int* tile = (const int*)(scales + at * L::SC_BUF + L::SG * L::SC_ROW);
-      const int o = tile[at_row], r = tile[128 + at_row], ct = tile[256], mine = tile[257];
+      const int o = tile[at_row], r = tile[128 + at_row], ct = tile[256];
       float acc[128];
 #pragma unroll
       for (int j = 0; j < 128; ++j) acc[j] = 0.f;
@@ -893,17 +909,18 @@ fp8_block_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
         ok = fb_wait_warp(&acc_full[buf], acc_phase, abort_flag);
         if (!ok) break;
         tc_fence_after();
-        if (32 * q < mine) {
+        // the next 16 columns are on their way while these are added.  (All warps do all of it: a branch around it for rows that the tile lacks costs 8192 x 5120 -> 34,816 1553 and not
+        // 1406 us, and without the loads ahead there are not registers enough.)
+        uint32_t v[2][16];
+        fb_ld(src + buf * 256, v[0]);
 #pragma unroll
-          for (int c = 0; c < 128; c += 16) {
-            uint32_t v[16];
-            fb_ld(src + buf * 256 + c, v);
-            fb_ld_wait(v);
+        for (int c = 0; c < 128; c += 16) {
+          fb_ld_wait(v[c / 16 & 1]);
+          if (c + 16 < 128) fb_ld(src + buf * 256 + c + 16, v[(c / 16 + 1) & 1]);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) acc[c + j] = fmaf(__uint_as_float(v[j]), scale, acc[c + j]);
-          }
-          tc_fence_before();
+          for (int j = 0; j < 16; ++j) acc[c + j] = fmaf(__uint_as_float(v[c / 16 & 1][j]), scale, acc[c + j]);
         }
+        tc_fence_before();
         __syncwarp();
         fb_arrive_warp(acc_free + 8 * buf);
         if (buf ^= 1; buf == 0) acc_phase ^= 1;
@@ -914,22 +931,31 @@ fp8_block_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
       }
       if (!ok) break;
       const int n = ct * 256 + 128 * side;
-      if (wa.parts == 1) {
+      if (!PARTS) {
         if (o >= 0 && n < a.N) fb_store_row(a, o, n, acc, EXPERTS && r < 0, wa.wide != 0);
       } else {
-        // one tile a cluster: the ring has been read to its end.  [256 columns][128 rows]
-        float* red = (float*)smem + 128 * side * 128 + at_row;
+        // One tile a cluster.  Once every CTA's ring has been read to its end, each part sends its sums of 16 columns to the part that adds them up (stores, which nobody waits for one by
+        // one; fetched instead, 333 x 10,240 -> 1000 in 8 parts took 20.0 and not 17.5 us).  There they stand [part][16 columns][4 of them][128 rows][4].
+        cluster_sync();
+        const int most = (16 + parts - 1) / parts;
 #pragma unroll
-        for (int j = 0; j < 128; ++j) red[j * 128] = acc[j];
+        for (int i = 0; i < 8; ++i) {
+          const int group = 8 * side + i, owner = ((group + 1) * parts - 1) / 16;
+          const uint32_t to = mapa_u32(smem_u32(smem), CG * owner + half) + (part * most + group - 16 * owner / parts) * (16 * 128 * 4) + at_row * 16;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) st_cluster_f4(to + u * (128 * 16), acc[16 * i + 4 * u], acc[16 * i + 4 * u + 1], acc[16 * i + 4 * u + 2], acc[16 * i + 4 * u + 3]);
+        }
       }
     }
+    __syncwarp();
+    if (PARTS && !ok) cluster_sync();
   }
   tc_fence_before();
   __syncthreads();
   if (CG == 2 && *abort_flag != 0 && threadIdx.x == 0)
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapa_u32(smem_u32((const void*)abort_flag), rank ^ 1)), "r"(1) : "memory");
   __syncwarp();
-  if (CG == 2 || wa.parts > 1) cluster_sync();
+  if (CG == 2 || PARTS) cluster_sync();
   if (*abort_flag != 0) {
     // Either CTA has given up, and the last copies may be under way.  A stage that only one CTA has issued its copies for gets the other's bytes here.
     if (half == 0 && threadIdx.x == 0) {
@@ -940,28 +966,27 @@ fp8_block_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
       ring_landed(full, L::STAGES, max(n0, n1));
     }
     __syncwarp();
-  } else if (wa.parts > 1 && unit < tiles) {
+  } else if (PARTS) {
     // each of the parts adds up its share of the columns, a thread 16 neighbouring ones of a row at a time
     const FbTile f = tile_of(unit);
     const int row = threadIdx.x & 127, out_row = f.row0 + 128 * half + row, n0 = f.ct * 256;
-    const int c1 = row < f.rows - 128 * half ? min(16 * (16 * (part + 1) / wa.parts), a.N - n0) : 0;
-    const uint32_t base = smem_u32(smem) + row * 4;
-    for (int c = 16 * (16 * part / wa.parts) + (threadIdx.x >> 7) * 16; c < c1; c += L::THREADS / 128 * 16) {
+    const int c1 = row < f.rows - 128 * half ? min(16 * (16 * (part + 1) / parts), a.N - n0) : 0;
+    const int first_c = 16 * (16 * part / parts), most = (16 + parts - 1) / parts;
+    for (int c = first_c + (threadIdx.x >> 7) * 16; c < c1; c += L::THREADS / 128 * 16) {
+      const float4* from = (const float4*)smem + (c - first_c) / 16 * (4 * 128) + row;
       float v[16];
 #pragma unroll
       for (int u = 0; u < 16; ++u) v[u] = 0.f;
-      for (int p = 0; p < wa.parts; ++p) {
-        const uint32_t from = mapa_u32(base, CG * p + half) + c * 512;
-        float x[16];
+      for (int p = 0; p < parts; ++p, from += most * (4 * 128))
 #pragma unroll
-        for (int u = 0; u < 16; ++u) x[u] = ld_cluster_f(from + u * 512);
-#pragma unroll
-        for (int u = 0; u < 16; ++u) v[u] += x[u];
-      }
+        for (int u = 0; u < 4; ++u) {
+          const float4 x = from[u * 128];
+          v[4 * u] += x.x, v[4 * u + 1] += x.y, v[4 * u + 2] += x.z, v[4 * u + 3] += x.w;
+        }
       fb_store_row(a, out_row, n0 + c, v, false, wa.wide != 0);
     }
   }
-  if (CG == 2 || wa.parts > 1) cluster_sync();
+  if (CG == 2) cluster_sync();
   if (warp == 9) {
     __syncwarp();
     if constexpr (CG == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
@@ -1026,24 +1051,22 @@ static int fb_launch_step(const void* q, long long ldq, const void* w, const FbA
 }
 
 // The registers that the sums' warps add come out of what the block was launched with, and they would wait for them: a build with fewer a thread is not launched.
-constexpr int FB_WIDE_REGS = 168;
-static_assert(8 * 208 + 4 * 88 <= 12 * FB_WIDE_REGS, "more registers than the block is launched with");
-template <int CG, bool EXPERTS>
+template <int CG, bool EXPERTS, bool PARTS>
 static int fb_wide_builds() {
   static const int regs = [] {
     cudaFuncAttributes at;
-    return cudaFuncGetAttributes(&at, fp8_block_wide_kernel<CG, EXPERTS>) == cudaSuccess ? at.numRegs : 0;
+    return cudaFuncGetAttributes(&at, fp8_block_wide_kernel<CG, EXPERTS, PARTS>) == cudaSuccess ? at.numRegs : 0;
   }();
   return regs == FB_WIDE_REGS ? 0 : (int)cudaErrorInvalidKernelImage;
 }
 
-template <int CG, bool EXPERTS>
+template <int CG, bool EXPERTS, bool PARTS>
 static int fb_launch_wide(const void* q, long long ldq, const void* w, const FbArgs& a, int parts, cudaStream_t st) {
   using L = FbWide<CG>;
-  auto kern = fp8_block_wide_kernel<CG, EXPERTS>;
+  auto kern = fp8_block_wide_kernel<CG, EXPERTS, PARTS>;
   const int smem = EXPERTS ? L::SMEM_EXPERTS : L::SMEM;
-  if (const int ce = fb_wide_builds<CG, EXPERTS>()) return ce;
-  if (const int ce = fb_allow<fp8_block_wide_kernel<CG, EXPERTS>>(smem)) return ce;
+  if (const int ce = fb_wide_builds<CG, EXPERTS, PARTS>()) return ce;
+  if (const int ce = fb_allow<fp8_block_wide_kernel<CG, EXPERTS, PARTS>>(smem)) return ce;
   CUtensorMap tw, tx;
   int e = fb_tmap(&tw, w, (uint64_t)a.N * (EXPERTS ? a.experts : 1), a.K, a.K, 256 / CG);
   if (e == 0) e = fb_tmap(&tx, q, a.rows, a.K, ldq, 128);
@@ -1060,7 +1083,7 @@ static int fb_launch_wide(const void* q, long long ldq, const void* w, const FbA
   wa.wide = ((uintptr_t)a.out | (uintptr_t)(a.ldo * size)) % 32 == 0;
   const long long tiles = (long long)wa.row_tiles * wa.col_tiles;
   if (tiles > (1 << 30)) return (int)cudaErrorInvalidValue;
-  const int units = parts > 1 || tiles < 148 / CG ? (int)tiles : 148 / CG;
+  const int units = PARTS || tiles < 148 / CG ? (int)tiles : 148 / CG;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(CG * parts * units), cfg.blockDim = dim3(L::THREADS), cfg.dynamicSmemBytes = smem, cfg.stream = st;
   cudaLaunchAttribute at[2];
@@ -1117,7 +1140,8 @@ static void fb_consider_wide(int dev, const FbArgs& a, FbChoice& best) {
   const long long row_tiles = (a.rows + 128 * CG - 1) / (128 * CG), tiles = row_tiles * ((a.N + 255) / 256);
   const double dram = (double)a.N * a.K, all = (double)tiles * CG * a.kblocks * ((a.rows < 128 ? a.rows : 128) * FB_K + L::B), mem = dram / 8e6 + (all - dram) / 22e6;
   for (int parts = 1; parts * CG <= 8 && parts <= a.kblocks; ++parts) {
-    const int slots = fb_at_once<fp8_block_wide_kernel<CG, false>>(dev, CG * parts, L::THREADS, L::SMEM);
+    const int slots = parts > 1 ? fb_at_once<fp8_block_wide_kernel<CG, false, true>>(dev, CG * parts, L::THREADS, L::SMEM)
+                                : fb_at_once<fp8_block_wide_kernel<CG, false, false>>(dev, CG, L::THREADS, L::SMEM);
     if (slots <= 0 || (parts > 1 && tiles > slots)) continue;      // (a cluster with parts has one tile)
     const double waves = (double)((tiles + slots - 1) / slots), blocks = (a.kblocks + parts - 1) / parts, k = waves * (blocks * 0.41 + 1.8);
     const double us = 4.0 + sqrt(k * k + mem * mem) + (parts > 1 ? 2.2 + 0.9 * parts : 0);
@@ -1158,8 +1182,8 @@ RX_API int rx_fp8_block_linear(const void* q, long long ldq, const void* s, long
     fb_consider_wide<2>(dev, a, c);
   }
   cudaStream_t st = (cudaStream_t)stream;
-  if (c.cg == 1) return fb_launch_wide<1, false>(q, ldq, w, a, c.parts, st);
-  if (c.cg == 2) return fb_launch_wide<2, false>(q, ldq, w, a, c.parts, st);
+  if (c.cg == 1) return c.parts > 1 ? fb_launch_wide<1, false, true>(q, ldq, w, a, c.parts, st) : fb_launch_wide<1, false, false>(q, ldq, w, a, 1, st);
+  if (c.cg == 2) return c.parts > 1 ? fb_launch_wide<2, false, true>(q, ldq, w, a, c.parts, st) : fb_launch_wide<2, false, false>(q, ldq, w, a, 1, st);
   if (c.T == 16) return fb_launch_step<16, false>(q, ldq, w, a, 1, c.parts, st);
   if (c.T == 32) return fb_launch_step<32, false>(q, ldq, w, a, 1, c.parts, st);
   if (c.T == 64) return fb_launch_step<64, false>(q, ldq, w, a, (rows + 63) / 64, c.parts, st);
@@ -1181,7 +1205,7 @@ RX_API int rx_fp8_block_experts(const void* q, long long ldq, const void* s, lon
   if (src != nullptr && (long long)rows * (ldq / 16) > 0xFFFFFFFFll) return (int)cudaErrorInvalidValue;      // a row's place is held in 32 bits, of 16 bytes
   cudaStream_t st = (cudaStream_t)stream;
   // Up to six positions an expert: tiles of 16 rows, whose CTAs begin sooner (8 of 128 experts, a row each 10 us and 17, 800 positions 65 and 67; 2000 positions 88 and 70).
-  if (cap > 6 * experts) return fb_launch_wide<1, true>(q, ldq, w, a, 1, st);
+  if (cap > 6 * experts) return fb_launch_wide<1, true, false>(q, ldq, w, a, 1, st);
   const int some = experts < cap ? experts : cap;
   const long long row_tiles = ((long long)cap + (long long)some * 15) / 16;          // the most tiles that `cap` rows of `some` experts can make
   return fb_launch_step<16, true>(q, ldq, w, a, (int)row_tiles, 1, st);
