@@ -4,7 +4,11 @@
 //
 // The inner sums are tensor-core products (kind::f8f6f4, float32 accumulators in tensor memory), one per block of k and from zero: a block's scales do not
 // factor out of the sum over blocks.  So a group of warps takes each block's accumulator out of tensor memory, multiplies and adds it into registers
-// while the next blocks' products fill the other accumulators.
+// while the next blocks' products fill the other accumulators.  Nothing is rounded to fewer than 32 bits before out.
+//
+// Two kernels.  Few rows: fp8_block_step_kernel, whose tensor-core rows are the weights' (128 columns of out) and whose columns are the rows (16, 32 or 64), so that a tile
+// of few rows wastes nothing; it is bound by the weights' way from memory.  Many rows: fp8_block_wide_kernel, tiles of 128 x 256 or, by pairs of CTAs, 256 x 256.  Each has a form
+// for routed experts.  An estimate of both chooses (below).
 #include <cuda.h>
 #include <math.h>
 #include <type_traits>
@@ -201,6 +205,9 @@ __device__ __forceinline__ int fb_count_tiles(const FbArgs& a, int lane, F&& eac
 
 // Few rows.  The weights are the M side: a CTA has a strip of 128 output columns (TMEM lanes) and T rows (TMEM columns), and the CTAs of a cluster share the
 // strip's blocks of k; their sums are added in the order of the CTAs through distributed shared memory.
+// What bounds it: memory.  1 x 5120 -> 34,816 27.6 us, 6.5 TB/s (what a copy takes); 16 rows x 8 of 128 experts, 2048 -> 1536, 41 us, 6.3 TB/s.  A CTA's block takes 0.19 to 0.28 us of handing
+// over (blocks by fours: one by one it was 0.5), so a strip with many blocks of k goes to several CTAs, which T = 64 has room for by whole clusters only: 64 x 17,408 -> 5120 has 40 strips
+// in 3 parts, 120 of 148 SMs, 20.6 us, 4.4 TB/s.  Two CTAs of T = 64 an SM (four stages, batches of two): 30 us.
 template <int T>
 struct FbStep {
   static constexpr int PER_SM = T <= 32 ? 2 : 1;   // CTAs of an SM
@@ -501,6 +508,10 @@ fp8_block_step_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
 // Many rows.  The rows are the M side: a CTA has 128 rows (TMEM lanes) and 256 columns, alone (CG 1) or as half of a pair that shares the weights of a tile of
 // 256 x 256 (CG 2).  A thread of the sums has one row, so a block's scale is one value for its 128 columns (a strip of the weights).  CTAs go from tile to tile; where
 // there are few tiles, `parts` of them (pairs of them) in a cluster share a tile's blocks of k, and their sums are added in order through distributed shared memory.
+// What bounds it: two accumulators of 256 columns are all of tensor memory, and one's round trip is the products (512 cycles), the sums (335: 128 multiply-adds and 8 loads of two warps
+// a scheduler) and the barriers between (some 900): 890 cycles a block.  8192 x 5120 -> 34,816 1406 to 1510 us by the clock that the power leaves, 1.93 to 2.08 PFLOP/s; without the sums it would be
+// 1125, without the products 960.  Slower: four accumulators of 128 columns (an operand is read from shared memory twice, 6%), 16 warps of sums (23%), one lane that waits for its warp (38%).
+// Routed experts: 2100 rows x 8 of 128 experts, 2048 -> 1536, 145 us: what passes from L2 (800 MB, weights 1.5 times, because 131 rows an expert are two tiles for half of them).
 template <int CG>
 struct FbWide {
   static constexpr int EW = 8, THREADS = 384;      // 0-7: sums; 8: copies, 9: products, 10: scales, 11: the watch over the waits
@@ -1204,9 +1215,10 @@ RX_API int rx_fp8_block_experts(const void* q, long long ldq, const void* s, lon
   if ((src == nullptr && cap > rows) || (dst == nullptr && cap > out_rows)) return (int)cudaErrorInvalidValue;
   if (src != nullptr && (long long)rows * (ldq / 16) > 0xFFFFFFFFll) return (int)cudaErrorInvalidValue;      // a row's place is held in 32 bits, of 16 bytes
   cudaStream_t st = (cudaStream_t)stream;
-  // Up to six positions an expert: tiles of 16 rows, whose CTAs begin sooner (8 of 128 experts, a row each 10 us and 17, 800 positions 65 and 67; 2000 positions 88 and 70).
-  if (cap > 6 * experts) return fb_launch_wide<1, true, false>(q, ldq, w, a, 1, st);
+  // Up to six positions an expert: tiles of 16 rows, whose CTAs begin sooner (8 of 128 experts, 2048 -> 1536: a row 10.2 us and 13.7, 768 positions 61 and 59, 2048 89 and 63; 2 of 16, 7168 -> 4096,
+  // 24 rows 67 and 79).  But each of them begins anew, so with few blocks of k they have to find room at once (768 -> 2048: 24 positions 12.5 us and 13.4, 96 27.7 and 21).
   const int some = experts < cap ? experts : cap;
+  if (cap > 6 * experts || (a.kblocks < 12 && (long long)some * ((N + 127) / 128) > 444)) return fb_launch_wide<1, true, false>(q, ldq, w, a, 1, st);
   const long long row_tiles = ((long long)cap + (long long)some * 15) / 16;          // the most tiles that `cap` rows of `some` experts can make
   return fb_launch_step<16, true>(q, ldq, w, a, (int)row_tiles, 1, st);
 }
