@@ -8,12 +8,29 @@ reference's runtime, crates/server/src/runtime.rs:603).  Per step the host uploa
 """
 from __future__ import annotations
 
+import contextlib
+import gc
+
 import numpy as np
 import torch
 
 from ..models.dense import PAGE, DenseGPU
 from ..sched import BlockPool
 from .backend import Backend, BackendError, RowOutput
+
+
+@contextlib.contextmanager
+def capturing(graph):
+    """`torch.cuda.graph(graph)` with Python's cycle collector off.  A backend that nobody holds any more is a cycle; collected in the middle of a capture, its own graphs would be
+    destroyed there, which a capture does not survive."""
+    on = gc.isenabled()
+    gc.disable()
+    try:
+        with torch.cuda.graph(graph):
+            yield
+    finally:
+        if on:
+            gc.enable()
 
 CTX_BUCKET = 2048   # decode graphs are captured per (rows, candidate count, context bucket)
 
@@ -714,7 +731,7 @@ class DenseGpuBackend(Backend):
         from ..ops import lib as _oplib
         g = torch.cuda.CUDAGraph()
         n0 = _oplib.launch_count
-        with torch.cuda.graph(g):
+        with capturing(g):
             self._window(M, count, bucket)
         self.graph_kernels[self._graph_key(M, count, bucket)] = _oplib.launch_count - n0
         self.graph_captures += 1
@@ -861,7 +878,7 @@ class DenseGpuBackend(Backend):
                 self._draft_chain(n, k, bucket)
                 torch.cuda.synchronize()
                 g = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(g):
+                with capturing(g):
                     self._draft_chain(n, k, bucket)
                 self.draft_graphs[key] = g
             g.replay()

@@ -18,7 +18,7 @@ import torch.distributed as dist
 from ..models.dense_tp import DenseTPShard
 from ..utils import trace
 from .backend import BackendError, RowOutput
-from .gpu_backend import DenseGpuBackend
+from .gpu_backend import DenseGpuBackend, capturing
 
 OP_STOP, OP_WINDOW, OP_PREFILL, OP_MARK, OP_SYNC, OP_TREE, OP_MOVES = 0, 1, 2, 3, 4, 5, 6
 # OP_TREE: a window of draft trees.  Payload: the rows, the dirty block-table rows, then tree_base [M], the private tables [M x W] and the
@@ -85,7 +85,7 @@ class _TpExec:
             torch.cuda.synchronize()
             g = torch.cuda.CUDAGraph()
             n0 = _oplib.launch_count
-            with torch.cuda.graph(g):
+            with capturing(g):
                 self.run_window_eager(M, count, bucket, tree_n)
             self.tp_graph_kernels[key] = _oplib.launch_count - n0
             self.tp_graphs[key] = g

@@ -1,4 +1,5 @@
 """Products of E4M3 rows and weights under scales for blocks of 128, dense and through routed experts, against the formula in 64 bits."""
+import gc
 import os
 import subprocess
 import sys
@@ -6,6 +7,7 @@ import sys
 import pytest
 import torch
 
+from rexl3_b200.engine.gpu_backend import capturing
 from rexl3_b200.ops import kernels as K
 from rexl3_b200.ops import lib as L
 
@@ -280,7 +282,7 @@ def test_a_feed_forward_block():
     # captured and replayed, beside eager calls on another stream with buffers of their own
     want = [t.clone() for t in (h, z, q3.view(torch.uint8), s3)]
     graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
+    with capturing(graph):
         block()
     other, so = torch.zeros_like(z), K.new_status()
     stream = torch.cuda.Stream()
@@ -440,6 +442,7 @@ def test_a_captured_call_follows_the_routing(rows):
         out, status, graph, stream = torch.zeros(rows * 3, 136, device="cuda"), K.new_status(), torch.cuda.CUDAGraph(), torch.cuda.Stream()
         K.fp8_block_experts(q, s, w, offs, out, status, src=pairs, src_div=3)
         torch.cuda.synchronize()
+        gc.collect()
         with torch.cuda.graph(graph, stream=stream):
             K.fp8_block_experts(q, s, w, offs, out, status, src=pairs, src_div=3)
         jobs.append((q, s, offs, pairs, out, status, graph, stream))

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from rexl3_b200.engine.gpu_backend import capturing
 from rexl3_b200.ops import kernels as K
 
 pytestmark = pytest.mark.gpu
@@ -205,7 +206,7 @@ def test_no_rows_and_captured_calls():
     torch.cuda.synchronize()
     want = [t.clone() for t in (q.view(torch.uint8), s, q2.view(torch.uint8), s2)]
     graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
+    with capturing(graph):
         K.add_norm_fp8(x, h, w, 1e-6, q, s)
         K.swiglu_fp8(h, q2, s2)
     for _ in range(3):
