@@ -1217,8 +1217,9 @@ RX_API int rx_fp8_block_experts(const void* q, long long ldq, const void* s, lon
   cudaStream_t st = (cudaStream_t)stream;
   // Up to six positions an expert: tiles of 16 rows, whose CTAs begin sooner (8 of 128 experts, 2048 -> 1536: a row 10.2 us and 13.7, 768 positions 61 and 59, 2048 89 and 63; 2 of 16, 7168 -> 4096,
   // 24 rows 67 and 79).  But each of them begins anew, so with few blocks of k they have to find room at once (768 -> 2048: 24 positions 12.5 us and 13.4, 96 27.7 and 21).
+  // And each of them counts all experts' tiles: 512 experts, 2048 -> 512, 128 positions 23.8 us and 26.7, 512 59.5 and 32; 4096 experts, 1536 -> 256, 4096 positions 768 and 62.
   const int some = experts < cap ? experts : cap;
-  if (cap > 6 * experts || (a.kblocks < 12 && (long long)some * ((N + 127) / 128) > 444)) return fb_launch_wide<1, true, false>(q, ldq, w, a, 1, st);
+  if (cap > 6 * experts || (long long)cap * experts > 65536 || (a.kblocks < 12 && (long long)some * ((N + 127) / 128) > 444)) return fb_launch_wide<1, true, false>(q, ldq, w, a, 1, st);
   const long long row_tiles = ((long long)cap + (long long)some * 15) / 16;          // the most tiles that `cap` rows of `some` experts can make
   return fb_launch_step<16, true>(q, ldq, w, a, (int)row_tiles, 1, st);
 }

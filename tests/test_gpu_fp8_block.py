@@ -385,7 +385,7 @@ def test_refusals():
 
 # ------------------------------------------------------------------------------------------------ what else a call may meet
 @pytest.mark.parametrize("first", [1, 2])
-@pytest.mark.parametrize("rows,picks", [(5000, 2), (13000, 2)])
+@pytest.mark.parametrize("rows,picks", [(8, 2), (5000, 2), (13000, 2)])
 def test_as_many_experts_as_there_may_be(rows, picks, first):
     g = gen(rows)
     w, status = weight_of(16 * first, 16, g, experts=4096), K.new_status()
